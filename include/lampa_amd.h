@@ -447,6 +447,88 @@ int lampa_gdr_traffic_probe_walk(const void* q, const void* k, const void* v, co
                                  const void* composites, void* o, int n_chunks, int H, int chunks_per_segment,
                                  void* stream);
 
+/* ------------------------------------------------------------------------------------- state-space operators */
+
+/* Selective scan of a state-space layer (the mixer of models/baselines/full_mamba2.py and hmamba.py, whose own scan lives in a
+ * package the reference imports): for every sequence and head, with the state S [N, P] in fp32,
+ *   delta_t = softplus(dt_t + dt_bias)  (softplus = 0: dt_t + dt_bias),
+ *   S_t = exp(delta_t A) S_{t-1} + delta_t B_t x_t^T,   y_t = S_t^T C_t + D x_t.
+ * Tensors of `dtype`: x, y [tokens, H, P], B, C [tokens, G, N] (head h reads group h / (H / G)), and dt [tokens, H] of dt_dtype
+ * (dtype or fp32), the last two dimensions contiguous and `*_stride` elements from one token to the next; A, D, dt_bias fp32 [H] (D, dt_bias may be NULL);
+ * states fp32 [n_seq, H, N, P]. Sequences: cu_seqlens (device int64 [n_seq + 1]: starts at 0, never decreases; boundaries
+ * outside 0 .. n_tokens are moved inside, and rows behind the last boundary come back as zero), or NULL for n_seq dense
+ * sequences of seq_len tokens. seg_tokens: length of the segments that run in parallel, a multiple of 64. N <= 128.
+ *
+ * slot_states [lampa_ss_slots, H, N, P] fp32 and slot_decay [lampa_ss_slots, H] fp32 are scratch of the forward; where a
+ * sequence may have more than one segment they must not be NULL. For gradients keep both (slot_states then holds the state at
+ * the start of every segment) and ht for lampa_ss_scan_bwd. */
+typedef struct {
+  const void *x, *dt, *B, *C;
+  const float *A, *D, *dt_bias, *h0;
+  void* y;
+  float* ht;
+  float *slot_states, *slot_decay;
+  const int64_t* cu_seqlens;
+  int64_t n_tokens, seq_len, seg_tokens;
+  int64_t x_stride, dt_stride, B_stride, C_stride, y_stride;
+  int32_t n_seq, H, P, G, N, dtype, dt_dtype, softplus;
+  /* gradients only: dy [tokens, H, P] contiguous and dht (or NULL) in; dx [tokens, H, P], dB, dC [tokens, G, N] in `dtype`,
+   * ddt [tokens, H] in dt_dtype, dA, dD, ddt_bias fp32 [H], dh0 fp32 (or NULL) out, all contiguous */
+  const void* dy;
+  const float* dht;
+  void *dx, *ddt, *dB, *dC;
+  float *dA, *dD, *ddt_bias, *dh0;
+  void* workspace;
+  int64_t workspace_bytes;
+} lampa_ss_args;
+
+int64_t lampa_ss_slots(const lampa_ss_args* args);
+int lampa_ss_scan_fwd(const lampa_ss_args* args, void* stream);
+int64_t lampa_ss_bwd_workspace_bytes(const lampa_ss_args* args);
+int lampa_ss_scan_bwd(const lampa_ss_args* args, void* stream);
+
+/* One token for each of n sequences: x, y [n, H, P], B, C [n, G, N] of dtype, dt [n, H] of dt_dtype (row strides in
+ * elements), A, D,
+ * dt_bias as above, state fp32 [n, H, N, P] read, new_state written (may be the same pointer: in place). Any N and P. */
+int lampa_ss_step(const void* x, int64_t x_stride, const void* dt, int64_t dt_stride, const void* B, int64_t B_stride,
+                  const void* C, int64_t C_stride, const float* A, const float* D, const float* dt_bias, const float* state,
+                  float* new_state, void* y, int n, int H, int P, int G, int N, int dtype, int dt_dtype, int softplus,
+                  void* stream);
+
+/* The causal short convolution (lampa_causal_conv1d_fwd) with what precedes and follows a call: x, y [n_tokens, D] of dtype (x with
+ * row stride x_stride, y contiguous), weight fp32 [D, W], bias fp32 [D] or NULL, activation 0 none / 1 SiLU. past [n_seq, D, W] of
+ * dtype or NULL: the W inputs before each sequence (the oldest is not read); last [n_seq, D, W] or NULL: the W inputs up to
+ * each sequence's end (not the same memory as past). Sequences as in lampa_ss_args. D % 8 == 0, W <= 8, 16-byte aligned rows. */
+int lampa_causal_conv1d_state_fwd(const void* x, int64_t x_stride, int64_t n_tokens, int D, int W, const float* weight,
+                                  const float* bias, const void* past, const int64_t* cu_seqlens, int n_seq, int64_t seq_len,
+                                  int activation, int dtype, void* y, void* last, void* stream);
+/* One token for each of n sequences: x, y [n, D], cache [n, D, W] moved on by x into new_cache (may be the same pointer). Any D. */
+int lampa_causal_conv1d_step(const void* x, int64_t x_stride, const void* cache, void* new_cache, const float* weight,
+                             const float* bias, int activation, int dtype, void* y, int64_t n, int D, int W, void* stream);
+/* Gradients of the convolution: dy, dx [n_tokens, D] contiguous, dweight_bias fp32 [D, W + 1] (a channel's taps, then its bias). */
+int64_t lampa_causal_conv1d_bwd_workspace_bytes(int64_t n_tokens, int D, int W, int dtype);
+int lampa_causal_conv1d_bwd(const void* x, int64_t x_stride, const void* dy, int64_t n_tokens, int D, int W, const float* weight,
+                            const float* bias, const void* past, const int64_t* cu_seqlens, int n_seq, int64_t seq_len,
+                            int activation, int dtype, void* dx, float* dweight_bias, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+
+/* Norm behind a block, its gate, the scaled residual add and the next block's norm (models/hattention/fused_norm.py:40-111 has
+ * the plain residual add + norm): a = x or rmsnorm(x) * post_weight (where post_weight is not NULL),
+ * r = residual + scale * act(gate) * a, y = rmsnorm(r) * weight. x, y [rows, D] of dtype; residual, residual_out of res_dtype
+ * (dtype or fp32); weights and scale fp32 [D] or NULL; gate_kind 0 none, 1 [rows, D], 2 [rows / seq_rows, D] (one row for every
+ * seq_rows rows); activation of the gate 0 none, 1 SiLU, 2 sigmoid. All contiguous, 16-byte aligned, D % 8 == 0, D <= 8192. */
+int lampa_residual_norm_fwd(const void* x, const void* residual, const float* weight, const float* post_weight, const void* gate,
+                            int gate_kind, int activation, const float* scale, int64_t rows, int64_t seq_rows, int D, float eps,
+                            int dtype, int res_dtype, void* y, void* residual_out, void* stream);
+/* Its gradients: dy of dtype and dres of res_dtype (either may be NULL: zero); dx, dgate of dtype, dresidual of res_dtype,
+ * dweight, dpost_weight, dscale fp32 [D] (those and dgate may be NULL where they are not wanted). */
+int64_t lampa_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t seq_rows, int D);
+int lampa_residual_norm_bwd(const void* x, const void* residual, const float* weight, const float* post_weight, const void* gate,
+                            int gate_kind, int activation, const float* scale, const void* dy, const void* dres, int64_t rows,
+                            int64_t seq_rows, int D, float eps, int dtype, int res_dtype, void* dx, void* dresidual, void* dgate,
+                            float* dweight, float* dpost_weight, float* dscale, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -93,6 +93,22 @@ _SIGNATURES = {
                                _i32, _i32, _f32, _i32, _vp]),
     "lampa_hgdn_tail": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _f32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32,
                                _i32, _i32, _i32, _f32, _i32, _vp]),
+    "lampa_ss_slots": (_i64, [_vp]),
+    "lampa_ss_scan_fwd": (_i32, [_vp, _vp]),
+    "lampa_ss_bwd_workspace_bytes": (_i64, [_vp]),
+    "lampa_ss_scan_bwd": (_i32, [_vp, _vp]),
+    "lampa_ss_step": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64] + [_vp] * 6 + [_i32] * 8 + [_vp]),
+    "lampa_causal_conv1d_state_fwd": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp,
+                                             _vp]),
+    "lampa_causal_conv1d_step": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _i32, _i32, _vp]),
+    "lampa_causal_conv1d_bwd_workspace_bytes": (_i64, [_i64, _i32, _i32, _i32]),
+    "lampa_causal_conv1d_bwd": (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp,
+                                       _vp, _i64, _vp]),
+    "lampa_residual_norm_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _i64, _i32, _f32, _i32, _i32, _vp, _vp,
+                                       _vp]),
+    "lampa_residual_norm_bwd_workspace_bytes": (_i64, [_i64, _i64, _i32]),
+    "lampa_residual_norm_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i32, _f32, _i32, _i32]
+                                + [_vp] * 7 + [_i64, _vp]),
 }
 
 _lib = None

@@ -1,0 +1,18 @@
+// What the state-space scan's kernels share beside the call's arguments: the buffers of the gradients, and the launchers of
+// the walks (token-serial for every type, chunks on the matrix cores for 16-bit types).
+#pragma once
+#include "ss_common.h"
+
+struct SsGrad {
+  float* adjoints;      // [slots, H, N, P]: the segments' local adjoints, then the adjoint at each segment's end
+  float *dB_part, *dC_part;  // [tokens, H * ceil(P / 64), N]: one part for each head and block of 64 columns of x
+  float* read;          // [tokens, H, parts]: dy_t . (S_t^T C_t), parts = ceil(P / 64) * ceil(N / 64)
+  float* written;       // [tokens, H, ceil(P / 64)]: x_t . (R_t^T B_t)
+  float* param_part;    // [slots, H, 2]: a segment's share of dA and d dt_bias
+  float* dD_part;       // [slots, H, ceil(P / 64)]
+};
+
+enum { SS_Y = 0, SS_DC = 1, SS_DX = 2, SS_DB = 3 };
+
+int ss_serial_maps(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s);
+int ss_serial_walk(const lampa_ss_args& a, int kind, const SsGrad& grad, hipStream_t s);

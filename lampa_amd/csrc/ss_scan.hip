@@ -1,0 +1,265 @@
+// The state-space scan's entry points on gfx950: checks, the scan over segments, the join of the gradients' parts.
+//
+// Replaces the selective scan behind Mamba2.forward (reference chengjiang123/Lampa: models/baselines/full_mamba2.py:221-430,
+// models/baselines/hmamba.py:356-460), whose kernels the reference imports from a package it does not hold.
+#include "ss_kernels.h"
+
+#define SS_BLOCK 256
+
+// S (or, from the end, R) across the segments of one sequence, one thread an element of the state: every slot's local state
+// is replaced by the state its segment starts from, and what is left after the last one goes to `out`. A thread reads
+// SS_AHEAD slots before it needs the first.
+#define SS_AHEAD 8
+template <bool REV>
+__global__ void __launch_bounds__(SS_BLOCK) ss_join_kernel(lampa_ss_args a, float* __restrict__ states,
+                                                           const float* __restrict__ init, float* __restrict__ out) {
+  const int64_t per_h = (int64_t)a.N * a.P;
+  const int64_t blocks = (per_h + SS_BLOCK - 1) / SS_BLOCK;
+  const int64_t e = (int64_t)(blockIdx.x % blocks) * SS_BLOCK + threadIdx.x;
+  const int h = (int)(blockIdx.x / blocks % a.H), seq = (int)(blockIdx.x / blocks / a.H);
+  if (e >= per_h) return;
+  const int64_t slot0 = a.n_tokens ? ss_first_slot(a, seq) : 0, len = ss_bound(a, seq + 1) - ss_bound(a, seq);
+  const int64_t n = a.n_tokens && len > 0 ? (len + a.seg_tokens - 1) / a.seg_tokens : (a.n_tokens ? 1 : 0);
+  const int64_t own = ((int64_t)seq * a.H + h) * per_h + e;
+  float S = init ? init[own] : 0.0f;
+  for (int64_t j0 = 0; j0 < n; j0 += SS_AHEAD) {
+    float local[SS_AHEAD], decay[SS_AHEAD];
+#pragma unroll
+    for (int i = 0; i < SS_AHEAD; ++i) {
+      const int64_t j = j0 + i, slot = slot0 + (REV ? n - 1 - j : j);
+      local[i] = j < n ? states[(slot * a.H + h) * per_h + e] : 0.0f;
+      decay[i] = j < n ? a.slot_decay[slot * a.H + h] : 1.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < SS_AHEAD; ++i) {
+      const int64_t j = j0 + i, slot = slot0 + (REV ? n - 1 - j : j);
+      if (j < n) states[(slot * a.H + h) * per_h + e] = S;
+      S = __builtin_fmaf(S, decay[i], local[i]);
+    }
+  }
+  if (out) out[own] = S;
+}
+
+template <bool REV>
+static int ss_join(const lampa_ss_args& a, float* states, const float* init, float* out, hipStream_t s) {
+  const int64_t blocks = ((int64_t)a.N * a.P + SS_BLOCK - 1) / SS_BLOCK * a.H * a.n_seq;
+  if (blocks > 0x7fffffff) return LAMPA_ERR_UNSUPPORTED;
+  LAMPA_PROF(s, "start");
+  hipLaunchKernelGGL((ss_join_kernel<REV>), dim3((unsigned)blocks), dim3(SS_BLOCK), 0, s, a, states, init, out);
+  LAMPA_PROF(s, "ss_join_kernel");
+  return lampa_launch_status();
+}
+
+// A segment's gradient of the decays: dg_t = dg_{t+1} + read_t - delta_t written_t from the segment's end, where it starts
+// from <R, S> of the states there, so that errors of the sum do not pass from one segment to the next. One workgroup a
+// segment and head, 256 tokens at a time from the end.
+template <typename T>
+__global__ void __launch_bounds__(SS_BLOCK) ss_decay_grad_kernel(lampa_ss_args a, SsGrad w) {
+  const SsSegment seg = ss_segment(a, blockIdx.x);
+  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = (int64_t)blockIdx.x * a.H + h;
+  if (!seg.live || seg.outside) {
+    if (tid < 2) w.param_part[row * 2 + tid] = 0.0f;
+    if (!seg.live) return;
+  }
+  __shared__ float part[4];
+  auto block_sum = [&](float x) {
+    x = ss_wave_sum(x);
+    __syncthreads();
+    if (lane == 0) part[wave] = x;
+    __syncthreads();
+    return (part[0] + part[1]) + (part[2] + part[3]);
+  };
+  const int npb = (a.P + 63) / 64, nnb = (a.N + 63) / 64;
+  const int64_t per_h = (int64_t)a.N * a.P;
+  const bool single = (a.cu_seqlens ? a.n_tokens : a.seq_len) <= a.seg_tokens;
+  const float* R = single || seg.last ? a.dht : w.adjoints;
+  const float* S = single || seg.last ? a.ht : a.slot_states;
+  float carry = 0.0f;
+  if (R && !seg.outside) {
+    const int64_t own = ((int64_t)seg.seq * a.H + h) * per_h;
+    R += single || seg.last ? own : row * per_h;
+    S += single || seg.last ? own : (row + a.H) * per_h;  // the next segment's initial state
+    float dot = 0.0f;
+    for (int64_t e = tid; e < per_h; e += SS_BLOCK) dot = __builtin_fmaf(R[e], S[e], dot);
+    carry = block_sum(dot);
+  }
+  const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
+  float dA = 0.0f, dbias = 0.0f;
+  for (int64_t hi = seg.t1; hi > seg.t0; hi -= SS_BLOCK) {
+    const int64_t tok = hi - 1 - tid;  // thread i: the i-th token from the end
+    const bool on = tok >= seg.t0;
+    float raw = 0.0f, delta = 0.0f, read = 0.0f, written = 0.0f;
+    if (on && !seg.outside) {
+      raw = ss_load_dt<T>(a.dt, a.dt_dtype, tok * a.dt_stride + h) + bias;
+      delta = ss_delta(raw, 0.0f, a.softplus);
+      for (int i = 0; i < npb * nnb; ++i) read += w.read[(tok * a.H + h) * npb * nnb + i];
+      for (int i = 0; i < npb; ++i) written += w.written[(tok * a.H + h) * npb + i];
+    }
+    float sum = on ? read - delta * written : 0.0f;  // inclusive prefix over the threads = suffix over the tokens
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const float up = __shfl_up(sum, off);
+      if (lane >= off) sum += up;
+    }
+    __syncthreads();
+    if (lane == 63) part[wave] = sum;
+    __syncthreads();
+    float before = carry;
+    for (int i = 0; i < wave; ++i) before += part[i];
+    const float dg = before + sum;
+    carry += (part[0] + part[1]) + (part[2] + part[3]);
+    if (on) {
+      float d = __builtin_fmaf(A, dg, written);
+      // the derivative of log(1 + e^x), which is used as x above 20
+      if (a.softplus) d *= raw > 20.0f ? 1.0f : 1.0f / (1.0f + expf(-raw));
+      if (seg.outside) d = 0.0f;
+      if (a.dt_dtype == GDR_FP32) ((float*)a.ddt)[tok * a.H + h] = d;
+      else ((T*)a.ddt)[tok * a.H + h] = GdrElem<T>::from_float(d);
+      dbias += d;
+      dA = __builtin_fmaf(delta, dg, dA);
+    }
+  }
+  dA = block_sum(dA);
+  dbias = block_sum(dbias);
+  if (tid == 0 && !seg.outside) {
+    w.param_part[row * 2] = dA;
+    w.param_part[row * 2 + 1] = dbias;
+  }
+}
+
+// The parts of dB and dC, one for each head and block of columns, added up over the heads of a group in their order.
+template <typename T>
+__global__ void __launch_bounds__(SS_BLOCK) ss_group_sum_kernel(const float* __restrict__ dB_part, const float* __restrict__ dC_part,
+                                                                T* __restrict__ dB, T* __restrict__ dC, int64_t n, int N, int parts) {
+  const int64_t i = (int64_t)blockIdx.x * SS_BLOCK + threadIdx.x;
+  if (i >= n) return;
+  const float* src = (blockIdx.y ? dC_part : dB_part) + (i / N) * parts * N + i % N;
+  float sum = 0.0f;
+  for (int j = 0; j < parts; ++j) sum += src[(int64_t)j * N];
+  (blockIdx.y ? dC : dB)[i] = GdrElem<T>::from_float(sum);
+}
+
+// dA, d dt_bias and dD of a head: its segments' shares in their order.
+__global__ void __launch_bounds__(SS_BLOCK) ss_param_sum_kernel(lampa_ss_args a, SsGrad w, int64_t slots) {
+  const int h = blockIdx.x, which = blockIdx.y, npb = (a.P + 63) / 64;
+  float* out = which == 0 ? a.dA : which == 1 ? a.ddt_bias : a.dD;
+  if (!out) return;
+  float sum = 0.0f;
+  for (int64_t slot = threadIdx.x; slot < slots; slot += SS_BLOCK) {
+    if (which < 2) sum += w.param_part[(slot * a.H + h) * 2 + which];
+    else if (ss_segment(a, slot).live)
+      for (int i = 0; i < npb; ++i) sum += w.dD_part[(slot * a.H + h) * npb + i];
+  }
+  __shared__ float part[4];
+  sum = ss_wave_sum(sum);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) out[h] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+static int ss_check(const lampa_ss_args* a) {
+  if (!a || !a->A || a->n_tokens < 0 || (a->n_tokens && (!a->x || !a->dt || !a->B || !a->C)) || a->n_seq < 1 || a->H < 1 || a->P < 1 || a->G < 1 ||
+      a->N < 1 || a->H % a->G || a->seg_tokens < 64 || a->seg_tokens % 64 || a->dtype < 0 || a->dtype > 2 ||
+      (a->dt_dtype != a->dtype && a->dt_dtype != GDR_FP32))
+    return LAMPA_ERR_INVALID;
+  if (!a->cu_seqlens && (a->seq_len < 0 || a->seq_len * a->n_seq != a->n_tokens)) return LAMPA_ERR_INVALID;
+  if (a->x_stride < (int64_t)a->H * a->P || a->dt_stride < a->H || a->B_stride < (int64_t)a->G * a->N ||
+      a->C_stride < (int64_t)a->G * a->N)
+    return LAMPA_ERR_INVALID;
+  if (a->N > 128) return LAMPA_ERR_UNSUPPORTED;
+  // the grids' limits: slots along x, heads and blocks along y
+  if (ss_slots(a) > 0x7fffffff || (int64_t)a->H * ss_blocks64(a->P) * 2 > 65535) return LAMPA_ERR_UNSUPPORTED;
+  return LAMPA_OK;
+}
+
+extern "C" int64_t lampa_ss_slots(const lampa_ss_args* a) { return ss_check(a) == LAMPA_OK ? ss_slots(a) : ss_check(a); }
+
+extern "C" int lampa_ss_scan_fwd(const lampa_ss_args* args, void* stream) {
+  const int rc = ss_check(args);
+  if (rc != LAMPA_OK) return rc;
+  const lampa_ss_args& a = *args;
+  hipStream_t s = (hipStream_t)stream;
+  if (!a.n_tokens) return a.ht ? ss_join<false>(a, nullptr, a.h0, a.ht, s) : LAMPA_OK;
+  if (!a.y || a.y_stride < (int64_t)a.H * a.P) return LAMPA_ERR_INVALID;
+  if (!ss_single(&a)) {
+    if (!a.slot_states || !a.slot_decay) return LAMPA_ERR_WORKSPACE;
+    int e = ss_serial_maps(a, nullptr, s);
+    if (e == LAMPA_OK) e = ss_join<false>(a, a.slot_states, a.h0, a.ht, s);
+    if (e != LAMPA_OK) return e;
+  }
+  return ss_serial_walk(a, SS_Y, SsGrad{}, s);
+}
+
+static int64_t ss_grad_layout(const lampa_ss_args& a, char* base, SsGrad* w) {
+  const int64_t slots = ss_slots(&a), npb = ss_blocks64(a.P), nnb = ss_blocks64(a.N);
+  int64_t at = 0;
+  auto take = [&](float*& p, int64_t n) {
+    p = base ? (float*)(base + at) : nullptr;
+    at += lampa_align_up(n * 4, 256);
+  };
+  SsGrad g;
+  take(g.adjoints, ss_single(&a) ? 0 : slots * a.H * a.N * a.P);
+  take(g.dB_part, a.n_tokens * a.H * npb * a.N);
+  take(g.dC_part, a.n_tokens * a.H * npb * a.N);
+  take(g.read, a.n_tokens * a.H * npb * nnb);
+  take(g.written, a.n_tokens * a.H * npb);
+  take(g.param_part, slots * a.H * 2);
+  take(g.dD_part, slots * a.H * npb);
+  if (w) *w = g;
+  return at;
+}
+
+extern "C" int64_t lampa_ss_bwd_workspace_bytes(const lampa_ss_args* a) {
+  const int rc = ss_check(a);
+  return rc == LAMPA_OK ? ss_grad_layout(*a, nullptr, nullptr) : rc;
+}
+
+extern "C" int lampa_ss_scan_bwd(const lampa_ss_args* args, void* stream) {
+  const int rc = ss_check(args);
+  if (rc != LAMPA_OK) return rc;
+  const lampa_ss_args& a = *args;
+  if (!a.dA) return LAMPA_ERR_INVALID;
+  if (a.n_tokens && (!a.dy || !a.dx || !a.ddt || !a.dB || !a.dC)) return LAMPA_ERR_INVALID;
+  if (a.dht && !a.ht) return LAMPA_ERR_INVALID;
+  const int64_t need = ss_grad_layout(a, nullptr, nullptr);
+  if (need && (!a.workspace || a.workspace_bytes < need)) return LAMPA_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  SsGrad w;
+  ss_grad_layout(a, (char*)a.workspace, &w);
+  const int64_t slots = a.n_tokens ? ss_slots(&a) : 0;
+  int e = LAMPA_OK;
+  if (!a.n_tokens) {
+    if (a.dh0) e = ss_join<true>(a, nullptr, a.dht, a.dh0, s);
+  } else {
+    if (!ss_single(&a)) {
+      if (!a.slot_states || !a.slot_decay || !a.ht) return LAMPA_ERR_WORKSPACE;
+      e = ss_serial_maps(a, &w, s);
+      if (e == LAMPA_OK) e = ss_join<true>(a, w.adjoints, a.dht, a.dh0, s);
+    }
+    for (int kind : {SS_DC, SS_DX, SS_DB})
+      if (e == LAMPA_OK) e = ss_serial_walk(a, kind, w, s);
+    if (e != LAMPA_OK) return e;
+    const int64_t n = a.n_tokens * a.G * a.N;
+    const dim3 sums((unsigned)((n + SS_BLOCK - 1) / SS_BLOCK), 2), segs((unsigned)slots, (unsigned)a.H);
+    const int parts = a.H / a.G * ss_blocks64(a.P);
+#define SS_TAIL(T)                                                                                                          \
+  hipLaunchKernelGGL((ss_decay_grad_kernel<T>), segs, dim3(SS_BLOCK), 0, s, a, w);                                          \
+  LAMPA_PROF(s, "ss_decay_grad_kernel");                                                                                    \
+  hipLaunchKernelGGL((ss_group_sum_kernel<T>), sums, dim3(SS_BLOCK), 0, s, w.dB_part, w.dC_part, (T*)a.dB, (T*)a.dC, n, a.N, \
+                     parts);                                                                                                \
+  LAMPA_PROF(s, "ss_group_sum_kernel");
+    if (n > (int64_t)0x7fffffff * SS_BLOCK) return LAMPA_ERR_UNSUPPORTED;
+    LAMPA_PROF(s, "start");
+    switch (a.dtype) {
+      case GDR_BF16: SS_TAIL(__bf16) break;
+      case GDR_FP16: SS_TAIL(_Float16) break;
+      default: SS_TAIL(float) break;
+    }
+#undef SS_TAIL
+  }
+  if (e != LAMPA_OK) return e;
+  hipLaunchKernelGGL(ss_param_sum_kernel, dim3((unsigned)a.H, 3), dim3(SS_BLOCK), 0, s, a, w, slots);
+  LAMPA_PROF(s, "ss_param_sum_kernel");
+  return lampa_launch_status();
+}

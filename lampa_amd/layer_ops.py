@@ -3,8 +3,10 @@
 
 Mirrors ``causal_conv1d`` / ``ShortConvolution`` (``models/hattention/short_convolution.py:426-458,528-721``) and
 ``rms_norm_gated`` / ``rms_norm`` / ``FusedRMSNormGated`` / ``FusedRMSNormSwishGate`` / ``RMSNorm``
-(``models/hattention/fused_norm.py:856-878,1003-1104,2094-2354``). Forward only; GPU tensors only (no CPU fallback).
+(``models/hattention/fused_norm.py:856-878,1003-1104,2094-2354``). ``causal_conv1d`` and ``residual_norm`` are
+differentiable, everything else is forward only; GPU tensors only (no CPU fallback).
 """
+import contextlib
 import weakref
 from typing import Optional, Tuple
 
@@ -34,6 +36,54 @@ def _code(dtype) -> int:
     if dtype not in _DTYPES:
         raise TypeError(f"lampa_amd: unsupported dtype {dtype} (bfloat16, float16 or float32)")
     return _DTYPES[dtype]
+
+
+def _on_device(device):
+    """The launches of a call go to its tensors' device, whichever is current."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _same_device(what, *tensors):
+    require_cuda(*tensors)
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: all tensors must be on one device, got {device} and {t.device}")
+    return device
+
+
+def _tokens(t: torch.Tensor, inner: int):
+    """(t, elements from one token to the next) of t [B, T, ...] whose dimensions behind T hold `inner` contiguous elements;
+    a copy only where the tokens do not lie evenly."""
+    B, T = t.shape[:2]
+    expect = 1
+    for size, stride in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
+        if size != 1 and stride != expect:
+            return t.contiguous(), inner
+        expect *= size
+    step = t.stride(1) if T > 1 else t.stride(0) if B > 1 else inner
+    if step < inner or (B > 1 and T > 1 and t.stride(0) != T * step):
+        return t.contiguous(), inner
+    return t, step
+
+
+def _sequences(what, cu_seqlens, batch, tokens, device):
+    """Boundaries as a device int64 tensor. On the host they are checked; on the device they are taken as they are (nothing
+    waits for the GPU, and a captured graph may be replayed with others): the kernels hold them inside the tensors."""
+    if cu_seqlens is None:
+        return None
+    if batch != 1:
+        raise ValueError(f"{what}: the batch size must be 1 rather than {batch} when cu_seqlens is given; flatten "
+                         f"variable-length inputs first")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.is_floating_point() or cu_seqlens.dtype == torch.bool:
+        raise ValueError(f"{what}: cu_seqlens must hold at least two whole numbers, got {cu_seqlens.dtype} "
+                         f"{tuple(cu_seqlens.shape)}")
+    if not cu_seqlens.is_cuda:
+        cu = cu_seqlens.tolist()
+        if cu[0] != 0 or cu[-1] != tokens or any(b < a for a, b in zip(cu[:-1], cu[1:])):
+            raise ValueError(f"{what}: cu_seqlens must start at 0, never decrease and end at the number of tokens ({tokens}); "
+                             f"got first = {cu[0]}, last = {cu[-1]}")
+    return cu_seqlens.to(device=device, dtype=torch.int64).contiguous()
 
 
 _F32_CACHE = {}
@@ -113,13 +163,86 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.as_strided((B * T, D), (t.stride(1), 1))
 
 
+def _conv_operands(x, weight, bias):
+    """x as rows of D, the taps and the bias in fp32 (a copy of this call's own)."""
+    D = x.shape[-1]
+    x2, step = _tokens(x, D)
+    if step % 8 or x2.data_ptr() % 16:
+        x2, step = x2.contiguous(), D
+        if x2.data_ptr() % 16:
+            x2 = x2.clone()
+    return x2, step, weight.detach().to(torch.float32).contiguous(), None if bias is None else bias.detach().to(torch.float32).contiguous()
+
+
+@torch.no_grad()
+def _conv_state_launch(x, weight, bias, activation, cu, past, want_last):
+    B, T, D = x.shape
+    W = weight.shape[-1]
+    n_seq = B if cu is None else cu.numel() - 1
+    x2, step, w32, b32 = _conv_operands(x, weight, bias)
+    past = None if past is None else past.detach().to(x.dtype).contiguous()
+    y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
+    last = torch.empty((n_seq, D, W), dtype=x.dtype, device=x.device) if want_last else None
+    with _on_device(x.device):
+        check(_capi.lib().lampa_causal_conv1d_state_fwd(
+            ptr(x2), step, B * T, D, W, ptr(w32), ptr(b32), ptr(past), ptr(cu), n_seq, T, _ACT[activation], _code(x.dtype),
+            ptr(y), ptr(last), stream_of(x)), "lampa_causal_conv1d_state_fwd")
+    return y, last
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, past, forward, activation, cu):
+        y, last = forward()
+        ctx.save_for_backward(x, weight, bias, past, cu)
+        ctx.activation = activation
+        ctx.residual_dtype = None if residual is None else residual.dtype
+        if last is not None:
+            ctx.mark_non_differentiable(last)
+        return y, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, _):
+        x, weight, bias, past, cu = ctx.saved_tensors
+        B, T, D = x.shape
+        w2 = weight.reshape(D, -1)
+        W = w2.shape[1]
+        x2, step, w32, b32 = _conv_operands(x, w2, bias)
+        past = None if past is None else past.detach().to(x.dtype).contiguous()
+        g = dy.to(x.dtype).contiguous()
+        if g.data_ptr() % 16:
+            g = g.clone()
+        dx = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
+        dwb = torch.empty((D, W + 1), dtype=torch.float32, device=x.device)
+        lib = _capi.lib()
+        with _on_device(x.device):
+            size = check(lib.lampa_causal_conv1d_bwd_workspace_bytes(B * T, D, W, _code(x.dtype)),
+                         "lampa_causal_conv1d_bwd_workspace_bytes")
+            ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+            check(lib.lampa_causal_conv1d_bwd(
+                ptr(x2), step, ptr(g), B * T, D, W, ptr(w32), ptr(b32), ptr(past), ptr(cu), B if cu is None else cu.numel() - 1,
+                T, _ACT[ctx.activation], _code(x.dtype), ptr(dx), ptr(dwb), ptr(ws), size, stream_of(x)),
+                "lampa_causal_conv1d_bwd")
+        dw = dwb[:, :W].to(weight.dtype).reshape(weight.shape) if ctx.needs_input_grad[1] else None
+        db = dwb[:, W].to(bias.dtype) if ctx.needs_input_grad[2] else None
+        return dx, dw, db, dy.to(ctx.residual_dtype) if ctx.needs_input_grad[3] else None, None, None, None, None
+
+
 def causal_conv1d(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                   residual: Optional[torch.Tensor] = None, activation: Optional[str] = None,
-                  cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  cu_seqlens: Optional[torch.Tensor] = None, initial_state: Optional[torch.Tensor] = None,
+                  output_final_state: bool = False):
     """``short_convolution.py:426-458``: x [B, T, D], weight [D, W] (tap W-1 on the current token), bias [D],
     residual [B, T, D]; activation ``None`` / ``'silu'`` / ``'swish'``; with ``cu_seqlens`` B must be 1 and taps never
-    cross a sequence start. Returns [B, T, D] in x's dtype (fp32 arithmetic)."""
-    require_cuda(x, weight, bias, residual, cu_seqlens)
+    cross a sequence start. Returns [B, T, D] in x's dtype (fp32 arithmetic). Differentiable in x, weight, bias and residual
+    (first order; repeated calls give the same bits).
+
+    ``initial_state`` [sequences, D, W] holds the W inputs before each sequence (a cache as ``causal_conv1d_step`` and
+    ``ShortConvolution`` keep it; its oldest column is not read), and ``output_final_state`` returns (y, the W inputs up to
+    each sequence's end). Both are data handed from call to call: no gradient runs through them. With either, cu_seqlens is
+    taken as ``state_space_scan`` takes it and there is no ``residual``."""
+    require_cuda(x, weight, bias, residual, initial_state)
     if activation not in (None, "silu", "swish"):
         raise ValueError(f"Activation `{activation}` not supported yet.")
     if x.dim() != 3:
@@ -127,14 +250,93 @@ def causal_conv1d(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: 
     B, T, D = x.shape
     if cu_seqlens is not None and B != 1:
         raise ValueError("causal_conv1d: batch size must be 1 when cu_seqlens is given")
+    with_state = initial_state is not None or output_final_state
+    if not with_state:
+        require_cuda(cu_seqlens)
     if weight is None:
         weight = torch.ones(D, 1, device=x.device)
-    w32, b32 = _f32(weight.reshape(D, -1), x.device), _f32(bias, x.device)
-    res2 = None if residual is None else _rows(residual.to(x.dtype))
-    x2 = _rows(x)
-    fn = lambda: _conv_launch(x2, w32, b32, res2, activation, cu_seqlens, max(T, 1)).view(B, T, D)  # noqa: E731
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        return _ForwardOnly.apply(fn, x, weight)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
+    if with_state or grad:
+        what = "causal_conv1d"
+        _same_device(what, x, weight, bias, residual, initial_state)
+        if weight.numel() % D or weight.shape[0] != D or (bias is not None and tuple(bias.shape) != (D,)):
+            raise ValueError(f"{what}: expected weight [{D}, W] and bias [{D}], got {tuple(weight.shape)} and "
+                             f"{None if bias is None else tuple(bias.shape)}")
+        W = weight.numel() // D
+        cu = _sequences(what, cu_seqlens, B, T, x.device)
+    if with_state:
+        n_seq = B if cu is None else cu.numel() - 1
+        if residual is not None:
+            raise ValueError(f"{what}: no residual together with initial_state or output_final_state")
+        if initial_state is not None and tuple(initial_state.shape) != (n_seq, D, W):
+            raise ValueError(f"{what}: initial_state must have shape {(n_seq, D, W)} ([sequences, D, W]), got "
+                             f"{tuple(initial_state.shape)}")
+        if initial_state is not None and initial_state.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what}: no gradient runs through initial_state; pass it detached")
+        forward = lambda: _conv_state_launch(x, weight.reshape(D, W), bias, activation, cu, initial_state,  # noqa: E731
+                                             output_final_state)
+    else:
+        if grad:  # a training step's weights are new every time
+            w32, b32 = weight.detach().reshape(D, -1).float().contiguous(), None if bias is None else bias.detach().float().contiguous()
+        else:
+            w32, b32 = _f32(weight.reshape(D, -1), x.device), _f32(bias, x.device)
+        res2 = None if residual is None else _rows(residual.to(x.dtype))
+        x2 = _rows(x)
+        forward = lambda: (_conv_launch(x2, w32, b32, res2, activation, cu_seqlens, max(T, 1)).view(B, T, D), None)  # noqa: E731
+    if grad:
+        y, last = _CausalConv.apply(x, weight, bias, residual, initial_state, forward, activation, cu)
+    else:
+        y, last = forward()
+    return (y, last) if output_final_state else y
+
+
+@torch.no_grad()
+def _conv_step_launch(x, cache, weight, bias, activation, target):
+    n, D = x.shape
+    W = weight.shape[-1]
+    if x.stride(1) != 1 and D > 1 or (n > 1 and x.stride(0) < D):
+        x = x.contiguous()
+    w32 = weight.detach().to(torch.float32).contiguous()
+    b32 = None if bias is None else bias.detach().to(torch.float32).contiguous()
+    y = torch.empty((n, D), dtype=x.dtype, device=x.device)
+    with _on_device(x.device):
+        check(_capi.lib().lampa_causal_conv1d_step(ptr(x), x.stride(0) if n > 1 else D, ptr(cache), ptr(target), ptr(w32), ptr(b32),
+                                                   _ACT[activation], _code(x.dtype), ptr(y), n, D, W, stream_of(x)),
+              "lampa_causal_conv1d_step")
+    return y
+
+
+def causal_conv1d_step(x: torch.Tensor, cache: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                       activation: Optional[str] = None, new_cache: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token for each of n sequences: x [n, D], ``cache`` [n, D, W] (x's type, contiguous) with the last W inputs, weight
+    [D, W], bias [D], W <= 8, any D. Returns y [n, D]; the cache is moved on in place, or, with ``new_cache`` (same shape, no
+    shared memory), left as it is and the next one written there. The arithmetic of ``causal_conv1d``, token by token.
+    Forward only: the backward raises."""
+    what = "causal_conv1d_step"
+    _same_device(what, x, cache, weight, bias, new_cache)
+    if activation not in (None, "silu", "swish"):
+        raise ValueError(f"Activation `{activation}` not supported yet.")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"{what}: x must be [n, D], got {tuple(x.shape)}")
+    n, D = x.shape
+    if weight.numel() % D or weight.shape[0] != D or weight.numel() == 0 or (bias is not None and tuple(bias.shape) != (D,)):
+        raise ValueError(f"{what}: expected weight [{D}, W] and bias [{D}], got {tuple(weight.shape)} and "
+                         f"{None if bias is None else tuple(bias.shape)}")
+    W = weight.numel() // D
+    for name, t in (("cache", cache), ("new_cache", new_cache)):
+        if t is not None and (tuple(t.shape) != (n, D, W) or t.dtype != x.dtype or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be a contiguous {x.dtype} tensor of shape {(n, D, W)}, got {t.dtype} "
+                             f"{tuple(t.shape)}")
+    if new_cache is not None and new_cache is not cache:
+        a, b, size = cache.data_ptr(), new_cache.data_ptr(), cache.numel() * cache.element_size()
+        if a != b and a < b + size and b < a + size:
+            raise ValueError(f"{what}: new_cache overlaps cache")
+    if n == 0:
+        return torch.empty_like(x)
+    target = cache if new_cache is None else new_cache
+    fn = lambda: _conv_step_launch(x, cache, weight.reshape(D, W), bias, activation, target)  # noqa: E731
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _ForwardOnly.apply(fn, x, weight, bias)
     return fn()
 
 
@@ -282,13 +484,12 @@ class ShortConvolution(nn.Conv1d):
         """One token per sequence: the cache is rolled in place, then the convolution runs over its W columns."""
         shape = x.shape
         D, W = self.hidden_size, self.kernel_size[0]
-        xt = x.reshape(-1, D)
+        held = cache if cache.is_contiguous() and cache.dtype == x.dtype else cache.to(x.dtype).contiguous()
         with torch.no_grad():
-            cache.copy_(cache.roll(shifts=-1, dims=-1))
-            cache[:, :, -1] = xt
-            window = cache.transpose(1, 2).contiguous()                                       # [N, W, D]
-        y = causal_conv1d(x=window, weight=self.weight.reshape(D, W), bias=self.bias, activation=self.activation)
-        y = y[:, -1].reshape(shape)
+            y = causal_conv1d_step(x.reshape(-1, D), held, self.weight.reshape(D, W), self.bias, self.activation)
+            if held is not cache:
+                cache.copy_(held)
+        y = y.reshape(shape)
         if residual is not None:
             y = y + residual
         return y, cache
@@ -358,6 +559,124 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, residual
              prenorm: bool = False, residual_in_fp32: bool = False):
     """``fused_norm.py:2094-2112``: y = rmsnorm(x + residual) * weight + bias; ``prenorm`` also returns x + residual."""
     return _rms_norm_any(x, None, weight, bias, None, residual, eps, prenorm, residual_in_fp32)
+
+
+_GATE_NONE, _GATE_TOKEN, _GATE_SEQUENCE = 0, 1, 2
+
+
+def _packed(t):
+    """Contiguous and 16-byte aligned, as the row kernels read it."""
+    if t is None:
+        return None
+    t = t.detach().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _vec32(t):
+    return None if t is None else _packed(t.to(torch.float32))
+
+
+def _norm_sizes(x, gate):
+    D = x.shape[-1]
+    rows = x.numel() // D
+    if gate is None:
+        return rows, max(rows, 1), D, _GATE_NONE
+    if gate.shape == x.shape:
+        return rows, max(rows, 1), D, _GATE_TOKEN
+    return rows, max(x.shape[1], 1), D, _GATE_SEQUENCE
+
+
+@torch.no_grad()
+def _residual_norm_launch(x, residual, weight, post_weight, gate, act, scale, eps):
+    rows, seq_rows, D, kind = _norm_sizes(x, gate)
+    x_, r_, g_ = _packed(x), _packed(residual), _packed(gate)
+    w, pw, sc = _vec32(weight), _vec32(post_weight), _vec32(scale)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    with _on_device(x.device):
+        check(_capi.lib().lampa_residual_norm_fwd(ptr(x_), ptr(r_), ptr(w), ptr(pw), ptr(g_), kind, act, ptr(sc), rows, seq_rows, D,
+                                                  float(eps), _code(x.dtype), _code(residual.dtype), ptr(y), ptr(out),
+                                                  stream_of(x)), "lampa_residual_norm_fwd")
+    return y, out
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, post_weight, gate, scale, act, eps):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, residual, weight, post_weight, gate, scale)
+        ctx.act, ctx.eps = act, eps
+        return _residual_norm_launch(x, residual, weight, post_weight, gate, act, scale, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dres):
+        x, residual, weight, post_weight, gate, scale = ctx.saved_tensors
+        rows, seq_rows, D, kind = _norm_sizes(x, gate)
+        x_, r_, g_ = _packed(x), _packed(residual), _packed(gate)
+        w, pw, sc = _vec32(weight), _vec32(post_weight), _vec32(scale)
+        dy = None if dy is None else _packed(dy.to(x.dtype))
+        dres = None if dres is None else _packed(dres.to(residual.dtype))
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dr = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+        make = torch.empty if rows else torch.zeros  # without rows nothing is launched
+        need = ctx.needs_input_grad
+        vec = lambda t, wanted: make(D, dtype=torch.float32, device=x.device) if t is not None and wanted else None  # noqa: E731
+        dw, dpw, dsc = vec(weight, need[2]), vec(post_weight, need[3]), vec(scale, need[5])
+        dg = make(gate.shape, dtype=gate.dtype, device=x.device) if gate is not None and need[4] else None
+        lib = _capi.lib()
+        with _on_device(x.device):
+            size = check(lib.lampa_residual_norm_bwd_workspace_bytes(rows, seq_rows, D), "lampa_residual_norm_bwd_workspace_bytes")
+            ws = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
+            check(lib.lampa_residual_norm_bwd(ptr(x_), ptr(r_), ptr(w), ptr(pw), ptr(g_), kind, ctx.act, ptr(sc), ptr(dy), ptr(dres),
+                                              rows, seq_rows, D, float(ctx.eps), _code(x.dtype), _code(residual.dtype), ptr(dx),
+                                              ptr(dr), ptr(dg), ptr(dw), ptr(dpw), ptr(dsc), ptr(ws), size, stream_of(x)),
+                  "lampa_residual_norm_bwd")
+        cast = lambda g, t: None if g is None else g.to(t.dtype)  # noqa: E731
+        return dx, dr, cast(dw, weight), cast(dpw, post_weight), dg, cast(dsc, scale), None, None
+
+
+def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                  post_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                  gate_activation: Optional[str] = None, residual_scale: Optional[torch.Tensor] = None, eps: float = 1e-5):
+    """The border between two blocks in one pass: x [..., D] is a block's output, ``residual`` (x's shape; x's type or
+    float32) the stream it is added to::
+
+        a = rms_norm(x, post_weight)            (x itself without post_weight)
+        r = residual + residual_scale * act(gate) * a
+        y = rms_norm(r, weight)
+
+    Returns (y in x's type, r in the residual's type); y comes from the unrounded r. ``weight``, ``post_weight`` and
+    ``residual_scale`` are [D] or None; ``gate`` has x's shape and type, or [B, 1, D] beside x [B, T, D] (one gate for each
+    sequence); ``gate_activation`` ``None`` / ``'sigmoid'`` / ``'silu'`` / ``'swish'``. D a multiple of 8, at most 8192.
+    Differentiable in every tensor (first order; repeated calls give the same bits)."""
+    what = "residual_norm"
+    _same_device(what, x, residual, weight, post_weight, gate, residual_scale)
+    if gate_activation not in _ACT:
+        raise ValueError(f"Activation `{gate_activation}` not supported yet.")
+    if x.dim() < 1 or residual.shape != x.shape:
+        raise ValueError(f"{what}: x and residual must have one shape [..., D], got {tuple(x.shape)} and {tuple(residual.shape)}")
+    D = x.shape[-1]
+    if D < 8 or D % 8 or D > 8192:
+        raise ValueError(f"{what}: the last dimension must be a multiple of 8 and at most 8192, got {D}")
+    if _code(x.dtype) != _code(residual.dtype) and residual.dtype != torch.float32:
+        raise TypeError(f"{what}: the residual must have x's type ({x.dtype}) or be float32, got {residual.dtype}")
+    for name, t in (("weight", weight), ("post_weight", post_weight), ("residual_scale", residual_scale)):
+        if t is not None and (tuple(t.shape) != (D,) or not t.is_floating_point()):
+            raise ValueError(f"{what}: {name} must be a floating-point tensor of shape ({D},), got {t.dtype} {tuple(t.shape)}")
+    if gate is not None:
+        if gate.shape != x.shape and not (x.dim() == 3 and tuple(gate.shape) == (x.shape[0], 1, D)):
+            raise ValueError(f"{what}: the gate must have x's shape {tuple(x.shape)}, or [B, 1, D] beside x [B, T, D], got "
+                             f"{tuple(gate.shape)}")
+        if gate.dtype != x.dtype:
+            raise TypeError(f"{what}: the gate must have x's type ({x.dtype}), got {gate.dtype}")
+        if gate.shape != x.shape and x.shape[0] > 65535:
+            raise ValueError(f"{what}: at most 65535 sequences with a gate each, got {x.shape[0]}")
+    act = _ACT[gate_activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, residual, weight, post_weight, gate, residual_scale)):
+        return _ResidualNorm.apply(x, residual, weight, post_weight, gate, residual_scale, act, eps)
+    return _residual_norm_launch(x, residual, weight, post_weight, gate, act, residual_scale, eps)
 
 
 class FusedRMSNormGated(nn.Module):

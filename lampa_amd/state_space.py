@@ -1,0 +1,224 @@
+"""The selective scan of a state-space layer, for prompts and for single tokens, on the GPU.
+
+For every sequence and head, with a state S [N, P] in float32 and a head's group of B and C shared by its heads::
+
+    delta_t = softplus(dt_t + dt_bias)
+    S_t = exp(delta_t A) S_{t-1} + delta_t B_t x_t^T          y_t = S_t^T C_t + D x_t
+
+``state_space_scan`` runs it over whole sequences (dense or packed) and is differentiable; ``state_space_step`` runs one
+token for each sequence on a kept state. It is the mixer behind the reference's LSH-ordered models
+(``models/baselines/full_mamba2.py:221-430``, ``models/baselines/hmamba.py:356-460``), whose scan lives in a package the
+reference imports. Names, state layout ([sequences, H, N, P], float32) and return tuples follow this package's
+``chunk_gated_delta_rule``. GPU tensors only; there is no CPU path.
+"""
+import struct
+from typing import Optional
+
+import torch
+
+from . import _capi
+from ._capi import check, ptr, require_cuda, stream_of
+from .gated_delta import _direct
+from .layer_ops import _DTYPES, _ForwardOnly, _on_device, _same_device, _sequences, _tokens
+
+MAX_STATE = 128  # N of state_space_scan; state_space_step takes any
+
+# lampa_ss_args: 13 pointers, 8 int64, 8 int32, 11 pointers, one int64
+_ARGS = struct.Struct("=13Q8q8i11Qq")
+
+
+def _f32(t):
+    return None if t is None else t.detach().to(torch.float32).contiguous()
+
+
+def _segment_tokens(longest: int, total: int, waves: int) -> int:
+    """Length of the segments that run in parallel, a multiple of 64: two waves a SIMD over the whole call."""
+    seg = -(-total * waves // 2048 // 64) * 64
+    return max(64, min(seg, -(-longest // 64) * 64))
+
+
+def _pack(x, dt, A, B, C, D, bias, h0, y, ht, states, decay, cu, longest, seg, n_seq, softplus, grad=None):
+    (x, xs), (dt, dts), (B, bs), (C, cs) = x, dt, B, C
+    H, P = x.shape[-2:]
+    G, N = B.shape[-2:]
+    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    total = x.shape[0] * x.shape[1]
+    extra = [0] * 12 if grad is None else [p(t) for t in grad[0]] + [grad[1]]
+    return _ARGS.pack(p(x), p(dt), p(B), p(C), p(A), p(D), p(bias), p(h0), p(y), p(ht), p(states), p(decay), p(cu), total,
+                      longest, seg, xs, dts, bs, cs, H * P, n_seq, H, P, G, N, _DTYPES[x.dtype], _DTYPES[dt.dtype],
+                      int(softplus), *extra)
+
+
+def _scan_launch(x, dt, A, B, C, D, bias, softplus, h0, want_final, cu, keep=False):
+    """(y, final state or None, kept): kept holds what the gradients need beside the inputs."""
+    nb, T, H, P = x.shape
+    G, N = B.shape[-2:]
+    n_seq = nb if cu is None else cu.numel() - 1
+    total, longest = nb * T, T
+    dev = x.device
+    x, dt = _tokens(x, H * P), _tokens(dt, H)
+    B, C = _tokens(B, G * N), _tokens(C, G * N)
+    A, D, bias, h0 = _f32(A), _f32(D), _f32(bias), _f32(h0)
+    seg = _segment_tokens(longest, total, H * -(-P // 64))
+    single = longest <= seg
+    y = torch.empty((nb, T, H, P), dtype=x[0].dtype, device=dev)
+    ht = torch.empty((n_seq, H, N, P), dtype=torch.float32, device=dev) if want_final or (keep and not single) else None
+    states = decay = None
+    if not single:
+        slots = n_seq * -(-T // seg) if cu is None else total // seg + n_seq + 1
+        states = torch.empty((slots, H, N, P), dtype=torch.float32, device=dev)
+        decay = torch.empty((slots, H), dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        check(_capi.lib().lampa_ss_scan_fwd(
+            _pack(x, dt, A, B, C, D, bias, h0, y, ht, states, decay, cu, longest, seg, n_seq, softplus),
+            stream_of(y)), "lampa_ss_scan_fwd")
+    return y, ht, (states, decay, seg, n_seq, longest)
+
+
+def _scan_backward(x, dt, A, B, C, D, bias, softplus, h0, cu, ht, kept, dy, dht):
+    states, decay, seg, n_seq, longest = kept
+    dev = x.device
+    nb, T, H, P = x.shape
+    G, N = B.shape[-2:]
+    dx, ddt, dB, dC = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (x, dt, B, C))
+    dA = torch.empty(H, dtype=torch.float32, device=dev)
+    dD = None if D is None else torch.empty_like(dA)
+    dbias = None if bias is None else torch.empty_like(dA)
+    dh0 = None if h0 is None else torch.empty((n_seq, H, N, P), dtype=torch.float32, device=dev)
+    dy = torch.zeros((nb, T, H, P), dtype=x.dtype, device=dev) if dy is None else dy.to(x.dtype).contiguous()
+    dht = _f32(dht)
+    x_, dt_ = _tokens(x, H * P), _tokens(dt, H)
+    B_, C_ = _tokens(B, G * N), _tokens(C, G * N)
+    A, D, bias, h0 = _f32(A), _f32(D), _f32(bias), _f32(h0)
+    pack = lambda ws, size: _pack(x_, dt_, A, B_, C_, D, bias, h0, None, ht, states, decay, cu, longest, seg, n_seq,  # noqa: E731
+                                  softplus, ((dy, dht, dx, ddt, dB, dC, dA, dD, dbias, dh0, ws), size))
+    lib = _capi.lib()
+    with _on_device(dev):
+        size = check(lib.lampa_ss_bwd_workspace_bytes(pack(None, 0)), "lampa_ss_bwd_workspace_bytes")
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        check(lib.lampa_ss_scan_bwd(pack(ws, size), stream_of(dx)), "lampa_ss_scan_bwd")
+    return dx, ddt, dA, dB, dC, dD, dbias, dh0
+
+
+class _StateSpaceScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, A, B, C, D, bias, h0, softplus, want_final, cu):
+        ctx.set_materialize_grads(False)
+        y, ht, kept = _scan_launch(x, dt, A, B, C, D, bias, softplus, h0, want_final, cu, keep=True)
+        ctx.save_for_backward(x, dt, A, B, C, D, bias, h0, cu, ht, kept[0], kept[1])
+        ctx.softplus, ctx.sizes = softplus, kept[2:]
+        return y, ht if want_final else None
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dht):
+        x, dt, A, B, C, D, bias, h0, cu, ht, states, decay = ctx.saved_tensors
+        dx, ddt, dA, dB, dC, dD, dbias, dh0 = _scan_backward(x, dt, A, B, C, D, bias, ctx.softplus, h0, cu, ht,
+                                                             (states, decay, *ctx.sizes), dy, dht)
+        as_type = lambda g, t: None if t is None else g.to(t.dtype)  # noqa: E731
+        return (dx, ddt, as_type(dA, A), dB, dC, as_type(dD, D), as_type(dbias, bias), as_type(dh0, h0), None, None, None)
+
+
+def _check_operands(what, x, dt, A, B, C, D, dt_bias, tokens):
+    """Shapes and types of a call; `tokens`: the leading dimensions of x."""
+    lead, (H, P) = tuple(x.shape[:tokens]), (x.shape[-2], x.shape[-1]) if x.dim() == tokens + 2 else (0, 0)
+    names = "B, T, " if tokens == 2 else "n, "
+    if x.dim() != tokens + 2 or tuple(dt.shape) != lead + (H,):
+        raise ValueError(f"{what}: expected x [{names}H, P] and dt [{names}H], got {tuple(x.shape)} and {tuple(dt.shape)}")
+    if B.dim() != tokens + 2 or B.shape != C.shape or tuple(B.shape[:tokens]) != lead or B.shape[-2] < 1 or H % max(1, B.shape[-2]):
+        raise ValueError(f"{what}: expected B, C [{names}G, N] with G a divisor of the {H} heads, got {tuple(B.shape)} and "
+                         f"{tuple(C.shape)}")
+    if H < 1 or P < 1 or B.shape[-1] < 1:
+        raise ValueError(f"{what}: heads, columns and states must be at least 1, got H = {H}, P = {P}, N = {B.shape[-1]}")
+    for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
+        if t is not None and tuple(t.shape) != (H,):
+            raise ValueError(f"{what}: {name} must have shape ({H},), one value per head, got {tuple(t.shape)}")
+        if t is not None and not t.is_floating_point():
+            raise TypeError(f"{what}: {name} must be a floating-point tensor, got {t.dtype}")
+    if x.dtype not in _DTYPES or B.dtype != x.dtype or C.dtype != x.dtype or dt.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"{what}: x, B and C must have one type (bfloat16, float16 or float32) and dt that type or float32, got "
+                        f"{x.dtype}, {B.dtype}, {C.dtype} and {dt.dtype}")
+
+
+def _check_state(what, name, state, shape):
+    if tuple(state.shape) != shape:
+        raise ValueError(f"{what}: {name} must have shape {shape} ([sequences, H, N, P]), got {tuple(state.shape)}")
+
+
+def state_space_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                     D: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None, dt_softplus: bool = False,
+                     initial_state: Optional[torch.Tensor] = None, output_final_state: bool = False,
+                     cu_seqlens: Optional[torch.Tensor] = None):
+    """x [B, T, H, P]; dt [B, T, H] (x's type or float32); A [H] (decay rates, normally negative); B, C [B, T, G, N] with G
+    dividing H (head h reads group h // (H // G)), N <= 128; D, dt_bias [H] or None. x, dt, B, C may be column slices of a
+    wider tensor. ``dt_softplus`` puts dt + dt_bias through softplus (as it is above 20). Returns (y [B, T, H, P] in x's type,
+    final state [sequences, H, N, P] float32 or None).
+
+    With ``cu_seqlens`` [sequences + 1] B must be 1 and the sequences lie one after the other: it starts at 0, never decreases
+    and ends at T. A tensor on the host is checked; one on the GPU is not read by the host (so a call can be captured in a
+    graph): boundaries outside the tokens are moved inside, and tokens behind the last boundary come back as zero.
+
+    A value that is not finite reaches the tokens from its own on, as in the recurrence, never earlier ones. Differentiable in every floating-point input (first order); the
+    gradients of B and C are summed over a group's heads in a fixed order, and repeated calls give the same bits."""
+    what = "state_space_scan"
+    device = _same_device(what, x, dt, A, B, C, D, dt_bias, initial_state)
+    _check_operands(what, x, dt, A, B, C, D, dt_bias, 2)
+    H, P = x.shape[-2:]
+    N = B.shape[-1]
+    if N > MAX_STATE:
+        raise ValueError(f"{what}: N must be at most {MAX_STATE}, got {N}")
+    cu = _sequences(what, cu_seqlens, x.shape[0], x.shape[1], device)
+    n_seq = x.shape[0] if cu is None else cu.numel() - 1
+    if n_seq < 1:
+        raise ValueError(f"{what}: the batch must hold at least one sequence")
+    if initial_state is not None:
+        _check_state(what, "initial_state", initial_state, (n_seq, H, N, P))
+    if _direct(x, dt, A, B, C, D, dt_bias, initial_state):
+        y, ht, _ = _scan_launch(x, dt, A, B, C, D, dt_bias, dt_softplus, initial_state, output_final_state, cu)
+        return y, ht
+    return _StateSpaceScan.apply(x, dt, A, B, C, D, dt_bias, initial_state, bool(dt_softplus), bool(output_final_state), cu)
+
+
+@torch.no_grad()
+def _step_launch(x, dt, A, B, C, D, dt_bias, softplus, state, new_state):
+    n, H, P = x.shape
+    G, N = B.shape[-2:]
+    rows = lambda t, inner: _tokens(t.unsqueeze(0), inner)  # noqa: E731
+    (x, xs), (dt, dts), (B, bs), (C, cs) = rows(x, H * P), rows(dt, H), rows(B, G * N), rows(C, G * N)
+    A, D, dt_bias = _f32(A), _f32(D), _f32(dt_bias)
+    y = torch.empty((n, H, P), dtype=x.dtype, device=x.device)
+    with _on_device(x.device):
+        check(_capi.lib().lampa_ss_step(ptr(x), xs, ptr(dt), dts, ptr(B), bs, ptr(C), cs, ptr(A), ptr(D), ptr(dt_bias),
+                                        ptr(state), ptr(new_state), ptr(y), n, H, P, G, N, _DTYPES[x.dtype],
+                                        _DTYPES[dt.dtype], int(softplus), stream_of(y)), "lampa_ss_step")
+    return y
+
+
+def state_space_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                     state: torch.Tensor, D: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None,
+                     dt_softplus: bool = False, new_state: Optional[torch.Tensor] = None):
+    """One token for each of n sequences on top of ``state`` [n, H, N, P] (float32, contiguous): x [n, H, P], dt [n, H],
+    B, C [n, G, N], everything else as in ``state_space_scan``; any N. Returns y [n, H, P] in x's type. ``state`` is moved on
+    in place, or, with ``new_state`` (same shape, no shared memory), left as it is and the next state written there. Forward
+    only: the backward raises."""
+    what = "state_space_step"
+    _same_device(what, x, dt, A, B, C, D, dt_bias, state, new_state)
+    _check_operands(what, x, dt, A, B, C, D, dt_bias, 1)
+    shape = (x.shape[0], x.shape[1], B.shape[-1], x.shape[2])
+    for name, t in (("state", state), ("new_state", new_state)):
+        if t is None:
+            continue
+        _check_state(what, name, t, shape)
+        if t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be float32 and contiguous, as it is read or written in place")
+    if new_state is not None and new_state is not state:
+        a, b, size = state.data_ptr(), new_state.data_ptr(), state.numel() * 4
+        if a != b and a < b + size and b < a + size:
+            raise ValueError(f"{what}: new_state overlaps state")
+    if x.shape[0] == 0:
+        return torch.empty_like(x)
+    target = state if new_state is None else new_state
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, dt, A, B, C, D, dt_bias, state)):
+        return _ForwardOnly.apply(lambda: _step_launch(x, dt, A, B, C, D, dt_bias, dt_softplus, state, target),
+                                  x, dt, A, B, C, D, dt_bias, state)
+    return _step_launch(x, dt, A, B, C, D, dt_bias, dt_softplus, state, target)
