@@ -1,0 +1,164 @@
+// Pieces of the chunked form of the state-space scan on the matrix cores (gfx950), 64 tokens at a time, for 16-bit types.
+//
+// With gamma_t the sum of the decay exponents of a chunk's tokens up to t and S the state before the chunk,
+//   y_t = e^{gamma_t} S^T C_t + sum_{s <= t} M[t, s] x_s,     M[t, s] = e^{gamma_t - gamma_s} delta_s (B_s . C_t),
+//   S  <- e^{gamma_end} S + sum_s B_s (delta_s e^{gamma_end - gamma_s} x_s)^T.
+// A workgroup of four waves walks a segment for one head and 64 columns of x; wave w keeps columns 16 w .. + 15 of the state in
+// accumulators (16 x 16 x 32 products). The accumulator layout of one product is the operand layout of the next: the state is
+// read out of the registers it is summed up in, and the pair weights go through LDS only because the four waves share them.
+//
+// Rounding: B, C, x (and dy) enter as they are. The pair weights are rounded once to the input type, as any operand of the
+// matrix cores has to be; they carry the same relative error as the output's own rounding. The state and the decayed x enter as
+// two operands of the input type each, value and remainder (2^-17 of the value is left in bf16): the state is handed from
+// chunk to chunk and out to the caller in fp32, and its sums are what the gradient of the decays is made of.
+#pragma once
+#include "ss_kernels.h"
+
+#define SC_BLOCK 256
+#define SC_LOG2E 1.44269504f
+
+template <typename T>
+using sc_x8 = typename OpVec<T>::x8;
+template <typename T>
+using sc_x4 = typename OpVec<T>::x4;
+
+// v as an operand value and the operand value of what that leaves out.
+template <typename T>
+__device__ __forceinline__ void sc_split(float v, T& hi, T& lo) {
+  hi = (T)v;
+  lo = (T)(v - (float)hi);
+}
+
+// fp16 has no room for every fp32 value: operands made from fp32 are scaled by a power of two that brings the largest of
+// them below 2^15 (and small ones up to it), and the product is scaled back. bf16 has fp32's range: 1.
+template <typename T>
+__device__ __forceinline__ float sc_scale_for(float largest) {
+  if constexpr (__is_same(T, _Float16)) {
+    if (!(largest > 0.0f) || !(largest < __builtin_inff())) return 1.0f;
+    int e = 14 - (int)((__float_as_uint(largest) >> 23) - 127);
+    e = e < -100 ? -100 : (e > 100 ? 100 : e);
+    return __uint_as_float((unsigned)(127 + e) << 23);
+  }
+  return 1.0f;
+}
+__device__ __forceinline__ float sc_inverse(float power_of_two) { return __uint_as_float((254u << 23) - __float_as_uint(power_of_two)); }
+
+__device__ __forceinline__ float sc_wave_max(float v) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) v = fmaxf(v, __shfl_xor(v, off));
+  return v;
+}
+
+// One thread's share of a [64, W] tile on its way from memory to LDS. Rows from `n` on and columns from `cols` on are zero.
+template <typename T, int W>
+struct ScTile {
+  sc_x8<T> v[W / 32];
+  __device__ __forceinline__ void fetch(const T* base, int64_t stride, int64_t t0, int n, int cols, bool vec) {
+#pragma unroll
+    for (int k = 0; k < W / 32; ++k) {
+      const int q = threadIdx.x + SC_BLOCK * k, row = q / (W / 8), c = q % (W / 8) * 8;
+      sc_x8<T> x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (T)0.0f;
+      if (row < n && c < cols) {
+        const T* p = base + (t0 + row) * stride + c;
+        if (vec) x = *reinterpret_cast<const sc_x8<T>*>(p);
+        else
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c + e < cols) x[e] = p[e];
+      }
+      v[k] = x;
+    }
+  }
+  // Stored in the column order of op_perm32: a lane's share of a 32-wide contraction step is one 16-byte piece.
+  __device__ __forceinline__ void put(T* tile, int stride) const {
+#pragma unroll
+    for (int k = 0; k < W / 32; ++k) {
+      const int q = threadIdx.x + SC_BLOCK * k, row = q / (W / 8), c = q % (W / 8) * 8;
+      T* p = tile + row * stride + (c & ~31) + op_perm32_piece((c >> 3) & 3);
+      sc_x4<T> a, b;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { a[e] = v[k][e]; b[e] = v[k][4 + e]; }
+      *reinterpret_cast<sc_x4<T>*>(p) = a;
+      *reinterpret_cast<sc_x4<T>*>(p + 8) = b;
+    }
+  }
+  // The first row of this thread that holds a value which is not finite, 64 if none.
+  __device__ __forceinline__ int first_bad() const {
+    int bad = 64;
+#pragma unroll
+    for (int k = W / 32 - 1; k >= 0; --k) {
+      typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+      const u32x4 w = __builtin_bit_cast(u32x4, v[k]);
+      constexpr unsigned E = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+      bool b = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b |= (w[e] & E) == E || (w[e] >> 16 & E) == E;
+      if (b) bad = (threadIdx.x + SC_BLOCK * k) / (W / 8);
+    }
+    return bad;
+  }
+};
+
+// What a chunk's steps and decays come to, one entry a token.
+struct ScDecay {
+  float gamma[64];  // gamma_t log2(e)
+  float delta[64];
+  float grow[64];   // e^{gamma_t}
+  float left[64];   // e^{gamma_end - gamma_t}
+  float end;        // e^{gamma_end}
+  float sum;        // gamma_end
+};
+// One wave, lane = token; tokens from n on have no step.
+__device__ __forceinline__ void sc_decays(ScDecay& d, float raw, int n, float bias, float A, int softplus) {
+  const int lane = lane_id();
+  const float delta = lane < n ? ss_delta(raw, bias, softplus) : 0.0f;
+  const float gamma = wave_cumulative_decay(lane < n ? ss_log_decay(delta, A) : 0.0f);
+  const float end = __shfl(gamma, 63);
+  d.gamma[lane] = gamma * SC_LOG2E;
+  d.delta[lane] = delta;
+  d.grow[lane] = __builtin_amdgcn_exp2f(gamma * SC_LOG2E);
+  d.left[lane] = __builtin_amdgcn_exp2f((end - gamma) * SC_LOG2E);
+  if (lane == 63) {
+    d.end = __builtin_amdgcn_exp2f(end * SC_LOG2E);
+    d.sum = end;
+  }
+}
+
+// Columns 16 w .. of a 64-row tile as an operand of the products over its rows (rows 32 kk ..): one for each kk.
+template <typename T>
+__device__ __forceinline__ void sc_columns(const T* tile, int stride, int col0, sc_x8<T> (&out)[2]) {
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) out[kk] = op_ld_tr16<T, true>(tile, stride, col0, 32 * kk, lane_id());
+}
+// The weights of a lane's rows in such an operand.
+__device__ __forceinline__ void sc_row_weights(const float* w, int kk, float (&out)[8]) {
+  const int g = lane_id() >> 4;
+  const f32x4 a = *reinterpret_cast<const f32x4*>(w + 32 * kk + 4 * g), b = *reinterpret_cast<const f32x4*>(w + 32 * kk + 16 + 4 * g);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) { out[e] = a[e]; out[4 + e] = b[e]; }
+}
+// A weighted operand in two parts.
+template <typename T>
+__device__ __forceinline__ void sc_weighted(const sc_x8<T>& x, const float (&w)[8], sc_x8<T>& hi, sc_x8<T>& lo) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    T h, l;
+    sc_split<T>((float)x[e] * w[e], h, l);
+    hi[e] = h;
+    lo[e] = l;
+  }
+}
+// Two accumulator tiles (32 rows) as an operand in two parts.
+template <typename T>
+__device__ __forceinline__ void sc_state_operand(const f32x4& a, const f32x4& b, float scale, sc_x8<T>& hi, sc_x8<T>& lo) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = e < 4 ? a[e] : b[e - 4];
+    T h, l;
+    sc_split<T>(__is_same(T, _Float16) ? v * scale : v, h, l);
+    hi[e] = h;
+    lo[e] = l;
+  }
+}

@@ -1,0 +1,387 @@
+// Chunked forward of the state-space scan on the matrix cores: the segments' local states, and the outputs (see ss_chunk.h).
+#include "ss_chunk.h"
+
+struct ScFlags {
+  bool x, B, C, dy, y;  // rows that can be read (y: written) in 16 (8) byte pieces
+};
+
+static ScFlags sc_flags(const lampa_ss_args& a) {
+  auto rows = [](const void* p, int64_t stride, int inner) { return (uintptr_t)p % 16 == 0 && stride % 8 == 0 && inner % 8 == 0; };
+  ScFlags f;
+  f.x = rows(a.x, a.x_stride, a.P);
+  f.B = rows(a.B, a.B_stride, a.N);
+  f.C = rows(a.C, a.C_stride, a.N);
+  f.dy = a.dy && rows(a.dy, (int64_t)a.H * a.P, a.P);
+  f.y = (uintptr_t)a.y % 8 == 0 && a.y_stride % 4 == 0 && a.P % 4 == 0;
+  return f;
+}
+
+// A segment's local state, or (REV) local adjoint: sum over its tokens of B_s (delta_s e^{gamma_end - gamma_s} x_s)^T, or of
+// C_t (e^{gamma_t} dy_t)^T with gamma counted from the segment's start. Reads x and B (dy and C) once.
+template <typename T, int NP, bool REV>
+__global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGrad w, ScFlags f) {
+  constexpr int NT = NP / 16, KS = NP + 8, VS = 64 + 8;
+  const SsSegment seg = ss_segment(a, blockIdx.x);
+  if (!seg.live) return;
+  const int npb = (a.P + 63) / 64, pb = blockIdx.y % npb, h = blockIdx.y / npb, grp = h / (a.H / a.G);
+  const int lane = lane_id(), wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  const int cols = a.P - 64 * pb < 64 ? a.P - 64 * pb : 64;
+  __shared__ __align__(16) T tk[64 * KS], tv[64 * VS];
+  __shared__ __align__(16) ScDecay dec;
+  const T* kb = (REV ? (const T*)a.C : (const T*)a.B) + (int64_t)grp * a.N;
+  const T* vb = (REV ? (const T*)a.dy : (const T*)a.x) + (int64_t)h * a.P + 64 * pb;
+  const int64_t ks = REV ? a.C_stride : a.B_stride, vs = REV ? (int64_t)a.H * a.P : a.x_stride;
+  const bool kvec = REV ? f.C : f.B, vvec = REV ? f.dy : f.x;
+  const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
+  const int64_t chunks = seg.outside ? 0 : (seg.t1 - seg.t0 + 63) / 64;
+
+  f32x4 S[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) S[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  ScTile<T, NP> pk;
+  ScTile<T, 64> pv;
+  float pdt = 0.0f, sum = 0.0f;
+  auto fetch = [&](int64_t c) {
+    const int64_t t0 = seg.t0 + 64 * (REV ? chunks - 1 - c : c);
+    const int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
+    pk.fetch(kb, ks, t0, n, a.N, kvec);
+    pv.fetch(vb, vs, t0, n, cols, vvec);
+    if (wave == 0 && lane < n) pdt = ss_load_dt<T>(a.dt, a.dt_dtype, (t0 + lane) * a.dt_stride + h);
+  };
+  if (chunks) fetch(0);
+  for (int64_t c = 0; c < chunks; ++c) {
+    const int64_t t0 = seg.t0 + 64 * (REV ? chunks - 1 - c : c);
+    const int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
+    pk.put(tk, KS);
+    pv.put(tv, VS);
+    if (wave == 0) sc_decays(dec, pdt, n, bias, A, a.softplus);
+    lds_barrier();
+    if (c + 1 < chunks) fetch(c + 1);
+    const float end = dec.end;
+    sum += dec.sum;
+    sc_x8<T> v[2], hi[2], lo[2];
+    sc_columns<T>(tv, VS, 16 * wave, v);
+    float wt[2][8], back = 1.0f;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      if constexpr (REV) {
+        sc_row_weights(dec.grow, kk, wt[kk]);
+      } else {
+        float d[8];
+        sc_row_weights(dec.left, kk, wt[kk]);
+        sc_row_weights(dec.delta, kk, d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) wt[kk][e] *= d[e];
+      }
+    }
+    if constexpr (__is_same(T, _Float16)) {  // the largest weight becomes 1 or a little less: x is in range by itself
+      float m = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(wt[kk][e]));
+      m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      const float s = sc_scale_for<T>(m) * 0x1p-15f;
+      back = sc_inverse(s);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) wt[kk][e] *= s;
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) sc_weighted<T>(v[kk], wt[kk], hi[kk], lo[kk]);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      sc_x8<T> k[2];
+      sc_columns<T>(tk, KS, 16 * nt, k);
+      if constexpr (__is_same(T, _Float16)) {
+        f32x4 d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) d = mfma16(k[kk], hi[kk], mfma16(k[kk], lo[kk], d));
+        S[nt] = S[nt] * end + d * back;
+      } else {
+        S[nt] *= end;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) S[nt] = mfma16(k[kk], hi[kk], mfma16(k[kk], lo[kk], S[nt]));
+      }
+    }
+    lds_barrier();
+  }
+  float* local = (REV ? w.adjoints : a.slot_states) + ((int64_t)blockIdx.x * a.H + h) * a.N * a.P;
+  const int p = 64 * pb + 16 * wave + i;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int n = 16 * nt + 4 * g + r;
+      if (n < a.N && p < a.P) local[(int64_t)n * a.P + p] = S[nt][r];
+    }
+  if (!REV && threadIdx.x == 0 && pb == 0) a.slot_decay[(int64_t)blockIdx.x * a.H + h] = expf(sum);
+}
+
+// Outputs of a segment from the state it starts from.
+template <typename T, int NP>
+__global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a, ScFlags f) {
+  constexpr int NT = NP / 16, KK = NP / 32, KS = NP + 8, VS = 64 + 8, MS = 64 + 8;
+  const SsSegment seg = ss_segment(a, blockIdx.x);
+  if (!seg.live) return;
+  const int npb = (a.P + 63) / 64, pb = blockIdx.y % npb, h = blockIdx.y / npb, grp = h / (a.H / a.G);
+  const int lane = lane_id(), wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  const int cols = a.P - 64 * pb < 64 ? a.P - 64 * pb : 64;
+  T* yb = (T*)a.y + (int64_t)h * a.P + 64 * pb;
+  if (seg.outside) {
+    for (int64_t e = threadIdx.x; e < (seg.t1 - seg.t0) * cols; e += SC_BLOCK) yb[(seg.t0 + e / cols) * a.y_stride + e % cols] = (T)0.0f;
+    return;
+  }
+  __shared__ __align__(16) T tb[64 * KS], tc[64 * KS], tx[64 * VS], tm[64 * MS];
+  __shared__ __align__(16) ScDecay dec;
+  __shared__ float mback[64];  // fp16: what the rows of the pair weights were scaled down by
+  __shared__ int first_bad;
+  const T* bb = (const T*)a.B + (int64_t)grp * a.N;
+  const T* cb = (const T*)a.C + (int64_t)grp * a.N;
+  const T* xb = (const T*)a.x + (int64_t)h * a.P + 64 * pb;
+  const float A = a.A[h], D = a.D ? a.D[h] : 0.0f, bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
+  const bool single = (a.cu_seqlens ? a.n_tokens : a.seq_len) <= a.seg_tokens;
+  const int p = 64 * pb + 16 * wave + i;
+
+  f32x4 S[NT];
+  const float* init = single ? a.h0 : a.slot_states;
+  if (init) init += ((single ? (int64_t)seg.seq : (int64_t)blockIdx.x) * a.H + h) * a.N * a.P;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int n = 16 * nt + 4 * g + r;
+      S[nt][r] = init && n < a.N && p < a.P ? init[(int64_t)n * a.P + p] : 0.0f;
+    }
+
+  ScTile<T, NP> pB, pC;
+  ScTile<T, 64> pX;
+  float pdt = 0.0f;
+  auto fetch = [&](int64_t t0) {
+    const int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
+    pB.fetch(bb, a.B_stride, t0, n, a.N, f.B);
+    pC.fetch(cb, a.C_stride, t0, n, a.N, f.C);
+    pX.fetch(xb, a.x_stride, t0, n, cols, f.x);
+    if (wave == 0 && lane < n) pdt = ss_load_dt<T>(a.dt, a.dt_dtype, (t0 + lane) * a.dt_stride + h);
+  };
+  if (threadIdx.x == 0) first_bad = 64;
+  if (seg.t0 < seg.t1) fetch(seg.t0);
+  lds_barrier();
+  for (int64_t t0 = seg.t0; t0 < seg.t1;) {
+    int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
+    pB.put(tb, KS);
+    pC.put(tc, KS);
+    pX.put(tx, VS);
+    {
+      const int bad = pX.first_bad();
+      if (bad < 64) atomicMin(&first_bad, bad);
+    }
+    if (wave == 0) sc_decays(dec, pdt, n, bias, A, a.softplus);
+    lds_barrier();
+    // An x that is not finite times a weight of zero would reach earlier tokens: such a token begins a chunk of its own.
+    const int bad = first_bad;
+    if (bad < n) {
+      n = bad ? bad : 1;
+      lds_barrier();
+      for (int e = threadIdx.x; e < (64 - n) * KS; e += SC_BLOCK) tb[n * KS + e] = (T)0.0f;
+      for (int e = threadIdx.x; e < (64 - n) * VS; e += SC_BLOCK) tx[n * VS + e] = (T)0.0f;
+      if (wave == 0) sc_decays(dec, pdt, n, bias, A, a.softplus);
+      if (threadIdx.x == 0) first_bad = 64;
+      lds_barrier();
+    }
+    if (t0 + n < seg.t1) fetch(t0 + n);
+
+    // Pair weights of tokens t = 16 wave + i with s = 0 .. t, as the operand of the products over s.
+    {
+      const float gt = dec.gamma[16 * wave + i];
+      sc_x8<T> q[KK];
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) q[kk] = *reinterpret_cast<const sc_x8<T>*>(tc + (16 * wave + i) * KS + 32 * kk + 8 * g);
+      f32x4 m[4];
+      float big = 0.0f;
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        m[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (st > wave) continue;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+          m[st] = mfma16(*reinterpret_cast<const sc_x8<T>*>(tb + (16 * st + i) * KS + 32 * kk + 8 * g), q[kk], m[st]);
+        const f32x4 gs = *reinterpret_cast<const f32x4*>(dec.gamma + 16 * st + 4 * g);
+        const f32x4 ds = *reinterpret_cast<const f32x4*>(dec.delta + 16 * st + 4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = m[st][r] * ds[r] * __builtin_amdgcn_exp2f(gt - gs[r]);
+          m[st][r] = 16 * st + 4 * g + r <= 16 * wave + i ? v : 0.0f;
+          if (__is_same(T, _Float16)) big = fmaxf(big, fabsf(m[st][r]));
+        }
+      }
+      if constexpr (__is_same(T, _Float16)) {
+        big = fmaxf(big, __shfl_xor(big, 16));
+        big = fmaxf(big, __shfl_xor(big, 32));
+        const float s = sc_scale_for<T>(big);
+#pragma unroll
+        for (int st = 0; st < 4; ++st) m[st] *= s;
+        if (g == 0) mback[16 * wave + i] = sc_inverse(s);
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+        if (2 * kk <= wave)
+          *reinterpret_cast<sc_x8<T>*>(tm + (16 * wave + i) * MS + 32 * kk + 8 * g) = acc2_to_op<T>(m[2 * kk], m[2 * kk + 1]);
+    }
+    lds_barrier();
+
+    // y^T of this wave's 16 columns: lane = token 16 tt + i, registers = columns 4 g .. + 3
+    f32x4 y[4];
+    float sback = 1.0f;
+    {
+      float s = 1.0f;
+      if constexpr (__is_same(T, _Float16)) {
+        float big = 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) big = fmaxf(big, fabsf(S[nt][r]));
+        s = sc_scale_for<T>(sc_wave_max(big));
+        sback = sc_inverse(s);
+      }
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) y[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        sc_x8<T> hi, lo;
+        sc_state_operand<T>(S[2 * kk], S[2 * kk + 1], s, hi, lo);
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          const sc_x8<T> q = *reinterpret_cast<const sc_x8<T>*>(tc + (16 * tt + i) * KS + 32 * kk + 8 * g);
+          y[tt] = mfma16(hi, q, mfma16(lo, q, y[tt]));
+        }
+      }
+    }
+    sc_x8<T> v[2];
+    sc_columns<T>(tx, VS, 16 * wave, v);
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+      const int t = 16 * tt + i;
+      const float back = __is_same(T, _Float16) ? mback[t] : 1.0f;
+      y[tt] *= __is_same(T, _Float16) ? dec.grow[t] * sback * sc_inverse(back) : dec.grow[t];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+        if (2 * kk <= tt) y[tt] = mfma16(v[kk], *reinterpret_cast<const sc_x8<T>*>(tm + t * MS + 32 * kk + 8 * g), y[tt]);
+      if (t < n) {
+        const sc_x4<T> xv = *reinterpret_cast<const sc_x4<T>*>(tx + t * VS + op_perm32_col(16 * wave + 4 * g));
+        sc_x4<T> o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float out = __is_same(T, _Float16) ? y[tt][r] * back : y[tt][r];
+          o[r] = (T)__builtin_fmaf(D, (float)xv[r], out);
+        }
+        const int c = 16 * wave + 4 * g;
+        T* dst = yb + (t0 + t) * a.y_stride + c;
+        if (f.y) {
+          if (c < cols) *reinterpret_cast<sc_x4<T>*>(dst) = o;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (c + r < cols) dst[r] = o[r];
+        }
+      }
+    }
+    // the state behind the chunk
+    {
+      float wt[2][8], back = 1.0f;
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        float d[8];
+        sc_row_weights(dec.left, kk, wt[kk]);
+        sc_row_weights(dec.delta, kk, d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) wt[kk][e] *= d[e];
+      }
+      if constexpr (__is_same(T, _Float16)) {
+        float m = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(wt[kk][e]));
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const float s = sc_scale_for<T>(m) * 0x1p-15f;
+        back = sc_inverse(s);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) wt[kk][e] *= s;
+      }
+      sc_x8<T> hi[2], lo[2];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) sc_weighted<T>(v[kk], wt[kk], hi[kk], lo[kk]);
+      const float end = dec.end;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        sc_x8<T> k[2];
+        sc_columns<T>(tb, KS, 16 * nt, k);
+        if constexpr (__is_same(T, _Float16)) {
+          f32x4 d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk) d = mfma16(k[kk], hi[kk], mfma16(k[kk], lo[kk], d));
+          S[nt] = S[nt] * end + d * back;
+        } else {
+          S[nt] *= end;
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk) S[nt] = mfma16(k[kk], hi[kk], mfma16(k[kk], lo[kk], S[nt]));
+        }
+      }
+    }
+    t0 += n;
+    lds_barrier();
+  }
+  if (single && a.ht) {
+    float* out = a.ht + ((int64_t)seg.seq * a.H + h) * a.N * a.P;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = 16 * nt + 4 * g + r;
+        if (n < a.N && p < a.P) out[(int64_t)n * a.P + p] = S[nt][r];
+      }
+  }
+}
+
+// Slots along x in a multiple of 8: workgroups are dealt to the 8 dies in turn, so the heads of a segment, which read the same
+// rows of B and C, meet in one die's L2.
+static dim3 sc_grid(const lampa_ss_args& a) {
+  return dim3((unsigned)((ss_slots(&a) + 7) / 8 * 8), (unsigned)(a.H * ss_blocks64(a.P)));
+}
+
+template <typename T>
+static int sc_maps_launch(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s) {
+  const ScFlags f = sc_flags(a);
+  const SsGrad w = grad ? *grad : SsGrad{};
+  LAMPA_PROF(s, "start");
+#define SC_GO(NP)                                                                                                     \
+  if (grad) hipLaunchKernelGGL((sc_map_kernel<T, NP, true>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f);              \
+  else hipLaunchKernelGGL((sc_map_kernel<T, NP, false>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f)
+  if (a.N <= 32) { SC_GO(32); } else if (a.N <= 64) { SC_GO(64); } else { SC_GO(128); }
+#undef SC_GO
+  LAMPA_PROF(s, "sc_map_kernel");
+  return lampa_launch_status();
+}
+int ss_chunk_maps(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s) {
+  return a.dtype == GDR_BF16 ? sc_maps_launch<__bf16>(a, grad, s) : sc_maps_launch<_Float16>(a, grad, s);
+}
+
+template <typename T>
+static int sc_out_launch(const lampa_ss_args& a, hipStream_t s) {
+  const ScFlags f = sc_flags(a);
+  LAMPA_PROF(s, "start");
+  if (a.N <= 32) hipLaunchKernelGGL((sc_out_kernel<T, 32>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, f);
+  else if (a.N <= 64) hipLaunchKernelGGL((sc_out_kernel<T, 64>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, f);
+  else hipLaunchKernelGGL((sc_out_kernel<T, 128>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, f);
+  LAMPA_PROF(s, "sc_out_kernel");
+  return lampa_launch_status();
+}
+int ss_chunk_out(const lampa_ss_args& a, hipStream_t s) {
+  return a.dtype == GDR_BF16 ? sc_out_launch<__bf16>(a, s) : sc_out_launch<_Float16>(a, s);
+}

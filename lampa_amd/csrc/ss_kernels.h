@@ -16,3 +16,6 @@ enum { SS_Y = 0, SS_DC = 1, SS_DX = 2, SS_DB = 3 };
 
 int ss_serial_maps(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s);
 int ss_serial_walk(const lampa_ss_args& a, int kind, const SsGrad& grad, hipStream_t s);
+
+int ss_chunk_maps(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s);
+int ss_chunk_out(const lampa_ss_args& a, hipStream_t s);

@@ -184,11 +184,11 @@ extern "C" int lampa_ss_scan_fwd(const lampa_ss_args* args, void* stream) {
   if (!a.y || a.y_stride < (int64_t)a.H * a.P) return LAMPA_ERR_INVALID;
   if (!ss_single(&a)) {
     if (!a.slot_states || !a.slot_decay) return LAMPA_ERR_WORKSPACE;
-    int e = ss_serial_maps(a, nullptr, s);
+    int e = a.dtype == GDR_FP32 ? ss_serial_maps(a, nullptr, s) : ss_chunk_maps(a, nullptr, s);
     if (e == LAMPA_OK) e = ss_join<false>(a, a.slot_states, a.h0, a.ht, s);
     if (e != LAMPA_OK) return e;
   }
-  return ss_serial_walk(a, SS_Y, SsGrad{}, s);
+  return a.dtype == GDR_FP32 ? ss_serial_walk(a, SS_Y, SsGrad{}, s) : ss_chunk_out(a, s);
 }
 
 static int64_t ss_grad_layout(const lampa_ss_args& a, char* base, SsGrad* w) {
@@ -234,7 +234,7 @@ extern "C" int lampa_ss_scan_bwd(const lampa_ss_args* args, void* stream) {
   } else {
     if (!ss_single(&a)) {
       if (!a.slot_states || !a.slot_decay || !a.ht) return LAMPA_ERR_WORKSPACE;
-      e = ss_serial_maps(a, &w, s);
+      e = a.dtype == GDR_FP32 ? ss_serial_maps(a, &w, s) : ss_chunk_maps(a, &w, s);
       if (e == LAMPA_OK) e = ss_join<true>(a, w.adjoints, a.dht, a.dh0, s);
     }
     for (int kind : {SS_DC, SS_DX, SS_DB})
