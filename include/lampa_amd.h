@@ -461,7 +461,7 @@ int lampa_gdr_traffic_probe_walk(const void* q, const void* k, const void* v, co
  *
  * slot_states [lampa_ss_slots, H, N, P] fp32 and slot_decay [lampa_ss_slots, H] fp32 are scratch of the forward; where a
  * sequence may have more than one segment they must not be NULL. For gradients keep both (slot_states then holds the state at
- * the start of every segment) and ht for lampa_ss_scan_bwd. */
+ * the start of every segment) for lampa_ss_scan_bwd. */
 typedef struct {
   const void *x, *dt, *B, *C;
   const float *A, *D, *dt_bias, *h0;

@@ -162,3 +162,41 @@ __device__ __forceinline__ void sc_state_operand(const f32x4& a, const f32x4& b,
     lo[e] = l;
   }
 }
+
+struct ScFlags {
+  bool x, B, C, dy;  // rows that can be read in 16-byte pieces
+  bool y, dx;        // rows that can be written in 8-byte pieces
+};
+
+static ScFlags sc_flags(const lampa_ss_args& a) {
+  auto rows = [](const void* p, int64_t stride, int inner) { return (uintptr_t)p % 16 == 0 && stride % 8 == 0 && inner % 8 == 0; };
+  ScFlags f;
+  f.x = rows(a.x, a.x_stride, a.P);
+  f.B = rows(a.B, a.B_stride, a.N);
+  f.C = rows(a.C, a.C_stride, a.N);
+  f.dy = a.dy && rows(a.dy, (int64_t)a.H * a.P, a.P);
+  f.dx = (uintptr_t)a.dx % 8 == 0 && a.P % 4 == 0;
+  f.y = (uintptr_t)a.y % 8 == 0 && a.y_stride % 4 == 0 && a.P % 4 == 0;
+  return f;
+}
+
+// Slots along x in a multiple of 8: workgroups are dealt to the 8 dies in turn, so the heads of a segment, which read the same
+// rows of B and C, meet in one die's L2.
+static dim3 sc_grid(const lampa_ss_args& a) {
+  return dim3((unsigned)((ss_slots(&a) + 7) / 8 * 8), (unsigned)(a.H * ss_blocks64(a.P)));
+}
+
+
+// Place of element (row 16 nt + row, column 16 w + col) of a chunk's kept state: float4 number (tile nt, columns 32 (w / 2) + 16
+// (w % 2) + 4 g ..) of lane 16 g + row, so that a lane of the gradients reads its operand's columns of one row in whole float4s, a
+// wave 1 KiB at a time.
+__device__ __forceinline__ int sc_kept_at(int nt, int w, int row, int col) { return ((nt * 4 + w) * 64 + 16 * (col >> 2) + row) * 4 + (col & 3); }
+
+// Sum over the 16 lanes of a row, in every lane of it.
+__device__ __forceinline__ float sc_row16_sum(float x) {
+  x += dpp_f32<GDR_DPP_QUAD_XOR1, 0xF>(0.0f, x);
+  x += dpp_f32<GDR_DPP_QUAD_XOR2, 0xF>(0.0f, x);
+  x += dpp_f32<0x141, 0xF>(0.0f, x);  // mirrored within 8 lanes
+  x += dpp_f32<0x140, 0xF>(0.0f, x);  // mirrored within 16
+  return x;
+}

@@ -1,24 +1,11 @@
 // Chunked forward of the state-space scan on the matrix cores: the segments' local states, and the outputs (see ss_chunk.h).
 #include "ss_chunk.h"
 
-struct ScFlags {
-  bool x, B, C, dy, y;  // rows that can be read (y: written) in 16 (8) byte pieces
-};
-
-static ScFlags sc_flags(const lampa_ss_args& a) {
-  auto rows = [](const void* p, int64_t stride, int inner) { return (uintptr_t)p % 16 == 0 && stride % 8 == 0 && inner % 8 == 0; };
-  ScFlags f;
-  f.x = rows(a.x, a.x_stride, a.P);
-  f.B = rows(a.B, a.B_stride, a.N);
-  f.C = rows(a.C, a.C_stride, a.N);
-  f.dy = a.dy && rows(a.dy, (int64_t)a.H * a.P, a.P);
-  f.y = (uintptr_t)a.y % 8 == 0 && a.y_stride % 4 == 0 && a.P % 4 == 0;
-  return f;
-}
-
 // A segment's local state, or (REV) local adjoint: sum over its tokens of B_s (delta_s e^{gamma_end - gamma_s} x_s)^T, or of
 // C_t (e^{gamma_t} dy_t)^T with gamma counted from the segment's start. Reads x and B (dy and C) once.
-template <typename T, int NP, bool REV>
+// KEEP: the walk starts from the segment's initial state and leaves the state in front of every chunk in w.chunk_states, in the
+// order in which the gradients' lanes read it (sc_kept_at).
+template <typename T, int NP, bool REV, bool KEEP>
 __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGrad w, ScFlags f) {
   constexpr int NT = NP / 16, KS = NP + 8, VS = 64 + 8;
   const SsSegment seg = ss_segment(a, blockIdx.x);
@@ -38,6 +25,19 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
   f32x4 S[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) S[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int p = 64 * pb + 16 * wave + i;
+  if (KEEP) {
+    const bool single = (a.cu_seqlens ? a.n_tokens : a.seq_len) <= a.seg_tokens;
+    const float* init = single ? a.h0 : a.slot_states;
+    if (init) init += ((single ? (int64_t)seg.seq : (int64_t)blockIdx.x) * a.H + h) * a.N * a.P;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = 16 * nt + 4 * g + r;
+        S[nt][r] = init && !seg.outside && n < a.N && p < a.P ? init[(int64_t)n * a.P + p] : 0.0f;
+      }
+  }
   ScTile<T, NP> pk;
   ScTile<T, 64> pv;
   float pdt = 0.0f, sum = 0.0f;
@@ -52,6 +52,13 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
   for (int64_t c = 0; c < chunks; ++c) {
     const int64_t t0 = seg.t0 + 64 * (REV ? chunks - 1 - c : c);
     const int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
+    if (KEEP) {
+      float* keep = w.chunk_states + ((seg.chunk0 + c) * a.H * npb + blockIdx.y) * (NP * 64);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) keep[sc_kept_at(nt, wave, 4 * g + r, i)] = S[nt][r];
+    }
     pk.put(tk, KS);
     pv.put(tv, VS);
     if (wave == 0) sc_decays(dec, pdt, n, bias, A, a.softplus);
@@ -108,8 +115,8 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
     }
     lds_barrier();
   }
+  if (KEEP) return;
   float* local = (REV ? w.adjoints : a.slot_states) + ((int64_t)blockIdx.x * a.H + h) * a.N * a.P;
-  const int p = 64 * pb + 16 * wave + i;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -349,27 +356,29 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a, Sc
   }
 }
 
-// Slots along x in a multiple of 8: workgroups are dealt to the 8 dies in turn, so the heads of a segment, which read the same
-// rows of B and C, meet in one die's L2.
-static dim3 sc_grid(const lampa_ss_args& a) {
-  return dim3((unsigned)((ss_slots(&a) + 7) / 8 * 8), (unsigned)(a.H * ss_blocks64(a.P)));
-}
-
+enum { SC_LOCAL_STATES, SC_LOCAL_ADJOINTS, SC_KEEP_STATES };
 template <typename T>
-static int sc_maps_launch(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s) {
+static int sc_maps_launch(const lampa_ss_args& a, int what, const SsGrad& w, hipStream_t s) {
   const ScFlags f = sc_flags(a);
-  const SsGrad w = grad ? *grad : SsGrad{};
   LAMPA_PROF(s, "start");
-#define SC_GO(NP)                                                                                                     \
-  if (grad) hipLaunchKernelGGL((sc_map_kernel<T, NP, true>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f);              \
-  else hipLaunchKernelGGL((sc_map_kernel<T, NP, false>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f)
-  if (a.N <= 32) { SC_GO(32); } else if (a.N <= 64) { SC_GO(64); } else { SC_GO(128); }
+#define SC_GO(NP)                                                                                                                   \
+  switch (what) {                                                                                                                   \
+    case SC_LOCAL_STATES: hipLaunchKernelGGL((sc_map_kernel<T, NP, false, false>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f); break; \
+    case SC_LOCAL_ADJOINTS: hipLaunchKernelGGL((sc_map_kernel<T, NP, true, false>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f); break; \
+    default: hipLaunchKernelGGL((sc_map_kernel<T, NP, false, true>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f); break;              \
+  }
+  if (a.N <= 32) { SC_GO(32) } else if (a.N <= 64) { SC_GO(64) } else { SC_GO(128) }
 #undef SC_GO
-  LAMPA_PROF(s, "sc_map_kernel");
+  LAMPA_PROF(s, what == SC_KEEP_STATES ? "sc_map_kernel<keep>" : "sc_map_kernel");
   return lampa_launch_status();
 }
 int ss_chunk_maps(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s) {
-  return a.dtype == GDR_BF16 ? sc_maps_launch<__bf16>(a, grad, s) : sc_maps_launch<_Float16>(a, grad, s);
+  const int what = grad ? SC_LOCAL_ADJOINTS : SC_LOCAL_STATES;
+  const SsGrad w = grad ? *grad : SsGrad{};
+  return a.dtype == GDR_BF16 ? sc_maps_launch<__bf16>(a, what, w, s) : sc_maps_launch<_Float16>(a, what, w, s);
+}
+int ss_chunk_keep(const lampa_ss_args& a, const SsGrad& w, hipStream_t s) {
+  return a.dtype == GDR_BF16 ? sc_maps_launch<__bf16>(a, SC_KEEP_STATES, w, s) : sc_maps_launch<_Float16>(a, SC_KEEP_STATES, w, s);
 }
 
 template <typename T>

@@ -23,6 +23,7 @@
 struct SsSegment {
   int64_t t0, t1;   // tokens of this segment
   int seq, index;   // sequence, place of the segment in it
+  int64_t chunk0;   // row of its first 64 tokens in tables with a row for every 64 tokens of a sequence
   bool live;        // false: this slot holds no segment
   bool first, last; // in its sequence
   bool outside;     // rows behind the last sequence: their outputs are zero
@@ -70,6 +71,7 @@ __device__ __forceinline__ SsSegment ss_segment(const lampa_ss_args& a, int64_t 
   s.t0 = b + (int64_t)s.index * a.seg_tokens;
   s.t1 = s.t0 + a.seg_tokens < e ? s.t0 + a.seg_tokens : e;
   if (s.t1 < s.t0) s.t1 = s.t0;
+  s.chunk0 = b / 64 + s.seq + (int64_t)s.index * (a.seg_tokens / 64);
   s.first = s.index == 0;
   s.last = s.t1 >= e;
   return s;
@@ -103,6 +105,8 @@ static inline int64_t ss_slots(const lampa_ss_args* a) {
   if (!a->cu_seqlens) return (int64_t)a->n_seq * ((a->seq_len + a->seg_tokens - 1) / a->seg_tokens);
   return a->n_tokens / a->seg_tokens + a->n_seq + 1;
 }
+// Rows of a table with one for every 64 tokens of a sequence: sequence i takes them from floor(begin / 64) + i on.
+static inline int64_t ss_chunk_rows(const lampa_ss_args* a) { return a->n_tokens / 64 + a->n_seq + 1; }
 // One segment holds any sequence: no scan over segments, the walks start from h0 and leave the final states themselves.
 static inline bool ss_single(const lampa_ss_args* a) {
   return (a->cu_seqlens ? a->n_tokens : a->seq_len) <= a->seg_tokens;

@@ -4,12 +4,15 @@
 #include "ss_common.h"
 
 struct SsGrad {
-  float* adjoints;      // [slots, H, N, P]: the segments' local adjoints, then the adjoint at each segment's end
-  float *dB_part, *dC_part;  // [tokens, H * ceil(P / 64), N]: one part for each head and block of 64 columns of x
-  float* read;          // [tokens, H, parts]: dy_t . (S_t^T C_t), parts = ceil(P / 64) * ceil(N / 64)
-  float* written;       // [tokens, H, ceil(P / 64)]: x_t . (R_t^T B_t)
-  float* param_part;    // [slots, H, 2]: a segment's share of dA and d dt_bias
-  float* dD_part;       // [slots, H, ceil(P / 64)]
+  float* adjoints;           // [slots, H, N, P]: the segments' local adjoints, then the adjoint at each segment's end
+  float *dB_part, *dC_part;  // [tokens, H * blocks, N]: one part for each head and block of 64 columns of x
+  float* dg;                 // [tokens, H, blocks]: the decay exponent's gradient (chunks), or dy_t . (S_t^T C_t) (token-serial)
+  float* reach;              // [tokens, H, blocks]: x_t . (R_t^T B_t)
+  float* chunk_states;       // chunks: the state in front of every 64 tokens, [rows, H, blocks, N padded, 64]
+                             // token-serial: the state behind them, [rows, H, N, P]
+  float* chunk_dots;         // token-serial: <R, S> behind every 64 tokens, [rows, H, blocks]
+  float* param_part;         // [slots, H, 2]: a segment's share of dA and d dt_bias
+  float* dD_part;            // [slots, H, blocks]
 };
 
 enum { SS_Y = 0, SS_DC = 1, SS_DX = 2, SS_DB = 3 };
@@ -19,3 +22,6 @@ int ss_serial_walk(const lampa_ss_args& a, int kind, const SsGrad& grad, hipStre
 
 int ss_chunk_maps(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s);
 int ss_chunk_out(const lampa_ss_args& a, hipStream_t s);
+int ss_chunk_keep(const lampa_ss_args& a, const SsGrad& w, hipStream_t s);
+int ss_chunk_grad(const lampa_ss_args& a, const SsGrad& w, hipStream_t s);
+static inline int ss_chunk_n(int N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }  // N as the chunk kernels are built for it

@@ -50,81 +50,61 @@ static int ss_join(const lampa_ss_args& a, float* states, const float* init, flo
   return lampa_launch_status();
 }
 
-// A segment's gradient of the decays: dg_t = dg_{t+1} + read_t - delta_t written_t from the segment's end, where it starts
-// from <R, S> of the states there, so that errors of the sum do not pass from one segment to the next. One workgroup a
-// segment and head, 256 tokens at a time from the end.
+// From the gradient of the decays to those of dt, A and dt_bias. One workgroup a segment and head; a wave takes 64 tokens at a
+// time, a lane one of them. Where dg has not been summed up yet (fp32), it is here, from the end of the 64 tokens:
+// dg_t = dg_{t+1} + read_t - delta_t reach_t, behind the last of them <R, S>. Starting anew every 64 tokens keeps rounding errors
+// of the sum, which pass on to every earlier token of it, from adding up over a segment (dA off by 2.5e-5 then, 60 000 tokens).
 template <typename T>
-__global__ void __launch_bounds__(SS_BLOCK) ss_decay_grad_kernel(lampa_ss_args a, SsGrad w) {
+__global__ void __launch_bounds__(SS_BLOCK) ss_decay_grad_kernel(lampa_ss_args a, SsGrad w, bool summed) {
   const SsSegment seg = ss_segment(a, blockIdx.x);
-  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = (int64_t)blockIdx.x * a.H + h;
-  if (!seg.live || seg.outside) {
-    if (tid < 2) w.param_part[row * 2 + tid] = 0.0f;
-    if (!seg.live) return;
-  }
-  __shared__ float part[4];
-  auto block_sum = [&](float x) {
-    x = ss_wave_sum(x);
-    __syncthreads();
-    if (lane == 0) part[wave] = x;
-    __syncthreads();
-    return (part[0] + part[1]) + (part[2] + part[3]);
-  };
-  const int npb = (a.P + 63) / 64, nnb = (a.N + 63) / 64;
-  const int64_t per_h = (int64_t)a.N * a.P;
-  const bool single = (a.cu_seqlens ? a.n_tokens : a.seq_len) <= a.seg_tokens;
-  const float* R = single || seg.last ? a.dht : w.adjoints;
-  const float* S = single || seg.last ? a.ht : a.slot_states;
-  float carry = 0.0f;
-  if (R && !seg.outside) {
-    const int64_t own = ((int64_t)seg.seq * a.H + h) * per_h;
-    R += single || seg.last ? own : row * per_h;
-    S += single || seg.last ? own : (row + a.H) * per_h;  // the next segment's initial state
-    float dot = 0.0f;
-    for (int64_t e = tid; e < per_h; e += SS_BLOCK) dot = __builtin_fmaf(R[e], S[e], dot);
-    carry = block_sum(dot);
-  }
+  const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t slot_row = (int64_t)blockIdx.x * a.H + h;
+  const int npb = (a.P + 63) / 64, reads = summed ? npb : npb * ((a.N + 63) / 64);
   const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
   float dA = 0.0f, dbias = 0.0f;
-  for (int64_t hi = seg.t1; hi > seg.t0; hi -= SS_BLOCK) {
-    const int64_t tok = hi - 1 - tid;  // thread i: the i-th token from the end
-    const bool on = tok >= seg.t0;
-    float raw = 0.0f, delta = 0.0f, read = 0.0f, written = 0.0f;
-    if (on && !seg.outside) {
+  for (int64_t t0 = seg.t0 + 64 * wave; seg.live && t0 < seg.t1; t0 += SS_BLOCK) {
+    const int64_t tok = t0 + lane;
+    const bool on = tok < seg.t1 && !seg.outside;
+    float raw = 0.0f, delta = 0.0f, dg = 0.0f, reach = 0.0f;
+    if (on) {
       raw = ss_load_dt<T>(a.dt, a.dt_dtype, tok * a.dt_stride + h) + bias;
       delta = ss_delta(raw, 0.0f, a.softplus);
-      for (int i = 0; i < npb * nnb; ++i) read += w.read[(tok * a.H + h) * npb * nnb + i];
-      for (int i = 0; i < npb; ++i) written += w.written[(tok * a.H + h) * npb + i];
+      for (int i = 0; i < reads; ++i) dg += w.dg[(tok * a.H + h) * reads + i];
+      for (int i = 0; i < npb; ++i) reach += w.reach[(tok * a.H + h) * npb + i];
     }
-    float sum = on ? read - delta * written : 0.0f;  // inclusive prefix over the threads = suffix over the tokens
+    if (!summed && !seg.outside) {
+      if (on) dg -= delta * reach;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const float up = __shfl_up(sum, off);
-      if (lane >= off) sum += up;
+      for (int off = 1; off < 64; off <<= 1) {
+        const float later = __shfl_down(dg, off);
+        if (lane + off < 64) dg += later;
+      }
+      const int64_t row = (seg.chunk0 + (t0 - seg.t0) / 64) * a.H + h;
+      for (int i = 0; i < npb; ++i) dg += w.chunk_dots[row * npb + i];
     }
-    __syncthreads();
-    if (lane == 63) part[wave] = sum;
-    __syncthreads();
-    float before = carry;
-    for (int i = 0; i < wave; ++i) before += part[i];
-    const float dg = before + sum;
-    carry += (part[0] + part[1]) + (part[2] + part[3]);
-    if (on) {
-      float d = __builtin_fmaf(A, dg, written);
+    if (tok < seg.t1) {
+      float d = on ? __builtin_fmaf(A, dg, reach) : 0.0f;
       // the derivative of log(1 + e^x), which is used as x above 20
-      if (a.softplus) d *= raw > 20.0f ? 1.0f : 1.0f / (1.0f + expf(-raw));
-      if (seg.outside) d = 0.0f;
+      if (on && a.softplus) d *= raw > 20.0f ? 1.0f : 1.0f / (1.0f + expf(-raw));
       if (a.dt_dtype == GDR_FP32) ((float*)a.ddt)[tok * a.H + h] = d;
       else ((T*)a.ddt)[tok * a.H + h] = GdrElem<T>::from_float(d);
-      dbias += d;
-      dA = __builtin_fmaf(delta, dg, dA);
+      if (on) {
+        dbias += d;
+        dA = __builtin_fmaf(delta, dg, dA);
+      }
     }
   }
-  dA = block_sum(dA);
-  dbias = block_sum(dbias);
-  if (tid == 0 && !seg.outside) {
-    w.param_part[row * 2] = dA;
-    w.param_part[row * 2 + 1] = dbias;
+  dA = ss_wave_sum(dA);
+  dbias = ss_wave_sum(dbias);
+  __shared__ float part[2][4];
+  if (lane == 0) {
+    part[0][wave] = dA;
+    part[1][wave] = dbias;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    const float* v = part[threadIdx.x];
+    w.param_part[slot_row * 2 + threadIdx.x] = (v[0] + v[1]) + (v[2] + v[3]);
   }
 }
 
@@ -202,8 +182,11 @@ static int64_t ss_grad_layout(const lampa_ss_args& a, char* base, SsGrad* w) {
   take(g.adjoints, ss_single(&a) ? 0 : slots * a.H * a.N * a.P);
   take(g.dB_part, a.n_tokens * a.H * npb * a.N);
   take(g.dC_part, a.n_tokens * a.H * npb * a.N);
-  take(g.read, a.n_tokens * a.H * npb * nnb);
-  take(g.written, a.n_tokens * a.H * npb);
+  const bool serial = a.dtype == GDR_FP32;
+  take(g.dg, a.n_tokens * a.H * npb * (serial ? nnb : 1));
+  take(g.reach, a.n_tokens * a.H * npb);
+  take(g.chunk_states, ss_chunk_rows(&a) * a.H * (serial ? (int64_t)a.N * a.P : npb * ss_chunk_n(a.N) * 64));
+  take(g.chunk_dots, serial ? ss_chunk_rows(&a) * a.H * npb : 0);
   take(g.param_part, slots * a.H * 2);
   take(g.dD_part, slots * a.H * npb);
   if (w) *w = g;
@@ -221,30 +204,35 @@ extern "C" int lampa_ss_scan_bwd(const lampa_ss_args* args, void* stream) {
   const lampa_ss_args& a = *args;
   if (!a.dA) return LAMPA_ERR_INVALID;
   if (a.n_tokens && (!a.dy || !a.dx || !a.ddt || !a.dB || !a.dC)) return LAMPA_ERR_INVALID;
-  if (a.dht && !a.ht) return LAMPA_ERR_INVALID;
   const int64_t need = ss_grad_layout(a, nullptr, nullptr);
   if (need && (!a.workspace || a.workspace_bytes < need)) return LAMPA_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   SsGrad w;
   ss_grad_layout(a, (char*)a.workspace, &w);
   const int64_t slots = a.n_tokens ? ss_slots(&a) : 0;
+  const bool serial = a.dtype == GDR_FP32;
   int e = LAMPA_OK;
   if (!a.n_tokens) {
     if (a.dh0) e = ss_join<true>(a, nullptr, a.dht, a.dh0, s);
   } else {
     if (!ss_single(&a)) {
-      if (!a.slot_states || !a.slot_decay || !a.ht) return LAMPA_ERR_WORKSPACE;
-      e = a.dtype == GDR_FP32 ? ss_serial_maps(a, &w, s) : ss_chunk_maps(a, &w, s);
+      if (!a.slot_states || !a.slot_decay) return LAMPA_ERR_WORKSPACE;
+      e = serial ? ss_serial_maps(a, &w, s) : ss_chunk_maps(a, &w, s);
       if (e == LAMPA_OK) e = ss_join<true>(a, w.adjoints, a.dht, a.dh0, s);
     }
-    for (int kind : {SS_DC, SS_DX, SS_DB})
-      if (e == LAMPA_OK) e = ss_serial_walk(a, kind, w, s);
+    if (serial) {
+      for (int kind : {SS_DC, SS_DX, SS_DB})
+        if (e == LAMPA_OK) e = ss_serial_walk(a, kind, w, s);
+    } else {
+      if (e == LAMPA_OK) e = ss_chunk_keep(a, w, s);
+      if (e == LAMPA_OK) e = ss_chunk_grad(a, w, s);
+    }
     if (e != LAMPA_OK) return e;
     const int64_t n = a.n_tokens * a.G * a.N;
     const dim3 sums((unsigned)((n + SS_BLOCK - 1) / SS_BLOCK), 2), segs((unsigned)slots, (unsigned)a.H);
     const int parts = a.H / a.G * ss_blocks64(a.P);
 #define SS_TAIL(T)                                                                                                          \
-  hipLaunchKernelGGL((ss_decay_grad_kernel<T>), segs, dim3(SS_BLOCK), 0, s, a, w);                                          \
+  hipLaunchKernelGGL((ss_decay_grad_kernel<T>), segs, dim3(SS_BLOCK), 0, s, a, w, !serial);                                          \
   LAMPA_PROF(s, "ss_decay_grad_kernel");                                                                                    \
   hipLaunchKernelGGL((ss_group_sum_kernel<T>), sums, dim3(SS_BLOCK), 0, s, w.dB_part, w.dC_part, (T*)a.dB, (T*)a.dC, n, a.N, \
                      parts);                                                                                                \

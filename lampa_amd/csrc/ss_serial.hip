@@ -132,6 +132,19 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
         if (MAP) sum_g += g;
         const float v = KIND == SS_Y || KIND == SS_DC ? delta * lv[t][lane] : lv[t][lane];
         const float s = REV ? carry : decay;
+        if constexpr (KIND == SS_DX && !MAP) {
+          const int64_t done = tok + 1 - seg.t0;
+          if (done % 64 == 0 || tok + 1 == seg.t1) {  // S times the last decay is the adjoint behind this token
+            const int64_t row = (seg.chunk0 + (done - 1) / 64) * a.H + h;
+            const float* kept = w.chunk_states + row * per_h;
+            float dot = 0.0f;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+              if (lane_on && r < rn) dot = __builtin_fmaf(S[r], kept[at(r)], dot);
+            dot = ss_wave_sum(dot) * carry;
+            if (lane == 0) w.chunk_dots[row * npb + pb] = dot;
+          }
+        }
         float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
@@ -151,12 +164,20 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
           if (lane_on) ((T*)a.dx)[tok * dy_stride + (int64_t)h * a.P + l] =
               GdrElem<T>::from_float(__builtin_fmaf(delta, out, D * dyv));
           const float q = ss_wave_sum(lane_on ? xv * out : 0.0f);
-          if (lane == 0) w.written[(tok * a.H + h) * npb + pb] = q;
+          if (lane == 0) w.reach[(tok * a.H + h) * npb + pb] = q;
           dD = __builtin_fmaf(xv, dyv, dD);
         } else if constexpr (KIND == SS_DC) {
           if (lane_on) w.dC_part[(tok * a.H * npb + h * npb + pb) * a.N + l] = out;
           const float u = ss_wave_sum(lane_on && !seg.outside ? le[t][lane] * out : 0.0f);
-          if (lane == 0) w.read[((tok * a.H + h) * npb + pb) * nnb + lane_block] = u;
+          if (lane == 0) w.dg[((tok * a.H + h) * npb + pb) * nnb + lane_block] = u;
+          // the state behind every 64 tokens (and behind the last one), for <R, S> there
+          const int64_t done = tok + 1 - seg.t0;
+          if (!seg.outside && (done % 64 == 0 || tok + 1 == seg.t1)) {
+            float* keep = w.chunk_states + ((seg.chunk0 + (done - 1) / 64) * a.H + h) * per_h;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+              if (lane_on && r < rn) keep[at(r)] = S[r];
+          }
         } else {
           if (lane_on) w.dB_part[(tok * a.H * npb + h * npb + pb) * a.N + l] = delta * out;
         }
