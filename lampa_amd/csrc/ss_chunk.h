@@ -15,16 +15,17 @@
 #include "ss_kernels.h"
 
 #define SC_BLOCK 256
-#define SC_LOG2E 1.44269504f
 
 template <typename T>
 using sc_x8 = typename OpVec<T>::x8;
 template <typename T>
 using sc_x4 = typename OpVec<T>::x4;
 
-// v as an operand value and the operand value of what that leaves out.
+// v as an operand value and the operand value of what that leaves out. v is taken out of the compiler's sight: it would form an
+// fp16 `hi` of a product in one rounding and the remainder from one of two, which now and then (ties) is another value.
 template <typename T>
 __device__ __forceinline__ void sc_split(float v, T& hi, T& lo) {
+  if constexpr (__is_same(T, _Float16)) asm("" : "+v"(v));
   hi = (T)v;
   lo = (T)(v - (float)hi);
 }
@@ -101,28 +102,50 @@ struct ScTile {
   }
 };
 
-// What a chunk's steps and decays come to, one entry a token.
+// What a chunk's steps and decays come to, one entry a token. gamma is summed up in 64 bits: it reaches -200 and beyond where a
+// head decays fast, and the exponents of neighbouring tokens are differences of it, which have to be right to 2^-24 for dA and
+// d dt_bias, sums over all tokens, to be.
 struct ScDecay {
-  float gamma[64];  // gamma_t log2(e)
+  float gamma[64];  // gamma_t log2(e), rounded ...
+  float rest[64];   // ... and 2 to the power of what the rounding left out
   float delta[64];
   float grow[64];   // e^{gamma_t}
   float left[64];   // e^{gamma_end - gamma_t}
   float end;        // e^{gamma_end}
-  float sum;        // gamma_end
+  float sum;        // gamma_end log2(e)
 };
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double sc_dpp_add(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xF, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xF, false);
+  return x + __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
 // One wave, lane = token; tokens from n on have no step.
 __device__ __forceinline__ void sc_decays(ScDecay& d, float raw, int n, float bias, float A, int softplus) {
   const int lane = lane_id();
   const float delta = lane < n ? ss_delta(raw, bias, softplus) : 0.0f;
-  const float gamma = wave_cumulative_decay(lane < n ? ss_log_decay(delta, A) : 0.0f);
-  const float end = __shfl(gamma, 63);
-  d.gamma[lane] = gamma * SC_LOG2E;
+  double g = 0.0;
+  if (lane < n) {
+    g = (double)delta * (double)A;
+    g = (g < SS_MIN_LOG_DECAY ? (double)SS_MIN_LOG_DECAY : g) * 1.4426950408889634;
+  }
+  g = sc_dpp_add<GDR_DPP_ROW_SHR(1), 0xF>(g);
+  g = sc_dpp_add<GDR_DPP_ROW_SHR(2), 0xF>(g);
+  g = sc_dpp_add<GDR_DPP_ROW_SHR(4), 0xF>(g);
+  g = sc_dpp_add<GDR_DPP_ROW_SHR(8), 0xF>(g);
+  g = sc_dpp_add<GDR_DPP_ROW_BCAST15, 0xA>(g);
+  g = sc_dpp_add<GDR_DPP_ROW_BCAST31, 0xC>(g);
+  const double end = __shfl(g, 63);
+  const float rounded = (float)g;
+  d.gamma[lane] = rounded;
+  d.rest[lane] = __builtin_amdgcn_exp2f((float)(g - (double)rounded));
   d.delta[lane] = delta;
-  d.grow[lane] = __builtin_amdgcn_exp2f(gamma * SC_LOG2E);
-  d.left[lane] = __builtin_amdgcn_exp2f((end - gamma) * SC_LOG2E);
+  d.grow[lane] = __builtin_amdgcn_exp2f(rounded);
+  d.left[lane] = __builtin_amdgcn_exp2f((float)(end - g));
   if (lane == 63) {
-    d.end = __builtin_amdgcn_exp2f(end * SC_LOG2E);
-    d.sum = end;
+    d.end = __builtin_amdgcn_exp2f((float)end);
+    d.sum = (float)end;
   }
 }
 

@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
     // S in front of the chunk: columns p of this wave's rows n, as the lane's share of an operand
     f32x4 S[NW][4];
     if (has_n) {
-      const f32x4* kept = reinterpret_cast<const f32x4*>(w.chunk_states + ((seg.chunk0 + c) * parts + blockIdx.y) * (NP * 64));
+      const f32x4* kept = reinterpret_cast<const f32x4*>(w.chunk_states + ((ss_row_of(seg, 64) + c) * parts + blockIdx.y) * (NP * 64));
 #pragma unroll
       for (int j = 0; j < NW; ++j)
 #pragma unroll
@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
     // Pair weights of tokens s = 16 wave + i with t = s ..: rows of m1 (L G) and m2 (delta_s L H), and the sums of their product.
     {
       const int s = 16 * wave + i;
-      const float gs = dec.gamma[s], ds = dec.delta[s];
+      // The exponents' rounding (2^rest) matters to the sums only: theirs of t goes in element by element, that of s at the end.
+      const float gs = dec.gamma[s], ds = dec.delta[s], rest_s = 1.0f / dec.rest[s], ds_rest = ds * rest_s;
       x8 qb[KK], qx[2];
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) qb[kk] = *reinterpret_cast<const x8*>(tb + s * KS + 32 * kk + 8 * g);
@@ -134,15 +135,16 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) Hm = mfma16(*reinterpret_cast<const x8*>(ty + (16 * tt + i) * VS + 32 * kk + 8 * g), qx[kk], Hm);
           const f32x4 gt = *reinterpret_cast<const f32x4*>(dec.gamma + 16 * tt + 4 * g);
+          const f32x4 rest = *reinterpret_cast<const f32x4*>(dec.rest + 16 * tt + 4 * g);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int t = 16 * tt + 4 * g + r;
             const float l = __builtin_amdgcn_exp2f(gt[r] - gs);
-            const float vg = t >= s ? l * G[r] : 0.0f, both = t >= s ? vg * Hm[r] : 0.0f;
+            const float vg = t >= s ? l * G[r] : 0.0f, both = t >= s ? vg * Hm[r] * rest[r] : 0.0f;
             lg[tt][r] = vg;
             lh[tt][r] = t >= s ? ds * l * Hm[r] : 0.0f;
             if (t == s) own = both; else sum += both;
-            rows[r] = sc_row16_sum(t == s ? 0.0f : ds * both);
+            rows[r] = sc_row16_sum(t == s ? 0.0f : ds_rest * both);
             if (F16) { big1 = fmaxf(big1, fabsf(vg)); big2 = fmaxf(big2, fabsf(lh[tt][r])); }
           }
         }
@@ -152,7 +154,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
       sum += __shfl_xor(sum, 32);
       own += __shfl_xor(own, 16);  // one lane of the four has it
       own += __shfl_xor(own, 32);
-      if (g == 0) { col_sum[s] = sum; diag[s] = own; }
+      if (g == 0) { col_sum[s] = sum * rest_s; diag[s] = own * rest_s; }
       if constexpr (F16) {
         big1 = fmaxf(big1, __shfl_xor(big1, 16));
         big1 = fmaxf(big1, __shfl_xor(big1, 32));

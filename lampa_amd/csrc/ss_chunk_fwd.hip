@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
     const int64_t t0 = seg.t0 + 64 * (REV ? chunks - 1 - c : c);
     const int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
     if (KEEP) {
-      float* keep = w.chunk_states + ((seg.chunk0 + c) * a.H * npb + blockIdx.y) * (NP * 64);
+      float* keep = w.chunk_states + ((ss_row_of(seg, 64) + c) * a.H * npb + blockIdx.y) * (NP * 64);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
       const int n = 16 * nt + 4 * g + r;
       if (n < a.N && p < a.P) local[(int64_t)n * a.P + p] = S[nt][r];
     }
-  if (!REV && threadIdx.x == 0 && pb == 0) a.slot_decay[(int64_t)blockIdx.x * a.H + h] = expf(sum);
+  if (!REV && threadIdx.x == 0 && pb == 0) a.slot_decay[(int64_t)blockIdx.x * a.H + h] = __builtin_amdgcn_exp2f(sum);
 }
 
 // Outputs of a segment from the state it starts from.

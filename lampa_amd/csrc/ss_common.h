@@ -23,7 +23,7 @@
 struct SsSegment {
   int64_t t0, t1;   // tokens of this segment
   int seq, index;   // sequence, place of the segment in it
-  int64_t chunk0;   // row of its first 64 tokens in tables with a row for every 64 tokens of a sequence
+  int64_t begin;    // first token of the sequence
   bool live;        // false: this slot holds no segment
   bool first, last; // in its sequence
   bool outside;     // rows behind the last sequence: their outputs are zero
@@ -71,7 +71,7 @@ __device__ __forceinline__ SsSegment ss_segment(const lampa_ss_args& a, int64_t 
   s.t0 = b + (int64_t)s.index * a.seg_tokens;
   s.t1 = s.t0 + a.seg_tokens < e ? s.t0 + a.seg_tokens : e;
   if (s.t1 < s.t0) s.t1 = s.t0;
-  s.chunk0 = b / 64 + s.seq + (int64_t)s.index * (a.seg_tokens / 64);
+  s.begin = b;
   s.first = s.index == 0;
   s.last = s.t1 >= e;
   return s;
@@ -82,6 +82,10 @@ template <typename T>
 __device__ __forceinline__ float ss_load_dt(const void* dt, int dt_dtype, int64_t i) {
   return dt_dtype == GDR_FP32 ? ((const float*)dt)[i] : GdrElem<T>::to_float(((const T*)dt)[i]);
 }
+// Row of a segment's first tokens in a table with one row for every `every` tokens of a sequence (a divisor of 64): sequence i
+// takes its rows from floor(begin / every) + i on, as it takes its slots.
+__device__ __forceinline__ int64_t ss_row_of(const SsSegment& s, int every) { return s.begin / every + s.seq + (s.t0 - s.begin) / every; }
+
 __device__ __forceinline__ float ss_delta(float raw, float bias, int softplus) {
   const float x = raw + bias;
   return softplus ? (x > 20.0f ? x : log1pf(expf(x))) : x;
@@ -105,8 +109,7 @@ static inline int64_t ss_slots(const lampa_ss_args* a) {
   if (!a->cu_seqlens) return (int64_t)a->n_seq * ((a->seq_len + a->seg_tokens - 1) / a->seg_tokens);
   return a->n_tokens / a->seg_tokens + a->n_seq + 1;
 }
-// Rows of a table with one for every 64 tokens of a sequence: sequence i takes them from floor(begin / 64) + i on.
-static inline int64_t ss_chunk_rows(const lampa_ss_args* a) { return a->n_tokens / 64 + a->n_seq + 1; }
+static inline int64_t ss_rows(const lampa_ss_args* a, int every) { return a->n_tokens / every + a->n_seq + 1; }  // of ss_row_of's tables
 // One segment holds any sequence: no scan over segments, the walks start from h0 and leave the final states themselves.
 static inline bool ss_single(const lampa_ss_args* a) {
   return (a->cu_seqlens ? a->n_tokens : a->seq_len) <= a->seg_tokens;

@@ -3,14 +3,16 @@
 #pragma once
 #include "ss_common.h"
 
+#define SS_DOT 16  // tokens between two places where the token-serial gradients form <R, S>
+
 struct SsGrad {
   float* adjoints;           // [slots, H, N, P]: the segments' local adjoints, then the adjoint at each segment's end
   float *dB_part, *dC_part;  // [tokens, H * blocks, N]: one part for each head and block of 64 columns of x
   float* dg;                 // [tokens, H, blocks]: the decay exponent's gradient (chunks), or dy_t . (S_t^T C_t) (token-serial)
   float* reach;              // [tokens, H, blocks]: x_t . (R_t^T B_t)
   float* chunk_states;       // chunks: the state in front of every 64 tokens, [rows, H, blocks, N padded, 64]
-                             // token-serial: the state behind them, [rows, H, N, P]
-  float* chunk_dots;         // token-serial: <R, S> behind every 64 tokens, [rows, H, blocks]
+                             // token-serial: the state behind every SS_DOT, [rows, H, N, P]
+  float* chunk_dots;         // token-serial: <R, S> behind every SS_DOT tokens, [rows, H, blocks]
   float* param_part;         // [slots, H, 2]: a segment's share of dA and d dt_bias
   float* dD_part;            // [slots, H, blocks]
 };

@@ -51,9 +51,9 @@ static int ss_join(const lampa_ss_args& a, float* states, const float* init, flo
 }
 
 // From the gradient of the decays to those of dt, A and dt_bias. One workgroup a segment and head; a wave takes 64 tokens at a
-// time, a lane one of them. Where dg has not been summed up yet (fp32), it is here, from the end of the 64 tokens:
-// dg_t = dg_{t+1} + read_t - delta_t reach_t, behind the last of them <R, S>. Starting anew every 64 tokens keeps rounding errors
-// of the sum, which pass on to every earlier token of it, from adding up over a segment (dA off by 2.5e-5 then, 60 000 tokens).
+// time, a lane one of them. Where dg has not been summed up yet (fp32), it is here, SS_DOT tokens at a time from their end:
+// dg_t = dg_{t+1} + read_t - delta_t reach_t, behind the last of them <R, S>. Starting anew that often keeps rounding errors of
+// the sum, which pass on to every earlier token of it, from adding up (dA off by 2.5e-5 over segments of 256 tokens, 6e-6 over 64).
 template <typename T>
 __global__ void __launch_bounds__(SS_BLOCK) ss_decay_grad_kernel(lampa_ss_args a, SsGrad w, bool summed) {
   const SsSegment seg = ss_segment(a, blockIdx.x);
@@ -75,12 +75,12 @@ __global__ void __launch_bounds__(SS_BLOCK) ss_decay_grad_kernel(lampa_ss_args a
     if (!summed && !seg.outside) {
       if (on) dg -= delta * reach;
 #pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
+      for (int off = 1; off < SS_DOT; off <<= 1) {
         const float later = __shfl_down(dg, off);
-        if (lane + off < 64) dg += later;
+        if (lane % SS_DOT + off < SS_DOT) dg += later;
       }
-      const int64_t row = (seg.chunk0 + (t0 - seg.t0) / 64) * a.H + h;
-      for (int i = 0; i < npb; ++i) dg += w.chunk_dots[row * npb + i];
+      const int64_t row = (ss_row_of(seg, SS_DOT) + (tok - seg.t0) / SS_DOT) * a.H + h;
+      for (int i = 0; on && i < npb; ++i) dg += w.chunk_dots[row * npb + i];
     }
     if (tok < seg.t1) {
       float d = on ? __builtin_fmaf(A, dg, reach) : 0.0f;
@@ -185,8 +185,8 @@ static int64_t ss_grad_layout(const lampa_ss_args& a, char* base, SsGrad* w) {
   const bool serial = a.dtype == GDR_FP32;
   take(g.dg, a.n_tokens * a.H * npb * (serial ? nnb : 1));
   take(g.reach, a.n_tokens * a.H * npb);
-  take(g.chunk_states, ss_chunk_rows(&a) * a.H * (serial ? (int64_t)a.N * a.P : npb * ss_chunk_n(a.N) * 64));
-  take(g.chunk_dots, serial ? ss_chunk_rows(&a) * a.H * npb : 0);
+  take(g.chunk_states, ss_rows(&a, serial ? SS_DOT : 64) * a.H * (serial ? (int64_t)a.N * a.P : npb * ss_chunk_n(a.N) * 64));
+  take(g.chunk_dots, serial ? ss_rows(&a, SS_DOT) * a.H * npb : 0);
   take(g.param_part, slots * a.H * 2);
   take(g.dD_part, slots * a.H * npb);
   if (w) *w = g;

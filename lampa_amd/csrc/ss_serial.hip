@@ -134,8 +134,8 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
         const float s = REV ? carry : decay;
         if constexpr (KIND == SS_DX && !MAP) {
           const int64_t done = tok + 1 - seg.t0;
-          if (done % 64 == 0 || tok + 1 == seg.t1) {  // S times the last decay is the adjoint behind this token
-            const int64_t row = (seg.chunk0 + (done - 1) / 64) * a.H + h;
+          if (done % SS_DOT == 0 || tok + 1 == seg.t1) {  // S times the last decay is the adjoint behind this token
+            const int64_t row = (ss_row_of(seg, SS_DOT) + (done - 1) / SS_DOT) * a.H + h;
             const float* kept = w.chunk_states + row * per_h;
             float dot = 0.0f;
 #pragma unroll
@@ -170,10 +170,10 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
           if (lane_on) w.dC_part[(tok * a.H * npb + h * npb + pb) * a.N + l] = out;
           const float u = ss_wave_sum(lane_on && !seg.outside ? le[t][lane] * out : 0.0f);
           if (lane == 0) w.dg[((tok * a.H + h) * npb + pb) * nnb + lane_block] = u;
-          // the state behind every 64 tokens (and behind the last one), for <R, S> there
+          // the state behind every SS_DOT tokens (and behind the last one), for <R, S> there
           const int64_t done = tok + 1 - seg.t0;
-          if (!seg.outside && (done % 64 == 0 || tok + 1 == seg.t1)) {
-            float* keep = w.chunk_states + ((seg.chunk0 + (done - 1) / 64) * a.H + h) * per_h;
+          if (!seg.outside && (done % SS_DOT == 0 || tok + 1 == seg.t1)) {
+            float* keep = w.chunk_states + ((ss_row_of(seg, SS_DOT) + (done - 1) / SS_DOT) * a.H + h) * per_h;
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
               if (lane_on && r < rn) keep[at(r)] = S[r];
