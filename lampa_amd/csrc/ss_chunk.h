@@ -50,24 +50,39 @@ __device__ __forceinline__ float sc_wave_max(float v) {
   return v;
 }
 
+// The compiler moves nothing across: left alone it requests the operands of many products at once and runs out of registers.
+__device__ __forceinline__ void sc_fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// The lane's number, as a value the compiler knows nothing about: addresses and comparisons made from it are formed anew in every
+// turn of a loop instead of being kept in registers all through it.
+__device__ __forceinline__ int sc_fresh(int lane) {
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
 // One thread's share of a [64, W] tile on its way from memory to LDS. Rows from `n` on and columns from `cols` on are zero.
 template <typename T, int W>
 struct ScTile {
   sc_x8<T> v[W / 32];
-  __device__ __forceinline__ void fetch(const T* base, int64_t stride, int64_t t0, int n, int cols, bool vec) {
+  // `base`: column 0 of row 0, the same in the whole workgroup, as are stride and n: a row's address is a scalar and the lane's
+  // offset within 32 bits, one for all rows (64-bit pointers of their own for each would cost more registers than the state).
+  template <bool VEC>
+  __device__ __forceinline__ void fetch(const T* base, int64_t stride, int n, int cols) {
+    const int row0 = threadIdx.x / (W / 8), c = threadIdx.x % (W / 8) * 8;
+    const unsigned off = (unsigned)(row0 * (int)stride + c) * (unsigned)sizeof(T);
 #pragma unroll
     for (int k = 0; k < W / 32; ++k) {
-      const int q = threadIdx.x + SC_BLOCK * k, row = q / (W / 8), c = q % (W / 8) * 8;
+      const int row = row0 + k * (2048 / W);
+      const char* p = reinterpret_cast<const char*>(base + (int64_t)(k * (2048 / W)) * stride);
       sc_x8<T> x;
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = (T)0.0f;
       if (row < n && c < cols) {
-        const T* p = base + (t0 + row) * stride + c;
-        if (vec) x = *reinterpret_cast<const sc_x8<T>*>(p);
+        if constexpr (VEC) x = *reinterpret_cast<const sc_x8<T>*>(p + off);
         else
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (c + e < cols) x[e] = p[e];
+            if (c + e < cols) x[e] = *reinterpret_cast<const T*>(p + (off + e * (unsigned)sizeof(T)));
       }
       v[k] = x;
     }
@@ -106,8 +121,7 @@ struct ScTile {
 // head decays fast, and the exponents of neighbouring tokens are differences of it, which have to be right to 2^-24 for dA and
 // d dt_bias, sums over all tokens, to be.
 struct ScDecay {
-  float gamma[64];  // gamma_t log2(e), rounded ...
-  float rest[64];   // ... and 2 to the power of what the rounding left out
+  float gamma[64];  // gamma_t log2(e), rounded (what that leaves out goes to `rest`, as 2 to its power)
   float delta[64];
   float grow[64];   // e^{gamma_t}
   float left[64];   // e^{gamma_end - gamma_t}
@@ -122,7 +136,7 @@ __device__ __forceinline__ double sc_dpp_add(double x) {
   return x + __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 // One wave, lane = token; tokens from n on have no step.
-__device__ __forceinline__ void sc_decays(ScDecay& d, float raw, int n, float bias, float A, int softplus) {
+__device__ __forceinline__ void sc_decays(ScDecay& d, float* rest, float raw, int n, float bias, float A, int softplus) {
   const int lane = lane_id();
   const float delta = lane < n ? ss_delta(raw, bias, softplus) : 0.0f;
   double g = 0.0;
@@ -139,7 +153,7 @@ __device__ __forceinline__ void sc_decays(ScDecay& d, float raw, int n, float bi
   const double end = __shfl(g, 63);
   const float rounded = (float)g;
   d.gamma[lane] = rounded;
-  d.rest[lane] = __builtin_amdgcn_exp2f((float)(g - (double)rounded));
+  if (rest) rest[lane] = __builtin_amdgcn_exp2f((float)(g - (double)rounded));
   d.delta[lane] = delta;
   d.grow[lane] = __builtin_amdgcn_exp2f(rounded);
   d.left[lane] = __builtin_amdgcn_exp2f((float)(end - g));
@@ -149,15 +163,21 @@ __device__ __forceinline__ void sc_decays(ScDecay& d, float raw, int n, float bi
   }
 }
 
+// Element (n, p) of a state [N, P], zero outside; the address is held inside, so that loads need no branch.
+__device__ __forceinline__ float sc_state_at(const float* state, int n, int p, int N, int P) {
+  const float v = state[(unsigned)((n < N ? n : N - 1) * P + (p < P ? p : P - 1))];
+  return n < N && p < P ? v : 0.0f;
+}
+
 // Columns 16 w .. of a 64-row tile as an operand of the products over its rows (rows 32 kk ..): one for each kk.
 template <typename T>
-__device__ __forceinline__ void sc_columns(const T* tile, int stride, int col0, sc_x8<T> (&out)[2]) {
+__device__ __forceinline__ void sc_columns(const T* tile, int stride, int col0, int lane, sc_x8<T> (&out)[2]) {
 #pragma unroll
-  for (int kk = 0; kk < 2; ++kk) out[kk] = op_ld_tr16<T, true>(tile, stride, col0, 32 * kk, lane_id());
+  for (int kk = 0; kk < 2; ++kk) out[kk] = op_ld_tr16<T, true>(tile, stride, col0, 32 * kk, lane);
 }
 // The weights of a lane's rows in such an operand.
-__device__ __forceinline__ void sc_row_weights(const float* w, int kk, float (&out)[8]) {
-  const int g = lane_id() >> 4;
+__device__ __forceinline__ void sc_row_weights(const float* w, int kk, int lane, float (&out)[8]) {
+  const int g = lane >> 4;
   const f32x4 a = *reinterpret_cast<const f32x4*>(w + 32 * kk + 4 * g), b = *reinterpret_cast<const f32x4*>(w + 32 * kk + 16 + 4 * g);
 #pragma unroll
   for (int e = 0; e < 4; ++e) { out[e] = a[e]; out[4 + e] = b[e]; }
@@ -186,21 +206,12 @@ __device__ __forceinline__ void sc_state_operand(const f32x4& a, const f32x4& b,
   }
 }
 
-struct ScFlags {
-  bool x, B, C, dy;  // rows that can be read in 16-byte pieces
-  bool y, dx;        // rows that can be written in 8-byte pieces
-};
-
-static ScFlags sc_flags(const lampa_ss_args& a) {
+// Whether every row of a call can be read in 16-byte pieces and written in 8-byte ones (the kernels are built for both: their
+// loads element by element would cost the others registers).
+static bool sc_vectors(const lampa_ss_args& a) {
   auto rows = [](const void* p, int64_t stride, int inner) { return (uintptr_t)p % 16 == 0 && stride % 8 == 0 && inner % 8 == 0; };
-  ScFlags f;
-  f.x = rows(a.x, a.x_stride, a.P);
-  f.B = rows(a.B, a.B_stride, a.N);
-  f.C = rows(a.C, a.C_stride, a.N);
-  f.dy = a.dy && rows(a.dy, (int64_t)a.H * a.P, a.P);
-  f.dx = (uintptr_t)a.dx % 8 == 0 && a.P % 4 == 0;
-  f.y = (uintptr_t)a.y % 8 == 0 && a.y_stride % 4 == 0 && a.P % 4 == 0;
-  return f;
+  return rows(a.x, a.x_stride, a.P) && rows(a.B, a.B_stride, a.N) && rows(a.C, a.C_stride, a.N) && rows(a.dy, 8, a.P) &&
+         rows(a.dx, 8, a.P) && (uintptr_t)a.y % 8 == 0 && a.y_stride % 4 == 0;
 }
 
 // Slots along x in a multiple of 8: workgroups are dealt to the 8 dies in turn, so the heads of a segment, which read the same

@@ -19,8 +19,8 @@
 // over p; summing it up twice costs fewer cycles than passing it through LDS.
 #include "ss_chunk.h"
 
-template <typename T, int NP>
-__global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, SsGrad w, ScFlags f) {
+template <typename T, int NP, bool VEC>
+__global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, SsGrad w) {
   constexpr int NT = NP / 16, KK = NP / 32, KS = NP + 8, VS = 64 + 8, MS = 64 + 8;
   constexpr int NW = NP == 128 ? 2 : 1;  // tiles of 16 columns n a wave has of dB, dC and the transposed R
   constexpr bool F16 = __is_same(T, _Float16);
@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
   const SsSegment seg = ss_segment(a, blockIdx.x);
   if (!seg.live) return;
   const int npb = (a.P + 63) / 64, pb = blockIdx.y % npb, h = blockIdx.y / npb, grp = h / (a.H / a.G);
-  const int lane = lane_id(), wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  const int lane0 = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cols = a.P - 64 * pb < 64 ? a.P - 64 * pb : 64;
   const int64_t row_p = (int64_t)a.H * a.P, parts = (int64_t)a.H * npb;
   T* dxb = (T*)a.dx + (int64_t)h * a.P + 64 * pb;
@@ -46,6 +46,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
   __shared__ __align__(16) T tb[64 * KS], tc[64 * KS], tx[64 * VS], ty[64 * VS], m1[64 * MS], m2[64 * MS];
   __shared__ __align__(16) ScDecay dec;
   __shared__ __align__(16) float row_part[4][64], col_sum[64], diag[64], left_part[4][64], read_part[4][64], dot_part[4];
+  __shared__ __align__(16) float rest2[64];
   __shared__ float back1[64], back2[64];  // fp16: what the rows of m1 and m2 were scaled down by
   const T* bb = (const T*)a.B + (int64_t)grp * a.N;
   const T* cb = (const T*)a.C + (int64_t)grp * a.N;
@@ -53,31 +54,33 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
   const T* yb = (const T*)a.dy + (int64_t)h * a.P + 64 * pb;
   const float A = a.A[h], D = a.D ? a.D[h] : 0.0f, bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
   const bool single = (a.cu_seqlens ? a.n_tokens : a.seq_len) <= a.seg_tokens;
-  const int p = 64 * pb + 16 * wave + i;
   const int nt0 = NW * wave;        // this wave's tiles of columns n
   const bool has_n = nt0 < NT;      // (a state of 32 has two of them only)
-  const bool part_vec = a.N % 4 == 0;
 
   f32x4 R[NT], RT[4][NW];
+  {
+  const int lane = lane0, g = lane >> 4, i = lane & 15, p = 64 * pb + 16 * wave + i;
   const float* init = single ? a.dht : w.adjoints;
   if (init) init += ((single ? (int64_t)seg.seq : (int64_t)blockIdx.x) * a.H + h) * a.N * a.P;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int n = 16 * nt + 4 * g + r;
-      R[nt][r] = init && n < a.N && p < a.P ? init[(int64_t)n * a.P + p] : 0.0f;
-    }
+  for (int nt = 0; nt < NT; ++nt) R[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int pt = 0; pt < 4; ++pt)
 #pragma unroll
-    for (int j = 0; j < NW; ++j)
+    for (int j = 0; j < NW; ++j) RT[pt][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (init) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = 16 * (nt0 + j) + i, q = 64 * pb + 16 * pt + 4 * g + r;
-        RT[pt][j][r] = init && n < a.N && q < a.P ? init[(int64_t)n * a.P + q] : 0.0f;
-      }
-
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) R[nt][r] = sc_state_at(init, 16 * nt + 4 * g + r, p, a.N, a.P);
+#pragma unroll
+    for (int pt = 0; pt < 4; ++pt)
+#pragma unroll
+      for (int j = 0; j < NW; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) RT[pt][j][r] = sc_state_at(init, 16 * (nt0 + j) + i, 64 * pb + 16 * pt + 4 * g + r, a.N, a.P);
+  }
+  }
   ScTile<T, NP> pB, pC;
   ScTile<T, 64> pX, pY;
   float pdt = 0.0f, dD = 0.0f;
@@ -85,38 +88,33 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
   auto fetch = [&](int64_t c) {
     const int64_t t0 = seg.t0 + 64 * c;
     const int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
-    pB.fetch(bb, a.B_stride, t0, n, a.N, f.B);
-    pC.fetch(cb, a.C_stride, t0, n, a.N, f.C);
-    pX.fetch(xb, a.x_stride, t0, n, cols, f.x);
-    pY.fetch(yb, row_p, t0, n, cols, f.dy);
-    if (wave == 0 && lane < n) pdt = ss_load_dt<T>(a.dt, a.dt_dtype, (t0 + lane) * a.dt_stride + h);
+    pB.template fetch<VEC>(bb + t0 * a.B_stride, a.B_stride, n, a.N);
+    pC.template fetch<VEC>(cb + t0 * a.C_stride, a.C_stride, n, a.N);
+    pX.template fetch<VEC>(xb + t0 * a.x_stride, a.x_stride, n, cols);
+    pY.template fetch<VEC>(yb + t0 * row_p, row_p, n, cols);
+    if (wave == 0 && lane0 < n) pdt = ss_load_dt<T>(a.dt, a.dt_dtype, (t0 + lane0) * a.dt_stride + h);
   };
-  if (chunks) fetch(chunks - 1);
+  // A wide state leaves no registers for the next chunk's tiles: they are fetched when they are due, and the other workgroup of
+  // the CU works meanwhile.
+  constexpr bool AHEAD = NP <= 64;
+  if (AHEAD && chunks) fetch(chunks - 1);
   for (int64_t c = chunks - 1; c >= 0; --c) {
+    const int lane = sc_fresh(lane0), g = lane >> 4, i = lane & 15;
     const int64_t t0 = seg.t0 + 64 * c;
     const int n_tok = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
+    if (!AHEAD) fetch(c);
     pB.put(tb, KS);
     pC.put(tc, KS);
     pX.put(tx, VS);
     pY.put(ty, VS);
-    if (wave == 0) sc_decays(dec, pdt, n_tok, bias, A, a.softplus);
+    if (wave == 0) sc_decays(dec, rest2, pdt, n_tok, bias, A, a.softplus);
     lds_barrier();
-    if (c > 0) fetch(c - 1);
-    // S in front of the chunk: columns p of this wave's rows n, as the lane's share of an operand
-    f32x4 S[NW][4];
-    if (has_n) {
-      const f32x4* kept = reinterpret_cast<const f32x4*>(w.chunk_states + ((ss_row_of(seg, 64) + c) * parts + blockIdx.y) * (NP * 64));
-#pragma unroll
-      for (int j = 0; j < NW; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) S[j][q] = kept[((nt0 + j) * 4 + q) * 64 + lane];
-    }
-
+    if (AHEAD && c > 0) fetch(c - 1);
     // Pair weights of tokens s = 16 wave + i with t = s ..: rows of m1 (L G) and m2 (delta_s L H), and the sums of their product.
     {
       const int s = 16 * wave + i;
       // The exponents' rounding (2^rest) matters to the sums only: theirs of t goes in element by element, that of s at the end.
-      const float gs = dec.gamma[s], ds = dec.delta[s], rest_s = 1.0f / dec.rest[s], ds_rest = ds * rest_s;
+      const float gs = dec.gamma[s], ds = dec.delta[s], rest_s = 1.0f / rest2[s], ds_rest = ds * rest_s;
       x8 qb[KK], qx[2];
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) qb[kk] = *reinterpret_cast<const x8*>(tb + s * KS + 32 * kk + 8 * g);
@@ -126,6 +124,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
       float sum = 0.0f, own = 0.0f, big1 = 0.0f, big2 = 0.0f;
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
+        sc_fence();
         lg[tt] = lh[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         f32x4 rows = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (tt >= wave) {
@@ -135,7 +134,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) Hm = mfma16(*reinterpret_cast<const x8*>(ty + (16 * tt + i) * VS + 32 * kk + 8 * g), qx[kk], Hm);
           const f32x4 gt = *reinterpret_cast<const f32x4*>(dec.gamma + 16 * tt + 4 * g);
-          const f32x4 rest = *reinterpret_cast<const f32x4*>(dec.rest + 16 * tt + 4 * g);
+          const f32x4 rest = *reinterpret_cast<const f32x4*>(rest2 + 16 * tt + 4 * g);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int t = 16 * tt + 4 * g + r;
@@ -175,11 +174,20 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
     }
     lds_barrier();
 
+    sc_fence();
+    // S in front of the chunk: columns p of this wave's rows n, as the lane's share of an operand, a tile of rows at a time
+    f32x4 S[4];
+    const f32x4* kept = reinterpret_cast<const f32x4*>(w.chunk_states + ((ss_row_of(seg, 64) + c) * parts + blockIdx.y) * (NP * 64));
+    if (has_n) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) S[q] = kept[(nt0 * 4 + q) * 64 + lane];
+    }
+
     const float end = dec.end;
     // dx of this wave's 16 columns: lane = token 16 st + i, registers = columns 4 g .. + 3
     {
       x8 vy[2];
-      sc_columns<T>(ty, VS, 16 * wave, vy);
+      sc_columns<T>(ty, VS, 16 * wave, lane, vy);
       float sc = 1.0f, sback = 1.0f;
       if constexpr (F16) {
         float big = 0.0f;
@@ -195,6 +203,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
       for (int st = 0; st < 4; ++st) acc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
+        sc_fence();
         x8 hi, lo;
         sc_state_operand<T>(R[2 * kk], R[2 * kk + 1], sc, hi, lo);
 #pragma unroll
@@ -205,6 +214,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
       }
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
+        sc_fence();
         const int s = 16 * st + i;
         acc[st] *= F16 ? dec.left[s] * sback : dec.left[s];
         const int at = s * VS + op_perm32_col(16 * wave + 4 * g);
@@ -230,8 +240,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[r] = (T)__builtin_fmaf(ds, near[r], D * (float)dyv[r]);
           const int c0 = 16 * wave + 4 * g;
-          T* dst = dxb + (t0 + s) * row_p + c0;
-          if (f.dx) {
+          T* dst = reinterpret_cast<T*>(reinterpret_cast<char*>(dxb + (t0 + 16 * st) * row_p) + (unsigned)(i * (int)row_p + c0) * (unsigned)sizeof(T));
+          if constexpr (VEC) {
             if (c0 < cols) *reinterpret_cast<x4*>(dst) = o;
           } else {
 #pragma unroll
@@ -241,14 +251,13 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
         }
       }
     }
+    sc_fence();
     // dB and dC of this wave's columns n: lane = token, registers = columns 4 g .. + 3 of a tile
     float dot = 0.0f;
     if (has_n) {
 #pragma unroll
       for (int j = 0; j < NW; ++j) {
-        x8 vb[2], vc[2];
-        sc_columns<T>(tb, KS, 16 * (nt0 + j), vb);
-        sc_columns<T>(tc, KS, 16 * (nt0 + j), vc);
+        sc_fence();
         float s1 = 1.0f, b1 = 1.0f, s2 = 1.0f, b2 = 1.0f;
         if constexpr (F16) {
           float big1 = 0.0f, big2 = 0.0f;
@@ -257,7 +266,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               big1 = fmaxf(big1, fabsf(RT[q][j][r]));
-              big2 = fmaxf(big2, fabsf(S[j][q][r]));
+              big2 = fmaxf(big2, fabsf(S[q][r]));
             }
           s1 = sc_scale_for<T>(sc_wave_max(big1));
           b1 = sc_inverse(s1);
@@ -269,6 +278,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
         for (int st = 0; st < 4; ++st) db[st] = dc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
+          sc_fence();
           x8 hi, lo;
           sc_state_operand<T>(RT[2 * kk][j], RT[2 * kk + 1][j], s1, hi, lo);
 #pragma unroll
@@ -276,7 +286,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
             const x8 q = *reinterpret_cast<const x8*>(tx + (16 * st + i) * VS + 32 * kk + 8 * g);
             db[st] = mfma16(hi, q, mfma16(lo, q, db[st]));
           }
-          sc_state_operand<T>(S[j][2 * kk], S[j][2 * kk + 1], s2, hi, lo);
+          sc_fence();
+          sc_state_operand<T>(S[2 * kk], S[2 * kk + 1], s2, hi, lo);
 #pragma unroll
           for (int tt = 0; tt < 4; ++tt) {
             const x8 q = *reinterpret_cast<const x8*>(ty + (16 * tt + i) * VS + 32 * kk + 8 * g);
@@ -286,10 +297,19 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) dot = __builtin_fmaf(RT[q][j][r], S[j][q][r], dot);
+          for (int r = 0; r < 4; ++r) dot = __builtin_fmaf(RT[q][j][r], S[q][r], dot);
+        if (j + 1 < NW) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) S[q] = kept[((nt0 + j + 1) * 4 + q) * 64 + lane];
+        }
+        sc_fence();
+        x8 vb[2], vc[2];
+        sc_columns<T>(tb, KS, 16 * (nt0 + j), lane, vb);
+        sc_columns<T>(tc, KS, 16 * (nt0 + j), lane, vc);
         const int c0 = 16 * (nt0 + j) + 4 * g;
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
+          sc_fence();
           const int s = 16 * st + i;
           db[st] *= dec.left[s] * dec.delta[s] * b1;
           if constexpr (F16) {
@@ -327,18 +347,21 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
               }
             }
           if (s < n_tok) {
-            const int64_t at = ((t0 + s) * parts + blockIdx.y) * a.N + c0;
-            if (part_vec) {
+            const int64_t row = ((t0 + 16 * st) * parts + blockIdx.y) * a.N;
+            const unsigned at = (unsigned)(i * (int)(parts * a.N) + c0) * 4u;
+            float* pdb = reinterpret_cast<float*>(reinterpret_cast<char*>(w.dB_part + row) + at);
+            float* pdc = reinterpret_cast<float*>(reinterpret_cast<char*>(w.dC_part + row) + at);
+            if constexpr (VEC) {
               if (c0 < a.N) {
-                *reinterpret_cast<f32x4*>(w.dB_part + at) = db[st];
-                *reinterpret_cast<f32x4*>(w.dC_part + at) = dc[st];
+                *reinterpret_cast<f32x4*>(pdb) = db[st];
+                *reinterpret_cast<f32x4*>(pdc) = dc[st];
               }
             } else {
 #pragma unroll
               for (int r = 0; r < 4; ++r)
                 if (c0 + r < a.N) {
-                  w.dB_part[at + r] = db[st][r];
-                  w.dC_part[at + r] = dc[st][r];
+                  pdb[r] = db[st][r];
+                  pdc[r] = dc[st][r];
                 }
             }
           }
@@ -350,12 +373,13 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
     dot = ss_wave_sum(dot);
     if (lane == 0) dot_part[wave] = dot;
 
+    sc_fence();
     // R in front of the chunk, both ways round. (fp16: the decayed operands' weights are at most about 1; where the chunk's
     // first token decays strongly they are all small, so they are scaled by the largest, which is the first.)
     {
       float wt[2][8], back = 1.0f;
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) sc_row_weights(dec.grow, kk, wt[kk]);
+      for (int kk = 0; kk < 2; ++kk) sc_row_weights(dec.grow, kk, lane, wt[kk]);
       if constexpr (F16) {
         float m = 0.0f;
 #pragma unroll
@@ -384,25 +408,28 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
         }
       };
       x8 v[2], hi[2], lo[2], left[2];
-      sc_columns<T>(ty, VS, 16 * wave, v);
+      sc_columns<T>(ty, VS, 16 * wave, lane, v);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) sc_weighted<T>(v[kk], wt[kk], hi[kk], lo[kk]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        sc_columns<T>(tc, KS, 16 * nt, left);
+        sc_columns<T>(tc, KS, 16 * nt, lane, left);
         add(R[nt], left, hi, lo);
+        sc_fence();
       }
       if (has_n) {
 #pragma unroll
         for (int j = 0; j < NW; ++j) {
-          sc_columns<T>(tc, KS, 16 * (nt0 + j), v);
+          sc_columns<T>(tc, KS, 16 * (nt0 + j), lane, v);
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) sc_weighted<T>(v[kk], wt[kk], hi[kk], lo[kk]);
 #pragma unroll
           for (int pt = 0; pt < 4; ++pt) {
-            sc_columns<T>(ty, VS, 16 * pt, left);
+            sc_columns<T>(ty, VS, 16 * pt, lane, left);
             add(RT[pt][j], left, hi, lo);
+            sc_fence();
           }
+          sc_fence();
         }
       }
     }
@@ -431,6 +458,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
       }
     }
   }
+  const int lane = lane0, g = lane >> 4, i = lane & 15, p = 64 * pb + 16 * wave + i;
   // shares of dD: every wave has its own columns
   dD = ss_wave_sum(dD);
   lds_barrier();
@@ -449,16 +477,16 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
   }
 }
 
-template <typename T>
+template <typename T, bool VEC>
 static int sc_grad_launch(const lampa_ss_args& a, const SsGrad& w, hipStream_t s) {
-  const ScFlags f = sc_flags(a);
   LAMPA_PROF(s, "start");
-  if (a.N <= 32) hipLaunchKernelGGL((sc_grad_kernel<T, 32>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f);
-  else if (a.N <= 64) hipLaunchKernelGGL((sc_grad_kernel<T, 64>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f);
-  else hipLaunchKernelGGL((sc_grad_kernel<T, 128>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f);
+  if (a.N <= 32) hipLaunchKernelGGL((sc_grad_kernel<T, 32, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w);
+  else if (a.N <= 64) hipLaunchKernelGGL((sc_grad_kernel<T, 64, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w);
+  else hipLaunchKernelGGL((sc_grad_kernel<T, 128, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w);
   LAMPA_PROF(s, "sc_grad_kernel");
   return lampa_launch_status();
 }
 int ss_chunk_grad(const lampa_ss_args& a, const SsGrad& w, hipStream_t s) {
-  return a.dtype == GDR_BF16 ? sc_grad_launch<__bf16>(a, w, s) : sc_grad_launch<_Float16>(a, w, s);
+  if (a.dtype == GDR_BF16) return sc_vectors(a) ? sc_grad_launch<__bf16, true>(a, w, s) : sc_grad_launch<__bf16, false>(a, w, s);
+  return sc_vectors(a) ? sc_grad_launch<_Float16, true>(a, w, s) : sc_grad_launch<_Float16, false>(a, w, s);
 }

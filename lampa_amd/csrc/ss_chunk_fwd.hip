@@ -5,38 +5,35 @@
 // C_t (e^{gamma_t} dy_t)^T with gamma counted from the segment's start. Reads x and B (dy and C) once.
 // KEEP: the walk starts from the segment's initial state and leaves the state in front of every chunk in w.chunk_states, in the
 // order in which the gradients' lanes read it (sc_kept_at).
-template <typename T, int NP, bool REV, bool KEEP>
-__global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGrad w, ScFlags f) {
+template <typename T, int NP, bool REV, bool KEEP, bool VEC>
+__global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGrad w) {
   constexpr int NT = NP / 16, KS = NP + 8, VS = 64 + 8;
   const SsSegment seg = ss_segment(a, blockIdx.x);
   if (!seg.live) return;
   const int npb = (a.P + 63) / 64, pb = blockIdx.y % npb, h = blockIdx.y / npb, grp = h / (a.H / a.G);
-  const int lane = lane_id(), wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  const int lane0 = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cols = a.P - 64 * pb < 64 ? a.P - 64 * pb : 64;
   __shared__ __align__(16) T tk[64 * KS], tv[64 * VS];
   __shared__ __align__(16) ScDecay dec;
   const T* kb = (REV ? (const T*)a.C : (const T*)a.B) + (int64_t)grp * a.N;
   const T* vb = (REV ? (const T*)a.dy : (const T*)a.x) + (int64_t)h * a.P + 64 * pb;
   const int64_t ks = REV ? a.C_stride : a.B_stride, vs = REV ? (int64_t)a.H * a.P : a.x_stride;
-  const bool kvec = REV ? f.C : f.B, vvec = REV ? f.dy : f.x;
   const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
   const int64_t chunks = seg.outside ? 0 : (seg.t1 - seg.t0 + 63) / 64;
 
   f32x4 S[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) S[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const int p = 64 * pb + 16 * wave + i;
+  const int p = 64 * pb + 16 * wave + (lane0 & 15);
   if (KEEP) {
     const bool single = (a.cu_seqlens ? a.n_tokens : a.seq_len) <= a.seg_tokens;
     const float* init = single ? a.h0 : a.slot_states;
     if (init) init += ((single ? (int64_t)seg.seq : (int64_t)blockIdx.x) * a.H + h) * a.N * a.P;
+    if (init && !seg.outside)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = 16 * nt + 4 * g + r;
-        S[nt][r] = init && !seg.outside && n < a.N && p < a.P ? init[(int64_t)n * a.P + p] : 0.0f;
-      }
+        for (int r = 0; r < 4; ++r) S[nt][r] = sc_state_at(init, 16 * nt + 4 * (lane0 >> 4) + r, p, a.N, a.P);
   }
   ScTile<T, NP> pk;
   ScTile<T, 64> pv;
@@ -44,12 +41,13 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
   auto fetch = [&](int64_t c) {
     const int64_t t0 = seg.t0 + 64 * (REV ? chunks - 1 - c : c);
     const int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
-    pk.fetch(kb, ks, t0, n, a.N, kvec);
-    pv.fetch(vb, vs, t0, n, cols, vvec);
-    if (wave == 0 && lane < n) pdt = ss_load_dt<T>(a.dt, a.dt_dtype, (t0 + lane) * a.dt_stride + h);
+    pk.template fetch<VEC>(kb + t0 * ks, ks, n, a.N);
+    pv.template fetch<VEC>(vb + t0 * vs, vs, n, cols);
+    if (wave == 0 && lane0 < n) pdt = ss_load_dt<T>(a.dt, a.dt_dtype, (t0 + lane0) * a.dt_stride + h);
   };
   if (chunks) fetch(0);
   for (int64_t c = 0; c < chunks; ++c) {
+    const int lane = sc_fresh(lane0), g = lane >> 4, i = lane & 15;
     const int64_t t0 = seg.t0 + 64 * (REV ? chunks - 1 - c : c);
     const int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
     if (KEEP) {
@@ -61,22 +59,22 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
     }
     pk.put(tk, KS);
     pv.put(tv, VS);
-    if (wave == 0) sc_decays(dec, pdt, n, bias, A, a.softplus);
+    if (wave == 0) sc_decays(dec, nullptr, pdt, n, bias, A, a.softplus);
     lds_barrier();
     if (c + 1 < chunks) fetch(c + 1);
     const float end = dec.end;
     sum += dec.sum;
     sc_x8<T> v[2], hi[2], lo[2];
-    sc_columns<T>(tv, VS, 16 * wave, v);
+    sc_columns<T>(tv, VS, 16 * wave, lane, v);
     float wt[2][8], back = 1.0f;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       if constexpr (REV) {
-        sc_row_weights(dec.grow, kk, wt[kk]);
+        sc_row_weights(dec.grow, kk, lane, wt[kk]);
       } else {
         float d[8];
-        sc_row_weights(dec.left, kk, wt[kk]);
-        sc_row_weights(dec.delta, kk, d);
+        sc_row_weights(dec.left, kk, lane, wt[kk]);
+        sc_row_weights(dec.delta, kk, lane, d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) wt[kk][e] *= d[e];
       }
@@ -101,7 +99,7 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       sc_x8<T> k[2];
-      sc_columns<T>(tk, KS, 16 * nt, k);
+      sc_columns<T>(tk, KS, 16 * nt, lane, k);
       if constexpr (__is_same(T, _Float16)) {
         f32x4 d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -121,20 +119,20 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int n = 16 * nt + 4 * g + r;
+      const int n = 16 * nt + 4 * (lane0 >> 4) + r;
       if (n < a.N && p < a.P) local[(int64_t)n * a.P + p] = S[nt][r];
     }
   if (!REV && threadIdx.x == 0 && pb == 0) a.slot_decay[(int64_t)blockIdx.x * a.H + h] = __builtin_amdgcn_exp2f(sum);
 }
 
 // Outputs of a segment from the state it starts from.
-template <typename T, int NP>
-__global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a, ScFlags f) {
+template <typename T, int NP, bool VEC>
+__global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
   constexpr int NT = NP / 16, KK = NP / 32, KS = NP + 8, VS = 64 + 8, MS = 64 + 8;
   const SsSegment seg = ss_segment(a, blockIdx.x);
   if (!seg.live) return;
   const int npb = (a.P + 63) / 64, pb = blockIdx.y % npb, h = blockIdx.y / npb, grp = h / (a.H / a.G);
-  const int lane = lane_id(), wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  const int lane0 = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cols = a.P - 64 * pb < 64 ? a.P - 64 * pb : 64;
   T* yb = (T*)a.y + (int64_t)h * a.P + 64 * pb;
   if (seg.outside) {
@@ -143,40 +141,41 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a, Sc
   }
   __shared__ __align__(16) T tb[64 * KS], tc[64 * KS], tx[64 * VS], tm[64 * MS];
   __shared__ __align__(16) ScDecay dec;
-  __shared__ float mback[64];  // fp16: what the rows of the pair weights were scaled down by
+  __shared__ float mback[__is_same(T, _Float16) ? 64 : 1];  // fp16: what the rows of the pair weights were scaled down by
   __shared__ int first_bad;
   const T* bb = (const T*)a.B + (int64_t)grp * a.N;
   const T* cb = (const T*)a.C + (int64_t)grp * a.N;
   const T* xb = (const T*)a.x + (int64_t)h * a.P + 64 * pb;
   const float A = a.A[h], D = a.D ? a.D[h] : 0.0f, bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
   const bool single = (a.cu_seqlens ? a.n_tokens : a.seq_len) <= a.seg_tokens;
-  const int p = 64 * pb + 16 * wave + i;
+  const int p = 64 * pb + 16 * wave + (lane0 & 15);
 
   f32x4 S[NT];
   const float* init = single ? a.h0 : a.slot_states;
   if (init) init += ((single ? (int64_t)seg.seq : (int64_t)blockIdx.x) * a.H + h) * a.N * a.P;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int nt = 0; nt < NT; ++nt) S[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (init)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int n = 16 * nt + 4 * g + r;
-      S[nt][r] = init && n < a.N && p < a.P ? init[(int64_t)n * a.P + p] : 0.0f;
-    }
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[nt][r] = sc_state_at(init, 16 * nt + 4 * (lane0 >> 4) + r, p, a.N, a.P);
 
   ScTile<T, NP> pB, pC;
   ScTile<T, 64> pX;
   float pdt = 0.0f;
   auto fetch = [&](int64_t t0) {
     const int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
-    pB.fetch(bb, a.B_stride, t0, n, a.N, f.B);
-    pC.fetch(cb, a.C_stride, t0, n, a.N, f.C);
-    pX.fetch(xb, a.x_stride, t0, n, cols, f.x);
-    if (wave == 0 && lane < n) pdt = ss_load_dt<T>(a.dt, a.dt_dtype, (t0 + lane) * a.dt_stride + h);
+    pB.template fetch<VEC>(bb + t0 * a.B_stride, a.B_stride, n, a.N);
+    pC.template fetch<VEC>(cb + t0 * a.C_stride, a.C_stride, n, a.N);
+    pX.template fetch<VEC>(xb + t0 * a.x_stride, a.x_stride, n, cols);
+    if (wave == 0 && lane0 < n) pdt = ss_load_dt<T>(a.dt, a.dt_dtype, (t0 + lane0) * a.dt_stride + h);
   };
   if (threadIdx.x == 0) first_bad = 64;
   if (seg.t0 < seg.t1) fetch(seg.t0);
   lds_barrier();
   for (int64_t t0 = seg.t0; t0 < seg.t1;) {
+    const int lane = sc_fresh(lane0), g = lane >> 4, i = lane & 15;
     int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
     pB.put(tb, KS);
     pC.put(tc, KS);
@@ -185,7 +184,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a, Sc
       const int bad = pX.first_bad();
       if (bad < 64) atomicMin(&first_bad, bad);
     }
-    if (wave == 0) sc_decays(dec, pdt, n, bias, A, a.softplus);
+    if (wave == 0) sc_decays(dec, nullptr, pdt, n, bias, A, a.softplus);
     lds_barrier();
     // An x that is not finite times a weight of zero would reach earlier tokens: such a token begins a chunk of its own.
     const int bad = first_bad;
@@ -194,7 +193,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a, Sc
       lds_barrier();
       for (int e = threadIdx.x; e < (64 - n) * KS; e += SC_BLOCK) tb[n * KS + e] = (T)0.0f;
       for (int e = threadIdx.x; e < (64 - n) * VS; e += SC_BLOCK) tx[n * VS + e] = (T)0.0f;
-      if (wave == 0) sc_decays(dec, pdt, n, bias, A, a.softplus);
+      if (wave == 0) sc_decays(dec, nullptr, pdt, n, bias, A, a.softplus);
       if (threadIdx.x == 0) first_bad = 64;
       lds_barrier();
     }
@@ -267,7 +266,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a, Sc
       }
     }
     sc_x8<T> v[2];
-    sc_columns<T>(tx, VS, 16 * wave, v);
+    sc_columns<T>(tx, VS, 16 * wave, lane, v);
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
       const int t = 16 * tt + i;
@@ -285,8 +284,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a, Sc
           o[r] = (T)__builtin_fmaf(D, (float)xv[r], out);
         }
         const int c = 16 * wave + 4 * g;
-        T* dst = yb + (t0 + t) * a.y_stride + c;
-        if (f.y) {
+        T* dst = reinterpret_cast<T*>(reinterpret_cast<char*>(yb + (t0 + 16 * tt) * a.y_stride) + (unsigned)(i * (int)a.y_stride + c) * (unsigned)sizeof(T));
+        if constexpr (VEC) {
           if (c < cols) *reinterpret_cast<sc_x4<T>*>(dst) = o;
         } else {
 #pragma unroll
@@ -301,8 +300,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a, Sc
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         float d[8];
-        sc_row_weights(dec.left, kk, wt[kk]);
-        sc_row_weights(dec.delta, kk, d);
+        sc_row_weights(dec.left, kk, lane, wt[kk]);
+        sc_row_weights(dec.delta, kk, lane, d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) wt[kk][e] *= d[e];
       }
@@ -328,7 +327,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a, Sc
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         sc_x8<T> k[2];
-        sc_columns<T>(tb, KS, 16 * nt, k);
+        sc_columns<T>(tb, KS, 16 * nt, lane, k);
         if constexpr (__is_same(T, _Float16)) {
           f32x4 d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -350,47 +349,46 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a, Sc
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int n = 16 * nt + 4 * g + r;
+        const int n = 16 * nt + 4 * (lane0 >> 4) + r;
         if (n < a.N && p < a.P) out[(int64_t)n * a.P + p] = S[nt][r];
       }
   }
 }
 
 enum { SC_LOCAL_STATES, SC_LOCAL_ADJOINTS, SC_KEEP_STATES };
-template <typename T>
+template <typename T, bool VEC>
 static int sc_maps_launch(const lampa_ss_args& a, int what, const SsGrad& w, hipStream_t s) {
-  const ScFlags f = sc_flags(a);
   LAMPA_PROF(s, "start");
-#define SC_GO(NP)                                                                                                                   \
-  switch (what) {                                                                                                                   \
-    case SC_LOCAL_STATES: hipLaunchKernelGGL((sc_map_kernel<T, NP, false, false>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f); break; \
-    case SC_LOCAL_ADJOINTS: hipLaunchKernelGGL((sc_map_kernel<T, NP, true, false>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f); break; \
-    default: hipLaunchKernelGGL((sc_map_kernel<T, NP, false, true>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w, f); break;              \
+#define SC_GO(NP)                                                                                                                      \
+  switch (what) {                                                                                                                      \
+    case SC_LOCAL_STATES: hipLaunchKernelGGL((sc_map_kernel<T, NP, false, false, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w); break; \
+    case SC_LOCAL_ADJOINTS: hipLaunchKernelGGL((sc_map_kernel<T, NP, true, false, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w); break; \
+    default: hipLaunchKernelGGL((sc_map_kernel<T, NP, false, true, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w); break;               \
   }
   if (a.N <= 32) { SC_GO(32) } else if (a.N <= 64) { SC_GO(64) } else { SC_GO(128) }
 #undef SC_GO
   LAMPA_PROF(s, what == SC_KEEP_STATES ? "sc_map_kernel<keep>" : "sc_map_kernel");
   return lampa_launch_status();
 }
+static int sc_maps(const lampa_ss_args& a, int what, const SsGrad& w, hipStream_t s) {
+  if (a.dtype == GDR_BF16) return sc_vectors(a) ? sc_maps_launch<__bf16, true>(a, what, w, s) : sc_maps_launch<__bf16, false>(a, what, w, s);
+  return sc_vectors(a) ? sc_maps_launch<_Float16, true>(a, what, w, s) : sc_maps_launch<_Float16, false>(a, what, w, s);
+}
 int ss_chunk_maps(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s) {
-  const int what = grad ? SC_LOCAL_ADJOINTS : SC_LOCAL_STATES;
-  const SsGrad w = grad ? *grad : SsGrad{};
-  return a.dtype == GDR_BF16 ? sc_maps_launch<__bf16>(a, what, w, s) : sc_maps_launch<_Float16>(a, what, w, s);
+  return sc_maps(a, grad ? SC_LOCAL_ADJOINTS : SC_LOCAL_STATES, grad ? *grad : SsGrad{}, s);
 }
-int ss_chunk_keep(const lampa_ss_args& a, const SsGrad& w, hipStream_t s) {
-  return a.dtype == GDR_BF16 ? sc_maps_launch<__bf16>(a, SC_KEEP_STATES, w, s) : sc_maps_launch<_Float16>(a, SC_KEEP_STATES, w, s);
-}
+int ss_chunk_keep(const lampa_ss_args& a, const SsGrad& w, hipStream_t s) { return sc_maps(a, SC_KEEP_STATES, w, s); }
 
-template <typename T>
+template <typename T, bool VEC>
 static int sc_out_launch(const lampa_ss_args& a, hipStream_t s) {
-  const ScFlags f = sc_flags(a);
   LAMPA_PROF(s, "start");
-  if (a.N <= 32) hipLaunchKernelGGL((sc_out_kernel<T, 32>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, f);
-  else if (a.N <= 64) hipLaunchKernelGGL((sc_out_kernel<T, 64>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, f);
-  else hipLaunchKernelGGL((sc_out_kernel<T, 128>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, f);
+  if (a.N <= 32) hipLaunchKernelGGL((sc_out_kernel<T, 32, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a);
+  else if (a.N <= 64) hipLaunchKernelGGL((sc_out_kernel<T, 64, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a);
+  else hipLaunchKernelGGL((sc_out_kernel<T, 128, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a);
   LAMPA_PROF(s, "sc_out_kernel");
   return lampa_launch_status();
 }
 int ss_chunk_out(const lampa_ss_args& a, hipStream_t s) {
-  return a.dtype == GDR_BF16 ? sc_out_launch<__bf16>(a, s) : sc_out_launch<_Float16>(a, s);
+  if (a.dtype == GDR_BF16) return sc_vectors(a) ? sc_out_launch<__bf16, true>(a, s) : sc_out_launch<__bf16, false>(a, s);
+  return sc_vectors(a) ? sc_out_launch<_Float16, true>(a, s) : sc_out_launch<_Float16, false>(a, s);
 }

@@ -108,16 +108,24 @@ __global__ void __launch_bounds__(SS_BLOCK) ss_decay_grad_kernel(lampa_ss_args a
   }
 }
 
-// The parts of dB and dC, one for each head and block of columns, added up over the heads of a group in their order.
-template <typename T>
+// The parts of dB and dC, one for each head and block of columns, added up over the heads of a group in their order. VW: columns
+// a thread takes (4 where N allows: a wave then reads 1 KiB at a time).
+template <typename T, int VW>
 __global__ void __launch_bounds__(SS_BLOCK) ss_group_sum_kernel(const float* __restrict__ dB_part, const float* __restrict__ dC_part,
                                                                 T* __restrict__ dB, T* __restrict__ dC, int64_t n, int N, int parts) {
-  const int64_t i = (int64_t)blockIdx.x * SS_BLOCK + threadIdx.x;
+  typedef float vec __attribute__((ext_vector_type(VW)));
+  typedef T out_vec __attribute__((ext_vector_type(VW)));
+  const int64_t i = ((int64_t)blockIdx.x * SS_BLOCK + threadIdx.x) * VW;
   if (i >= n) return;
-  const float* src = (blockIdx.y ? dC_part : dB_part) + (i / N) * parts * N + i % N;
-  float sum = 0.0f;
-  for (int j = 0; j < parts; ++j) sum += src[(int64_t)j * N];
-  (blockIdx.y ? dC : dB)[i] = GdrElem<T>::from_float(sum);
+  const int64_t row = i / N;
+  const float* src = (blockIdx.y ? dC_part : dB_part) + row * parts * N + (i - row * N);
+  vec sum = *reinterpret_cast<const vec*>(src);
+#pragma unroll 4
+  for (int j = 1; j < parts; ++j) sum += *reinterpret_cast<const vec*>(src + (int64_t)j * N);
+  out_vec o;
+#pragma unroll
+  for (int e = 0; e < VW; ++e) o[e] = GdrElem<T>::from_float(sum[e]);
+  *reinterpret_cast<out_vec*>((blockIdx.y ? dC : dB) + i) = o;
 }
 
 // dA, d dt_bias and dD of a head: its segments' shares in their order.
@@ -148,6 +156,10 @@ static int ss_check(const lampa_ss_args* a) {
       a->C_stride < (int64_t)a->G * a->N)
     return LAMPA_ERR_INVALID;
   if (a->N > 128) return LAMPA_ERR_UNSUPPORTED;
+  // a lane's offset within 64 rows is formed in 32 bits
+  if (a->x_stride >= 1 << 24 || a->B_stride >= 1 << 24 || a->C_stride >= 1 << 24 || a->y_stride >= 1 << 24 ||
+      (int64_t)a->H * (a->P + 63) * a->N >= 1 << 28)
+    return LAMPA_ERR_UNSUPPORTED;
   // the grids' limits: slots along x, heads and blocks along y
   if (ss_slots(a) > 0x7fffffff || (int64_t)a->H * ss_blocks64(a->P) * 2 > 65535) return LAMPA_ERR_UNSUPPORTED;
   return LAMPA_OK;
@@ -229,13 +241,17 @@ extern "C" int lampa_ss_scan_bwd(const lampa_ss_args* args, void* stream) {
     }
     if (e != LAMPA_OK) return e;
     const int64_t n = a.n_tokens * a.G * a.N;
-    const dim3 sums((unsigned)((n + SS_BLOCK - 1) / SS_BLOCK), 2), segs((unsigned)slots, (unsigned)a.H);
+    const bool wide = a.N % 4 == 0 && ((uintptr_t)a.dB | (uintptr_t)a.dC) % 16 == 0;
+    const int64_t per = SS_BLOCK * (wide ? 4 : 1);
+    const dim3 sums((unsigned)((n + per - 1) / per), 2), segs((unsigned)slots, (unsigned)a.H);
     const int parts = a.H / a.G * ss_blocks64(a.P);
 #define SS_TAIL(T)                                                                                                          \
   hipLaunchKernelGGL((ss_decay_grad_kernel<T>), segs, dim3(SS_BLOCK), 0, s, a, w, !serial);                                          \
   LAMPA_PROF(s, "ss_decay_grad_kernel");                                                                                    \
-  hipLaunchKernelGGL((ss_group_sum_kernel<T>), sums, dim3(SS_BLOCK), 0, s, w.dB_part, w.dC_part, (T*)a.dB, (T*)a.dC, n, a.N, \
-                     parts);                                                                                                \
+  if (wide)                                                                                                                 \
+    hipLaunchKernelGGL((ss_group_sum_kernel<T, 4>), sums, dim3(SS_BLOCK), 0, s, w.dB_part, w.dC_part, (T*)a.dB, (T*)a.dC, n, a.N, parts); \
+  else                                                                                                                      \
+    hipLaunchKernelGGL((ss_group_sum_kernel<T, 1>), sums, dim3(SS_BLOCK), 0, s, w.dB_part, w.dC_part, (T*)a.dB, (T*)a.dC, n, a.N, parts); \
   LAMPA_PROF(s, "ss_group_sum_kernel");
     if (n > (int64_t)0x7fffffff * SS_BLOCK) return LAMPA_ERR_UNSUPPORTED;
     LAMPA_PROF(s, "start");

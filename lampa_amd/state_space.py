@@ -31,10 +31,19 @@ def _f32(t):
     return None if t is None else t.detach().to(torch.float32).contiguous()
 
 
-def _segment_tokens(longest: int, total: int, waves: int) -> int:
-    """Length of the segments that run in parallel, a multiple of 64: two waves a SIMD over the whole call."""
-    seg = -(-total * waves // 2048 // 64) * 64
-    return max(64, min(seg, -(-longest // 64) * 64))
+def _segment_tokens(longest: int, total: int, heads: int, N: int, dtype, grad: bool) -> int:
+    """Length of the segments that run in parallel, a multiple of 64: as many workgroups as the chip holds at once, in one round.
+    ``heads`` counts blocks of 64 columns. The chunk kernels (16-bit types) run two workgroups a CU, three without gradients and
+    N <= 64; the token-serial ones (float32) one wave a workgroup, eight a CU. 60 000 tokens x 8 heads, segments of 256 / 640 /
+    960 / 1920 tokens: forward at N = 64 126 / 97 / 106 / - us, with gradients at N = 128 1098 / - / 810 / 1039 us. Segments of
+    fewer tokens than `shortest` are not worth the two further launches of joining them: fp32 gradients of 6 007 tokens x 4
+    heads with 64 / 128 / 256 tokens 335 / 579 / 1061 us, but 77 tokens whole 48 us, in two segments 72; 16-bit forward of 15 000
+    x 6 with 64 / 256 / 512 tokens 41 / 42 / 58 us."""
+    serial = dtype == torch.float32
+    per_cu = 8 if serial else 3 if N <= 64 and not grad else 2
+    shortest = 256 if not serial else 128 if longest <= 128 else 64
+    seg = -(-total * heads // (256 * per_cu) // 64) * 64
+    return max(shortest, min(seg, -(-longest // 64) * 64))
 
 
 def _pack(x, dt, A, B, C, D, bias, h0, y, ht, states, decay, cu, longest, seg, n_seq, softplus, grad=None):
@@ -59,7 +68,7 @@ def _scan_launch(x, dt, A, B, C, D, bias, softplus, h0, want_final, cu, keep=Fal
     x, dt = _tokens(x, H * P), _tokens(dt, H)
     B, C = _tokens(B, G * N), _tokens(C, G * N)
     A, D, bias, h0 = _f32(A), _f32(D), _f32(bias), _f32(h0)
-    seg = _segment_tokens(longest, total, H * -(-P // 64))
+    seg = _segment_tokens(longest, total, H * -(-P // 64), N, x[0].dtype, keep)
     single = longest <= seg
     y = torch.empty((nb, T, H, P), dtype=x[0].dtype, device=dev)
     ht = torch.empty((n_seq, H, N, P), dtype=torch.float32, device=dev) if want_final or (keep and not single) else None
