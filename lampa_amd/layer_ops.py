@@ -38,23 +38,46 @@ def _code(dtype) -> int:
     return _DTYPES[dtype]
 
 
-def _on_device(device):
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_here = contextlib.nullcontext()
+
+
+def _on_device(device: int):
     """The launches of a call go to its tensors' device, whichever is current."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _here if device == _current_device() else torch.cuda.device(device)
 
 
-def _same_device(what, *tensors):
-    require_cuda(*tensors)
-    device = tensors[0].device
+def _same_device(what, *tensors) -> int:
+    device = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: all tensors must be on one device, got {device} and {t.device}")
+        if t is not None and t.get_device() != device:
+            require_cuda(*tensors)
+            raise ValueError(f"{what}: all tensors must be on one device, got cuda:{device} and {t.device}")
+    if device < 0:
+        require_cuda(*tensors)
     return device
+
+
+def _wants_grad(*tensors) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _plain_f32(t):
+    """t in float32 and contiguous, for its pointer: t itself where it is."""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().to(torch.float32).contiguous()
 
 
 def _tokens(t: torch.Tensor, inner: int):
     """(t, elements from one token to the next) of t [B, T, ...] whose dimensions behind T hold `inner` contiguous elements;
     a copy only where the tokens do not lie evenly."""
+    if t.is_contiguous():
+        return t, inner
     B, T = t.shape[:2]
     expect = 1
     for size, stride in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
@@ -171,7 +194,7 @@ def _conv_operands(x, weight, bias):
         x2, step = x2.contiguous(), D
         if x2.data_ptr() % 16:
             x2 = x2.clone()
-    return x2, step, weight.detach().to(torch.float32).contiguous(), None if bias is None else bias.detach().to(torch.float32).contiguous()
+    return x2, step, _plain_f32(weight), _plain_f32(bias)
 
 
 @torch.no_grad()
@@ -183,7 +206,7 @@ def _conv_state_launch(x, weight, bias, activation, cu, past, want_last):
     past = None if past is None else past.detach().to(x.dtype).contiguous()
     y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
     last = torch.empty((n_seq, D, W), dtype=x.dtype, device=x.device) if want_last else None
-    with _on_device(x.device):
+    with _on_device(x.get_device()):
         check(_capi.lib().lampa_causal_conv1d_state_fwd(
             ptr(x2), step, B * T, D, W, ptr(w32), ptr(b32), ptr(past), ptr(cu), n_seq, T, _ACT[activation], _code(x.dtype),
             ptr(y), ptr(last), stream_of(x)), "lampa_causal_conv1d_state_fwd")
@@ -216,7 +239,7 @@ class _CausalConv(torch.autograd.Function):
         dx = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
         dwb = torch.empty((D, W + 1), dtype=torch.float32, device=x.device)
         lib = _capi.lib()
-        with _on_device(x.device):
+        with _on_device(x.get_device()):
             size = check(lib.lampa_causal_conv1d_bwd_workspace_bytes(B * T, D, W, _code(x.dtype)),
                          "lampa_causal_conv1d_bwd_workspace_bytes")
             ws = torch.empty(size, dtype=torch.uint8, device=x.device)
@@ -255,7 +278,7 @@ def causal_conv1d(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: 
         require_cuda(cu_seqlens)
     if weight is None:
         weight = torch.ones(D, 1, device=x.device)
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
+    grad = _wants_grad(x, weight, bias, residual)
     if with_state or grad:
         what = "causal_conv1d"
         _same_device(what, x, weight, bias, residual, initial_state)
@@ -277,7 +300,7 @@ def causal_conv1d(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: 
                                              output_final_state)
     else:
         if grad:  # a training step's weights are new every time
-            w32, b32 = weight.detach().reshape(D, -1).float().contiguous(), None if bias is None else bias.detach().float().contiguous()
+            w32, b32 = _plain_f32(weight.detach().reshape(D, -1)), _plain_f32(bias)
         else:
             w32, b32 = _f32(weight.reshape(D, -1), x.device), _f32(bias, x.device)
         res2 = None if residual is None else _rows(residual.to(x.dtype))
@@ -290,18 +313,16 @@ def causal_conv1d(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: 
     return (y, last) if output_final_state else y
 
 
-@torch.no_grad()
 def _conv_step_launch(x, cache, weight, bias, activation, target):
     n, D = x.shape
-    W = weight.shape[-1]
-    if x.stride(1) != 1 and D > 1 or (n > 1 and x.stride(0) < D):
-        x = x.contiguous()
-    w32 = weight.detach().to(torch.float32).contiguous()
-    b32 = None if bias is None else bias.detach().to(torch.float32).contiguous()
+    step = x.stride(0) if n > 1 else D
+    if step < D or (D > 1 and x.stride(1) != 1):
+        x, step = x.contiguous(), D
+    w32, b32 = _plain_f32(weight), _plain_f32(bias)
     y = torch.empty((n, D), dtype=x.dtype, device=x.device)
-    with _on_device(x.device):
-        check(_capi.lib().lampa_causal_conv1d_step(ptr(x), x.stride(0) if n > 1 else D, ptr(cache), ptr(target), ptr(w32), ptr(b32),
-                                                   _ACT[activation], _code(x.dtype), ptr(y), n, D, W, stream_of(x)),
+    with _on_device(x.get_device()):
+        check(_capi.lib().lampa_causal_conv1d_step(ptr(x), step, ptr(cache), ptr(target), ptr(w32), ptr(b32), _ACT[activation],
+                                                   _code(x.dtype), ptr(y), n, D, weight.numel() // D, stream_of(x)),
               "lampa_causal_conv1d_step")
     return y
 
@@ -334,10 +355,9 @@ def causal_conv1d_step(x: torch.Tensor, cache: torch.Tensor, weight: torch.Tenso
     if n == 0:
         return torch.empty_like(x)
     target = cache if new_cache is None else new_cache
-    fn = lambda: _conv_step_launch(x, cache, weight.reshape(D, W), bias, activation, target)  # noqa: E731
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _ForwardOnly.apply(fn, x, weight, bias)
-    return fn()
+    if _wants_grad(x, weight, bias):
+        return _ForwardOnly.apply(lambda: _conv_step_launch(x, cache, weight, bias, activation, target), x, weight, bias)
+    return _conv_step_launch(x, cache, weight, bias, activation, target)
 
 
 @torch.no_grad()
@@ -566,14 +586,14 @@ _GATE_NONE, _GATE_TOKEN, _GATE_SEQUENCE = 0, 1, 2
 
 def _packed(t):
     """Contiguous and 16-byte aligned, as the row kernels read it."""
-    if t is None:
-        return None
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
     t = t.detach().contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _vec32(t):
-    return None if t is None else _packed(t.to(torch.float32))
+    return _packed(_plain_f32(t))
 
 
 def _norm_sizes(x, gate):
@@ -586,14 +606,13 @@ def _norm_sizes(x, gate):
     return rows, max(x.shape[1], 1), D, _GATE_SEQUENCE
 
 
-@torch.no_grad()
 def _residual_norm_launch(x, residual, weight, post_weight, gate, act, scale, eps):
     rows, seq_rows, D, kind = _norm_sizes(x, gate)
     x_, r_, g_ = _packed(x), _packed(residual), _packed(gate)
     w, pw, sc = _vec32(weight), _vec32(post_weight), _vec32(scale)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     out = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    with _on_device(x.device):
+    with _on_device(x.get_device()):
         check(_capi.lib().lampa_residual_norm_fwd(ptr(x_), ptr(r_), ptr(w), ptr(pw), ptr(g_), kind, act, ptr(sc), rows, seq_rows, D,
                                                   float(eps), _code(x.dtype), _code(residual.dtype), ptr(y), ptr(out),
                                                   stream_of(x)), "lampa_residual_norm_fwd")
@@ -625,7 +644,7 @@ class _ResidualNorm(torch.autograd.Function):
         dw, dpw, dsc = vec(weight, need[2]), vec(post_weight, need[3]), vec(scale, need[5])
         dg = make(gate.shape, dtype=gate.dtype, device=x.device) if gate is not None and need[4] else None
         lib = _capi.lib()
-        with _on_device(x.device):
+        with _on_device(x.get_device()):
             size = check(lib.lampa_residual_norm_bwd_workspace_bytes(rows, seq_rows, D), "lampa_residual_norm_bwd_workspace_bytes")
             ws = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
             check(lib.lampa_residual_norm_bwd(ptr(x_), ptr(r_), ptr(w), ptr(pw), ptr(g_), kind, ctx.act, ptr(sc), ptr(dy), ptr(dres),
@@ -673,8 +692,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torc
         if gate.shape != x.shape and x.shape[0] > 65535:
             raise ValueError(f"{what}: at most 65535 sequences with a gate each, got {x.shape[0]}")
     act = _ACT[gate_activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, residual, weight, post_weight, gate, residual_scale)):
+    if _wants_grad(x, residual, weight, post_weight, gate, residual_scale):
         return _ResidualNorm.apply(x, residual, weight, post_weight, gate, residual_scale, act, eps)
     return _residual_norm_launch(x, residual, weight, post_weight, gate, act, residual_scale, eps)
 

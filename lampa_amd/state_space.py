@@ -19,16 +19,12 @@ import torch
 from . import _capi
 from ._capi import check, ptr, require_cuda, stream_of
 from .gated_delta import _direct
-from .layer_ops import _DTYPES, _ForwardOnly, _on_device, _same_device, _sequences, _tokens
+from .layer_ops import _DTYPES, _ForwardOnly, _on_device, _plain_f32, _same_device, _sequences, _tokens, _wants_grad
 
 MAX_STATE = 128  # N of state_space_scan; state_space_step takes any
 
 # lampa_ss_args: 13 pointers, 8 int64, 8 int32, 11 pointers, one int64
 _ARGS = struct.Struct("=13Q8q8i11Qq")
-
-
-def _f32(t):
-    return None if t is None else t.detach().to(torch.float32).contiguous()
 
 
 def _segment_tokens(longest: int, total: int, heads: int, N: int, dtype, grad: bool) -> int:
@@ -67,7 +63,7 @@ def _scan_launch(x, dt, A, B, C, D, bias, softplus, h0, want_final, cu, keep=Fal
     dev = x.device
     x, dt = _tokens(x, H * P), _tokens(dt, H)
     B, C = _tokens(B, G * N), _tokens(C, G * N)
-    A, D, bias, h0 = _f32(A), _f32(D), _f32(bias), _f32(h0)
+    A, D, bias, h0 = _plain_f32(A), _plain_f32(D), _plain_f32(bias), _plain_f32(h0)
     seg = _segment_tokens(longest, total, H * -(-P // 64), N, x[0].dtype, keep)
     single = longest <= seg
     y = torch.empty((nb, T, H, P), dtype=x[0].dtype, device=dev)
@@ -77,7 +73,7 @@ def _scan_launch(x, dt, A, B, C, D, bias, softplus, h0, want_final, cu, keep=Fal
         slots = n_seq * -(-T // seg) if cu is None else total // seg + n_seq + 1
         states = torch.empty((slots, H, N, P), dtype=torch.float32, device=dev)
         decay = torch.empty((slots, H), dtype=torch.float32, device=dev)
-    with _on_device(dev):
+    with _on_device(dev.index):
         check(_capi.lib().lampa_ss_scan_fwd(
             _pack(x, dt, A, B, C, D, bias, h0, y, ht, states, decay, cu, longest, seg, n_seq, softplus),
             stream_of(y)), "lampa_ss_scan_fwd")
@@ -95,14 +91,14 @@ def _scan_backward(x, dt, A, B, C, D, bias, softplus, h0, cu, ht, kept, dy, dht)
     dbias = None if bias is None else torch.empty_like(dA)
     dh0 = None if h0 is None else torch.empty((n_seq, H, N, P), dtype=torch.float32, device=dev)
     dy = torch.zeros((nb, T, H, P), dtype=x.dtype, device=dev) if dy is None else dy.to(x.dtype).contiguous()
-    dht = _f32(dht)
+    dht = _plain_f32(dht)
     x_, dt_ = _tokens(x, H * P), _tokens(dt, H)
     B_, C_ = _tokens(B, G * N), _tokens(C, G * N)
-    A, D, bias, h0 = _f32(A), _f32(D), _f32(bias), _f32(h0)
+    A, D, bias, h0 = _plain_f32(A), _plain_f32(D), _plain_f32(bias), _plain_f32(h0)
     pack = lambda ws, size: _pack(x_, dt_, A, B_, C_, D, bias, h0, None, ht, states, decay, cu, longest, seg, n_seq,  # noqa: E731
                                   softplus, ((dy, dht, dx, ddt, dB, dC, dA, dD, dbias, dh0, ws), size))
     lib = _capi.lib()
-    with _on_device(dev):
+    with _on_device(dev.index):
         size = check(lib.lampa_ss_bwd_workspace_bytes(pack(None, 0)), "lampa_ss_bwd_workspace_bytes")
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
         check(lib.lampa_ss_scan_bwd(pack(ws, size), stream_of(dx)), "lampa_ss_scan_bwd")
@@ -130,23 +126,27 @@ class _StateSpaceScan(torch.autograd.Function):
 
 def _check_operands(what, x, dt, A, B, C, D, dt_bias, tokens):
     """Shapes and types of a call; `tokens`: the leading dimensions of x."""
-    lead, (H, P) = tuple(x.shape[:tokens]), (x.shape[-2], x.shape[-1]) if x.dim() == tokens + 2 else (0, 0)
-    names = "B, T, " if tokens == 2 else "n, "
-    if x.dim() != tokens + 2 or tuple(dt.shape) != lead + (H,):
-        raise ValueError(f"{what}: expected x [{names}H, P] and dt [{names}H], got {tuple(x.shape)} and {tuple(dt.shape)}")
-    if B.dim() != tokens + 2 or B.shape != C.shape or tuple(B.shape[:tokens]) != lead or B.shape[-2] < 1 or H % max(1, B.shape[-2]):
-        raise ValueError(f"{what}: expected B, C [{names}G, N] with G a divisor of the {H} heads, got {tuple(B.shape)} and "
+    xs, bs, own = x.shape, B.shape, x.dtype
+    if len(xs) != tokens + 2 or dt.shape != xs[:-1]:
+        names = "B, T, " if tokens == 2 else "n, "
+        raise ValueError(f"{what}: expected x [{names}H, P] and dt [{names}H], got {tuple(xs)} and {tuple(dt.shape)}")
+    H = xs[-2]
+    if len(bs) != tokens + 2 or bs != C.shape or bs[:tokens] != xs[:tokens] or bs[-2] < 1 or H % bs[-2]:
+        names = "B, T, " if tokens == 2 else "n, "
+        raise ValueError(f"{what}: expected B, C [{names}G, N] with G a divisor of the {H} heads, got {tuple(bs)} and "
                          f"{tuple(C.shape)}")
-    if H < 1 or P < 1 or B.shape[-1] < 1:
-        raise ValueError(f"{what}: heads, columns and states must be at least 1, got H = {H}, P = {P}, N = {B.shape[-1]}")
+    if H < 1 or xs[-1] < 1 or bs[-1] < 1:
+        raise ValueError(f"{what}: heads, columns and states must be at least 1, got H = {H}, P = {xs[-1]}, N = {bs[-1]}")
     for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
-        if t is not None and tuple(t.shape) != (H,):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != H:
             raise ValueError(f"{what}: {name} must have shape ({H},), one value per head, got {tuple(t.shape)}")
-        if t is not None and not t.is_floating_point():
+        if not t.is_floating_point():
             raise TypeError(f"{what}: {name} must be a floating-point tensor, got {t.dtype}")
-    if x.dtype not in _DTYPES or B.dtype != x.dtype or C.dtype != x.dtype or dt.dtype not in (x.dtype, torch.float32):
+    if own not in _DTYPES or B.dtype != own or C.dtype != own or (dt.dtype != own and dt.dtype != torch.float32):
         raise TypeError(f"{what}: x, B and C must have one type (bfloat16, float16 or float32) and dt that type or float32, got "
-                        f"{x.dtype}, {B.dtype}, {C.dtype} and {dt.dtype}")
+                        f"{own}, {B.dtype}, {C.dtype} and {dt.dtype}")
 
 
 def _check_state(what, name, state, shape):
@@ -170,13 +170,13 @@ def state_space_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torc
     A value that is not finite reaches the tokens from its own on, as in the recurrence, never earlier ones. Differentiable in every floating-point input (first order); the
     gradients of B and C are summed over a group's heads in a fixed order, and repeated calls give the same bits."""
     what = "state_space_scan"
-    device = _same_device(what, x, dt, A, B, C, D, dt_bias, initial_state)
+    _same_device(what, x, dt, A, B, C, D, dt_bias, initial_state)
     _check_operands(what, x, dt, A, B, C, D, dt_bias, 2)
     H, P = x.shape[-2:]
     N = B.shape[-1]
     if N > MAX_STATE:
         raise ValueError(f"{what}: N must be at most {MAX_STATE}, got {N}")
-    cu = _sequences(what, cu_seqlens, x.shape[0], x.shape[1], device)
+    cu = _sequences(what, cu_seqlens, x.shape[0], x.shape[1], x.device)
     n_seq = x.shape[0] if cu is None else cu.numel() - 1
     if n_seq < 1:
         raise ValueError(f"{what}: the batch must hold at least one sequence")
@@ -188,15 +188,18 @@ def state_space_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torc
     return _StateSpaceScan.apply(x, dt, A, B, C, D, dt_bias, initial_state, bool(dt_softplus), bool(output_final_state), cu)
 
 
-@torch.no_grad()
+def _rows(t, inner):
+    """(t, elements from one row to the next) of t [n, ...] whose rows are contiguous."""
+    return (t, inner) if t.is_contiguous() else _tokens(t.unsqueeze(0), inner)
+
+
 def _step_launch(x, dt, A, B, C, D, dt_bias, softplus, state, new_state):
     n, H, P = x.shape
     G, N = B.shape[-2:]
-    rows = lambda t, inner: _tokens(t.unsqueeze(0), inner)  # noqa: E731
-    (x, xs), (dt, dts), (B, bs), (C, cs) = rows(x, H * P), rows(dt, H), rows(B, G * N), rows(C, G * N)
-    A, D, dt_bias = _f32(A), _f32(D), _f32(dt_bias)
+    (x, xs), (dt, dts), (B, bs), (C, cs) = _rows(x, H * P), _rows(dt, H), _rows(B, G * N), _rows(C, G * N)
+    A, D, dt_bias = _plain_f32(A), _plain_f32(D), _plain_f32(dt_bias)
     y = torch.empty((n, H, P), dtype=x.dtype, device=x.device)
-    with _on_device(x.device):
+    with _on_device(x.get_device()):
         check(_capi.lib().lampa_ss_step(ptr(x), xs, ptr(dt), dts, ptr(B), bs, ptr(C), cs, ptr(A), ptr(D), ptr(dt_bias),
                                         ptr(state), ptr(new_state), ptr(y), n, H, P, G, N, _DTYPES[x.dtype],
                                         _DTYPES[dt.dtype], int(softplus), stream_of(y)), "lampa_ss_step")
@@ -227,7 +230,7 @@ def state_space_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torc
     if x.shape[0] == 0:
         return torch.empty_like(x)
     target = state if new_state is None else new_state
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, dt, A, B, C, D, dt_bias, state)):
+    if _wants_grad(x, dt, A, B, C, D, dt_bias, state):
         return _ForwardOnly.apply(lambda: _step_launch(x, dt, A, B, C, D, dt_bias, dt_softplus, state, target),
                                   x, dt, A, B, C, D, dt_bias, state)
     return _step_launch(x, dt, A, B, C, D, dt_bias, dt_softplus, state, target)
