@@ -37,6 +37,20 @@ __device__ __forceinline__ int cc_seq_of(const CcSeq& q, int64_t t) {
   return lo;
 }
 
+template <typename T>
+__device__ __forceinline__ void cc_store8(T* dst, const float* v) {
+  if constexpr (sizeof(T) == 2) {
+    typedef T vec8 __attribute__((ext_vector_type(8)));
+    vec8 o;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) o[c] = GdrElem<T>::from_float(v[c]);
+    *reinterpret_cast<vec8*>(dst) = o;
+  } else {
+    *reinterpret_cast<f32x4*>(dst) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4*>(dst + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ forward with state
 // One thread: 8 channels x CF_TOKENS tokens, its W - 1 rows of history in registers. The workgroups behind the tokens' ones
 // write the caches. Rows behind the last sequence come back as zero.
@@ -107,17 +121,7 @@ __global__ void __launch_bounds__(CC_BLOCK) cc_fwd_kernel(const T* __restrict__ 
       if (act) v *= cc_sigmoid(v);
       out[c] = seq < q.n_seq ? v : 0.0f;
     }
-    T* dst = y + t * D + c0;
-    if constexpr (sizeof(T) == 2) {
-      typedef T vec8 __attribute__((ext_vector_type(8)));
-      vec8 o;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) o[c] = GdrElem<T>::from_float(out[c]);
-      *reinterpret_cast<vec8*>(dst) = o;
-    } else {
-      *reinterpret_cast<f32x4*>(dst) = f32x4{out[0], out[1], out[2], out[3]};
-      *reinterpret_cast<f32x4*>(dst + 4) = f32x4{out[4], out[5], out[6], out[7]};
-    }
+    cc_store8(y + t * D + c0, out);
   }
 }
 
@@ -146,86 +150,99 @@ __global__ void __launch_bounds__(CC_BLOCK) cc_step_kernel(const T* __restrict__
 }
 
 // ------------------------------------------------------------------------------------------------------- gradients
-// A workgroup takes 16 groups of 8 channels and, side by side, 16 runs of CB_TOKENS tokens; it goes over the tokens in
-// strides of the whole grid and leaves one share of dw and dbias, added up over its runs in a fixed order.
-template <typename T> struct CcBwdTokens { static const int n = 16; };
-template <> struct CcBwdTokens<float> { static const int n = 8; };
+// A workgroup takes 32 groups of 4 channels and, side by side, 8 runs of CB_TOKENS tokens; it goes over the tokens in strides of
+// the whole grid and leaves one share of dw and dbias, added up over its runs in a fixed order. Rows are requested four at a
+// time, one four ahead. (Eight channels a thread, or all rows of a run requested at once, take over 200 registers: 138 and
+// 151 us at 60 000 x 640 in bf16.)
+#define CB_CH 4
+#define CB_TOKENS 16
+#define CB_LANES 32
+#define CB_RUNS (CC_BLOCK / CB_LANES)
 
-template <typename T, int W>
-__global__ void __launch_bounds__(CC_BLOCK) cc_bwd_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ dy,
-                                                          int D, CcSeq q, const float* __restrict__ weight,
-                                                          const float* __restrict__ bias, const T* __restrict__ past, int act,
-                                                          T* __restrict__ dx, float* __restrict__ parts) {
-  constexpr int N = CcBwdTokens<T>::n, ROWS = N + W - 1;
-  const int groups = D / 8, cl = threadIdx.x & 15, run = threadIdx.x >> 4;
-  const int cg = blockIdx.x * 16 + cl, c0 = cg * 8;
-  const bool on = cg < groups;
-  float w[W][8], bv[8], dw[W][8], db[8];
+template <typename T>
+struct CbRaw { typedef T vec __attribute__((ext_vector_type(CB_CH))); };
+
+// One run of tokens of one thread. EDGE: a sequence may begin or end among the rows that are looked at (t0 - (W-1) .. t0 +
+// CB_TOKENS + W-2); without, no row is masked.
+template <typename T, int W, bool EDGE>
+__device__ __forceinline__ void cc_bwd_run(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ dy, int D, const CcSeq& q,
+                                           const float (&w)[W][CB_CH], const float (&bv)[CB_CH], const T* __restrict__ past, int act,
+                                           T* __restrict__ dx, int64_t t0, int c0, int seq, int64_t b, int64_t e,
+                                           float (&dw)[W][CB_CH], float (&db)[CB_CH]) {
+  typedef typename CbRaw<T>::vec raw;
+  constexpr int ROWS = CB_TOKENS + W - 1, GROUPS = (ROWS + 3) / 4;
+  float win[W][CB_CH], dpre[W][CB_CH];  // x of the last W rows; dpre of the last W tokens
+  int64_t begins[W];                    // where the sequences of the last W tokens begin
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    bv[c] = on && bias ? bias[c0 + c] : 0.0f;
-    db[c] = 0.0f;
+  for (int r = 0; r < W; ++r) {
+    begins[r] = 0;
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      w[j][c] = on ? weight[(int64_t)(c0 + c) * W + j] : 0.0f;
-      dw[j][c] = 0.0f;
+    for (int c = 0; c < CB_CH; ++c) win[r][c] = dpre[r][c] = 0.0f;
+  }
+  raw rx[2][4], ry[2][4];
+  auto fetch = [&](int group) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = 4 * group + k;
+      if (i >= ROWS) continue;
+      int64_t t = t0 + i;
+      if (EDGE && t >= q.n_tokens) t = q.n_tokens - 1;  // not used
+      rx[group & 1][k] = *reinterpret_cast<const raw*>(x + t * x_stride + c0);
+      ry[group & 1][k] = *reinterpret_cast<const raw*>(dy + t * D + c0);
+    }
+  };
+  fetch(0);
+#pragma unroll
+  for (int r = 0; r < W - 1; ++r) {
+    const int64_t t = t0 - (W - 1) + r;
+    if (!EDGE || t >= 0) {
+      const raw v = *reinterpret_cast<const raw*>(x + t * x_stride + c0);
+#pragma unroll
+      for (int c = 0; c < CB_CH; ++c) win[r + 1][c] = GdrElem<T>::to_float(v[c]);
     }
   }
-  for (int64_t t0 = ((int64_t)blockIdx.y * 16 + run) * N; t0 < q.n_tokens && on; t0 += (int64_t)gridDim.y * 16 * N) {
-    // x[t0 - (W-1) .. t0 + N + W-2] and dy[t0 .. t0 + N + W-2], in a sliding window: tokens past the run are needed for dx
-    float win[W][8], dpre[W][8];  // x of the last W rows; dpre of the last W tokens
 #pragma unroll
-    for (int r = 0; r < W; ++r)
+  for (int group = 0; group < GROUPS; ++group) {
+    if (group + 1 < GROUPS) fetch(group + 1);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) win[r][c] = dpre[r][c] = 0.0f;
-    int seq = cc_seq_of(q, t0);
-    int64_t b = cc_bound(q, seq), e = cc_bound(q, seq + 1);
-#pragma unroll
-    for (int r = 0; r < W - 1; ++r) {
-      const int64_t t = t0 - (W - 1) + r;
-      if (t >= 0) load8(x + t * x_stride + c0, win[r + 1]);
-    }
-    int64_t begins[W];            // where the sequences of the last W tokens begin
-#pragma unroll
-    for (int r = 0; r < W; ++r) begins[r] = 0;
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
+    for (int k = 0; k < 4; ++k) {
+      const int i = 4 * group + k;
+      if (i >= ROWS) continue;
       const int64_t t = t0 + i;
 #pragma unroll
       for (int r = 0; r + 1 < W; ++r) {
         begins[r] = begins[r + 1];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) { win[r][c] = win[r + 1][c]; dpre[r][c] = dpre[r + 1][c]; }
+        for (int c = 0; c < CB_CH; ++c) { win[r][c] = win[r + 1][c]; dpre[r][c] = dpre[r + 1][c]; }
       }
-      if (t < q.n_tokens) {
-        load8(x + t * x_stride + c0, win[W - 1]);
-        float g[8];
-        load8(dy + t * D + c0, g);
-        if (t >= e) {
+      if (!EDGE || t < q.n_tokens) {
+        if (EDGE && t >= e) {
           seq = cc_seq_of(q, t);
           b = cc_bound(q, seq);
           e = cc_bound(q, seq + 1);
         }
         begins[W - 1] = b;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < CB_CH; ++c) {
+          win[W - 1][c] = GdrElem<T>::to_float(rx[group & 1][k][c]);
           float taps[W], pre = 0.0f;
 #pragma unroll
           for (int j = 0; j < W; ++j) {
             const int64_t src = t - (W - 1) + j;
             taps[j] = win[j][c];
-            if (src < b)
+            if (EDGE && src < b)
               taps[j] = past && seq < q.n_seq ? GdrElem<T>::to_float(past[((int64_t)seq * D + c0 + c) * W + W + (src - b)]) : 0.0f;
             pre = __builtin_fmaf(taps[j], w[j][c], pre);
           }
           pre += bv[c];
-          float d = seq < q.n_seq ? g[c] : 0.0f;
+          float d = !EDGE || seq < q.n_seq ? GdrElem<T>::to_float(ry[group & 1][k][c]) : 0.0f;
           if (act) {
             const float s = cc_sigmoid(pre);
             d *= s * __builtin_fmaf(pre, 1.0f - s, 1.0f);
           }
           dpre[W - 1][c] = d;
-          if (i < N) {
+          if (i < CB_TOKENS) {
             db[c] += d;
 #pragma unroll
             for (int j = 0; j < W; ++j) dw[j][c] = __builtin_fmaf(d, taps[j], dw[j][c]);
@@ -234,56 +251,77 @@ __global__ void __launch_bounds__(CC_BLOCK) cc_bwd_kernel(const T* __restrict__ 
       } else {
         begins[W - 1] = INT64_MAX;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) win[W - 1][c] = dpre[W - 1][c] = 0.0f;
+        for (int c = 0; c < CB_CH; ++c) win[W - 1][c] = dpre[W - 1][c] = 0.0f;
       }
       const int64_t s = t - (W - 1);
-      if (i >= W - 1 && s < q.n_tokens) {  // dx of token s: dpre[r] belongs to token s + r
-        float out[8];
+      if (i >= W - 1 && (!EDGE || s < q.n_tokens)) {  // dx of token s: dpre[r] belongs to token s + r
+        raw out;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < CB_CH; ++c) {
           float v = 0.0f;
 #pragma unroll
-          for (int r = 0; r < W; ++r) v = __builtin_fmaf(begins[r] <= s ? dpre[r][c] : 0.0f, w[W - 1 - r][c], v);
-          out[c] = v;
+          for (int r = 0; r < W; ++r) v = __builtin_fmaf(!EDGE || begins[r] <= s ? dpre[r][c] : 0.0f, w[W - 1 - r][c], v);
+          out[c] = GdrElem<T>::from_float(v);
         }
-        T* dst = dx + s * D + c0;
-        if constexpr (sizeof(T) == 2) {
-          typedef T vec8 __attribute__((ext_vector_type(8)));
-          vec8 o;
-#pragma unroll
-          for (int c = 0; c < 8; ++c) o[c] = GdrElem<T>::from_float(out[c]);
-          *reinterpret_cast<vec8*>(dst) = o;
-        } else {
-          *reinterpret_cast<f32x4*>(dst) = f32x4{out[0], out[1], out[2], out[3]};
-          *reinterpret_cast<f32x4*>(dst + 4) = f32x4{out[4], out[5], out[6], out[7]};
-        }
+        *reinterpret_cast<raw*>(dx + s * D + c0) = out;
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
-  // over the 16 runs: 4 in a wave, then the 4 waves
-  __shared__ float red[4][16][8 * (W + 1)];
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(CC_BLOCK) cc_bwd_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ dy,
+                                                          int D, CcSeq q, const float* __restrict__ weight,
+                                                          const float* __restrict__ bias, const T* __restrict__ past, int act,
+                                                          T* __restrict__ dx, float* __restrict__ parts) {
+  constexpr int ROWS = CB_TOKENS + W - 1;
+  const int groups = D / CB_CH, cl = threadIdx.x % CB_LANES, run = threadIdx.x / CB_LANES;
+  const int cg = blockIdx.x * CB_LANES + cl, c0 = cg * CB_CH;
+  const bool on = cg < groups;
+  float w[W][CB_CH], bv[CB_CH], dw[W][CB_CH], db[CB_CH];
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
+  for (int c = 0; c < CB_CH; ++c) {
+    bv[c] = on && bias ? bias[c0 + c] : 0.0f;
+    db[c] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      w[j][c] = on ? weight[(int64_t)(c0 + c) * W + j] : 0.0f;
+      dw[j][c] = 0.0f;
+    }
+  }
+  for (int64_t t0 = ((int64_t)blockIdx.y * CB_RUNS + run) * CB_TOKENS; t0 < q.n_tokens && on;
+       t0 += (int64_t)gridDim.y * CB_RUNS * CB_TOKENS) {
+    const int seq = cc_seq_of(q, t0);
+    const int64_t b = cc_bound(q, seq), e = cc_bound(q, seq + 1);
+    if (__all(seq < q.n_seq && t0 - (W - 1) >= b && t0 + ROWS <= e))
+      cc_bwd_run<T, W, false>(x, x_stride, dy, D, q, w, bv, past, act, dx, t0, c0, seq, b, e, dw, db);
+    else
+      cc_bwd_run<T, W, true>(x, x_stride, dy, D, q, w, bv, past, act, dx, t0, c0, seq, b, e, dw, db);
+  }
+  // over the 8 runs: 2 in a wave, then the 4 waves
+  __shared__ float red[4][CB_LANES][CB_CH * (W + 1)];
+#pragma unroll
+  for (int c = 0; c < CB_CH; ++c)
 #pragma unroll
     for (int j = 0; j <= W; ++j) {
       float v = j < W ? dw[j < W ? j : 0][c] : db[c];
-      v += __shfl_xor(v, 16);
-      v += __shfl_xor(v, 32);
-      if ((threadIdx.x & 63) < 16) red[threadIdx.x >> 6][cl][c * (W + 1) + j] = v;
+      v += __shfl_xor(v, CB_LANES);
+      if ((threadIdx.x & 63) < CB_LANES) red[threadIdx.x >> 6][cl][c * (W + 1) + j] = v;
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * 8 * (W + 1); i += CC_BLOCK) {
-    const int g = i / (8 * (W + 1)), k = i % (8 * (W + 1));
-    if (blockIdx.x * 16 + g < groups)
-      parts[((int64_t)blockIdx.y * D + (blockIdx.x * 16 + g) * 8) * (W + 1) + k] =
+  for (int i = threadIdx.x; i < CB_LANES * CB_CH * (W + 1); i += CC_BLOCK) {
+    const int g = i / (CB_CH * (W + 1)), k = i % (CB_CH * (W + 1));
+    if (blockIdx.x * CB_LANES + g < groups)
+      parts[((int64_t)blockIdx.y * D + (blockIdx.x * CB_LANES + g) * CB_CH) * (W + 1) + k] =
           (red[0][g][k] + red[1][g][k]) + (red[2][g][k] + red[3][g][k]);
   }
 }
 
-// Workgroups along the tokens, so that about four a CU are left where there are tokens enough.
-static int cc_bwd_runs(int64_t n_tokens, int D, int dtype) {
-  const int64_t per = 16 * (dtype == GDR_FP32 ? 8 : 16);
-  const int64_t need = (n_tokens + per - 1) / per, most = 1280 / ((D / 8 + 15) / 16) + 1;
+// Workgroups along the tokens: eight a CU over the whole call where there are tokens enough (each leaves a row of sums).
+static int cc_bwd_runs(int64_t n_tokens, int D) {
+  const int64_t need = (n_tokens + CB_RUNS * CB_TOKENS - 1) / (CB_RUNS * CB_TOKENS);
+  const int64_t most = 2048 / ((D / CB_CH + CB_LANES - 1) / CB_LANES) + 1;
   return (int)(need < 1 ? 1 : (need < most ? need : most));
 }
 
@@ -368,13 +406,13 @@ extern "C" int lampa_causal_conv1d_step(const void* x, int64_t x_stride, const v
 
 extern "C" int64_t lampa_causal_conv1d_bwd_workspace_bytes(int64_t n_tokens, int D, int W, int dtype) {
   if (n_tokens < 0 || D < 8 || D % 8 || W < 1 || W > CC_MAX_W || dtype < 0 || dtype > 2) return LAMPA_ERR_INVALID;
-  return (int64_t)cc_bwd_runs(n_tokens, D, dtype) * D * (W + 1) * 4;
+  return (int64_t)cc_bwd_runs(n_tokens, D) * D * (W + 1) * 4;
 }
 
 template <typename T>
 static int cc_bwd_launch(const void* x, int64_t x_stride, const void* dy, int D, int W, CcSeq q, const float* weight,
                          const float* bias, const void* past, int act, void* dx, float* parts, int runs, hipStream_t s) {
-  const dim3 grid((unsigned)((D / 8 + 15) / 16), (unsigned)runs);
+  const dim3 grid((unsigned)((D / CB_CH + CB_LANES - 1) / CB_LANES), (unsigned)runs);
   LAMPA_PROF(s, "start");
 #define CC_GO(WW)                                                                                                            \
   case WW:                                                                                                                   \
@@ -396,7 +434,7 @@ extern "C" int lampa_causal_conv1d_bwd(const void* x, int64_t x_stride, const vo
   if (!dweight_bias || (n_tokens && (!dy || !dx || ((uintptr_t)dy | (uintptr_t)dx) % 16))) return LAMPA_ERR_INVALID;
   if (!workspace || workspace_bytes < lampa_causal_conv1d_bwd_workspace_bytes(n_tokens, D, W, dtype)) return LAMPA_ERR_WORKSPACE;
   const CcSeq q{cu_seqlens, n_seq, seq_len, n_tokens};
-  const int runs = cc_bwd_runs(n_tokens, D, dtype);
+  const int runs = cc_bwd_runs(n_tokens, D);
   float* parts = (float*)workspace;
   hipStream_t s = (hipStream_t)stream;
   int e;
@@ -407,5 +445,5 @@ extern "C" int lampa_causal_conv1d_bwd(const void* x, int64_t x_stride, const vo
   }
   if (e != LAMPA_OK) return e;
   const int64_t cols = (int64_t)D * (W + 1);
-  return row_sums_launch<float>(parts, runs, cols, cols, 0, 1, dweight_bias, 0, s);
+  return row_sums_launch<float>(parts, runs, cols, cols, 0, 1, RowSumsOut<float>{{dweight_bias, nullptr, nullptr}, 0}, s);
 }

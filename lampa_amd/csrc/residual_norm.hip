@@ -43,6 +43,21 @@ __device__ __forceinline__ void rn_store8(T* p, const float* v) {
   }
 }
 
+// 8 consecutive elements as loaded.
+template <typename T>
+struct RnRaw {
+  typedef T vec __attribute__((ext_vector_type(sizeof(T) == 2 ? 8 : 4)));
+  vec v[sizeof(T) == 2 ? 1 : 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int k = 0; k < (sizeof(T) == 2 ? 1 : 2); ++k) v[k] = reinterpret_cast<const vec*>(p)[k];
+  }
+  __device__ __forceinline__ void get(float* out) const {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) out[c] = GdrElem<T>::to_float(sizeof(T) == 2 ? v[0][c] : v[c / 4 < (sizeof(T) == 2 ? 1 : 2) ? c / 4 : 0][c % 4]);
+  }
+};
+
 // Sum over the lanes of a row (every lane gets it). `part`: LDS of 2 x 4 floats for rows of a whole workgroup; `turn`
 // alternates, so that one barrier a sum is enough.
 template <int LPR>
@@ -84,10 +99,28 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
 #pragma unroll
       for (int c = 0; c < 8; ++c) dw[st][c] = dpw[st][c] = dsc[st][c] = dga[st][c] = 0.0f;
   }
+  // The next row's operands are requested while this one is worked on, where they fit the registers (one stride a row).
+  constexpr bool AHEAD = GRAD && STEPS == 1;
+  RnRaw<T> nx, ng, ndy;
+  RnRaw<RT> nh, ndr;
+  auto request = [&](int64_t r0) {
+    const int c0 = sub * 8;
+    if (!(r0 + slot < n_rows && c0 < a.D)) return;
+    const int64_t row = row_base + r0 + slot, at = row * a.D + c0;
+    nx.load((const T*)a.x + at);
+    nh.load((const RT*)a.residual + at);
+    if (a.gate_kind) ng.load((const T*)a.gate + (a.gate_kind == RN_GATE_SEQ ? row / a.seq_rows : row) * a.D + c0);
+    if (a.dy) ndy.load((const T*)a.dy + at);
+    if (a.dres) ndr.load((const RT*)a.dres + at);
+  };
+  if (AHEAD) request((int64_t)blockIdx.x * ROWS);
   // every thread makes the same number of turns: rows past the end are worked on as zeros and not stored
   for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < n_rows; r0 += stride) {
     const bool live = r0 + slot < n_rows;
     const int64_t row = row_base + r0 + slot;
+    const RnRaw<T> cx = nx, cg = ng, cdy = ndy;
+    const RnRaw<RT> ch = nh, cdr = ndr;
+    if (AHEAD) request(r0 + stride);
     float x[STEPS][8], h[STEPS][8], sq = 0.0f;
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
@@ -96,8 +129,13 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
 #pragma unroll
       for (int c = 0; c < 8; ++c) x[st][c] = h[st][c] = 0.0f;
       if (on) {
-        load8((const T*)a.x + row * a.D + c0, x[st]);
-        load8((const RT*)a.residual + row * a.D + c0, h[st]);
+        if constexpr (AHEAD) {
+          cx.get(x[st]);
+          ch.get(h[st]);
+        } else {
+          load8((const T*)a.x + row * a.D + c0, x[st]);
+          load8((const RT*)a.residual + row * a.D + c0, h[st]);
+        }
       }
 #pragma unroll
       for (int c = 0; c < 8; ++c) sq = __builtin_fmaf(x[st][c], x[st][c], sq);
@@ -115,7 +153,10 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
 #pragma unroll
       for (int c = 0; c < 8; ++c) { pw[c] = 1.0f; g[c] = 1.0f; sc[c] = 1.0f; }
       if (on && a.post_weight) load8(a.post_weight + c0, pw);
-      if (on && a.gate_kind) load8((const T*)a.gate + gate_row * a.D + c0, g);
+      if (on && a.gate_kind) {
+        if constexpr (AHEAD) cg.get(g);
+        else load8((const T*)a.gate + gate_row * a.D + c0, g);
+      }
       if (on && a.scale) load8(a.scale + c0, sc);
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
@@ -154,7 +195,10 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
         float w[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) { dh[st][c] = 0.0f; w[c] = 1.0f; }
-        if (on && a.dy) load8((const T*)a.dy + row * a.D + c0, dh[st]);
+        if (on && a.dy) {
+          if constexpr (AHEAD) cdy.get(dh[st]);
+          else load8((const T*)a.dy + row * a.D + c0, dh[st]);
+        }
         if (on && a.weight) load8(a.weight + c0, w);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -173,7 +217,10 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
         float dr[8], sc[8], pw[8], dg[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) { dr[c] = 0.0f; sc[c] = 1.0f; pw[c] = 1.0f; }
-        if (on && a.dres) load8((const RT*)a.dres + row * a.D + c0, dr);
+        if (on && a.dres) {
+          if constexpr (AHEAD) cdr.get(dr);
+          else load8((const RT*)a.dres + row * a.D + c0, dr);
+        }
         if (on && a.scale) load8(a.scale + c0, sc);
         if (on && a.post_weight) load8(a.post_weight + c0, pw);
 #pragma unroll
@@ -367,18 +414,19 @@ extern "C" int lampa_residual_norm_bwd(const void* x, const void* residual, cons
   const int64_t per_seq = rn_grad_blocks(seq_rows, n_seq, lpr);
   hipStream_t s = (hipStream_t)stream;
   rc = rn_types<true>(a, dtype, res_dtype, lpr, steps, dim3((unsigned)per_seq, (unsigned)n_seq), s);
-  // [n_seq, per_seq, n_sums, D]: a weight's sums are columns of rows of n_sums * D
+  // [n_seq, per_seq, n_sums, D]: a weight's sums are columns of rows of n_sums * D, the weights' ones side by side
   const int64_t width = (int64_t)a.n_sums * D;
-  float* const outs[3] = {dweight, dpost_weight, dscale};
-  const int ats[3] = {a.at_weight, a.at_post, a.at_scale};
-  for (int i = 0; i < 3 && rc == LAMPA_OK; ++i)
-    if (outs[i]) rc = row_sums_launch<float>(a.parts + (int64_t)ats[i] * D, n_seq * per_seq, D, width, 0, 1, outs[i], 0, s);
+  RowSumsOut<float> to = {{nullptr, nullptr, nullptr}, 0};
+  int sets = 0;
+  for (float* out : {dweight, dpost_weight, dscale})
+    if (out) to.out[sets++] = out;
+  if (rc == LAMPA_OK && sets) rc = row_sums_launch<float>(a.parts, n_seq * per_seq, D, width, D, sets, to, s);
   if (rc == LAMPA_OK && a.at_gate >= 0) {
     const float* src = a.parts + (int64_t)a.at_gate * D;
     const int64_t set = per_seq * width;
-    if (dtype == GDR_BF16) rc = row_sums_launch<__bf16>(src, per_seq, D, width, set, (int)n_seq, (__bf16*)dgate, D, s);
-    else if (dtype == GDR_FP16) rc = row_sums_launch<_Float16>(src, per_seq, D, width, set, (int)n_seq, (_Float16*)dgate, D, s);
-    else rc = row_sums_launch<float>(src, per_seq, D, width, set, (int)n_seq, (float*)dgate, D, s);
+    if (dtype == GDR_BF16) rc = row_sums_launch<__bf16>(src, per_seq, D, width, set, (int)n_seq, RowSumsOut<__bf16>{{(__bf16*)dgate, nullptr, nullptr}, D}, s);
+    else if (dtype == GDR_FP16) rc = row_sums_launch<_Float16>(src, per_seq, D, width, set, (int)n_seq, RowSumsOut<_Float16>{{(_Float16*)dgate, nullptr, nullptr}, D}, s);
+    else rc = row_sums_launch<float>(src, per_seq, D, width, set, (int)n_seq, RowSumsOut<float>{{(float*)dgate, nullptr, nullptr}, D}, s);
   }
   return rc;
 }
