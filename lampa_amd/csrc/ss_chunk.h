@@ -9,8 +9,8 @@
 //
 // Rounding: B, C, x (and dy) enter as they are. The pair weights are rounded once to the input type, as any operand of the
 // matrix cores has to be; they carry the same relative error as the output's own rounding. The state and the decayed x enter as
-// two operands of the input type each, value and remainder (2^-17 of the value is left in bf16): the state is handed from
-// chunk to chunk and out to the caller in fp32, and its sums are what the gradient of the decays is made of.
+// two or three operands of the input type each, value and remainders (ScParts): the state is handed from chunk to chunk and out
+// to the caller in fp32, and its sums are what the gradient of the decays is made of.
 #pragma once
 #include "ss_kernels.h"
 
@@ -21,13 +21,21 @@ using sc_x8 = typename OpVec<T>::x8;
 template <typename T>
 using sc_x4 = typename OpVec<T>::x4;
 
-// v as an operand value and the operand value of what that leaves out. v is taken out of the compiler's sight: it would form an
-// fp16 `hi` of a product in one rounding and the remainder from one of two, which now and then (ties) is another value.
+// An fp32 value as a sum of operand values: fp16 has it to 2^-22 in two, bf16 to 2^-17 in two and whole in three. Three go in
+// wherever a state or adjoint that is handed on, or a sum that dA and d dt_bias are made of, comes out; two where the product
+// itself is rounded to the input type.
 template <typename T>
-__device__ __forceinline__ void sc_split(float v, T& hi, T& lo) {
+struct ScParts { static const int n = __is_same(T, __bf16) ? 3 : 2; };
+// v is taken out of the compiler's sight: it would form an fp16 `hi` of a product in one rounding and the remainder from one of
+// two, which now and then (ties) is another value.
+template <typename T, int PARTS>
+__device__ __forceinline__ void sc_split(float v, T (&part)[PARTS]) {
   if constexpr (__is_same(T, _Float16)) asm("" : "+v"(v));
-  hi = (T)v;
-  lo = (T)(v - (float)hi);
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k) {
+    part[k] = (T)v;
+    v -= (float)part[k];
+  }
 }
 
 // fp16 has no room for every fp32 value: operands made from fp32 are scaled by a power of two that brings the largest of
@@ -182,28 +190,41 @@ __device__ __forceinline__ void sc_row_weights(const float* w, int kk, int lane,
 #pragma unroll
   for (int e = 0; e < 4; ++e) { out[e] = a[e]; out[4 + e] = b[e]; }
 }
-// A weighted operand in two parts.
-template <typename T>
-__device__ __forceinline__ void sc_weighted(const sc_x8<T>& x, const float (&w)[8], sc_x8<T>& hi, sc_x8<T>& lo) {
+// A weighted operand in parts.
+template <typename T, int PARTS>
+__device__ __forceinline__ void sc_weighted(const sc_x8<T>& x, const float (&w)[8], sc_x8<T> (&out)[PARTS]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    T h, l;
-    sc_split<T>((float)x[e] * w[e], h, l);
-    hi[e] = h;
-    lo[e] = l;
+    T part[PARTS];
+    sc_split<T, PARTS>((float)x[e] * w[e], part);
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) out[k][e] = part[k];
   }
 }
-// Two accumulator tiles (32 rows) as an operand in two parts.
-template <typename T>
-__device__ __forceinline__ void sc_state_operand(const f32x4& a, const f32x4& b, float scale, sc_x8<T>& hi, sc_x8<T>& lo) {
+// Two accumulator tiles (32 rows) as an operand in parts.
+template <typename T, int PARTS>
+__device__ __forceinline__ void sc_state_operand(const f32x4& a, const f32x4& b, float scale, sc_x8<T> (&out)[PARTS]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float v = e < 4 ? a[e] : b[e - 4];
-    T h, l;
-    sc_split<T>(__is_same(T, _Float16) ? v * scale : v, h, l);
-    hi[e] = h;
-    lo[e] = l;
+    T part[PARTS];
+    sc_split<T, PARTS>(__is_same(T, _Float16) ? v * scale : v, part);
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) out[k][e] = part[k];
   }
+}
+// acc + left * (the operand's parts), the smallest first
+template <typename X8, int PARTS>
+__device__ __forceinline__ f32x4 sc_mfma_left(const X8& left, const X8 (&right)[PARTS], f32x4 acc) {
+#pragma unroll
+  for (int k = PARTS - 1; k >= 0; --k) acc = mfma16(left, right[k], acc);
+  return acc;
+}
+template <typename X8, int PARTS>
+__device__ __forceinline__ f32x4 sc_mfma_right(const X8 (&left)[PARTS], const X8& right, f32x4 acc) {
+#pragma unroll
+  for (int k = PARTS - 1; k >= 0; --k) acc = mfma16(left[k], right, acc);
+  return acc;
 }
 
 // Whether every row of a call can be read in 16-byte pieces and written in 8-byte ones (the kernels are built for both: their

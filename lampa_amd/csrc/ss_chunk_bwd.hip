@@ -26,6 +26,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
   constexpr bool F16 = __is_same(T, _Float16);
   typedef sc_x8<T> x8;
   typedef sc_x4<T> x4;
+  constexpr int PARTS = ScParts<T>::n;
   const SsSegment seg = ss_segment(a, blockIdx.x);
   if (!seg.live) return;
   const int npb = (a.P + 63) / 64, pb = blockIdx.y % npb, h = blockIdx.y / npb, grp = h / (a.H / a.G);
@@ -204,12 +205,12 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         sc_fence();
-        x8 hi, lo;
-        sc_state_operand<T>(R[2 * kk], R[2 * kk + 1], sc, hi, lo);
+        x8 st8[PARTS];
+        sc_state_operand<T, PARTS>(R[2 * kk], R[2 * kk + 1], sc, st8);
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
           const x8 q = *reinterpret_cast<const x8*>(tb + (16 * st + i) * KS + 32 * kk + 8 * g);
-          acc[st] = mfma16(hi, q, mfma16(lo, q, acc[st]));
+          acc[st] = sc_mfma_right(st8, q, acc[st]);
         }
       }
 #pragma unroll
@@ -279,19 +280,19 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
           sc_fence();
-          x8 hi, lo;
-          sc_state_operand<T>(RT[2 * kk][j], RT[2 * kk + 1][j], s1, hi, lo);
+          x8 adj[2], state[PARTS];
+          sc_state_operand<T, 2>(RT[2 * kk][j], RT[2 * kk + 1][j], s1, adj);
 #pragma unroll
           for (int st = 0; st < 4; ++st) {
             const x8 q = *reinterpret_cast<const x8*>(tx + (16 * st + i) * VS + 32 * kk + 8 * g);
-            db[st] = mfma16(hi, q, mfma16(lo, q, db[st]));
+            db[st] = sc_mfma_right(adj, q, db[st]);
           }
           sc_fence();
-          sc_state_operand<T>(S[2 * kk], S[2 * kk + 1], s2, hi, lo);
+          sc_state_operand<T, PARTS>(S[2 * kk], S[2 * kk + 1], s2, state);
 #pragma unroll
           for (int tt = 0; tt < 4; ++tt) {
             const x8 q = *reinterpret_cast<const x8*>(ty + (16 * tt + i) * VS + 32 * kk + 8 * g);
-            dc[tt] = mfma16(hi, q, mfma16(lo, q, dc[tt]));
+            dc[tt] = sc_mfma_right(state, q, dc[tt]);
           }
         }
 #pragma unroll
@@ -395,26 +396,26 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
           for (int e = 0; e < 8; ++e) wt[kk][e] *= s;
       }
-      auto add = [&](f32x4& acc, const x8 (&left)[2], const x8 (&hi)[2], const x8 (&lo)[2]) {
+      auto add = [&](f32x4& acc, const x8 (&left)[2], const x8 (&right)[2][PARTS]) {
         if constexpr (F16) {
           f32x4 d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk) d = mfma16(left[kk], hi[kk], mfma16(left[kk], lo[kk], d));
+          for (int kk = 0; kk < 2; ++kk) d = sc_mfma_left(left[kk], right[kk], d);
           acc = acc * end + d * back;
         } else {
           acc *= end;
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk) acc = mfma16(left[kk], hi[kk], mfma16(left[kk], lo[kk], acc));
+          for (int kk = 0; kk < 2; ++kk) acc = sc_mfma_left(left[kk], right[kk], acc);
         }
       };
-      x8 v[2], hi[2], lo[2], left[2];
+      x8 v[2], vw[2][PARTS], left[2];
       sc_columns<T>(ty, VS, 16 * wave, lane, v);
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) sc_weighted<T>(v[kk], wt[kk], hi[kk], lo[kk]);
+      for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         sc_columns<T>(tc, KS, 16 * nt, lane, left);
-        add(R[nt], left, hi, lo);
+        add(R[nt], left, vw);
         sc_fence();
       }
       if (has_n) {
@@ -422,11 +423,11 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
         for (int j = 0; j < NW; ++j) {
           sc_columns<T>(tc, KS, 16 * (nt0 + j), lane, v);
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk) sc_weighted<T>(v[kk], wt[kk], hi[kk], lo[kk]);
+          for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
 #pragma unroll
           for (int pt = 0; pt < 4; ++pt) {
             sc_columns<T>(ty, VS, 16 * pt, lane, left);
-            add(RT[pt][j], left, hi, lo);
+            add(RT[pt][j], left, vw);
             sc_fence();
           }
           sc_fence();
@@ -437,12 +438,32 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
     if (wave == 0) {  // lane = token: what passes across it
       const float d = dec.delta[lane];
       const float col = col_sum[lane];
-      const float row = (row_part[0][lane] + row_part[1][lane]) + (row_part[2][lane] + row_part[3][lane]);
+      const float r0 = row_part[0][lane], r1 = row_part[1][lane], r2 = row_part[2][lane], r3 = row_part[3][lane];
       const float left = (left_part[0][lane] + left_part[1][lane]) + (left_part[2][lane] + left_part[3][lane]);
       const float read = (read_part[0][lane] + read_part[1][lane]) + (read_part[2][lane] + read_part[3][lane]);
       const float all = end * ((dot_part[0] + dot_part[1]) + (dot_part[2] + dot_part[3]));
-      float before = d * (col + left) - row;  // summed over the tokens before this one ...
-      float later = read;                     // ... and this over this one and those behind it
+      // Pairs across the first token of each 16: of the tiles of pairs, those of later tokens with earlier ones ...
+      const int tile = lane >> 4;
+      const float from0 = sc_row16_sum(r0), from1 = sc_row16_sum(r1), from2 = sc_row16_sum(r2);
+      float across1 = tile >= 1 ? from0 : 0.0f, across2 = tile >= 2 ? from0 + from1 : 0.0f,
+            across3 = tile >= 3 ? (from0 + from1) + from2 : 0.0f;
+#pragma unroll
+      for (int off = 16; off < 64; off <<= 1) {
+        across1 += __shfl_xor(across1, off);
+        across2 += __shfl_xor(across2, off);
+        across3 += __shfl_xor(across3, off);
+      }
+      // ... and from there on a prefix sum of column minus row sums. (Over all 64 tokens its rounding errors, which stay in every
+      // later token, are 3e-6 of dA and d dt_bias.)
+      float pairs = d * col - ((r0 + r1) + (r2 + r3));
+      pairs += dpp_f32<GDR_DPP_ROW_SHR(1), 0xF>(0.0f, pairs);
+      pairs += dpp_f32<GDR_DPP_ROW_SHR(2), 0xF>(0.0f, pairs);
+      pairs += dpp_f32<GDR_DPP_ROW_SHR(4), 0xF>(0.0f, pairs);
+      pairs += dpp_f32<GDR_DPP_ROW_SHR(8), 0xF>(0.0f, pairs);
+      pairs = dpp_f32<GDR_DPP_ROW_SHR(1), 0xF>(0.0f, pairs);
+      pairs += tile == 0 ? 0.0f : tile == 1 ? across1 : tile == 2 ? across2 : across3;
+      float before = d * left;  // summed over the tokens before this one ...
+      float later = read;       // ... and this over this one and those behind it
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
         const float up = __shfl_up(before, off), down = __shfl_down(later, off);
@@ -453,7 +474,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
       if (lane == 0) before = 0.0f;
       if (lane < n_tok) {
         const int64_t at = (t0 + lane) * parts + blockIdx.y;
-        w.dg[at] = before + later + all;
+        w.dg[at] = (pairs + before) + (later + all);
         w.reach[at] = col + diag[lane] + left;
       }
     }

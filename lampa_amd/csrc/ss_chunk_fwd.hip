@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
     if (c + 1 < chunks) fetch(c + 1);
     const float end = dec.end;
     sum += dec.sum;
-    sc_x8<T> v[2], hi[2], lo[2];
+    constexpr int PARTS = ScParts<T>::n;
+    sc_x8<T> v[2], vw[2][PARTS];
     sc_columns<T>(tv, VS, 16 * wave, lane, v);
     float wt[2][8], back = 1.0f;
 #pragma unroll
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
         for (int e = 0; e < 8; ++e) wt[kk][e] *= s;
     }
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) sc_weighted<T>(v[kk], wt[kk], hi[kk], lo[kk]);
+    for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       sc_x8<T> k[2];
@@ -103,12 +104,12 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
       if constexpr (__is_same(T, _Float16)) {
         f32x4 d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) d = mfma16(k[kk], hi[kk], mfma16(k[kk], lo[kk], d));
+        for (int kk = 0; kk < 2; ++kk) d = sc_mfma_left(k[kk], vw[kk], d);
         S[nt] = S[nt] * end + d * back;
       } else {
         S[nt] *= end;
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) S[nt] = mfma16(k[kk], hi[kk], mfma16(k[kk], lo[kk], S[nt]));
+        for (int kk = 0; kk < 2; ++kk) S[nt] = sc_mfma_left(k[kk], vw[kk], S[nt]);
       }
     }
     lds_barrier();
@@ -148,6 +149,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
   const T* xb = (const T*)a.x + (int64_t)h * a.P + 64 * pb;
   const float A = a.A[h], D = a.D ? a.D[h] : 0.0f, bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
   const bool single = (a.cu_seqlens ? a.n_tokens : a.seq_len) <= a.seg_tokens;
+  const bool handed_on = single && a.ht;
   const int p = 64 * pb + 16 * wave + (lane0 & 15);
 
   f32x4 S[NT];
@@ -256,12 +258,12 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
       for (int tt = 0; tt < 4; ++tt) y[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
-        sc_x8<T> hi, lo;
-        sc_state_operand<T>(S[2 * kk], S[2 * kk + 1], s, hi, lo);
+        sc_x8<T> st[2];
+        sc_state_operand<T, 2>(S[2 * kk], S[2 * kk + 1], s, st);
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
           const sc_x8<T> q = *reinterpret_cast<const sc_x8<T>*>(tc + (16 * tt + i) * KS + 32 * kk + 8 * g);
-          y[tt] = mfma16(hi, q, mfma16(lo, q, y[tt]));
+          y[tt] = sc_mfma_right(st, q, y[tt]);
         }
       }
     }
@@ -320,9 +322,11 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) wt[kk][e] *= s;
       }
-      sc_x8<T> hi[2], lo[2];
+      // the third part only where the state goes to the caller
+      constexpr int PARTS = ScParts<T>::n;
+      sc_x8<T> vw[2][PARTS];
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) sc_weighted<T>(v[kk], wt[kk], hi[kk], lo[kk]);
+      for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
       const float end = dec.end;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -331,12 +335,15 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
         if constexpr (__is_same(T, _Float16)) {
           f32x4 d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk) d = mfma16(k[kk], hi[kk], mfma16(k[kk], lo[kk], d));
+          for (int kk = 0; kk < 2; ++kk) d = sc_mfma_left(k[kk], vw[kk], d);
           S[nt] = S[nt] * end + d * back;
         } else {
           S[nt] *= end;
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk) S[nt] = mfma16(k[kk], hi[kk], mfma16(k[kk], lo[kk], S[nt]));
+          for (int kk = 0; kk < 2; ++kk) {
+            if (handed_on) S[nt] = mfma16(k[kk], vw[kk][2], S[nt]);
+            S[nt] = mfma16(k[kk], vw[kk][0], mfma16(k[kk], vw[kk][1], S[nt]));
+          }
         }
       }
     }
