@@ -78,6 +78,12 @@ struct ScTile {
   __device__ __forceinline__ void fetch(const T* base, int64_t stride, int n, int cols) {
     const int row0 = threadIdx.x / (W / 8), c = threadIdx.x % (W / 8) * 8;
     const unsigned off = (unsigned)(row0 * (int)stride + c) * (unsigned)sizeof(T);
+    if (VEC && n == 64 && cols >= W) {  // nothing to leave out
+#pragma unroll
+      for (int k = 0; k < W / 32; ++k)
+        v[k] = *reinterpret_cast<const sc_x8<T>*>(reinterpret_cast<const char*>(base + (int64_t)(k * (2048 / W)) * stride) + off);
+      return;
+    }
 #pragma unroll
     for (int k = 0; k < W / 32; ++k) {
       const int row = row0 + k * (2048 / W);
@@ -225,6 +231,25 @@ __device__ __forceinline__ f32x4 sc_mfma_right(const X8 (&left)[PARTS], const X8
 #pragma unroll
   for (int k = PARTS - 1; k >= 0; --k) acc = mfma16(left[k], right, acc);
   return acc;
+}
+
+// acc[nt] += (columns 16 nt .. of the tile)^T * (the first `parts` parts of an operand over its 64 rows). Every product goes to
+// another tile than the one before it, which it would otherwise wait for.
+template <typename T, int NT, int PARTS>
+__device__ __forceinline__ void sc_add_products(const T* tile, int stride, int lane, const sc_x8<T> (&right)[2][PARTS], int parts,
+                                                f32x4 (&acc)[NT]) {
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) {
+    sc_x8<T> left[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) left[nt] = op_ld_tr16<T, true>(tile, stride, 16 * nt, 32 * kk, lane);
+#pragma unroll
+    for (int k = PARTS - 1; k >= 0; --k) {
+      if (k >= parts) continue;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) acc[nt] = mfma16(left[nt], right[kk][k], acc[nt]);
+    }
+  }
 }
 
 // Whether every row of a call can be read in 16-byte pieces and written in 8-byte ones (the kernels are built for both: their

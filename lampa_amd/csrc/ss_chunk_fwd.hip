@@ -21,6 +21,8 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
   const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
   const int64_t chunks = seg.outside ? 0 : (seg.t1 - seg.t0 + 63) / 64;
 
+  // the third part only where the states go to the caller or into gradients
+  const bool whole = REV || KEEP || a.ht;
   f32x4 S[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) S[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -97,20 +99,18 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
     }
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
+    // (a product of one tile after the other: no product waits for the one before it)
+    if constexpr (__is_same(T, _Float16)) {
+      f32x4 d[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      sc_x8<T> k[2];
-      sc_columns<T>(tk, KS, 16 * nt, lane, k);
-      if constexpr (__is_same(T, _Float16)) {
-        f32x4 d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int nt = 0; nt < NT; ++nt) d[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      sc_add_products<T, NT, PARTS>(tk, KS, lane, vw, PARTS, d);
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) d = sc_mfma_left(k[kk], vw[kk], d);
-        S[nt] = S[nt] * end + d * back;
-      } else {
-        S[nt] *= end;
+      for (int nt = 0; nt < NT; ++nt) S[nt] = S[nt] * end + d[nt] * back;
+    } else {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) S[nt] = sc_mfma_left(k[kk], vw[kk], S[nt]);
-      }
+      for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
+      sc_add_products<T, NT, PARTS>(tk, KS, lane, vw, whole ? PARTS : 2, S);
     }
     lds_barrier();
   }
@@ -328,23 +328,17 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
       const float end = dec.end;
+      if constexpr (__is_same(T, _Float16)) {
+        f32x4 d[NT];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        sc_x8<T> k[2];
-        sc_columns<T>(tb, KS, 16 * nt, lane, k);
-        if constexpr (__is_same(T, _Float16)) {
-          f32x4 d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int nt = 0; nt < NT; ++nt) d[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        sc_add_products<T, NT, PARTS>(tb, KS, lane, vw, PARTS, d);
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk) d = sc_mfma_left(k[kk], vw[kk], d);
-          S[nt] = S[nt] * end + d * back;
-        } else {
-          S[nt] *= end;
+        for (int nt = 0; nt < NT; ++nt) S[nt] = S[nt] * end + d[nt] * back;
+      } else {
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk) {
-            if (handed_on) S[nt] = mfma16(k[kk], vw[kk][2], S[nt]);
-            S[nt] = mfma16(k[kk], vw[kk][0], mfma16(k[kk], vw[kk][1], S[nt]));
-          }
-        }
+        for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
+        sc_add_products<T, NT, PARTS>(tb, KS, lane, vw, handed_on ? PARTS : 2, S);
       }
     }
     t0 += n;
