@@ -514,13 +514,14 @@ int lampa_causal_conv1d_bwd(const void* x, int64_t x_stride, const void* dy, int
 
 /* Norm behind a block, its gate, the scaled residual add and the next block's norm (models/hattention/fused_norm.py:40-111 has
  * the plain residual add + norm): a = x or rmsnorm(x) * post_weight (where post_weight is not NULL),
- * r = residual + scale * act(gate) * a, y = rmsnorm(r) * weight. x, y [rows, D] of dtype; residual, residual_out of res_dtype
- * (dtype or fp32); weights and scale fp32 [D] or NULL; gate_kind 0 none, 1 [rows, D], 2 [rows / seq_rows, D] (one row for every
+ * r = residual + scale * act(gate) * a, y = rmsnorm(r) * weight. x, y [rows, D] of dtype; residual, residual_out (r) of res_dtype
+ * (dtype or fp32), residual NULL for zero (residual_out may then be NULL as well); weights and scale fp32 [D] or NULL; gate_kind 0 none, 1 [rows, D], 2 [rows / seq_rows, D] (one row for every
  * seq_rows rows); activation of the gate 0 none, 1 SiLU, 2 sigmoid. All contiguous, 16-byte aligned, D % 8 == 0, D <= 8192. */
 int lampa_residual_norm_fwd(const void* x, const void* residual, const float* weight, const float* post_weight, const void* gate,
                             int gate_kind, int activation, const float* scale, int64_t rows, int64_t seq_rows, int D, float eps,
                             int dtype, int res_dtype, void* y, void* residual_out, void* stream);
-/* Its gradients: dy of dtype and dres of res_dtype (either may be NULL: zero); dx, dgate of dtype, dresidual of res_dtype,
+/* Its gradients: dy of dtype and dres of res_dtype (either may be NULL: zero); dx, dgate of dtype, dresidual of res_dtype (NULL without a
+ * residual),
  * dweight, dpost_weight, dscale fp32 [D] (those and dgate may be NULL where they are not wanted). */
 int64_t lampa_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t seq_rows, int D);
 int lampa_residual_norm_bwd(const void* x, const void* residual, const float* weight, const float* post_weight, const void* gate,

@@ -7,6 +7,11 @@ gated by swish(g_proj(x)) -> output projection. ``LshgdBlock`` is the benchmark 
 the hits, pre-norm residual layers (the fused add + norm of ``GatedDeltaProductBlock.forward``, ``:1029-1056``), unsort
 and an embedding head. The projections are plain library GEMMs (one fused GEMM per layer for q|k|v|g|b|a); everything
 else runs in this package's HIP kernels. Forward only.
+
+``StateSpaceLayer`` and ``StateSpaceBlock`` are the state-space counterpart (the mixer and residual wiring behind
+``models/baselines/full_mamba2.py:221-430``): projection -> short convolution + SiLU -> selective scan -> gated norm -> output
+projection, with the norms at the borders fused with the residual add. They train (every operator has its gradients), take
+packed sequences, and continue from caches with whole prompts or one token at a time.
 """
 import math
 
@@ -16,8 +21,9 @@ import torch.nn.functional as F
 
 from . import lsh
 from .gated_delta import chunk_gated_delta_rule
-from .layer_ops import (PROJ_CONV_HIDDEN, FusedRMSNormSwishGate, RMSNorm, ShortConvolution, causal_conv1d,
-                        causal_conv1d_split, gdr_gates, norm_proj, norm_proj_supported, proj_conv)
+from .layer_ops import (PROJ_CONV_HIDDEN, FusedRMSNormSwishGate, RMSNorm, ShortConvolution, causal_conv1d, causal_conv1d_split,
+                        causal_conv1d_step, gdr_gates, norm_proj, norm_proj_supported, proj_conv, residual_norm)
+from .state_space import state_space_scan, state_space_step
 
 
 class GatedDeltaLayer(nn.Module):
@@ -194,3 +200,104 @@ class LshgdBlock(nn.Module):
                 raise lsh.LampaError("LshgdBlock: the bucket key of the first hash table does not fit 32 bits; the "
                                      "sequence order would be meaningless")
         return out
+
+
+class StateSpaceLayer(nn.Module):
+    """in_proj -> z | x | B | C | dt; causal convolution + SiLU over x | B | C; selective scan with delta = softplus(dt + dt_bias),
+    A = -exp(A_log) and the skip D; rms norm of silu(z) * y; out_proj. ``expand * hidden_size`` columns in heads of ``head_dim``,
+    B and C shared by the heads of a group."""
+
+    def __init__(self, hidden_size: int = 128, d_state: int = 64, head_dim: int = 64, expand: int = 2, n_groups: int = 1,
+                 conv_size: int = 4, norm_eps: float = 1e-5):
+        super().__init__()
+        inner = expand * hidden_size
+        if inner % head_dim or (inner // head_dim) % n_groups:
+            raise ValueError(f"StateSpaceLayer: {inner} columns do not divide into heads of {head_dim} and {n_groups} groups")
+        self.hidden_size, self.d_state, self.head_dim, self.n_groups = hidden_size, d_state, head_dim, n_groups
+        self.inner, self.num_heads, self.conv_size, self.norm_eps = inner, inner // head_dim, conv_size, norm_eps
+        self.conv_dim = inner + 2 * n_groups * d_state
+        self.in_proj = nn.Linear(hidden_size, inner + self.conv_dim + self.num_heads, bias=False)
+        bound = conv_size ** -0.5
+        self.conv_weight = nn.Parameter(torch.empty(self.conv_dim, conv_size).uniform_(-bound, bound))
+        self.conv_bias = nn.Parameter(torch.empty(self.conv_dim).uniform_(-bound, bound))
+        self.A_log = nn.Parameter(torch.log(torch.empty(self.num_heads).uniform_(1, 16)))
+        step = torch.exp(torch.rand(self.num_heads) * (math.log(0.1) - math.log(0.001)) + math.log(0.001)).clamp(min=1e-4)
+        self.dt_bias = nn.Parameter(step + torch.log(-torch.expm1(-step)))
+        self.D = nn.Parameter(torch.ones(self.num_heads))
+        self.norm_weight = nn.Parameter(torch.ones(inner))
+        self.out_proj = nn.Linear(inner, hidden_size, bias=False)
+
+    def _split(self, hidden):
+        return self.in_proj(hidden).split([self.inner, self.conv_dim, self.num_heads], dim=-1)
+
+    def _heads(self, xbc):
+        gn = self.n_groups * self.d_state
+        x, B, C = xbc.split([self.inner, gn, gn], dim=-1)
+        return x.unflatten(-1, (self.num_heads, self.head_dim)), *(t.unflatten(-1, (self.n_groups, self.d_state)) for t in (B, C))
+
+    def _out(self, y, z):
+        return self.out_proj(residual_norm(y.flatten(-2), None, self.norm_weight, gate=z, gate_activation="silu", eps=self.norm_eps))
+
+    def forward(self, hidden_states: torch.Tensor, cu_seqlens=None, cache=None, output_cache: bool = False):
+        """hidden_states [B, T, hidden] -> (out [B, T, hidden], cache or None). ``cache`` = (the last inputs of the convolution
+        [sequences, conv_dim, conv_size], the states [sequences, heads, d_state, head_dim] float32) as a call or ``step`` left
+        them; no gradient runs through the convolution's part."""
+        z, xbc, dt = self._split(hidden_states)
+        conv_cache, state = (None, None) if cache is None else cache
+        conv = causal_conv1d(xbc, self.conv_weight, self.conv_bias, activation="silu", cu_seqlens=cu_seqlens,
+                             initial_state=conv_cache, output_final_state=output_cache)
+        xbc, conv_cache = conv if output_cache else (conv, None)
+        x, B, C = self._heads(xbc)
+        y, state = state_space_scan(x, dt, -torch.exp(self.A_log.float()), B, C, D=self.D, dt_bias=self.dt_bias, dt_softplus=True,
+                                    initial_state=state, output_final_state=output_cache, cu_seqlens=cu_seqlens)
+        return self._out(y, z), (conv_cache, state) if output_cache else None
+
+    @torch.no_grad()
+    def step(self, hidden_states: torch.Tensor, cache):
+        """One token for each sequence: hidden_states [sequences, hidden] -> [sequences, hidden]; the cache is moved on in place."""
+        z, xbc, dt = self._split(hidden_states)
+        xbc = causal_conv1d_step(xbc, cache[0], self.conv_weight, self.conv_bias, "silu")
+        x, B, C = self._heads(xbc)
+        y = state_space_step(x, dt, -torch.exp(self.A_log.float()), B, C, cache[1], D=self.D, dt_bias=self.dt_bias, dt_softplus=True)
+        return self._out(y, z)
+
+
+class StateSpaceBlock(nn.Module):
+    """``n_layers`` pre-norm residual ``StateSpaceLayer``s and a final norm. The residual add, its learned scale
+    (``residual_scale``: one value per channel and layer, starting at the given number) and the next norm are one operator;
+    ``residual_in_fp32`` keeps the stream in float32 beside 16-bit layers."""
+
+    def __init__(self, hidden_size: int = 128, n_layers: int = 4, residual_scale: float = None, residual_in_fp32: bool = True,
+                 norm_eps: float = 1e-5, **layer_args):
+        super().__init__()
+        self.layers = nn.ModuleList([StateSpaceLayer(hidden_size, norm_eps=norm_eps, **layer_args) for _ in range(n_layers)])
+        self.norm_weights = nn.ParameterList([nn.Parameter(torch.ones(hidden_size)) for _ in range(n_layers + 1)])
+        self.scales = None if residual_scale is None else nn.ParameterList(
+            [nn.Parameter(torch.full((hidden_size,), float(residual_scale))) for _ in range(n_layers)])
+        self.residual_in_fp32, self.norm_eps = residual_in_fp32, norm_eps
+
+    def _enter(self, x):
+        h = residual_norm(x, None, self.norm_weights[0], eps=self.norm_eps)
+        return h, x.float() if self.residual_in_fp32 else x
+
+    def _border(self, i, out, residual):
+        return residual_norm(out, residual, self.norm_weights[i + 1], residual_scale=None if self.scales is None else self.scales[i],
+                             eps=self.norm_eps)
+
+    def forward(self, x: torch.Tensor, cu_seqlens=None, caches=None, output_caches: bool = False):
+        """x [B, T, hidden] -> (normed output [B, T, hidden], the layers' caches or None)."""
+        h, residual = self._enter(x)
+        new = []
+        for i, layer in enumerate(self.layers):
+            out, cache = layer(h, cu_seqlens, None if caches is None else caches[i], output_caches)
+            new.append(cache)
+            h, residual = self._border(i, out, residual)
+        return h, new if output_caches else None
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, caches):
+        """One token for each sequence: x [sequences, hidden]; the caches are moved on in place."""
+        h, residual = self._enter(x)
+        for i, layer in enumerate(self.layers):
+            h, residual = self._border(i, layer.step(h, caches[i]), residual)
+        return h

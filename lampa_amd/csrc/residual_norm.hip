@@ -1,7 +1,7 @@
 // The border between two blocks of a pre-norm stack, in one pass over the rows (gfx950): the norm behind a block, its gate, the
 // scaled residual add and the norm in front of the next block,
 //   a = x  or  x / rms(x) * post_weight,   m = scale * act(gate) * a,   r = residual + m,   y = r / rms(r) * weight,
-// with rms(v) = sqrt(mean(v^2) + eps) over the last dimension, and its gradients. Every factor is optional.
+// with rms(v) = sqrt(mean(v^2) + eps) over the last dimension, and its gradients. Every factor and the residual are optional.
 // Bound by bytes: each input is read once, each output written once; sums and everything between load and store are fp32 (y
 // comes from the unrounded r). The gradients recompute a, r and both rms from the inputs, which costs the bytes of x and the
 // residual instead of those of kept intermediates, and is exact where a kept r would be rounded to the residual's type.
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
     if (!(r0 + slot < n_rows && c0 < a.D)) return;
     const int64_t row = row_base + r0 + slot, at = row * a.D + c0;
     nx.load((const T*)a.x + at);
-    nh.load((const RT*)a.residual + at);
+    if (a.residual) nh.load((const RT*)a.residual + at);
     if (a.gate_kind) ng.load((const T*)a.gate + (a.gate_kind == RN_GATE_SEQ ? row / a.seq_rows : row) * a.D + c0);
     if (a.dy) ndy.load((const T*)a.dy + at);
     if (a.dres) ndr.load((const RT*)a.dres + at);
@@ -131,10 +131,10 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
       if (on) {
         if constexpr (AHEAD) {
           cx.get(x[st]);
-          ch.get(h[st]);
+          if (a.residual) ch.get(h[st]);
         } else {
           load8((const T*)a.x + row * a.D + c0, x[st]);
-          load8((const RT*)a.residual + row * a.D + c0, h[st]);
+          if (a.residual) load8((const RT*)a.residual + row * a.D + c0, h[st]);
         }
       }
 #pragma unroll
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
         sq2 = __builtin_fmaf(h[st][c], h[st][c], sq2);
       }
       if constexpr (!GRAD)
-        if (on) rn_store8((RT*)a.res_out + row * a.D + c0, h[st]);
+        if (on && a.res_out) rn_store8((RT*)a.res_out + row * a.D + c0, h[st]);
     }
     const float i2 = 1.0f / sqrtf(rn_row_sum<LPR>(sq2, part, turn) * inv_d + a.eps);
     if constexpr (!GRAD) {
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
           dh[st][c] = da;
         }
         if (on) {
-          rn_store8((RT*)a.dresidual + row * a.D + c0, dr);
+          if (a.dresidual) rn_store8((RT*)a.dresidual + row * a.D + c0, dr);
           if (a.gate_kind == RN_GATE_TOKEN && a.dgate) rn_store8((T*)a.dgate + row * a.D + c0, dg);
         }
       }
@@ -355,7 +355,7 @@ static int rn_types(const RnArgs& a, int dtype, int res_dtype, int lpr, int step
 static int rn_check(const void* x, const void* residual, const void* gate, int gate_kind, int act, int64_t rows, int64_t seq_rows,
                     int D, int dtype, int res_dtype) {
   if (rows < 0 || D < 1 || dtype < 0 || dtype > 2 || (res_dtype != dtype && res_dtype != GDR_FP32) || act < 0 || act > 2 ||
-      gate_kind < 0 || gate_kind > 2 || (rows && (!x || !residual || (gate_kind && !gate))) || seq_rows < 1 || rows % seq_rows)
+      gate_kind < 0 || gate_kind > 2 || (rows && (!x || (gate_kind && !gate))) || seq_rows < 1 || rows % seq_rows)
     return LAMPA_ERR_INVALID;
   if (D % 8 || D > 8192 || ((uintptr_t)x | (uintptr_t)residual | (uintptr_t)gate) % 16) return LAMPA_ERR_UNSUPPORTED;
   return LAMPA_OK;
@@ -369,7 +369,7 @@ extern "C" int lampa_residual_norm_fwd(const void* x, const void* residual, cons
   if (rc == LAMPA_OK) rc = rn_shape(D, &lpr, &steps);
   if (rc != LAMPA_OK) return rc;
   if (rows == 0) return LAMPA_OK;
-  if (!y || !residual_out) return LAMPA_ERR_INVALID;
+  if (!y || (residual && !residual_out)) return LAMPA_ERR_INVALID;
   if (((uintptr_t)y | (uintptr_t)residual_out) % 16) return LAMPA_ERR_UNSUPPORTED;
   RnArgs a = {};
   a.x = x; a.residual = residual; a.gate = gate; a.weight = weight; a.post_weight = post_weight; a.scale = scale;
@@ -398,7 +398,7 @@ extern "C" int lampa_residual_norm_bwd(const void* x, const void* residual, cons
   if (rc != LAMPA_OK) return rc;
   const int64_t n_seq = rows / seq_rows;
   if (rows == 0) return LAMPA_OK;  // nothing to sum: the caller's zeros stand
-  if (!dx || !dresidual || (!weight && dweight) || (!post_weight && dpost_weight) || (!scale && dscale) || (!gate_kind && dgate))
+  if (!dx || (residual && !dresidual) || (!weight && dweight) || (!post_weight && dpost_weight) || (!scale && dscale) || (!gate_kind && dgate))
     return LAMPA_ERR_INVALID;
   if (((uintptr_t)dx | (uintptr_t)dresidual | (uintptr_t)dgate | (uintptr_t)dy | (uintptr_t)dres) % 16) return LAMPA_ERR_UNSUPPORTED;
   if (n_seq > 65535) return LAMPA_ERR_UNSUPPORTED;

@@ -611,11 +611,11 @@ def _residual_norm_launch(x, residual, weight, post_weight, gate, act, scale, ep
     x_, r_, g_ = _packed(x), _packed(residual), _packed(gate)
     w, pw, sc = _vec32(weight), _vec32(post_weight), _vec32(scale)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    out = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    out = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
     with _on_device(x.get_device()):
         check(_capi.lib().lampa_residual_norm_fwd(ptr(x_), ptr(r_), ptr(w), ptr(pw), ptr(g_), kind, act, ptr(sc), rows, seq_rows, D,
-                                                  float(eps), _code(x.dtype), _code(residual.dtype), ptr(y), ptr(out),
-                                                  stream_of(x)), "lampa_residual_norm_fwd")
+                                                  float(eps), _code(x.dtype), _code((x if residual is None else residual).dtype),
+                                                  ptr(y), ptr(out), stream_of(x)), "lampa_residual_norm_fwd")
     return y, out
 
 
@@ -635,9 +635,10 @@ class _ResidualNorm(torch.autograd.Function):
         x_, r_, g_ = _packed(x), _packed(residual), _packed(gate)
         w, pw, sc = _vec32(weight), _vec32(post_weight), _vec32(scale)
         dy = None if dy is None else _packed(dy.to(x.dtype))
-        dres = None if dres is None else _packed(dres.to(residual.dtype))
+        dres = None if dres is None or residual is None else _packed(dres.to(residual.dtype))
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dr = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+        res_dtype = (x if residual is None else residual).dtype
+        dr = None if residual is None else torch.empty(x.shape, dtype=res_dtype, device=x.device)
         make = torch.empty if rows else torch.zeros  # without rows nothing is launched
         need = ctx.needs_input_grad
         vec = lambda t, wanted: make(D, dtype=torch.float32, device=x.device) if t is not None and wanted else None  # noqa: E731
@@ -648,14 +649,14 @@ class _ResidualNorm(torch.autograd.Function):
             size = check(lib.lampa_residual_norm_bwd_workspace_bytes(rows, seq_rows, D), "lampa_residual_norm_bwd_workspace_bytes")
             ws = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
             check(lib.lampa_residual_norm_bwd(ptr(x_), ptr(r_), ptr(w), ptr(pw), ptr(g_), kind, ctx.act, ptr(sc), ptr(dy), ptr(dres),
-                                              rows, seq_rows, D, float(ctx.eps), _code(x.dtype), _code(residual.dtype), ptr(dx),
+                                              rows, seq_rows, D, float(ctx.eps), _code(x.dtype), _code(res_dtype), ptr(dx),
                                               ptr(dr), ptr(dg), ptr(dw), ptr(dpw), ptr(dsc), ptr(ws), size, stream_of(x)),
                   "lampa_residual_norm_bwd")
         cast = lambda g, t: None if g is None else g.to(t.dtype)  # noqa: E731
         return dx, dr, cast(dw, weight), cast(dpw, post_weight), dg, cast(dsc, scale), None, None
 
 
-def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor] = None,
+def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor] = None,
                   post_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
                   gate_activation: Optional[str] = None, residual_scale: Optional[torch.Tensor] = None, eps: float = 1e-5):
     """The border between two blocks in one pass: x [..., D] is a block's output, ``residual`` (x's shape; x's type or
@@ -665,7 +666,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torc
         r = residual + residual_scale * act(gate) * a
         y = rms_norm(r, weight)
 
-    Returns (y in x's type, r in the residual's type); y comes from the unrounded r. ``weight``, ``post_weight`` and
+    Returns (y in x's type, r in the residual's type), or y alone where there is no residual (None): the gated norm behind a mixer,
+    norm of act(gate) * a. y comes from the unrounded r. ``weight``, ``post_weight`` and
     ``residual_scale`` are [D] or None; ``gate`` has x's shape and type, or [B, 1, D] beside x [B, T, D] (one gate for each
     sequence); ``gate_activation`` ``None`` / ``'sigmoid'`` / ``'silu'`` / ``'swish'``. D a multiple of 8, at most 8192.
     Differentiable in every tensor (first order; repeated calls give the same bits)."""
@@ -673,12 +675,13 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torc
     _same_device(what, x, residual, weight, post_weight, gate, residual_scale)
     if gate_activation not in _ACT:
         raise ValueError(f"Activation `{gate_activation}` not supported yet.")
-    if x.dim() < 1 or residual.shape != x.shape:
-        raise ValueError(f"{what}: x and residual must have one shape [..., D], got {tuple(x.shape)} and {tuple(residual.shape)}")
+    if x.dim() < 1 or (residual is not None and residual.shape != x.shape):
+        raise ValueError(f"{what}: x and residual must have one shape [..., D], got {tuple(x.shape)} and "
+                         f"{None if residual is None else tuple(residual.shape)}")
     D = x.shape[-1]
     if D < 8 or D % 8 or D > 8192:
         raise ValueError(f"{what}: the last dimension must be a multiple of 8 and at most 8192, got {D}")
-    if _code(x.dtype) != _code(residual.dtype) and residual.dtype != torch.float32:
+    if _code(x.dtype) != _code((x if residual is None else residual).dtype) and residual.dtype != torch.float32:
         raise TypeError(f"{what}: the residual must have x's type ({x.dtype}) or be float32, got {residual.dtype}")
     for name, t in (("weight", weight), ("post_weight", post_weight), ("residual_scale", residual_scale)):
         if t is not None and (tuple(t.shape) != (D,) or not t.is_floating_point()):
@@ -693,8 +696,10 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torc
             raise ValueError(f"{what}: at most 65535 sequences with a gate each, got {x.shape[0]}")
     act = _ACT[gate_activation]
     if _wants_grad(x, residual, weight, post_weight, gate, residual_scale):
-        return _ResidualNorm.apply(x, residual, weight, post_weight, gate, residual_scale, act, eps)
-    return _residual_norm_launch(x, residual, weight, post_weight, gate, act, residual_scale, eps)
+        y, r = _ResidualNorm.apply(x, residual, weight, post_weight, gate, residual_scale, act, eps)
+    else:
+        y, r = _residual_norm_launch(x, residual, weight, post_weight, gate, act, residual_scale, eps)
+    return y if residual is None else (y, r)
 
 
 class FusedRMSNormGated(nn.Module):

@@ -113,6 +113,21 @@ def test_against_the_plain_norm(device):
     assert torch.equal(y, y2) and torch.equal(out, out2)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_without_a_residual(device, dtype):
+    """The gated norm alone: the same bits as on a residual of zeros, and no second output."""
+    d, dy, dres = _data((2, 40, 128), dtype, "same", "token", False, False, True, 7, device)
+    d["residual"] = torch.zeros_like(d["residual"])
+    leaves = [d[k].requires_grad_(True) for k in ("x", "gate", "weight")]
+    y = lo.residual_norm(leaves[0], None, leaves[2], gate=leaves[1], gate_activation="silu")
+    y2, _ = lo.residual_norm(leaves[0], d["residual"], leaves[2], gate=leaves[1], gate_activation="silu")
+    assert torch.equal(y, y2)
+    for a, b in zip(torch.autograd.grad(y, leaves, dy), torch.autograd.grad(y2, leaves, dy)):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        assert torch.equal(lo.residual_norm(leaves[0], None, leaves[2], gate=leaves[1], gate_activation="silu"), y)
+
+
 def test_one_gradient_and_strides(device):
     d, dy, dres = _data((2, 30, 64), torch.bfloat16, "same", "token", True, True, True, 1, device)
     leaves = {k: v.detach().requires_grad_(True) for k, v in d.items()}
