@@ -95,11 +95,9 @@ __device__ __forceinline__ float ss_log_decay(float delta, float A) {
   return g < SS_MIN_LOG_DECAY ? SS_MIN_LOG_DECAY : g;  // a NaN stays one
 }
 
-// Sum over the 64 lanes of a wave, in every lane.
+// Sum over the 64 lanes of a wave, in every lane (the last lane of a prefix sum has it; no LDS round trips).
 __device__ __forceinline__ float ss_wave_sum(float x) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off);
-  return x;
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_inclusive_scan(x)), 63));
 }
 
 static inline int ss_blocks64(int n) { return (n + 63) / 64; }

@@ -16,6 +16,7 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
   constexpr bool REV = KIND == SS_DX || KIND == SS_DB;  // from the end of the segment
   constexpr bool LANE_P = KIND == SS_Y || KIND == SS_DX;
   constexpr int PIECES = ROWS * SS_TILE / 64;
+  constexpr int UNROLL = ROWS <= 64 ? 4 : 2;
   const SsSegment seg = ss_segment(a, blockIdx.x);
   if (!seg.live) return;
   const int lane = threadIdx.x;
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
   };
 
   float carry = 1.0f;   // reverse walks: the decay between the token before (later in time) and this one
-  float sum_g = 0.0f;   // maps: the segment's whole exponent
+  float sum_g = 0.0f;   // maps: this lane's share of the segment's whole exponent
   float dD = 0.0f;
   if (tiles && !seg.outside) fetch(0);
   for (int64_t tile = 0; tile < tiles; ++tile) {
@@ -116,25 +117,30 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
       }
       if (lane < SS_TILE) {
         const float d = lane < n ? ss_delta(pdt, bias, a.softplus) : 0.0f;
+        const float g = lane < n ? ss_log_decay(d, A) : 0.0f;
         ldelta[lane] = d;
-        ldecay[lane] = lane < n ? ss_log_decay(d, A) : 0.0f;
+        ldecay[lane] = expf(g);
+        if (MAP) sum_g += g;
       }
       if (tile + 1 < tiles) fetch(tile + 1);
     }
     __syncthreads();
-    for (int i = 0; i < n; ++i) {
-      const int t = REV ? n - 1 - i : i;
+    // Tokens behind the segment's last one have no step, no input and a decay of one: every tile is walked whole, so that the
+    // staged rows of one token can be read while the one before is worked on.
+#pragma unroll UNROLL
+    for (int i = 0; i < SS_TILE; ++i) {
+      const int t = REV ? SS_TILE - 1 - i : i;
       const int64_t tok = t0 + t;
+      const bool real = t < n;
       float out = 0.0f, delta = 0.0f;
       if (!seg.outside) {
         delta = ldelta[t];
-        const float g = ldecay[t], decay = expf(g);
-        if (MAP) sum_g += g;
+        const float decay = ldecay[t];
         const float v = KIND == SS_Y || KIND == SS_DC ? delta * lv[t][lane] : lv[t][lane];
         const float s = REV ? carry : decay;
         if constexpr (KIND == SS_DX && !MAP) {
           const int64_t done = tok + 1 - seg.t0;
-          if (done % SS_DOT == 0 || tok + 1 == seg.t1) {  // S times the last decay is the adjoint behind this token
+          if (real && (done % SS_DOT == 0 || tok + 1 == seg.t1)) {  // S times the last decay is the adjoint behind this token
             const int64_t row = (ss_row_of(seg, SS_DOT) + (done - 1) / SS_DOT) * a.H + h;
             const float* kept = w.chunk_states + row * per_h;
             float dot = 0.0f;
@@ -154,6 +160,7 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
         out = (o[0] + o[1]) + (o[2] + o[3]);
         carry = decay;
       }
+      if (!real) continue;
       if constexpr (!MAP) {
         if constexpr (KIND == SS_Y) {
           if (lane_on)
@@ -190,6 +197,7 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
       if (lane_on && r < rn) local[at(r)] = REV ? S[r] * carry : S[r];
+    sum_g = ss_wave_sum(sum_g);
     if (!REV && lane == 0 && pb == 0) a.slot_decay[(int64_t)blockIdx.x * a.H + h] = expf(sum_g);
   } else if (LANE_P) {
     if (KIND == SS_DX) {
