@@ -5,16 +5,22 @@
 // C_t (e^{gamma_t} dy_t)^T with gamma counted from the segment's start. Reads x and B (dy and C) once.
 // KEEP: the walk starts from the segment's initial state and leaves the state in front of every chunk in w.chunk_states, in the
 // order in which the gradients' lanes read it (sc_kept_at).
+template <typename T, int NP>
+struct ScMapTiles {
+  static const int KS = NP + 8, VS = 64 + 8;
+  __align__(16) T k[64 * KS], v[64 * VS];
+  __align__(16) ScDecay dec;
+};
 template <typename T, int NP, bool REV, bool KEEP, bool VEC>
-__global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGrad w) {
+__device__ __forceinline__ void sc_map(const lampa_ss_args& a, const SsGrad& w, ScMapTiles<T, NP>& tiles) {
   constexpr int NT = NP / 16, KS = NP + 8, VS = 64 + 8;
   const SsSegment seg = ss_segment(a, blockIdx.x);
   if (!seg.live) return;
   const int npb = (a.P + 63) / 64, pb = blockIdx.y % npb, h = blockIdx.y / npb, grp = h / (a.H / a.G);
   const int lane0 = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cols = a.P - 64 * pb < 64 ? a.P - 64 * pb : 64;
-  __shared__ __align__(16) T tk[64 * KS], tv[64 * VS];
-  __shared__ __align__(16) ScDecay dec;
+  T *tk = tiles.k, *tv = tiles.v;
+  ScDecay& dec = tiles.dec;
   const T* kb = (REV ? (const T*)a.C : (const T*)a.B) + (int64_t)grp * a.N;
   const T* vb = (REV ? (const T*)a.dy : (const T*)a.x) + (int64_t)h * a.P + 64 * pb;
   const int64_t ks = REV ? a.C_stride : a.B_stride, vs = REV ? (int64_t)a.H * a.P : a.x_stride;
@@ -124,6 +130,24 @@ __global__ void __launch_bounds__(SC_BLOCK) sc_map_kernel(lampa_ss_args a, SsGra
       if (n < a.N && p < a.P) local[(int64_t)n * a.P + p] = S[nt][r];
     }
   if (!REV && threadIdx.x == 0 && pb == 0) a.slot_decay[(int64_t)blockIdx.x * a.H + h] = __builtin_amdgcn_exp2f(sum);
+}
+
+// Waves a SIMD that fit without spilling (element-by-element loads and fp16's scales take more registers).
+template <typename T, int NP, bool VEC>
+constexpr int sc_map_waves() { return !VEC ? 2 : NP <= 64 ? (__is_same(T, __bf16) ? 4 : 3) : (__is_same(T, __bf16) ? 3 : 2); }
+
+template <typename T, int NP, bool VEC>
+__global__ void __launch_bounds__(SC_BLOCK, (sc_map_waves<T, NP, VEC>())) sc_map_kernel(lampa_ss_args a, SsGrad w) {
+  __shared__ ScMapTiles<T, NP> tiles;
+  sc_map<T, NP, false, false, VEC>(a, w, tiles);
+}
+// Before the gradients: the states in front of the chunks (first half of the grid) and the local adjoints, which do not depend on
+// each other, side by side: neither fills the chip by itself (60 000 tokens x 8 heads, N = 128: 62 and 120 us in turn).
+template <typename T, int NP, bool VEC>
+__global__ void __launch_bounds__(SC_BLOCK, (sc_map_waves<T, NP, VEC>())) sc_prepare_kernel(lampa_ss_args a, SsGrad w) {
+  __shared__ ScMapTiles<T, NP> tiles;
+  if (blockIdx.z == 0) sc_map<T, NP, false, true, VEC>(a, w, tiles);
+  else sc_map<T, NP, true, false, VEC>(a, w, tiles);
 }
 
 // Outputs of a segment from the state it starts from.
@@ -356,29 +380,24 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
   }
 }
 
-enum { SC_LOCAL_STATES, SC_LOCAL_ADJOINTS, SC_KEEP_STATES };
 template <typename T, bool VEC>
-static int sc_maps_launch(const lampa_ss_args& a, int what, const SsGrad& w, hipStream_t s) {
+static int sc_maps_launch(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s) {
+  dim3 grid = sc_grid(a);
+  if (grad) grid.z = ss_single(&a) ? 1 : 2;  // a sequence of one segment starts from dht: no local adjoints
   LAMPA_PROF(s, "start");
-#define SC_GO(NP)                                                                                                                      \
-  switch (what) {                                                                                                                      \
-    case SC_LOCAL_STATES: hipLaunchKernelGGL((sc_map_kernel<T, NP, false, false, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w); break; \
-    case SC_LOCAL_ADJOINTS: hipLaunchKernelGGL((sc_map_kernel<T, NP, true, false, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w); break; \
-    default: hipLaunchKernelGGL((sc_map_kernel<T, NP, false, true, VEC>), sc_grid(a), dim3(SC_BLOCK), 0, s, a, w); break;               \
-  }
-  if (a.N <= 32) { SC_GO(32) } else if (a.N <= 64) { SC_GO(64) } else { SC_GO(128) }
+#define SC_GO(NP)                                                                                           \
+  if (grad) hipLaunchKernelGGL((sc_prepare_kernel<T, NP, VEC>), grid, dim3(SC_BLOCK), 0, s, a, *grad);      \
+  else hipLaunchKernelGGL((sc_map_kernel<T, NP, VEC>), grid, dim3(SC_BLOCK), 0, s, a, SsGrad{})
+  if (a.N <= 32) { SC_GO(32); } else if (a.N <= 64) { SC_GO(64); } else { SC_GO(128); }
 #undef SC_GO
-  LAMPA_PROF(s, what == SC_KEEP_STATES ? "sc_map_kernel<keep>" : "sc_map_kernel");
+  LAMPA_PROF(s, grad ? "sc_prepare_kernel" : "sc_map_kernel");
   return lampa_launch_status();
 }
-static int sc_maps(const lampa_ss_args& a, int what, const SsGrad& w, hipStream_t s) {
-  if (a.dtype == GDR_BF16) return sc_vectors(a) ? sc_maps_launch<__bf16, true>(a, what, w, s) : sc_maps_launch<__bf16, false>(a, what, w, s);
-  return sc_vectors(a) ? sc_maps_launch<_Float16, true>(a, what, w, s) : sc_maps_launch<_Float16, false>(a, what, w, s);
-}
+// The segments' local states, or, with `grad`, what the gradients start from.
 int ss_chunk_maps(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s) {
-  return sc_maps(a, grad ? SC_LOCAL_ADJOINTS : SC_LOCAL_STATES, grad ? *grad : SsGrad{}, s);
+  if (a.dtype == GDR_BF16) return sc_vectors(a) ? sc_maps_launch<__bf16, true>(a, grad, s) : sc_maps_launch<__bf16, false>(a, grad, s);
+  return sc_vectors(a) ? sc_maps_launch<_Float16, true>(a, grad, s) : sc_maps_launch<_Float16, false>(a, grad, s);
 }
-int ss_chunk_keep(const lampa_ss_args& a, const SsGrad& w, hipStream_t s) { return sc_maps(a, SC_KEEP_STATES, w, s); }
 
 template <typename T, bool VEC>
 static int sc_out_launch(const lampa_ss_args& a, hipStream_t s) {

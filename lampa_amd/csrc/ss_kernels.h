@@ -13,7 +13,7 @@ struct SsGrad {
   float* chunk_states;       // chunks: the state in front of every 64 tokens, [rows, H, blocks, N padded, 64]
                              // token-serial: the state behind every SS_DOT, [rows, H, N, P]
   float* chunk_dots;         // token-serial: <R, S> behind every SS_DOT tokens, [rows, H, blocks]
-  float* param_part;         // [slots, H, 2]: a segment's share of dA and d dt_bias
+  float* param_part;         // [slots * pieces, H, 2]: 256 tokens' share of dA and d dt_bias (pieces of a segment)
   float* dD_part;            // [slots, H, blocks]
 };
 
@@ -24,6 +24,5 @@ int ss_serial_walk(const lampa_ss_args& a, int kind, const SsGrad& grad, hipStre
 
 int ss_chunk_maps(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s);
 int ss_chunk_out(const lampa_ss_args& a, hipStream_t s);
-int ss_chunk_keep(const lampa_ss_args& a, const SsGrad& w, hipStream_t s);
 int ss_chunk_grad(const lampa_ss_args& a, const SsGrad& w, hipStream_t s);
 static inline int ss_chunk_n(int N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }  // N as the chunk kernels are built for it

@@ -9,7 +9,7 @@
 // S (or, from the end, R) across the segments of one sequence, one thread an element of the state: every slot's local state
 // is replaced by the state its segment starts from, and what is left after the last one goes to `out`. A thread reads
 // SS_AHEAD slots before it needs the first.
-#define SS_AHEAD 8
+#define SS_AHEAD 16
 template <bool REV>
 __global__ void __launch_bounds__(SS_BLOCK) ss_join_kernel(lampa_ss_args a, float* __restrict__ states,
                                                            const float* __restrict__ init, float* __restrict__ out) {
@@ -50,19 +50,20 @@ static int ss_join(const lampa_ss_args& a, float* states, const float* init, flo
   return lampa_launch_status();
 }
 
-// From the gradient of the decays to those of dt, A and dt_bias. One workgroup a segment and head; a wave takes 64 tokens at a
-// time, a lane one of them. Where dg has not been summed up yet (fp32), it is here, SS_DOT tokens at a time from their end:
+// From the gradient of the decays to those of dt, A and dt_bias. One workgroup takes 256 tokens of a segment and head,
+// a wave 64, a lane one. Where dg has not been summed up yet (fp32), it is here, SS_DOT tokens at a time from their end:
 // dg_t = dg_{t+1} + read_t - delta_t reach_t, behind the last of them <R, S>. Starting anew that often keeps rounding errors of
 // the sum, which pass on to every earlier token of it, from adding up (dA off by 2.5e-5 over segments of 256 tokens, 6e-6 over 64).
 template <typename T>
 __global__ void __launch_bounds__(SS_BLOCK) ss_decay_grad_kernel(lampa_ss_args a, SsGrad w, bool summed) {
   const SsSegment seg = ss_segment(a, blockIdx.x);
   const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t slot_row = (int64_t)blockIdx.x * a.H + h;
+  const int64_t part_row = ((int64_t)blockIdx.x * gridDim.z + blockIdx.z) * a.H + h;
   const int npb = (a.P + 63) / 64, reads = summed ? npb : npb * ((a.N + 63) / 64);
   const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
   float dA = 0.0f, dbias = 0.0f;
-  for (int64_t t0 = seg.t0 + 64 * wave; seg.live && t0 < seg.t1; t0 += SS_BLOCK) {
+  const int64_t t0 = seg.t0 + (int64_t)SS_BLOCK * blockIdx.z + 64 * wave;
+  if (seg.live && t0 < seg.t1) {
     const int64_t tok = t0 + lane;
     const bool on = tok < seg.t1 && !seg.outside;
     float raw = 0.0f, delta = 0.0f, dg = 0.0f, reach = 0.0f;
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(SS_BLOCK) ss_decay_grad_kernel(lampa_ss_args a
   __syncthreads();
   if (threadIdx.x < 2) {
     const float* v = part[threadIdx.x];
-    w.param_part[slot_row * 2 + threadIdx.x] = (v[0] + v[1]) + (v[2] + v[3]);
+    w.param_part[part_row * 2 + threadIdx.x] = (v[0] + v[1]) + (v[2] + v[3]);
   }
 }
 
@@ -129,15 +130,17 @@ __global__ void __launch_bounds__(SS_BLOCK) ss_group_sum_kernel(const float* __r
 }
 
 // dA, d dt_bias and dD of a head: its segments' shares in their order.
-__global__ void __launch_bounds__(SS_BLOCK) ss_param_sum_kernel(lampa_ss_args a, SsGrad w, int64_t slots) {
+__global__ void __launch_bounds__(SS_BLOCK) ss_param_sum_kernel(lampa_ss_args a, SsGrad w, int64_t slots, int64_t pieces) {
   const int h = blockIdx.x, which = blockIdx.y, npb = (a.P + 63) / 64;
   float* out = which == 0 ? a.dA : which == 1 ? a.ddt_bias : a.dD;
   if (!out) return;
   float sum = 0.0f;
-  for (int64_t slot = threadIdx.x; slot < slots; slot += SS_BLOCK) {
-    if (which < 2) sum += w.param_part[(slot * a.H + h) * 2 + which];
-    else if (ss_segment(a, slot).live)
-      for (int i = 0; i < npb; ++i) sum += w.dD_part[(slot * a.H + h) * npb + i];
+  if (which < 2) {
+    for (int64_t row = threadIdx.x; row < slots * pieces; row += SS_BLOCK) sum += w.param_part[(row * a.H + h) * 2 + which];
+  } else {
+    for (int64_t slot = threadIdx.x; slot < slots; slot += SS_BLOCK)
+      if (ss_segment(a, slot).live)
+        for (int i = 0; i < npb; ++i) sum += w.dD_part[(slot * a.H + h) * npb + i];
   }
   __shared__ float part[4];
   sum = ss_wave_sum(sum);
@@ -161,7 +164,7 @@ static int ss_check(const lampa_ss_args* a) {
       (int64_t)a->H * (a->P + 63) * a->N >= 1 << 28)
     return LAMPA_ERR_UNSUPPORTED;
   // the grids' limits: slots along x, heads and blocks along y
-  if (ss_slots(a) > 0x7fffffff || (int64_t)a->H * ss_blocks64(a->P) * 2 > 65535) return LAMPA_ERR_UNSUPPORTED;
+  if (ss_slots(a) > 0x7fffffff || a->seg_tokens > (int64_t)65535 * SS_BLOCK || (int64_t)a->H * ss_blocks64(a->P) * 2 > 65535) return LAMPA_ERR_UNSUPPORTED;
   return LAMPA_OK;
 }
 
@@ -183,6 +186,12 @@ extern "C" int lampa_ss_scan_fwd(const lampa_ss_args* args, void* stream) {
   return a.dtype == GDR_FP32 ? ss_serial_walk(a, SS_Y, SsGrad{}, s) : ss_chunk_out(a, s);
 }
 
+// Workgroups of 256 tokens a segment takes.
+static int64_t ss_pieces(const lampa_ss_args& a) {
+  const int64_t most = a.cu_seqlens ? a.n_tokens : a.seq_len, longest = a.seg_tokens < most ? a.seg_tokens : most;
+  return longest < 1 ? 1 : (longest + SS_BLOCK - 1) / SS_BLOCK;
+}
+
 static int64_t ss_grad_layout(const lampa_ss_args& a, char* base, SsGrad* w) {
   const int64_t slots = ss_slots(&a), npb = ss_blocks64(a.P), nnb = ss_blocks64(a.N);
   int64_t at = 0;
@@ -199,7 +208,7 @@ static int64_t ss_grad_layout(const lampa_ss_args& a, char* base, SsGrad* w) {
   take(g.reach, a.n_tokens * a.H * npb);
   take(g.chunk_states, ss_rows(&a, serial ? SS_DOT : 64) * a.H * (serial ? (int64_t)a.N * a.P : npb * ss_chunk_n(a.N) * 64));
   take(g.chunk_dots, serial ? ss_rows(&a, SS_DOT) * a.H * npb : 0);
-  take(g.param_part, slots * a.H * 2);
+  take(g.param_part, slots * ss_pieces(a) * a.H * 2);
   take(g.dD_part, slots * a.H * npb);
   if (w) *w = g;
   return at;
@@ -227,23 +236,22 @@ extern "C" int lampa_ss_scan_bwd(const lampa_ss_args* args, void* stream) {
   if (!a.n_tokens) {
     if (a.dh0) e = ss_join<true>(a, nullptr, a.dht, a.dh0, s);
   } else {
-    if (!ss_single(&a)) {
-      if (!a.slot_states || !a.slot_decay) return LAMPA_ERR_WORKSPACE;
-      e = serial ? ss_serial_maps(a, &w, s) : ss_chunk_maps(a, &w, s);
-      if (e == LAMPA_OK) e = ss_join<true>(a, w.adjoints, a.dht, a.dh0, s);
-    }
+    const bool single = ss_single(&a);
+    if (!single && (!a.slot_states || !a.slot_decay)) return LAMPA_ERR_WORKSPACE;
+    if (!serial) e = ss_chunk_maps(a, &w, s);
+    else if (!single) e = ss_serial_maps(a, &w, s);
+    if (e == LAMPA_OK && !single) e = ss_join<true>(a, w.adjoints, a.dht, a.dh0, s);
     if (serial) {
       for (int kind : {SS_DC, SS_DX, SS_DB})
         if (e == LAMPA_OK) e = ss_serial_walk(a, kind, w, s);
-    } else {
-      if (e == LAMPA_OK) e = ss_chunk_keep(a, w, s);
-      if (e == LAMPA_OK) e = ss_chunk_grad(a, w, s);
+    } else if (e == LAMPA_OK) {
+      e = ss_chunk_grad(a, w, s);
     }
     if (e != LAMPA_OK) return e;
     const int64_t n = a.n_tokens * a.G * a.N;
     const bool wide = a.N % 4 == 0 && ((uintptr_t)a.dB | (uintptr_t)a.dC) % 16 == 0;
     const int64_t per = SS_BLOCK * (wide ? 4 : 1);
-    const dim3 sums((unsigned)((n + per - 1) / per), 2), segs((unsigned)slots, (unsigned)a.H);
+    const dim3 sums((unsigned)((n + per - 1) / per), 2), segs((unsigned)slots, (unsigned)a.H, (unsigned)ss_pieces(a));
     const int parts = a.H / a.G * ss_blocks64(a.P);
 #define SS_TAIL(T)                                                                                                          \
   hipLaunchKernelGGL((ss_decay_grad_kernel<T>), segs, dim3(SS_BLOCK), 0, s, a, w, !serial);                                          \
@@ -263,7 +271,7 @@ extern "C" int lampa_ss_scan_bwd(const lampa_ss_args* args, void* stream) {
 #undef SS_TAIL
   }
   if (e != LAMPA_OK) return e;
-  hipLaunchKernelGGL(ss_param_sum_kernel, dim3((unsigned)a.H, 3), dim3(SS_BLOCK), 0, s, a, w, slots);
+  hipLaunchKernelGGL(ss_param_sum_kernel, dim3((unsigned)a.H, 3), dim3(SS_BLOCK), 0, s, a, w, slots, ss_pieces(a));
   LAMPA_PROF(s, "ss_param_sum_kernel");
   return lampa_launch_status();
 }
