@@ -26,15 +26,19 @@ using sc_x4 = typename OpVec<T>::x4;
 // itself is rounded to the input type.
 template <typename T>
 struct ScParts { static const int n = __is_same(T, __bf16) ? 3 : 2; };
-// v is taken out of the compiler's sight: it would form an fp16 `hi` of a product in one rounding and the remainder from one of
-// two, which now and then (ties) is another value.
+// Two values at a time, as they are converted. fp16: the values are taken out of the compiler's sight, which would form the first
+// part of a product in one rounding and the remainder from one of two, which now and then (ties) is another value.
 template <typename T, int PARTS>
-__device__ __forceinline__ void sc_split(float v, T (&part)[PARTS]) {
-  if constexpr (__is_same(T, _Float16)) asm("" : "+v"(v));
+__device__ __forceinline__ void sc_split(float a, float b, typename OpVec<T>::x2 (&part)[PARTS]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  if constexpr (__is_same(T, _Float16)) asm("" : "+v"(a), "+v"(b));
 #pragma unroll
   for (int k = 0; k < PARTS; ++k) {
-    part[k] = (T)v;
-    v -= (float)part[k];
+    part[k] = __builtin_convertvector(f32x2{a, b}, typename OpVec<T>::x2);
+    if (k + 1 < PARTS) {
+      a -= (float)part[k][0];
+      b -= (float)part[k][1];
+    }
   }
 }
 
@@ -200,23 +204,30 @@ __device__ __forceinline__ void sc_row_weights(const float* w, int kk, int lane,
 template <typename T, int PARTS>
 __device__ __forceinline__ void sc_weighted(const sc_x8<T>& x, const float (&w)[8], sc_x8<T> (&out)[PARTS]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    T part[PARTS];
-    sc_split<T, PARTS>((float)x[e] * w[e], part);
+  for (int e = 0; e < 8; e += 2) {
+    typename OpVec<T>::x2 part[PARTS];
+    sc_split<T, PARTS>((float)x[e] * w[e], (float)x[e + 1] * w[e + 1], part);
 #pragma unroll
-    for (int k = 0; k < PARTS; ++k) out[k][e] = part[k];
+    for (int k = 0; k < PARTS; ++k) {
+      out[k][e] = part[k][0];
+      out[k][e + 1] = part[k][1];
+    }
   }
 }
 // Two accumulator tiles (32 rows) as an operand in parts.
 template <typename T, int PARTS>
 __device__ __forceinline__ void sc_state_operand(const f32x4& a, const f32x4& b, float scale, sc_x8<T> (&out)[PARTS]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float v = e < 4 ? a[e] : b[e - 4];
-    T part[PARTS];
-    sc_split<T, PARTS>(__is_same(T, _Float16) ? v * scale : v, part);
+  for (int e = 0; e < 8; e += 2) {
+    const float u = e < 4 ? a[e] : b[e - 4], v = e < 4 ? a[e + 1] : b[e - 3];
+    typename OpVec<T>::x2 part[PARTS];
+    if constexpr (__is_same(T, _Float16)) sc_split<T, PARTS>(u * scale, v * scale, part);
+    else sc_split<T, PARTS>(u, v, part);
 #pragma unroll
-    for (int k = 0; k < PARTS; ++k) out[k][e] = part[k];
+    for (int k = 0; k < PARTS; ++k) {
+      out[k][e] = part[k][0];
+      out[k][e + 1] = part[k][1];
+    }
   }
 }
 // acc + left * (the operand's parts), the smallest first
@@ -233,10 +244,10 @@ __device__ __forceinline__ f32x4 sc_mfma_right(const X8 (&left)[PARTS], const X8
   return acc;
 }
 
-// acc[nt] += (columns 16 nt .. of the tile)^T * (the first `parts` parts of an operand over its 64 rows). Every product goes to
+// acc[nt] += (columns 16 nt .. of the tile)^T * (an operand over its 64 rows, in parts). Every product goes to
 // another tile than the one before it, which it would otherwise wait for.
 template <typename T, int NT, int PARTS>
-__device__ __forceinline__ void sc_add_products(const T* tile, int stride, int lane, const sc_x8<T> (&right)[2][PARTS], int parts,
+__device__ __forceinline__ void sc_add_products(const T* tile, int stride, int lane, const sc_x8<T> (&right)[2][PARTS],
                                                 f32x4 (&acc)[NT]) {
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) {
@@ -245,10 +256,44 @@ __device__ __forceinline__ void sc_add_products(const T* tile, int stride, int l
     for (int nt = 0; nt < NT; ++nt) left[nt] = op_ld_tr16<T, true>(tile, stride, 16 * nt, 32 * kk, lane);
 #pragma unroll
     for (int k = PARTS - 1; k >= 0; --k) {
-      if (k >= parts) continue;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) acc[nt] = mfma16(left[nt], right[kk][k], acc[nt]);
     }
+  }
+}
+
+// S <- end S + (tile)^T * (v, its rows weighted), the product of a wave's 16 columns with all rows of the state.
+template <typename T, int NT, int PARTS>
+__device__ __forceinline__ void sc_update(const T* tile, int stride, int lane, const sc_x8<T> (&v)[2], float (&wt)[2][8], float end,
+                                          f32x4 (&S)[NT]) {
+  sc_x8<T> vw[2][PARTS];
+  if constexpr (__is_same(T, _Float16)) {  // the largest weight becomes 1 or a little less: v is in range by itself
+    float m = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(wt[kk][e]));
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    const float s = sc_scale_for<T>(m) * 0x1p-15f, back = sc_inverse(s);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wt[kk][e] *= s;
+      sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
+    }
+    f32x4 d[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) d[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    sc_add_products<T, NT, PARTS>(tile, stride, lane, vw, d);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) S[nt] = S[nt] * end + d[nt] * back;
+  } else {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
+    sc_add_products<T, NT, PARTS>(tile, stride, lane, vw, S);
   }
 }
 

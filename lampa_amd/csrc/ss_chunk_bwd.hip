@@ -140,11 +140,13 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
           for (int r = 0; r < 4; ++r) {
             const int t = 16 * tt + 4 * g + r;
             const float l = __builtin_amdgcn_exp2f(gt[r] - gs);
-            const float vg = t >= s ? l * G[r] : 0.0f, both = t >= s ? vg * Hm[r] * rest[r] : 0.0f;
+            const bool on = tt > wave || t >= s;
+            const float vg = on ? l * G[r] : 0.0f, both = on ? vg * Hm[r] * rest[r] : 0.0f;
             lg[tt][r] = vg;
-            lh[tt][r] = t >= s ? ds * l * Hm[r] : 0.0f;
-            if (t == s) own = both; else sum += both;
-            rows[r] = sc_row16_sum(t == s ? 0.0f : ds_rest * both);
+            lh[tt][r] = on ? ds * l * Hm[r] : 0.0f;
+            const bool self = tt == wave && t == s;
+            if (self) own = both; else sum += both;
+            rows[r] = sc_row16_sum(self ? 0.0f : ds_rest * both);
             if (F16) { big1 = fmaxf(big1, fabsf(vg)); big2 = fmaxf(big2, fabsf(lh[tt][r])); }
           }
         }

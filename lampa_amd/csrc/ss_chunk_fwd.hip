@@ -11,7 +11,7 @@ struct ScMapTiles {
   __align__(16) T k[64 * KS], v[64 * VS];
   __align__(16) ScDecay dec;
 };
-template <typename T, int NP, bool REV, bool KEEP, bool VEC>
+template <typename T, int NP, bool REV, bool KEEP, bool VEC, int PARTS>
 __device__ __forceinline__ void sc_map(const lampa_ss_args& a, const SsGrad& w, ScMapTiles<T, NP>& tiles) {
   constexpr int NT = NP / 16, KS = NP + 8, VS = 64 + 8;
   const SsSegment seg = ss_segment(a, blockIdx.x);
@@ -27,8 +27,6 @@ __device__ __forceinline__ void sc_map(const lampa_ss_args& a, const SsGrad& w, 
   const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
   const int64_t chunks = seg.outside ? 0 : (seg.t1 - seg.t0 + 63) / 64;
 
-  // the third part only where the states go to the caller or into gradients
-  const bool whole = REV || KEEP || a.ht;
   f32x4 S[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) S[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -72,10 +70,9 @@ __device__ __forceinline__ void sc_map(const lampa_ss_args& a, const SsGrad& w, 
     if (c + 1 < chunks) fetch(c + 1);
     const float end = dec.end;
     sum += dec.sum;
-    constexpr int PARTS = ScParts<T>::n;
-    sc_x8<T> v[2], vw[2][PARTS];
+    sc_x8<T> v[2];
     sc_columns<T>(tv, VS, 16 * wave, lane, v);
-    float wt[2][8], back = 1.0f;
+    float wt[2][8];
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       if constexpr (REV) {
@@ -88,36 +85,7 @@ __device__ __forceinline__ void sc_map(const lampa_ss_args& a, const SsGrad& w, 
         for (int e = 0; e < 8; ++e) wt[kk][e] *= d[e];
       }
     }
-    if constexpr (__is_same(T, _Float16)) {  // the largest weight becomes 1 or a little less: x is in range by itself
-      float m = 0.0f;
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(wt[kk][e]));
-      m = fmaxf(m, __shfl_xor(m, 16));
-      m = fmaxf(m, __shfl_xor(m, 32));
-      const float s = sc_scale_for<T>(m) * 0x1p-15f;
-      back = sc_inverse(s);
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) wt[kk][e] *= s;
-    }
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
-    // (a product of one tile after the other: no product waits for the one before it)
-    if constexpr (__is_same(T, _Float16)) {
-      f32x4 d[NT];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) d[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      sc_add_products<T, NT, PARTS>(tk, KS, lane, vw, PARTS, d);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) S[nt] = S[nt] * end + d[nt] * back;
-    } else {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
-      sc_add_products<T, NT, PARTS>(tk, KS, lane, vw, whole ? PARTS : 2, S);
-    }
+    sc_update<T, NT, PARTS>(tk, KS, lane, v, wt, end, S);
     lds_barrier();
   }
   if (KEEP) return;
@@ -136,18 +104,19 @@ __device__ __forceinline__ void sc_map(const lampa_ss_args& a, const SsGrad& w, 
 template <typename T, int NP, bool VEC>
 constexpr int sc_map_waves() { return !VEC ? 2 : NP <= 64 ? (__is_same(T, __bf16) ? 4 : 3) : (__is_same(T, __bf16) ? 3 : 2); }
 
-template <typename T, int NP, bool VEC>
+// PARTS: all of them where the states go to the caller or into gradients, two where they only go into outputs.
+template <typename T, int NP, bool VEC, int PARTS>
 __global__ void __launch_bounds__(SC_BLOCK, (sc_map_waves<T, NP, VEC>())) sc_map_kernel(lampa_ss_args a, SsGrad w) {
   __shared__ ScMapTiles<T, NP> tiles;
-  sc_map<T, NP, false, false, VEC>(a, w, tiles);
+  sc_map<T, NP, false, false, VEC, PARTS>(a, w, tiles);
 }
 // Before the gradients: the states in front of the chunks (first half of the grid) and the local adjoints, which do not depend on
 // each other, side by side: neither fills the chip by itself (60 000 tokens x 8 heads, N = 128: 62 and 120 us in turn).
 template <typename T, int NP, bool VEC>
 __global__ void __launch_bounds__(SC_BLOCK, (sc_map_waves<T, NP, VEC>())) sc_prepare_kernel(lampa_ss_args a, SsGrad w) {
   __shared__ ScMapTiles<T, NP> tiles;
-  if (blockIdx.z == 0) sc_map<T, NP, false, true, VEC>(a, w, tiles);
-  else sc_map<T, NP, true, false, VEC>(a, w, tiles);
+  if (blockIdx.z == 0) sc_map<T, NP, false, true, VEC, ScParts<T>::n>(a, w, tiles);
+  else sc_map<T, NP, true, false, VEC, ScParts<T>::n>(a, w, tiles);
 }
 
 // Outputs of a segment from the state it starts from.
@@ -245,7 +214,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float v = m[st][r] * ds[r] * __builtin_amdgcn_exp2f(gt - gs[r]);
-          m[st][r] = 16 * st + 4 * g + r <= 16 * wave + i ? v : 0.0f;
+          m[st][r] = st < wave || 4 * g + r <= i ? v : 0.0f;
           if (__is_same(T, _Float16)) big = fmaxf(big, fabsf(m[st][r]));
         }
       }
@@ -322,7 +291,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
     }
     // the state behind the chunk
     {
-      float wt[2][8], back = 1.0f;
+      float wt[2][8];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         float d[8];
@@ -331,39 +300,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) wt[kk][e] *= d[e];
       }
-      if constexpr (__is_same(T, _Float16)) {
-        float m = 0.0f;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(wt[kk][e]));
-        m = fmaxf(m, __shfl_xor(m, 16));
-        m = fmaxf(m, __shfl_xor(m, 32));
-        const float s = sc_scale_for<T>(m) * 0x1p-15f;
-        back = sc_inverse(s);
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) wt[kk][e] *= s;
-      }
-      // the third part only where the state goes to the caller
-      constexpr int PARTS = ScParts<T>::n;
-      sc_x8<T> vw[2][PARTS];
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
-      const float end = dec.end;
-      if constexpr (__is_same(T, _Float16)) {
-        f32x4 d[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) d[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        sc_add_products<T, NT, PARTS>(tb, KS, lane, vw, PARTS, d);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) S[nt] = S[nt] * end + d[nt] * back;
-      } else {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
-        sc_add_products<T, NT, PARTS>(tb, KS, lane, vw, handed_on ? PARTS : 2, S);
-      }
+      if (handed_on) sc_update<T, NT, ScParts<T>::n>(tb, KS, lane, v, wt, dec.end, S);
+      else sc_update<T, NT, 2>(tb, KS, lane, v, wt, dec.end, S);
     }
     t0 += n;
     lds_barrier();
@@ -387,7 +325,8 @@ static int sc_maps_launch(const lampa_ss_args& a, const SsGrad* grad, hipStream_
   LAMPA_PROF(s, "start");
 #define SC_GO(NP)                                                                                           \
   if (grad) hipLaunchKernelGGL((sc_prepare_kernel<T, NP, VEC>), grid, dim3(SC_BLOCK), 0, s, a, *grad);      \
-  else hipLaunchKernelGGL((sc_map_kernel<T, NP, VEC>), grid, dim3(SC_BLOCK), 0, s, a, SsGrad{})
+  else if (a.ht) hipLaunchKernelGGL((sc_map_kernel<T, NP, VEC, ScParts<T>::n>), grid, dim3(SC_BLOCK), 0, s, a, SsGrad{}); \
+  else hipLaunchKernelGGL((sc_map_kernel<T, NP, VEC, 2>), grid, dim3(SC_BLOCK), 0, s, a, SsGrad{})
   if (a.N <= 32) { SC_GO(32); } else if (a.N <= 64) { SC_GO(64); } else { SC_GO(128); }
 #undef SC_GO
   LAMPA_PROF(s, grad ? "sc_prepare_kernel" : "sc_map_kernel");
