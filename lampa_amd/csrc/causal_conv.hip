@@ -6,6 +6,10 @@
 //   dpre[t] = dy[t] y'(pre[t]),  dx[s] = sum_j w[j] dpre[s + W-1 - j],  dw[j] = sum_t dpre[t] x[t - (W-1) + j],  dbias = sum_t dpre[t]
 // Bound by bytes: every row of x (and dy) is read once, plus W - 1 (and 2 (W - 1)) rows of history for every run of tokens,
 // which hit in L2. Arithmetic is fp32, results are rounded once.
+//
+// Measured: gradients of 60 000 x 640 in bf16 66 us (230 MB, 3.5 TB/s) and 10 us for the sums over the workgroups' rows (the
+// vector instructions, about 30 a value, are what is left: 40 us of it); 24 packed sequences, 15 000 x 224 in fp16, with state
+// 20 us.
 #include "gdr_common.h"
 #include "row_sums.h"
 

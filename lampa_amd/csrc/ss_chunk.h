@@ -11,6 +11,11 @@
 // matrix cores has to be; they carry the same relative error as the output's own rounding. The state and the decayed x enter as
 // two or three operands of the input type each, value and remainders (ScParts): the state is handed from chunk to chunk and out
 // to the caller in fp32, and its sums are what the gradient of the decays is made of.
+//
+// Measured, 60 000 tokens x 8 heads of 64 in bf16, one group of B and C. N = 64, forward: local states 32 us, join 15, outputs 64 (137
+// MB; 600 vector instructions a wave and chunk keep the vector units two thirds busy, the matrix cores a sixth). N = 128 with
+// gradients: local states 62, join 33 both ways, outputs 115, kept states and local adjoints 163 (of them 246 MB of kept
+// states written), gradients 350, sums of dB and dC over the heads 125 (490 MB, 3.9 TB/s).
 #pragma once
 #include "ss_kernels.h"
 
@@ -297,8 +302,8 @@ __device__ __forceinline__ void sc_update(const T* tile, int stride, int lane, c
   }
 }
 
-// Whether every row of a call can be read in 16-byte pieces and written in 8-byte ones (the kernels are built for both: their
-// loads element by element would cost the others registers).
+// Whether every row of a call can be read in 16-byte pieces and written in 8-byte ones. The kernels are built for both: loads
+// element by element beside the others would cost those registers (local states at N = 64: 182 against 122).
 static bool sc_vectors(const lampa_ss_args& a) {
   auto rows = [](const void* p, int64_t stride, int inner) { return (uintptr_t)p % 16 == 0 && stride % 8 == 0 && inner % 8 == 0; };
   return rows(a.x, a.x_stride, a.P) && rows(a.B, a.B_stride, a.N) && rows(a.C, a.C_stride, a.N) && rows(a.dy, 8, a.P) &&

@@ -3,6 +3,8 @@
 // Bound by the state's bytes, read once and written once. A workgroup takes PB columns (all N rows) of one head's state:
 // PB / VW lanes side by side over the columns, the rest of the 256 threads over the rows, so that every load of the state
 // can be under way at once; y is then summed over the rows' threads.
+//
+// Measured, bf16, 8 heads of 64: 250 sequences at N = 128 26 us (139 MB, 5.3 TB/s), one sequence at N = 64 6.5 us.
 #include "ss_common.h"
 
 #define SP_BLOCK 256
@@ -90,7 +92,9 @@ static int ss_step_launch(const void* x, int64_t xs, const void* dt, int dt_dtyp
                           float* new_state, void* y, int n, int H, int P, int G, int N, int softplus, hipStream_t s) {
   const bool vec = P % 4 == 0 && ((uintptr_t)state | (uintptr_t)new_state) % 16 == 0;
   const int64_t wide = (int64_t)n * H * ((P + 63) / 64), narrow = (int64_t)n * H * ((P + 15) / 16);
-  const bool few = wide < 256;  // fewer workgroups than CUs: narrower ones, more loads under way
+  // Fewer workgroups than CUs: narrower ones. 16 against 64 columns a workgroup, us, sequences x N (8 heads of 64): 1 x 128 6.7 / 8.0,
+  // 16 x 128 7.4 / 8.7, 32 x 64 8.2 / 7.6, 64 x 128 16.7 / 10.6, 250 x 128 42.8 / 26.0.
+  const bool few = wide < 256;
   if ((few ? narrow : wide) > 0x7fffffff) return LAMPA_ERR_UNSUPPORTED;
   LAMPA_PROF(s, "start");
 #define SP_GO(PB, VW)                                                                                                     \

@@ -274,6 +274,34 @@ def test_rows_outside_the_boundaries(device, dtype, monkeypatch):
     assert torch.equal(beyond, inside)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_where_the_operands_lie(device, dtype):
+    """Slices off every alignment, tokens and batches out of order, broadcast tensors, gradients that are no tensors of their own:
+    the bits of contiguous copies."""
+    gen = torch.Generator().manual_seed(50)
+    r = lambda *s: torch.randn(*s, generator=gen).to(dtype).to(device)  # noqa: E731
+    i = _to(_inputs((3, 90), 2, 16, 1, 24, dtype, 51, 3), device)
+    wide = r(3, 90, 100)
+    forms = [
+        {"x": wide[..., 3:35].unflatten(-1, (2, 16)), "B": wide[..., 37:61].unsqueeze(2), "C": wide[..., 75:99].unsqueeze(2), "dt": wide[..., 35:37]},
+        {"x": r(90, 3, 2, 16).transpose(0, 1), "B": r(3, 1, 90, 24).transpose(1, 2), "C": r(90, 3, 1, 24).transpose(0, 1), "dt": r(90, 2, 3).permute(2, 0, 1)},
+        {"x": r(3, 90, 16, 2).transpose(2, 3), "B": r(1, 1, 1, 24).expand(3, 90, 1, 24), "C": r(3, 1, 1, 24).expand(3, 90, 1, 24), "dt": r(3, 1, 2).expand(3, 90, 2)},
+    ]
+    dy = r(3, 2, 90, 16).transpose(1, 2)
+    for form in forms:
+        out = []
+        for copy in (False, True):
+            d = {**i, **form}
+            d = {k: (t.contiguous().clone() if copy else t).detach().requires_grad_(True) for k, t in d.items()}
+            y, ht = _call(d)
+            out.append([y, ht, *torch.autograd.grad(y, [d[k] for k in ("x", "dt", "A", "B", "C", "D", "dt_bias", "h0")],
+                                                    dy.contiguous() if copy else dy)])
+        for a, b in zip(*out):
+            assert torch.equal(a, b)
+    y, _ = _call({**i, "x": i["x"].requires_grad_(True)})
+    assert torch.equal(torch.autograd.grad(y.sum(), i["x"], retain_graph=True)[0], torch.autograd.grad(y, i["x"], torch.ones_like(y))[0])
+
+
 def test_no_tokens(device):
     i = _to(_inputs((2, 0), 2, 16, 1, 8, torch.bfloat16, 16, 2), device, grad=True)
     y, ht = _call(i)
