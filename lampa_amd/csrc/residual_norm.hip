@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
     if (a.dres) ndr.load((const RT*)a.dres + at);
   };
   if (AHEAD) request((int64_t)blockIdx.x * ROWS);
-  // every thread makes the same number of turns: rows past the end are worked on as zeros and not stored
+  // every thread makes the same number of turns: rows past the end are worked on as zeros, with a norm of zero (eps may be 0),
+  // and not stored
   for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < n_rows; r0 += stride) {
     const bool live = r0 + slot < n_rows;
     const int64_t row = row_base + r0 + slot;
@@ -145,7 +146,10 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
       for (int c = 0; c < 8; ++c) sq = __builtin_fmaf(x[st][c], x[st][c], sq);
     }
     float i1 = 1.0f;
-    if (a.post_weight) i1 = 1.0f / sqrtf(rn_row_sum<LPR>(sq, part, turn) * inv_d + a.eps);
+    if (a.post_weight) {
+      const float mean = rn_row_sum<LPR>(sq, part, turn) * inv_d;
+      i1 = live ? 1.0f / sqrtf(mean + a.eps) : 0.0f;
+    }
     const int64_t gate_row = a.gate_kind == RN_GATE_SEQ ? row / a.seq_rows : row;
     float am[GRAD ? STEPS : 1][8], act[GRAD ? STEPS : 1][8], slope[GRAD ? STEPS : 1][8];  // a; act(gate); its derivative
     float sq2 = 0.0f;
@@ -175,7 +179,8 @@ __global__ void __launch_bounds__(RN_BLOCK) rn_kernel(RnArgs a) {
       if constexpr (!GRAD)
         if (on && a.res_out) rn_store8((RT*)a.res_out + row * a.D + c0, h[st]);
     }
-    const float i2 = 1.0f / sqrtf(rn_row_sum<LPR>(sq2, part, turn) * inv_d + a.eps);
+    const float mean2 = rn_row_sum<LPR>(sq2, part, turn) * inv_d;
+    const float i2 = live ? 1.0f / sqrtf(mean2 + a.eps) : 0.0f;
     if constexpr (!GRAD) {
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {

@@ -59,6 +59,11 @@ __device__ __forceinline__ float sc_scale_for(float largest) {
   }
   return 1.0f;
 }
+// The largest so far: a value that is not finite does not set the scale of the others that share it.
+__device__ __forceinline__ float sc_larger(float big, float v) {
+  v = fabsf(v);
+  return v < __builtin_inff() ? fmaxf(big, v) : big;
+}
 __device__ __forceinline__ float sc_inverse(float power_of_two) { return __uint_as_float((254u << 23) - __float_as_uint(power_of_two)); }
 
 __device__ __forceinline__ float sc_wave_max(float v) {

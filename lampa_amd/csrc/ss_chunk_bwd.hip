@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) big = fmaxf(big, fabsf(R[nt][r]));
+          for (int r = 0; r < 4; ++r) big = sc_larger(big, R[nt][r]);
         sc = sc_scale_for<T>(sc_wave_max(big));
         sback = sc_inverse(sc);
       }
@@ -268,8 +268,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
           for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              big1 = fmaxf(big1, fabsf(RT[q][j][r]));
-              big2 = fmaxf(big2, fabsf(S[q][r]));
+              big1 = sc_larger(big1, RT[q][j][r]);
+              big2 = sc_larger(big2, S[q][r]);
             }
           s1 = sc_scale_for<T>(sc_wave_max(big1));
           b1 = sc_inverse(s1);

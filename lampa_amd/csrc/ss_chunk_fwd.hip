@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) big = fmaxf(big, fabsf(S[nt][r]));
+          for (int r = 0; r < 4; ++r) big = sc_larger(big, S[nt][r]);
         s = sc_scale_for<T>(sc_wave_max(big));
         sback = sc_inverse(s);
       }

@@ -25,7 +25,6 @@ struct SsSegment {
   int seq, index;   // sequence, place of the segment in it
   int64_t begin;    // first token of the sequence
   bool live;        // false: this slot holds no segment
-  bool first, last; // in its sequence
   bool outside;     // rows behind the last sequence: their outputs are zero
 };
 
@@ -72,8 +71,6 @@ __device__ __forceinline__ SsSegment ss_segment(const lampa_ss_args& a, int64_t 
   s.t1 = s.t0 + a.seg_tokens < e ? s.t0 + a.seg_tokens : e;
   if (s.t1 < s.t0) s.t1 = s.t0;
   s.begin = b;
-  s.first = s.index == 0;
-  s.last = s.t1 >= e;
   return s;
 }
 

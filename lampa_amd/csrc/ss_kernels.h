@@ -1,5 +1,5 @@
 // What the state-space scan's kernels share beside the call's arguments: the buffers of the gradients, and the launchers of
-// the walks (token-serial for every type, chunks on the matrix cores for 16-bit types).
+// the walks (token-serial for fp32, chunks on the matrix cores for 16-bit types).
 #pragma once
 #include "ss_common.h"
 

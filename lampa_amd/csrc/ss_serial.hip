@@ -15,7 +15,7 @@
 
 #define SS_TILE 8  // tokens staged at once
 
-template <typename T, int ROWS, int KIND, bool MAP>
+template <int ROWS, int KIND, bool MAP>
 __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w) {
   constexpr bool REV = KIND == SS_DX || KIND == SS_DB;  // from the end of the segment
   constexpr bool LANE_P = KIND == SS_Y || KIND == SS_DX;
@@ -58,12 +58,12 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
     }
   }
 
-  const T* x = (const T*)a.x + (int64_t)h * a.P;
-  const T* dy = (const T*)a.dy + (int64_t)h * a.P;
-  const T* Bm = (const T*)a.B + (int64_t)grp * a.N;
-  const T* Cm = (const T*)a.C + (int64_t)grp * a.N;
+  const float* x = (const float*)a.x + (int64_t)h * a.P;
+  const float* dy = (const float*)a.dy + (int64_t)h * a.P;
+  const float* Bm = (const float*)a.B + (int64_t)grp * a.N;
+  const float* Cm = (const float*)a.C + (int64_t)grp * a.N;
   const int64_t dy_stride = (int64_t)a.H * a.P;
-  const T *U, *Q, *V;
+  const float *U, *Q, *V;
   int64_t us, qs, vs;
   if constexpr (KIND == SS_Y) { U = Bm; us = a.B_stride; Q = Cm; qs = a.C_stride; V = x; vs = a.x_stride; }
   else if constexpr (KIND == SS_DC) { U = x; us = a.x_stride; Q = dy; qs = dy_stride; V = Bm; vs = a.B_stride; }
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
   else { U = dy; us = dy_stride; Q = x; qs = a.x_stride; V = Cm; vs = a.C_stride; }
   // a second lane vector: C (dC's dot with it), x (dx's)
   constexpr bool EXTRA = !MAP && (KIND == SS_DC || KIND == SS_DX);
-  const T* E = KIND == SS_DC ? Cm : x;
+  const float* E = KIND == SS_DC ? Cm : x;
   const int64_t es = KIND == SS_DC ? a.C_stride : a.x_stride;
   const float A = a.A[h], D = a.D ? a.D[h] : 0.0f, bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
 
@@ -87,16 +87,16 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
     for (int k = 0; k < PIECES; ++k) {
       const int i = lane + 64 * k, t = i / ROWS, r = i % ROWS;
       const bool on = t < n && r < rn;
-      pu[k] = on ? GdrElem<T>::to_float(U[(t0 + t) * us + r0 + r]) : 0.0f;
-      if (!MAP) pq[k] = on ? GdrElem<T>::to_float(Q[(t0 + t) * qs + r0 + r]) : 0.0f;
+      pu[k] = on ? U[(t0 + t) * us + r0 + r] : 0.0f;
+      if (!MAP) pq[k] = on ? Q[(t0 + t) * qs + r0 + r] : 0.0f;
     }
 #pragma unroll
     for (int t = 0; t < SS_TILE; ++t) {
       const bool on = t < n && lane_on;
-      pv[t] = on ? GdrElem<T>::to_float(V[(t0 + t) * vs + l]) : 0.0f;
-      if (EXTRA) pe[t] = on ? GdrElem<T>::to_float(E[(t0 + t) * es + l]) : 0.0f;
+      pv[t] = on ? V[(t0 + t) * vs + l] : 0.0f;
+      if (EXTRA) pe[t] = on ? E[(t0 + t) * es + l] : 0.0f;
     }
-    if (lane < n) pdt = ss_load_dt<T>(a.dt, a.dt_dtype, (t0 + lane) * a.dt_stride + h);
+    if (lane < n) pdt = ((const float*)a.dt)[(t0 + lane) * a.dt_stride + h];
   };
 
   float carry = 1.0f;   // reverse walks: the decay between the token before (later in time) and this one
@@ -168,12 +168,12 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
       if constexpr (!MAP) {
         if constexpr (KIND == SS_Y) {
           if (lane_on)
-            ((T*)a.y)[tok * a.y_stride + (int64_t)h * a.P + l] =
-                GdrElem<T>::from_float(seg.outside ? 0.0f : __builtin_fmaf(D, lv[t][lane], out));
+            ((float*)a.y)[tok * a.y_stride + (int64_t)h * a.P + l] =
+                seg.outside ? 0.0f : __builtin_fmaf(D, lv[t][lane], out);
         } else if constexpr (KIND == SS_DX) {
           const float dyv = seg.outside ? 0.0f : lv[t][lane], xv = seg.outside ? 0.0f : le[t][lane];
-          if (lane_on) ((T*)a.dx)[tok * dy_stride + (int64_t)h * a.P + l] =
-              GdrElem<T>::from_float(__builtin_fmaf(delta, out, D * dyv));
+          if (lane_on) ((float*)a.dx)[tok * dy_stride + (int64_t)h * a.P + l] =
+              __builtin_fmaf(delta, out, D * dyv);
           const float q = ss_wave_sum(lane_on ? xv * out : 0.0f);
           if (lane == 0) w.reach[(tok * a.H + h) * npb + pb] = q;
           dD = __builtin_fmaf(xv, dyv, dD);
@@ -218,37 +218,29 @@ __global__ void __launch_bounds__(64) ss_serial_kernel(lampa_ss_args a, SsGrad w
   }
 }
 
-template <typename T, int KIND, bool MAP>
+template <int KIND, bool MAP>
 static int ss_serial_launch(const lampa_ss_args& a, const SsGrad& w, hipStream_t s) {
   const int npb = ss_blocks64(a.P), nnb = ss_blocks64(a.N);
   constexpr bool LANE_P = KIND == SS_Y || KIND == SS_DX;
   const dim3 grid((unsigned)ss_slots(&a), (unsigned)(a.H * npb * (LANE_P ? 1 : nnb)));
   const int rows = LANE_P ? a.N : (a.P < 64 ? a.P : 64);
   LAMPA_PROF(s, "start");
-  if (rows <= 32) hipLaunchKernelGGL((ss_serial_kernel<T, 32, KIND, MAP>), grid, dim3(64), 0, s, a, w);
-  else if (rows <= 64) hipLaunchKernelGGL((ss_serial_kernel<T, 64, KIND, MAP>), grid, dim3(64), 0, s, a, w);
-  else if constexpr (LANE_P) hipLaunchKernelGGL((ss_serial_kernel<T, 128, KIND, MAP>), grid, dim3(64), 0, s, a, w);
+  if (rows <= 32) hipLaunchKernelGGL((ss_serial_kernel<32, KIND, MAP>), grid, dim3(64), 0, s, a, w);
+  else if (rows <= 64) hipLaunchKernelGGL((ss_serial_kernel<64, KIND, MAP>), grid, dim3(64), 0, s, a, w);
+  else if constexpr (LANE_P) hipLaunchKernelGGL((ss_serial_kernel<128, KIND, MAP>), grid, dim3(64), 0, s, a, w);
   LAMPA_PROF(s, MAP ? "ss_serial_kernel<map>" : "ss_serial_kernel<walk>");
   return lampa_launch_status();
 }
 
-#define SS_TYPES(CALL)                                     \
-  switch (a.dtype) {                                       \
-    case GDR_BF16: { typedef __bf16 T; return CALL; }      \
-    case GDR_FP16: { typedef _Float16 T; return CALL; }    \
-    default: { typedef float T; return CALL; }             \
-  }
-
 int ss_serial_maps(const lampa_ss_args& a, const SsGrad* grad, hipStream_t s) {
-  if (grad) { SS_TYPES((ss_serial_launch<T, SS_DX, true>(a, *grad, s))) }
-  SS_TYPES((ss_serial_launch<T, SS_Y, true>(a, SsGrad{}, s)))
+  return grad ? ss_serial_launch<SS_DX, true>(a, *grad, s) : ss_serial_launch<SS_Y, true>(a, SsGrad{}, s);
 }
 
 int ss_serial_walk(const lampa_ss_args& a, int kind, const SsGrad& grad, hipStream_t s) {
   switch (kind) {
-    case SS_Y: SS_TYPES((ss_serial_launch<T, SS_Y, false>(a, grad, s)))
-    case SS_DC: SS_TYPES((ss_serial_launch<T, SS_DC, false>(a, grad, s)))
-    case SS_DX: SS_TYPES((ss_serial_launch<T, SS_DX, false>(a, grad, s)))
-    default: SS_TYPES((ss_serial_launch<T, SS_DB, false>(a, grad, s)))
+    case SS_Y: return ss_serial_launch<SS_Y, false>(a, grad, s);
+    case SS_DC: return ss_serial_launch<SS_DC, false>(a, grad, s);
+    case SS_DX: return ss_serial_launch<SS_DX, false>(a, grad, s);
+    default: return ss_serial_launch<SS_DB, false>(a, grad, s);
   }
 }

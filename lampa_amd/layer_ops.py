@@ -12,6 +12,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd.graph import increment_version
 
 from . import _capi
 from ._capi import check, ptr, require_cuda, stream_of
@@ -229,6 +230,10 @@ class _CausalConv(torch.autograd.Function):
     def backward(ctx, dy, _):
         x, weight, bias, past, cu = ctx.saved_tensors
         B, T, D = x.shape
+        if x.numel() == 0:
+            zero = lambda i, t: torch.zeros_like(t) if ctx.needs_input_grad[i] else None  # noqa: E731
+            return (zero(0, x), zero(1, weight), zero(2, bias),
+                    dy.to(ctx.residual_dtype) if ctx.needs_input_grad[3] else None, None, None, None, None)
         w2 = weight.reshape(D, -1)
         W = w2.shape[1]
         x2, step, w32, b32 = _conv_operands(x, w2, bias)
@@ -259,7 +264,7 @@ def causal_conv1d(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: 
     """``short_convolution.py:426-458``: x [B, T, D], weight [D, W] (tap W-1 on the current token), bias [D],
     residual [B, T, D]; activation ``None`` / ``'silu'`` / ``'swish'``; with ``cu_seqlens`` B must be 1 and taps never
     cross a sequence start. Returns [B, T, D] in x's dtype (fp32 arithmetic). Differentiable in x, weight, bias and residual
-    (first order; repeated calls give the same bits).
+    (first order; repeated calls give the same bits); the gradients take cu_seqlens to end at T.
 
     ``initial_state`` [sequences, D, W] holds the W inputs before each sequence (a cache as ``causal_conv1d_step`` and
     ``ShortConvolution`` keep it; its oldest column is not read), and ``output_final_state`` returns (y, the W inputs up to
@@ -355,6 +360,7 @@ def causal_conv1d_step(x: torch.Tensor, cache: torch.Tensor, weight: torch.Tenso
     if n == 0:
         return torch.empty_like(x)
     target = cache if new_cache is None else new_cache
+    increment_version(target)  # written through its pointer: a backward that saved it must notice
     if _wants_grad(x, weight, bias):
         return _ForwardOnly.apply(lambda: _conv_step_launch(x, cache, weight, bias, activation, target), x, weight, bias)
     return _conv_step_launch(x, cache, weight, bias, activation, target)

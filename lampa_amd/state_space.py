@@ -15,6 +15,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _capi
 from ._capi import check, ptr, require_cuda, stream_of
@@ -179,8 +180,11 @@ def state_space_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torc
     and ends at T. A tensor on the host is checked; one on the GPU is not read by the host (so a call can be captured in a
     graph): boundaries outside the tokens are moved inside, and tokens behind the last boundary come back as zero.
 
-    A value that is not finite reaches the tokens from its own on, as in the recurrence, never earlier ones. Differentiable in every floating-point input (first order); the
-    gradients of B and C are summed over a group's heads in a fixed order, and repeated calls give the same bits."""
+    A value that is not finite reaches the tokens from its own on, as in the recurrence, never earlier ones (in gradients a
+    dy, B or C that is not finite may reach every token of its 64). Growth (delta A > 0) is taken as it is; where it passes
+    float32's range within 64 tokens or a segment the result may be NaN where the recurrence, on zeros, is not.
+    Differentiable in every floating-point input (first order); the gradients of B and C are summed over a group's heads in
+    a fixed order, and repeated calls give the same bits."""
     what = "state_space_scan"
     _same_device(what, x, dt, A, B, C, D, dt_bias, initial_state)
     _check_operands(what, x, dt, A, B, C, D, dt_bias, 2)
@@ -242,6 +246,7 @@ def state_space_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torc
     if x.shape[0] == 0:
         return torch.empty_like(x)
     target = state if new_state is None else new_state
+    increment_version(target)  # written through its pointer: a backward that saved it must notice
     if _wants_grad(x, dt, A, B, C, D, dt_bias, state):
         return _ForwardOnly.apply(lambda: _step_launch(x, dt, A, B, C, D, dt_bias, dt_softplus, state, target),
                                   x, dt, A, B, C, D, dt_bias, state)
