@@ -505,7 +505,8 @@ int lampa_causal_conv1d_state_fwd(const void* x, int64_t x_stride, int64_t n_tok
 /* One token for each of n sequences: x, y [n, D], cache [n, D, W] moved on by x into new_cache (may be the same pointer). Any D. */
 int lampa_causal_conv1d_step(const void* x, int64_t x_stride, const void* cache, void* new_cache, const float* weight,
                              const float* bias, int activation, int dtype, void* y, int64_t n, int D, int W, void* stream);
-/* Gradients of the convolution: dy, dx [n_tokens, D] contiguous, dweight_bias fp32 [D, W + 1] (a channel's taps, then its bias). */
+/* Gradients of the convolution: dy, dx [n_tokens, D] contiguous, dweight_bias fp32 [D, W + 1] (a channel's taps, then its bias). Rows
+ * behind the last boundary get zero and enter no sum, whatever they hold. */
 int64_t lampa_causal_conv1d_bwd_workspace_bytes(int64_t n_tokens, int D, int W, int dtype);
 int lampa_causal_conv1d_bwd(const void* x, int64_t x_stride, const void* dy, int64_t n_tokens, int D, int W, const float* weight,
                             const float* bias, const void* past, const int64_t* cu_seqlens, int n_seq, int64_t seq_len,

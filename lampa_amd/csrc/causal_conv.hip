@@ -227,6 +227,7 @@ __device__ __forceinline__ void cc_bwd_run(const T* __restrict__ x, int64_t x_st
           e = cc_bound(q, seq + 1);
         }
         begins[W - 1] = b;
+        const bool inside = !EDGE || seq < q.n_seq;  // rows behind the last sequence may hold anything: no share in any sum
 #pragma unroll
         for (int c = 0; c < CB_CH; ++c) {
           win[W - 1][c] = GdrElem<T>::to_float(rx[group & 1][k][c]);
@@ -236,15 +237,17 @@ __device__ __forceinline__ void cc_bwd_run(const T* __restrict__ x, int64_t x_st
             const int64_t src = t - (W - 1) + j;
             taps[j] = win[j][c];
             if (EDGE && src < b)
-              taps[j] = past && seq < q.n_seq ? GdrElem<T>::to_float(past[((int64_t)seq * D + c0 + c) * W + W + (src - b)]) : 0.0f;
+              taps[j] = past && inside ? GdrElem<T>::to_float(past[((int64_t)seq * D + c0 + c) * W + W + (src - b)]) : 0.0f;
+            if (EDGE && !inside) taps[j] = 0.0f;
             pre = __builtin_fmaf(taps[j], w[j][c], pre);
           }
           pre += bv[c];
-          float d = !EDGE || seq < q.n_seq ? GdrElem<T>::to_float(ry[group & 1][k][c]) : 0.0f;
+          float d = GdrElem<T>::to_float(ry[group & 1][k][c]);
           if (act) {
             const float s = cc_sigmoid(pre);
             d *= s * __builtin_fmaf(pre, 1.0f - s, 1.0f);
           }
+          if (EDGE && !inside) d = 0.0f;
           dpre[W - 1][c] = d;
           if (i < CB_TOKENS) {
             db[c] += d;

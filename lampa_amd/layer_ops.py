@@ -264,7 +264,8 @@ def causal_conv1d(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: 
     """``short_convolution.py:426-458``: x [B, T, D], weight [D, W] (tap W-1 on the current token), bias [D],
     residual [B, T, D]; activation ``None`` / ``'silu'`` / ``'swish'``; with ``cu_seqlens`` B must be 1 and taps never
     cross a sequence start. Returns [B, T, D] in x's dtype (fp32 arithmetic). Differentiable in x, weight, bias and residual
-    (first order; repeated calls give the same bits); the gradients take cu_seqlens to end at T.
+    (first order; repeated calls give the same bits); rows behind the last boundary of cu_seqlens have gradients of zero, and
+    nothing of them, whatever they hold, enters the others.
 
     ``initial_state`` [sequences, D, W] holds the W inputs before each sequence (a cache as ``causal_conv1d_step`` and
     ``ShortConvolution`` keep it; its oldest column is not read), and ``output_final_state`` returns (y, the W inputs up to
