@@ -508,14 +508,23 @@ class ShortConvolution(nn.Conv1d):
 
     def step(self, x: torch.Tensor, residual: Optional[torch.Tensor], cache: torch.Tensor,
              cu_seqlens: Optional[torch.LongTensor] = None):
-        """One token per sequence: the cache is rolled in place, then the convolution runs over its W columns."""
+        """One token per sequence: the cache is moved on in place, and the convolution runs over its W columns. Differentiable in x, the
+        taps and the bias, as the call on more tokens is; no gradient runs through the cache."""
         shape = x.shape
         D, W = self.hidden_size, self.kernel_size[0]
+        weight = self.weight.reshape(D, W)
         held = cache if cache.is_contiguous() and cache.dtype == x.dtype else cache.to(x.dtype).contiguous()
-        with torch.no_grad():
-            y = causal_conv1d_step(x.reshape(-1, D), held, self.weight.reshape(D, W), self.bias, self.activation)
-            if held is not cache:
-                cache.copy_(held)
+        if _wants_grad(x, weight, self.bias):
+            past = held.detach().clone()  # the backward's own: the cache moves on
+            y, last = causal_conv1d(x.reshape(-1, 1, D), weight, self.bias, activation=self.activation, initial_state=past,
+                                    output_final_state=True)
+            with torch.no_grad():
+                cache.copy_(last)
+        else:
+            with torch.no_grad():
+                y = causal_conv1d_step(x.reshape(-1, D), held, weight, self.bias, self.activation)
+                if held is not cache:
+                    cache.copy_(held)
         y = y.reshape(shape)
         if residual is not None:
             y = y + residual

@@ -4,6 +4,8 @@ import pytest
 import torch
 
 from lampa_amd import layer_ops as lo
+from oracle import state_space as os_
+from test_gpu_conv_state import HALF32, _close, _np, _want
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +37,34 @@ def test_convolution_gradients_leave_out_what_lies_behind_the_sequences(device, 
     # sums of 137 terms over the same rows, in an order that depends on the rows in all
     bound = 2 * used * 2.0 ** -24 * (dy[:, :used].abs().float().sum(1) * 1.1).max().item() * max(1.0, x[:, :used].abs().max().item())
     assert (dw - dw2).abs().max().item() <= bound and (db - db2).abs().max().item() <= bound
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("packed", [False, True])
+def test_short_convolution_trains_through_a_single_token(device, dtype, packed):
+    """One token with a cache, or with the cache asked for, has the gradients that more tokens have; the cache moves on as without
+    gradients, and moving it on again does not disturb the backward. Tolerances as in test_gpu_conv_state.test_gradients."""
+    D, W, n = 24, 4, 3
+    gen = torch.Generator().manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=gen).to(dtype).to(device)  # noqa: E731
+    conv = lo.ShortConvolution(D, W, bias=True).to(device)
+    shape, cu = ((1, n, D), torch.arange(n + 1, device=device)) if packed else ((n, 1, D), None)
+    for given in (True, False):
+        x, dy, cache = r(*shape), r(*shape), r(n, D, W) if given else None
+        start = torch.zeros(n, D, W, device=device, dtype=dtype) if cache is None else cache.clone()
+        with torch.no_grad():
+            want_y, want_cache = conv(x, cache=start.clone(), cu_seqlens=cu)
+        leaf = x.clone().requires_grad_(True)
+        y, cache = conv(leaf, cache=cache, output_final_state=True, cu_seqlens=cu)
+        assert torch.equal(y, want_y) and torch.equal(cache, want_cache)
+        with torch.no_grad():
+            conv(x, cache=cache, cu_seqlens=cu)
+        got = torch.autograd.grad(y, [leaf, conv.weight, conv.bias], dy)
+        rows = lambda t: _np(t).reshape(-1, D)  # noqa: E731
+        w, b = _np(conv.weight).reshape(D, W), _np(conv.bias)
+        want = os_.conv_grads(rows(x), w, b, "silu", rows(dy), [1] * n, _np(start))
+        _, _, pre = _want(x.reshape(1, n, D), conv.weight.reshape(D, W), conv.bias, start, "silu", [1] * n)
+        slack = abs(rows(dy)) * (1 + pre.reshape(-1, D)) * 20
+        mag = os_.conv_grads(abs(rows(x)), abs(w), None, None, slack, [1] * n, abs(_np(start)))
+        for name, a, v, m, terms in zip(("x", "weight", "bias"), got, want, mag, (W, n, n)):
+            _close(name, a.reshape(v.shape), v, (2 + terms) * HALF32 * m + 1e-30)
