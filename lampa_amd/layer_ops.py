@@ -509,11 +509,13 @@ class ShortConvolution(nn.Conv1d):
     def step(self, x: torch.Tensor, residual: Optional[torch.Tensor], cache: torch.Tensor,
              cu_seqlens: Optional[torch.LongTensor] = None):
         """One token per sequence: the cache is moved on in place, and the convolution runs over its W columns. Differentiable in x, the
-        taps and the bias, as the call on more tokens is; no gradient runs through the cache."""
+        taps and the bias, as the call on more tokens is; no gradient runs through the cache. Computed and returned in the
+        cache's type: a cache wider than x keeps its bits."""
         shape = x.shape
+        x = x.to(cache.dtype)
         D, W = self.hidden_size, self.kernel_size[0]
         weight = self.weight.reshape(D, W)
-        held = cache if cache.is_contiguous() and cache.dtype == x.dtype else cache.to(x.dtype).contiguous()
+        held = cache.contiguous()
         if _wants_grad(x, weight, self.bias):
             past = held.detach().clone()  # the backward's own: the cache moves on
             y, last = causal_conv1d(x.reshape(-1, 1, D), weight, self.bias, activation=self.activation, initial_state=past,

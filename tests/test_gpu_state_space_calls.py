@@ -68,3 +68,24 @@ def test_short_convolution_trains_through_a_single_token(device, dtype, packed):
         mag = os_.conv_grads(abs(rows(x)), abs(w), None, None, slack, [1] * n, abs(_np(start)))
         for name, a, v, m, terms in zip(("x", "weight", "bias"), got, want, mag, (W, n, n)):
             _close(name, a.reshape(v.shape), v, (2 + terms) * HALF32 * m + 1e-30)
+
+
+@pytest.mark.parametrize("x_type,cache_type", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32), (torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_cache_of_another_type_sets_the_type_of_the_step(device, x_type, cache_type, grad):
+    """The step's window, sums and output are of the cache's type, as the convolution of that window is; what it holds is kept to
+    the bit, also where the cache is no contiguous tensor."""
+    D, W, n = 16, 4, 3
+    gen = torch.Generator().manual_seed(8)
+    conv = lo.ShortConvolution(D, W, bias=True).to(device).requires_grad_(grad)
+    start = torch.randn(n, D, W, generator=gen).to(cache_type).to(device)
+    cache = start.transpose(0, 1).contiguous().transpose(0, 1)
+    assert not cache.is_contiguous()
+    window = start
+    for _ in range(W + 1):
+        x = torch.randn(n, 1, D, generator=gen).to(x_type).to(device)
+        y, back = conv(x, cache=cache)
+        assert back is cache
+        window = torch.cat([window[..., 1:], x.transpose(1, 2).to(cache_type)], -1)
+        want = lo.causal_conv1d(window.transpose(1, 2), conv.weight.reshape(D, W), conv.bias, activation="silu")[:, -1:]
+        assert y.dtype == cache_type and torch.equal(y, want) and torch.equal(cache, window)
