@@ -66,6 +66,19 @@ __device__ __forceinline__ float sc_larger(float big, float v) {
 }
 __device__ __forceinline__ float sc_inverse(float power_of_two) { return __uint_as_float((254u << 23) - __float_as_uint(power_of_two)); }
 
+// The scale of a lane's column (row or column i of an operand whose values lie in the lanes i, 16 + i, 32 + i and 48 + i), from the
+// largest value of each lane, and its inverse for the rows 4 g + r of a product that has the operand on the left. A scale of its own
+// for each: a column of small values loses no bits to a large one beside it.
+template <typename T>
+__device__ __forceinline__ float sc_column_scale(float largest, int lane, f32x4& back) {
+  largest = fmaxf(largest, __shfl_xor(largest, 16));
+  largest = fmaxf(largest, __shfl_xor(largest, 32));
+  const float s = sc_scale_for<T>(largest), inverse = sc_inverse(s);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) back[r] = __shfl(inverse, 4 * (lane >> 4) + r);
+  return s;
+}
+
 __device__ __forceinline__ float sc_wave_max(float v) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) v = fmaxf(v, __shfl_xor(v, off));
@@ -210,19 +223,42 @@ __device__ __forceinline__ void sc_row_weights(const float* w, int kk, int lane,
 #pragma unroll
   for (int e = 0; e < 4; ++e) { out[e] = a[e]; out[4 + e] = b[e]; }
 }
-// A weighted operand in parts.
+// An operand over a chunk's 64 rows, weighted row by row, in parts. Returns what a product with it on the right is to be multiplied with:
+// fp16's weighted values are scaled so that the largest of a lane's column (the product's column) comes to between 2^14 and 2^15. The
+// scale is made from the values, not from the weights alone: x or dy of 1e-4 would leave remainders below fp16's smallest step (states
+// were off by 3e-4, now by 1e-7 as with any other size of x).
 template <typename T, int PARTS>
-__device__ __forceinline__ void sc_weighted(const sc_x8<T>& x, const float (&w)[8], sc_x8<T> (&out)[PARTS]) {
+__device__ __forceinline__ float sc_weighted(const sc_x8<T> (&x)[2], const float (&w)[2][8], sc_x8<T> (&out)[2][PARTS]) {
+  constexpr bool F16 = __is_same(T, _Float16);
+  float s = 1.0f;
+  if constexpr (F16) {
+    float big = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    typename OpVec<T>::x2 part[PARTS];
-    sc_split<T, PARTS>((float)x[e] * w[e], (float)x[e + 1] * w[e + 1], part);
+    for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-    for (int k = 0; k < PARTS; ++k) {
-      out[k][e] = part[k][0];
-      out[k][e + 1] = part[k][1];
-    }
+      for (int e = 0; e < 8; ++e) big = sc_larger(big, (float)x[kk][e] * w[kk][e]);
+    big = fmaxf(big, __shfl_xor(big, 16));
+    big = fmaxf(big, __shfl_xor(big, 32));
+    s = sc_scale_for<T>(big);
   }
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      float a = (float)x[kk][e] * w[kk][e], b = (float)x[kk][e + 1] * w[kk][e + 1];
+      if constexpr (F16) {
+        a *= s;
+        b *= s;
+      }
+      typename OpVec<T>::x2 part[PARTS];
+      sc_split<T, PARTS>(a, b, part);
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) {
+        out[kk][k][e] = part[k][0];
+        out[kk][k][e + 1] = part[k][1];
+      }
+    }
+  return sc_inverse(s);
 }
 // Two accumulator tiles (32 rows) as an operand in parts.
 template <typename T, int PARTS>
@@ -274,24 +310,11 @@ __device__ __forceinline__ void sc_add_products(const T* tile, int stride, int l
 
 // S <- end S + (tile)^T * (v, its rows weighted), the product of a wave's 16 columns with all rows of the state.
 template <typename T, int NT, int PARTS>
-__device__ __forceinline__ void sc_update(const T* tile, int stride, int lane, const sc_x8<T> (&v)[2], float (&wt)[2][8], float end,
+__device__ __forceinline__ void sc_update(const T* tile, int stride, int lane, const sc_x8<T> (&v)[2], const float (&wt)[2][8], float end,
                                           f32x4 (&S)[NT]) {
   sc_x8<T> vw[2][PARTS];
-  if constexpr (__is_same(T, _Float16)) {  // the largest weight becomes 1 or a little less: v is in range by itself
-    float m = 0.0f;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(wt[kk][e]));
-    m = fmaxf(m, __shfl_xor(m, 16));
-    m = fmaxf(m, __shfl_xor(m, 32));
-    const float s = sc_scale_for<T>(m) * 0x1p-15f, back = sc_inverse(s);
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) wt[kk][e] *= s;
-      sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
-    }
+  const float back = sc_weighted<T, PARTS>(v, wt, vw);
+  if constexpr (__is_same(T, _Float16)) {
     f32x4 d[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) d[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -299,8 +322,6 @@ __device__ __forceinline__ void sc_update(const T* tile, int stride, int lane, c
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) S[nt] = S[nt] * end + d[nt] * back;
   } else {
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) S[nt] *= end;
     sc_add_products<T, NT, PARTS>(tile, stride, lane, vw, S);

@@ -191,15 +191,15 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
     {
       x8 vy[2];
       sc_columns<T>(ty, VS, 16 * wave, lane, vy);
-      float sc = 1.0f, sback = 1.0f;
+      float sc = 1.0f;
+      f32x4 sback;
       if constexpr (F16) {
         float big = 0.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) big = sc_larger(big, R[nt][r]);
-        sc = sc_scale_for<T>(sc_wave_max(big));
-        sback = sc_inverse(sc);
+        sc = sc_column_scale<T>(big, lane, sback);
       }
       f32x4 acc[4];
 #pragma unroll
@@ -219,7 +219,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
       for (int st = 0; st < 4; ++st) {
         sc_fence();
         const int s = 16 * st + i;
-        acc[st] *= F16 ? dec.left[s] * sback : dec.left[s];
+        if constexpr (F16) acc[st] *= sback * dec.left[s];
+        else acc[st] *= dec.left[s];
         const int at = s * VS + op_perm32_col(16 * wave + 4 * g);
         const x4 xv = *reinterpret_cast<const x4*>(tx + at), dyv = *reinterpret_cast<const x4*>(ty + at);
         float dot = 0.0f;
@@ -261,7 +262,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
       for (int j = 0; j < NW; ++j) {
         sc_fence();
-        float s1 = 1.0f, b1 = 1.0f, s2 = 1.0f, b2 = 1.0f;
+        float s1 = 1.0f, s2 = 1.0f;
+        f32x4 b1, b2;
         if constexpr (F16) {
           float big1 = 0.0f, big2 = 0.0f;
 #pragma unroll
@@ -271,10 +273,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
               big1 = sc_larger(big1, RT[q][j][r]);
               big2 = sc_larger(big2, S[q][r]);
             }
-          s1 = sc_scale_for<T>(sc_wave_max(big1));
-          b1 = sc_inverse(s1);
-          s2 = sc_scale_for<T>(sc_wave_max(big2));
-          b2 = sc_inverse(s2);
+          s1 = sc_column_scale<T>(big1, lane, b1);
+          s2 = sc_column_scale<T>(big2, lane, b2);
         }
         f32x4 db[4], dc[4];
 #pragma unroll
@@ -314,7 +314,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
         for (int st = 0; st < 4; ++st) {
           sc_fence();
           const int s = 16 * st + i;
-          db[st] *= dec.left[s] * dec.delta[s] * b1;
+          db[st] *= dec.left[s] * dec.delta[s];
+          if constexpr (F16) db[st] *= b1;
           if constexpr (F16) {
             f32x4 near = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -326,7 +327,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
             for (int kk = 0; kk < 2; ++kk)
               if (2 * kk + 1 >= st) db[st] = mfma16(vc[kk], *reinterpret_cast<const x8*>(m2 + s * MS + 32 * kk + 8 * g), db[st]);
           }
-          dc[st] *= dec.grow[s] * b2;
+          dc[st] *= dec.grow[s];
+          if constexpr (F16) dc[st] *= b2;
           const x4 cv = *reinterpret_cast<const x4*>(tc + s * KS + op_perm32_col(c0));
           float read = 0.0f;
 #pragma unroll
@@ -377,28 +379,12 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
     if (lane == 0) dot_part[wave] = dot;
 
     sc_fence();
-    // R in front of the chunk, both ways round. (fp16: the decayed operands' weights are at most about 1; where the chunk's
-    // first token decays strongly they are all small, so they are scaled by the largest, which is the first.)
+    // R in front of the chunk, both ways round.
     {
-      float wt[2][8], back = 1.0f;
+      float wt[2][8];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) sc_row_weights(dec.grow, kk, lane, wt[kk]);
-      if constexpr (F16) {
-        float m = 0.0f;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) m = fmaxf(m, wt[kk][e]);
-        m = fmaxf(m, __shfl_xor(m, 16));
-        m = fmaxf(m, __shfl_xor(m, 32));
-        const float s = sc_scale_for<T>(m) * 0x1p-15f;
-        back = sc_inverse(s);
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) wt[kk][e] *= s;
-      }
-      auto add = [&](f32x4& acc, const x8 (&left)[2], const x8 (&right)[2][PARTS]) {
+      auto add = [&](f32x4& acc, const x8 (&left)[2], const x8 (&right)[2][PARTS], float back) {
         if constexpr (F16) {
           f32x4 d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -412,24 +398,22 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
       };
       x8 v[2], vw[2][PARTS], left[2];
       sc_columns<T>(ty, VS, 16 * wave, lane, v);
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
+      float back = sc_weighted<T, PARTS>(v, wt, vw);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         sc_columns<T>(tc, KS, 16 * nt, lane, left);
-        add(R[nt], left, vw);
+        add(R[nt], left, vw, back);
         sc_fence();
       }
       if (has_n) {
 #pragma unroll
         for (int j = 0; j < NW; ++j) {
           sc_columns<T>(tc, KS, 16 * (nt0 + j), lane, v);
-#pragma unroll
-          for (int kk = 0; kk < 2; ++kk) sc_weighted<T, PARTS>(v[kk], wt[kk], vw[kk]);
+          back = sc_weighted<T, PARTS>(v, wt, vw);
 #pragma unroll
           for (int pt = 0; pt < 4; ++pt) {
             sc_columns<T>(ty, VS, 16 * pt, lane, left);
-            add(RT[pt][j], left, vw);
+            add(RT[pt][j], left, vw, back);
             sc_fence();
           }
           sc_fence();

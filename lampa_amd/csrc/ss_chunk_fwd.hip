@@ -102,7 +102,7 @@ __device__ __forceinline__ void sc_map(const lampa_ss_args& a, const SsGrad& w, 
 
 // Waves a SIMD that fit without spilling (element-by-element loads and fp16's scales take more registers).
 template <typename T, int NP, bool VEC>
-constexpr int sc_map_waves() { return !VEC ? 2 : NP <= 64 ? (__is_same(T, __bf16) ? 4 : 3) : (__is_same(T, __bf16) ? 3 : 2); }
+constexpr int sc_map_waves() { return !VEC ? (NP <= 64 && __is_same(T, __bf16) ? 3 : 2) : NP <= 32 ? 5 : NP <= 64 ? 4 : (__is_same(T, __bf16) ? 3 : 2); }
 
 // PARTS: all of them where the states go to the caller or into gradients, two where they only go into outputs.
 template <typename T, int NP, bool VEC, int PARTS>
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
 
     // y^T of this wave's 16 columns: lane = token 16 tt + i, registers = columns 4 g .. + 3
     f32x4 y[4];
-    float sback = 1.0f;
+    f32x4 sback;
     {
       float s = 1.0f;
       if constexpr (__is_same(T, _Float16)) {
@@ -244,8 +244,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) big = sc_larger(big, S[nt][r]);
-        s = sc_scale_for<T>(sc_wave_max(big));
-        sback = sc_inverse(s);
+        s = sc_column_scale<T>(big, lane, sback);
       }
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) y[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -266,7 +265,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_out_kernel(lampa_ss_args a) {
     for (int tt = 0; tt < 4; ++tt) {
       const int t = 16 * tt + i;
       const float back = __is_same(T, _Float16) ? mback[t] : 1.0f;
-      y[tt] *= __is_same(T, _Float16) ? dec.grow[t] * sback * sc_inverse(back) : dec.grow[t];
+      if constexpr (__is_same(T, _Float16)) y[tt] *= sback * (dec.grow[t] * sc_inverse(back));
+      else y[tt] *= dec.grow[t];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
         if (2 * kk <= tt) y[tt] = mfma16(v[kk], *reinterpret_cast<const sc_x8<T>*>(tm + t * MS + 32 * kk + 8 * g), y[tt]);

@@ -4,8 +4,10 @@ import pytest
 import torch
 
 from lampa_amd import layer_ops as lo
+from lampa_amd import state_space as ss
 from oracle import state_space as os_
 from test_gpu_conv_state import HALF32, _close, _np, _want
+from test_gpu_state_space import _bound, _call, _check, _inputs, _oracle, _to
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +91,45 @@ def test_a_cache_of_another_type_sets_the_type_of_the_step(device, x_type, cache
         window = torch.cat([window[..., 1:], x.transpose(1, 2).to(cache_type)], -1)
         want = lo.causal_conv1d(window.transpose(1, 2), conv.weight.reshape(D, W), conv.bias, activation="silu")[:, -1:]
         assert y.dtype == cache_type and torch.equal(y, want) and torch.equal(cache, window)
+
+
+NAMES = ["x", "dt", "A", "B", "C", "D", "dt_bias", "h0"]
+
+
+def _scan_against_float64(device, i, dy, dht, dtype, T, P, N, H, G):
+    """Outputs and gradients of one sequence within the bounds of test_gpu_state_space."""
+    (y, last, g), (ym, lastm, gm) = _oracle(i, [T], dy=dy, dht=dht)
+    d = _to(i, device, grad=True)
+    got, ht = _call(d)
+    _check("y", got, y, _bound(dtype, T, y, ym, N), dtype)
+    _check("last", ht, last, _bound(dtype, T, last, lastm, 0, False))
+    grads = torch.autograd.grad([got, ht], [d[k] for k in NAMES], [dy.to(device), dht.to(device)])
+    for k, a in zip(NAMES, grads):
+        wide = {"x": N, "B": P * H // G, "C": P * H // G, "h0": 0, "D": T * P}.get(k, N * P + T)
+        _check(k, a, g[k], _bound(dtype, T, g[k], gm[k], wide, k in ("x", "B", "C")), d[k].dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e-2, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("seg", [None, 64])
+def test_small_values_keep_the_bits_of_states_and_adjoints(device, dtype, size, seg, monkeypatch):
+    """x or C, which the states and adjoints are made of beside dy, small all over or in every other column: two operands of 11
+    bits hold a state as they do where x is about one."""
+    if seg:
+        monkeypatch.setattr(ss, "_segment_tokens", lambda *a: seg)
+    T, H, P, G, N = 200, 2, 32, 1, 40
+    gen = torch.Generator().manual_seed(3)
+    for small, alternate in (("x", False), ("dy", False), ("C", False), ("x", True), ("C", True)):
+        i = _inputs((1, T), H, P, G, N, dtype, 80, 1)
+        dy, dht = torch.randn(1, T, H, P, generator=gen).to(dtype), torch.randn(1, H, N, P, generator=gen)
+        step = 2 if alternate else 1
+        if small == "dy":
+            dy, dht = dy * size, dht * size
+        else:
+            i[small] = i[small].clone()
+            i[small][..., ::step] = (i[small].float() * size).to(dtype)[..., ::step]
+            if small == "x":
+                i["h0"][..., ::step] *= size
+            else:
+                dht[..., ::step, :] *= size
+        _scan_against_float64(device, i, dy, dht, dtype, T, P, N, H, G)
