@@ -12,6 +12,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _capi
@@ -60,6 +61,10 @@ def _same_device(what, *tensors) -> int:
 
 
 def _wants_grad(*tensors) -> bool:
+    """Whether a call has to go through its autograd function: a gradient can be asked for, or forward-mode gradients are being
+    computed (the function raises where one of its inputs has a tangent; past it the tangent would be dropped)."""
+    if _forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -363,7 +368,7 @@ def causal_conv1d_step(x: torch.Tensor, cache: torch.Tensor, weight: torch.Tenso
     target = cache if new_cache is None else new_cache
     increment_version(target)  # written through its pointer: a backward that saved it must notice
     if _wants_grad(x, weight, bias):
-        return _ForwardOnly.apply(lambda: _conv_step_launch(x, cache, weight, bias, activation, target), x, weight, bias)
+        return _ForwardOnly.apply(lambda: _conv_step_launch(x, cache, weight, bias, activation, target), x, weight, bias, cache)
     return _conv_step_launch(x, cache, weight, bias, activation, target)
 
 

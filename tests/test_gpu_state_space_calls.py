@@ -2,6 +2,7 @@
 the last sequence, gradients through a single token, forward-mode gradients, slices of long tensors, parameters without gradients."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from lampa_amd import layer_ops as lo
 from lampa_amd import state_space as ss
@@ -133,3 +134,36 @@ def test_small_values_keep_the_bits_of_states_and_adjoints(device, dtype, size, 
             else:
                 dht[..., ::step, :] *= size
         _scan_against_float64(device, i, dy, dht, dtype, T, P, N, H, G)
+
+
+def test_forward_mode_gradients_are_refused(device):
+    """No operator has forward-mode gradients: a tangent on any input raises instead of coming back without one, with gradients
+    enabled or not; in the same context inputs without tangents are taken as ever."""
+    gen = torch.Generator().manual_seed(9)
+    r = lambda *s: torch.randn(*s, generator=gen).to(device)  # noqa: E731
+    conv = dict(x=r(2, 5, 16), weight=r(16, 4), bias=r(16))
+    step = dict(x=r(2, 16), cache=r(2, 16, 4), weight=r(16, 4), bias=r(16))
+    norm = dict(x=r(2, 5, 16), residual=r(2, 5, 16), weight=r(16), post_weight=r(16), gate=r(2, 5, 16), residual_scale=r(16))
+    scan = dict(x=r(2, 5, 2, 8), dt=r(2, 5, 2), A=-r(2).abs(), B=r(2, 5, 1, 8), C=r(2, 5, 1, 8), D=r(2), dt_bias=r(2),
+                initial_state=r(2, 2, 8, 8))
+    token = {k: t[:, 0] if k in ("x", "dt", "B", "C") else t for k, t in scan.items() if k != "initial_state"}
+    short = lo.ShortConvolution(16, 4, bias=True).to(device).requires_grad_(False)
+    calls = [
+        (lo.causal_conv1d, conv), (lo.causal_conv1d, dict(conv, residual=r(2, 5, 16))),
+        (lambda **k: lo.causal_conv1d(**k, output_final_state=True), dict(conv, initial_state=r(2, 16, 4))),
+        (lambda **k: lo.causal_conv1d_step(**k, new_cache=torch.empty(2, 16, 4, device=device)), step),
+        (lo.residual_norm, norm), (lambda **k: ss.state_space_scan(**k, output_final_state=True), scan),
+        (lambda **k: ss.state_space_step(**k, new_state=torch.empty(2, 2, 8, 8, device=device)), dict(token, state=r(2, 2, 8, 8))),
+        (lambda x: short(x, cache=torch.zeros(2, 16, 4, device=device)), dict(x=r(2, 1, 16))),
+    ]
+    for call, inputs in calls:
+        want = call(**inputs)
+        for enabled in (True, False):
+            with forward_ad.dual_level(), torch.set_grad_enabled(enabled):
+                got = call(**inputs)
+                for a, b in zip(*((t if isinstance(t, tuple) else (t,)) for t in (got, want))):
+                    assert torch.equal(a, b)
+                for name in inputs:
+                    dual = forward_ad.make_dual(inputs[name], torch.ones_like(inputs[name]))
+                    with pytest.raises(RuntimeError, match="jvp"):  # (NotImplementedError is one)
+                        call(**dict(inputs, **{name: dual}))
