@@ -367,7 +367,7 @@ def causal_conv1d_step(x: torch.Tensor, cache: torch.Tensor, weight: torch.Tenso
         return torch.empty_like(x)
     target = cache if new_cache is None else new_cache
     increment_version(target)  # written through its pointer: a backward that saved it must notice
-    if _wants_grad(x, weight, bias):
+    if _wants_grad(x, weight, bias, cache):
         return _ForwardOnly.apply(lambda: _conv_step_launch(x, cache, weight, bias, activation, target), x, weight, bias, cache)
     return _conv_step_launch(x, cache, weight, bias, activation, target)
 

@@ -167,3 +167,11 @@ def test_forward_mode_gradients_are_refused(device):
                     dual = forward_ad.make_dual(inputs[name], torch.ones_like(inputs[name]))
                     with pytest.raises(RuntimeError, match="jvp"):  # (NotImplementedError is one)
                         call(**dict(inputs, **{name: dual}))
+
+
+def test_a_cache_with_a_gradient_is_refused_in_the_backward(device):
+    """The token steps have no gradients, of what they are handed in their caches neither."""
+    cache = torch.randn(2, 16, 4, device=device, requires_grad=True)
+    y = lo.causal_conv1d_step(torch.randn(2, 16, device=device), cache * 1.0, torch.randn(16, 4, device=device))
+    with pytest.raises(NotImplementedError):
+        y.sum().backward()
