@@ -23,6 +23,7 @@ from .gated_delta import _direct
 from .layer_ops import _DTYPES, _ForwardOnly, _on_device, _plain_f32, _same_device, _sequences, _tokens, _wants_grad
 
 MAX_STATE = 128  # N of state_space_scan; state_space_step takes any
+MAX_STRIDE = 1 << 24  # elements between tokens, as lampa_ss_scan_fwd takes them
 
 # lampa_ss_args: 13 pointers, 8 int64, 8 int32, 11 pointers, one int64
 _ARGS = struct.Struct("=13Q8q8i11Qq")
@@ -44,11 +45,12 @@ def _segment_tokens(longest: int, total: int, heads: int, N: int, dtype, grad: b
 
 
 def _vectors(t, inner, width):
-    """``_tokens`` of a 16-bit tensor whose rows of ``width`` the chunk kernels can read in 16-byte pieces; a copy where only its
-    place in memory is in the way (60 000 tokens x 8 heads of 64 one element off: 303 us read as they lie, 111 us aligned, a
-    copy takes 25)."""
+    """``_tokens`` as the kernels read them. A copy where tokens lie 2^24 elements apart or more (a token of each of several
+    long sequences: the kernels form offsets within 64 rows in 32 bits), and where a 16-bit tensor's rows of ``width`` could be
+    read in 16-byte pieces but for their place in memory (60 000 tokens x 8 heads of 64 one element off: 303 us read as they
+    lie, 111 us aligned, a copy takes 25)."""
     t, step = _tokens(t, inner)
-    if t.element_size() == 2 and width % 8 == 0 and (step % 8 or t.data_ptr() % 16):
+    if step >= MAX_STRIDE or (t.element_size() == 2 and width % 8 == 0 and (step % 8 or t.data_ptr() % 16)):
         return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t), inner
     return t, step
 

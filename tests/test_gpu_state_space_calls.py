@@ -175,3 +175,32 @@ def test_a_cache_with_a_gradient_is_refused_in_the_backward(device):
     y = lo.causal_conv1d_step(torch.randn(2, 16, device=device), cache * 1.0, torch.randn(16, 4, device=device))
     with pytest.raises(NotImplementedError):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1, 2])
+def test_tokens_out_of_long_sequences(device, dtype, T):
+    """The next token of each of several sequences, sliced out of tensors whose sequences lie more than 2^24 elements apart: the
+    bits of a contiguous copy, gradients too."""
+    long = dict(x=torch.zeros(3, 17000, 2, 512, device=device, dtype=dtype), B=torch.zeros(3, 17000, 16, 64, device=device, dtype=dtype),
+                C=torch.zeros(3, 17000, 16, 64, device=device, dtype=dtype), dt=torch.zeros(3, 17000, 1000, device=device, dtype=dtype))
+    gen = torch.Generator().manual_seed(10)
+    sizes = dict(x=(3, T, 2, 512), B=(3, T, 1, 64), C=(3, T, 1, 64), dt=(3, T, 2))
+    ends = dict(x=slice(None), B=slice(5, 6), C=slice(0, 1), dt=slice(7, 9))
+    parts = {}
+    for k, t in long.items():
+        assert t.stride(0) > 2 ** 24
+        parts[k] = t[:, 9000:9000 + T, ends[k]]
+        parts[k].copy_(torch.randn(*sizes[k], generator=gen))
+    shared = dict(A=-torch.rand(2, generator=gen).to(device), D=None, dt_bias=None, h0=torch.randn(3, 2, 64, 512, generator=gen).to(device))
+    dy = torch.randn(3, T, 2, 512, generator=gen).to(dtype).to(device)
+    out = []
+    for copy in (False, True):
+        d = {k: (t.contiguous().clone() if copy else t).detach().requires_grad_(True) for k, t in parts.items()}
+        y, ht = _call({**d, **shared})
+        with torch.no_grad():
+            plain = _call({**d, **shared})
+        assert torch.equal(y, plain[0]) and torch.equal(ht, plain[1])
+        out.append([y, ht, *torch.autograd.grad([y, ht], list(d.values()), [dy, ht.detach()])])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
