@@ -122,10 +122,11 @@ def _scan_backward(x, dt, A, B, C, D, bias, softplus, h0, cu, ht, kept, dy, dht)
 
 class _StateSpaceScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, dt, A, B, C, D, bias, h0, softplus, want_final, cu):
+    def forward(ctx, x, dt, A, B, C, D, bias, h0, softplus, want_final, cu, keep):
         ctx.set_materialize_grads(False)
-        y, ht, kept = _scan_launch(x, dt, A, B, C, D, bias, softplus, h0, want_final, cu, keep=True)
-        ctx.save_for_backward(x, dt, A, B, C, D, bias, h0, cu, ht, kept[0], kept[1])
+        y, ht, kept = _scan_launch(x, dt, A, B, C, D, bias, softplus, h0, want_final, cu, keep=keep)
+        if keep:
+            ctx.save_for_backward(x, dt, A, B, C, D, bias, h0, cu, ht, kept[0], kept[1])
         ctx.softplus, ctx.sizes = softplus, kept[2:]
         return y, ht if want_final else None
 
@@ -136,7 +137,7 @@ class _StateSpaceScan(torch.autograd.Function):
         dx, ddt, dA, dB, dC, dD, dbias, dh0 = _scan_backward(x, dt, A, B, C, D, bias, ctx.softplus, h0, cu, ht,
                                                              (states, decay, *ctx.sizes), dy, dht)
         as_type = lambda g, t: None if t is None else g.to(t.dtype)  # noqa: E731
-        return (dx, ddt, as_type(dA, A), dB, dC, as_type(dD, D), as_type(dbias, bias), as_type(dh0, h0), None, None, None)
+        return (dx, ddt, as_type(dA, A), dB, dC, as_type(dD, D), as_type(dbias, bias), as_type(dh0, h0), None, None, None, None)
 
 
 def _check_operands(what, x, dt, A, B, C, D, dt_bias, tokens):
@@ -203,7 +204,9 @@ def state_space_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torc
     if _direct(x, dt, A, B, C, D, dt_bias, initial_state):
         y, ht, _ = _scan_launch(x, dt, A, B, C, D, dt_bias, dt_softplus, initial_state, output_final_state, cu)
         return y, ht
-    return _StateSpaceScan.apply(x, dt, A, B, C, D, dt_bias, initial_state, bool(dt_softplus), bool(output_final_state), cu)
+    # a call that goes through the function without gradients (parameters under no_grad) is launched as the direct one
+    keep = _wants_grad(x, dt, A, B, C, D, dt_bias, initial_state)
+    return _StateSpaceScan.apply(x, dt, A, B, C, D, dt_bias, initial_state, bool(dt_softplus), bool(output_final_state), cu, keep)
 
 
 def _rows(t, inner):

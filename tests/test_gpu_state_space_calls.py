@@ -204,3 +204,25 @@ def test_tokens_out_of_long_sequences(device, dtype, T):
         out.append([y, ht, *torch.autograd.grad([y, ht], list(d.values()), [dy, ht.detach()])])
     for a, b in zip(*out):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_parameters_without_gradients_are_launched_as_plain_tensors(device, dtype, monkeypatch):
+    """Under no_grad a layer's parameters make no training call: the segments and the bits of the call on plain tensors, and
+    nothing kept of it."""
+    asked = []
+    rule = ss._segment_tokens
+    monkeypatch.setattr(ss, "_segment_tokens", lambda *a: asked.append(a[-1]) or rule(*a))
+    T, H, P, N = 40000, 8, 64, 64
+    d = _to(_inputs((1, T), H, P, 1, N, dtype, 90, 1), device)
+    held = {k: torch.nn.Parameter(t) if k in ("A", "D", "dt_bias", "h0") else t for k, t in d.items()}
+    assert rule(T, T, H, N, torch.bfloat16, True) != rule(T, T, H, N, torch.bfloat16, False)
+    with torch.no_grad():
+        want = _call(d)
+        before = torch.cuda.memory_allocated()
+        got = _call(held)
+        kept = torch.cuda.memory_allocated() - before - sum(t.numel() * t.element_size() for t in got)
+    assert asked == [False, False] and all(torch.equal(a, b) for a, b in zip(got, want))
+    assert kept < 2 ** 16  # the outputs alone, as the allocator rounds them up
+    _call(held)
+    assert asked[2:] == [True]
