@@ -460,8 +460,8 @@ int lampa_gdr_traffic_probe_walk(const void* q, const void* k, const void* v, co
  * sequences of seq_len tokens. seg_tokens: length of the segments that run in parallel, a multiple of 64. N <= 128.
  *
  * slot_states [lampa_ss_slots, H, N, P] fp32 and slot_decay [lampa_ss_slots, H] fp32 are scratch of the forward; where a
- * sequence may have more than one segment they must not be NULL. For gradients keep both (slot_states then holds the state at
- * the start of every segment) for lampa_ss_scan_bwd. */
+ * sequence may have more than one segment they must not be NULL. For gradients set for_grad in the forward and keep both
+ * (slot_states then holds the state at the start of every segment) for lampa_ss_scan_bwd, which reads neither y nor ht. */
 typedef struct {
   const void *x, *dt, *B, *C;
   const float *A, *D, *dt_bias, *h0;
@@ -472,6 +472,7 @@ typedef struct {
   int64_t n_tokens, seq_len, seg_tokens;
   int64_t x_stride, dt_stride, B_stride, C_stride, y_stride;
   int32_t n_seq, H, P, G, N, dtype, dt_dtype, softplus;
+  int32_t for_grad, reserved;  /* for_grad: not 0 where lampa_ss_scan_bwd follows the forward (slot_states whole to fp32) */
   /* gradients only: dy [tokens, H, P] contiguous and dht (or NULL) in; dx [tokens, H, P], dB, dC [tokens, G, N] in `dtype`,
    * ddt [tokens, H] in dt_dtype, dA, dD, ddt_bias fp32 [H], dh0 fp32 (or NULL) out, all contiguous */
   const void* dy;

@@ -325,7 +325,7 @@ static int sc_maps_launch(const lampa_ss_args& a, const SsGrad* grad, hipStream_
   LAMPA_PROF(s, "start");
 #define SC_GO(NP)                                                                                           \
   if (grad) hipLaunchKernelGGL((sc_prepare_kernel<T, NP, VEC>), grid, dim3(SC_BLOCK), 0, s, a, *grad);      \
-  else if (a.ht) hipLaunchKernelGGL((sc_map_kernel<T, NP, VEC, ScParts<T>::n>), grid, dim3(SC_BLOCK), 0, s, a, SsGrad{}); \
+  else if (a.ht || a.for_grad) hipLaunchKernelGGL((sc_map_kernel<T, NP, VEC, ScParts<T>::n>), grid, dim3(SC_BLOCK), 0, s, a, SsGrad{}); \
   else hipLaunchKernelGGL((sc_map_kernel<T, NP, VEC, 2>), grid, dim3(SC_BLOCK), 0, s, a, SsGrad{})
   if (a.N <= 32) { SC_GO(32); } else if (a.N <= 64) { SC_GO(64); } else { SC_GO(128); }
 #undef SC_GO

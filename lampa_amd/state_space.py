@@ -12,6 +12,7 @@ reference imports. Names, state layout ([sequences, H, N, P], float32) and retur
 ``chunk_gated_delta_rule``. GPU tensors only; there is no CPU path.
 """
 import struct
+import weakref
 from typing import Optional
 
 import torch
@@ -25,8 +26,8 @@ from .layer_ops import _DTYPES, _ForwardOnly, _on_device, _plain_f32, _same_devi
 MAX_STATE = 128  # N of state_space_scan; state_space_step takes any
 MAX_STRIDE = 1 << 24  # elements between tokens, as lampa_ss_scan_fwd takes them
 
-# lampa_ss_args: 13 pointers, 8 int64, 8 int32, 11 pointers, one int64
-_ARGS = struct.Struct("=13Q8q8i11Qq")
+# lampa_ss_args: 13 pointers, 8 int64, 10 int32, 11 pointers, one int64
+_ARGS = struct.Struct("=13Q8q10i11Qq")
 
 
 def _segment_tokens(longest: int, total: int, heads: int, N: int, dtype, grad: bool) -> int:
@@ -55,7 +56,7 @@ def _vectors(t, inner, width):
     return t, step
 
 
-def _pack(x, dt, A, B, C, D, bias, h0, y, ht, states, decay, cu, longest, seg, n_seq, softplus, grad=None):
+def _pack(x, dt, A, B, C, D, bias, h0, y, ht, states, decay, cu, longest, seg, n_seq, softplus, for_grad, grad=None):
     (x, xs), (dt, dts), (B, bs), (C, cs) = x, dt, B, C
     H, P = x.shape[-2:]
     G, N = B.shape[-2:]
@@ -64,7 +65,7 @@ def _pack(x, dt, A, B, C, D, bias, h0, y, ht, states, decay, cu, longest, seg, n
     extra = [0] * 12 if grad is None else [p(t) for t in grad[0]] + [grad[1]]
     return _ARGS.pack(p(x), p(dt), p(B), p(C), p(A), p(D), p(bias), p(h0), p(y), p(ht), p(states), p(decay), p(cu), total,
                       longest, seg, xs, dts, bs, cs, H * P, n_seq, H, P, G, N, _DTYPES[x.dtype], _DTYPES[dt.dtype],
-                      int(softplus), *extra)
+                      int(softplus), int(for_grad), 0, *extra)
 
 
 def _scan_launch(x, dt, A, B, C, D, bias, softplus, h0, want_final, cu, keep=False):
@@ -80,7 +81,7 @@ def _scan_launch(x, dt, A, B, C, D, bias, softplus, h0, want_final, cu, keep=Fal
     seg = _segment_tokens(longest, total, H * -(-P // 64), N, x[0].dtype, keep)
     single = longest <= seg
     y = torch.empty((nb, T, H, P), dtype=x[0].dtype, device=dev)
-    ht = torch.empty((n_seq, H, N, P), dtype=torch.float32, device=dev) if want_final or (keep and not single) else None
+    ht = torch.empty((n_seq, H, N, P), dtype=torch.float32, device=dev) if want_final else None
     states = decay = None
     if not single:
         slots = n_seq * -(-T // seg) if cu is None else total // seg + n_seq + 1
@@ -88,12 +89,12 @@ def _scan_launch(x, dt, A, B, C, D, bias, softplus, h0, want_final, cu, keep=Fal
         decay = torch.empty((slots, H), dtype=torch.float32, device=dev)
     with _on_device(dev.index):
         check(_capi.lib().lampa_ss_scan_fwd(
-            _pack(x, dt, A, B, C, D, bias, h0, y, ht, states, decay, cu, longest, seg, n_seq, softplus),
+            _pack(x, dt, A, B, C, D, bias, h0, y, ht, states, decay, cu, longest, seg, n_seq, softplus, keep),
             stream_of(y)), "lampa_ss_scan_fwd")
     return y, ht, (states, decay, seg, n_seq, longest)
 
 
-def _scan_backward(x, dt, A, B, C, D, bias, softplus, h0, cu, ht, kept, dy, dht):
+def _scan_backward(x, dt, A, B, C, D, bias, softplus, h0, cu, kept, dy, dht):
     states, decay, seg, n_seq, longest = kept
     dev = x.device
     nb, T, H, P = x.shape
@@ -110,8 +111,8 @@ def _scan_backward(x, dt, A, B, C, D, bias, softplus, h0, cu, ht, kept, dy, dht)
     x_, dt_ = _vectors(x, H * P, P), _tokens(dt, H)
     B_, C_ = _vectors(B, G * N, N), _vectors(C, G * N, N)
     A, D, bias, h0 = _plain_f32(A), _plain_f32(D), _plain_f32(bias), _plain_f32(h0)
-    pack = lambda ws, size: _pack(x_, dt_, A, B_, C_, D, bias, h0, None, ht, states, decay, cu, longest, seg, n_seq,  # noqa: E731
-                                  softplus, ((dy, dht, dx, ddt, dB, dC, dA, dD, dbias, dh0, ws), size))
+    pack = lambda ws, size: _pack(x_, dt_, A, B_, C_, D, bias, h0, None, None, states, decay, cu, longest, seg, n_seq,  # noqa: E731
+                                  softplus, True, ((dy, dht, dx, ddt, dB, dC, dA, dD, dbias, dh0, ws), size))
     lib = _capi.lib()
     with _on_device(dev.index):
         size = check(lib.lampa_ss_bwd_workspace_bytes(pack(None, 0)), "lampa_ss_bwd_workspace_bytes")
@@ -126,15 +127,22 @@ class _StateSpaceScan(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         y, ht, kept = _scan_launch(x, dt, A, B, C, D, bias, softplus, h0, want_final, cu, keep=keep)
         if keep:
-            ctx.save_for_backward(x, dt, A, B, C, D, bias, h0, cu, ht, kept[0], kept[1])
+            ctx.save_for_backward(x, dt, A, B, C, D, bias, h0, cu, kept[0], kept[1])
+        # The gradients do not read the final state, so it is not kept; but a gradient through it would be that of the state as
+        # it was returned, so one that has been moved on in place is noticed as long as somebody holds it.
+        ctx.final = (weakref.ref(ht), ht._version) if keep and want_final else None
         ctx.softplus, ctx.sizes = softplus, kept[2:]
         return y, ht if want_final else None
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dht):
-        x, dt, A, B, C, D, bias, h0, cu, ht, states, decay = ctx.saved_tensors
-        dx, ddt, dA, dB, dC, dD, dbias, dh0 = _scan_backward(x, dt, A, B, C, D, bias, ctx.softplus, h0, cu, ht,
+        x, dt, A, B, C, D, bias, h0, cu, states, decay = ctx.saved_tensors
+        final = None if ctx.final is None else ctx.final[0]()
+        if final is not None and final._version != ctx.final[1]:
+            raise RuntimeError("state_space_scan: the final state has been modified by an inplace operation (a step that moved it "
+                               "on) before the gradients of the scan that returned it; give state_space_step a new_state")
+        dx, ddt, dA, dB, dC, dD, dbias, dh0 = _scan_backward(x, dt, A, B, C, D, bias, ctx.softplus, h0, cu,
                                                              (states, decay, *ctx.sizes), dy, dht)
         as_type = lambda g, t: None if t is None else g.to(t.dtype)  # noqa: E731
         return (dx, ddt, as_type(dA, A), dB, dC, as_type(dD, D), as_type(dbias, bias), as_type(dh0, h0), None, None, None, None)
@@ -187,7 +195,9 @@ def state_space_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torc
     dy, B or C that is not finite may reach every token of its 64). Growth (delta A > 0) is taken as it is; where it passes
     float32's range within 64 tokens or a segment the result may be NaN where the recurrence, on zeros, is not.
     Differentiable in every floating-point input (first order); the gradients of B and C are summed over a group's heads in
-    a fixed order, and repeated calls give the same bits."""
+    a fixed order, and repeated calls give the same bits. (Calls that differ in what else is asked for, gradients or the final
+    state, may differ in the last bits of y: they run in other segments and hand states on with more bits.) The backward raises where
+    the final state it returned has been moved on in place since: use ``state_space_step(..., new_state=)`` until then."""
     what = "state_space_scan"
     _same_device(what, x, dt, A, B, C, D, dt_bias, initial_state)
     _check_operands(what, x, dt, A, B, C, D, dt_bias, 2)

@@ -226,3 +226,45 @@ def test_parameters_without_gradients_are_launched_as_plain_tensors(device, dtyp
     assert kept < 2 ** 16  # the outputs alone, as the allocator rounds them up
     _call(held)
     assert asked[2:] == [True]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_final_state_is_not_kept_for_the_gradients(device, dtype):
+    """Between forward and backward a call holds its segments' states and no final state, asked for or not, unless the caller does;
+    the gradients are the same bits either way."""
+    n, T, H, P, N = 40, 500, 2, 64, 128
+    d = _to(_inputs((n, T), H, P, 1, N, dtype, 91, n), device, grad=True)
+    dy = torch.randn(n, T, H, P, device=device).to(dtype)
+    size = n * H * N * P * 4
+    assert ss._segment_tokens(T, n * T, H, N, dtype, True) < T  # more than one segment a sequence
+    held, grads = [], []
+    for final in (False, True):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        y, ht = _call(d, final=final)
+        assert (ht is None) == (not final)
+        del ht
+        held.append(torch.cuda.memory_allocated() - before - y.numel() * y.element_size())
+        grads.append(torch.autograd.grad(y, [d[k] for k in NAMES], dy))
+        del y
+    seg = ss._segment_tokens(T, n * T, H, N, dtype, True)
+    slots = n * -(-T // seg)
+    for h in held:
+        assert h < slots * H * N * P * 4 + size / 2, (h, size)
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
+def test_a_final_state_moved_on_in_place_is_noticed(device):
+    """With another state for the step the scan's gradients are there; with the state moved on itself its backward raises."""
+    d = _to(_inputs((1, 700), 2, 64, 1, 64, torch.bfloat16, 92, 1), device, grad=True)
+    token = lambda state, **k: ss.state_space_step(  # noqa: E731
+        *(d[k][:, 0].detach() if k in ("x", "dt", "B", "C") else d[k].detach() for k in ("x", "dt", "A", "B", "C")), state.detach(), **k)
+    y, ht = _call(d)
+    want = torch.autograd.grad([y, ht], d["x"], [torch.ones_like(y), torch.ones_like(ht)], retain_graph=True)[0]
+    token(ht, new_state=torch.empty_like(ht))
+    again = torch.autograd.grad([y, ht], d["x"], [torch.ones_like(y), torch.ones_like(ht)], retain_graph=True)[0]
+    assert torch.equal(want, again)
+    token(ht)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad([y, ht], d["x"], [torch.ones_like(y), torch.ones_like(ht)])
