@@ -15,9 +15,10 @@
 #include "../../include/lampa_amd.h"
 #include "gdr_ops.h"
 
-// Decay exponents below this leave nothing of an fp32 value (exp(-104) is below the smallest denormal): clamping them
-// there keeps sums over a chunk, whose differences are taken, small enough to stay exact to about 1e-4 even where a
-// token cuts the past off.
+// Decay exponents below this leave nothing of an fp32 value (exp(-104) is below the smallest denormal): clamped there, a sum over the
+// 64 tokens of a chunk stays within 9 600 (as an exponent of 2) however strongly tokens cut the past off. The chunk kernels sum in
+// 64 bits; a pair's weight takes the difference of two such sums rounded to fp32, each off by half a step: 2^-16 each behind two
+// clamped tokens of a chunk, 2^-11 each (7e-4 of the weight) behind 63.
 #define SS_MIN_LOG_DECAY (-104.0f)
 
 struct SsSegment {

@@ -1,14 +1,16 @@
 """Calls of the state-space operators, the convolution and the norms that a program may make beside the ordinary ones: rubbish behind
 the last sequence, gradients through a single token, forward-mode gradients, slices of long tensors, parameters without gradients."""
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+from lampa_amd import block
 from lampa_amd import layer_ops as lo
 from lampa_amd import state_space as ss
 from oracle import state_space as os_
 from test_gpu_conv_state import HALF32, _close, _np, _want
-from test_gpu_state_space import _bound, _call, _check, _inputs, _oracle, _to
+from test_gpu_state_space import _bound, _call, _check, _half, _inputs, _oracle, _to
 
 pytestmark = pytest.mark.gpu
 
@@ -268,3 +270,81 @@ def test_a_final_state_moved_on_in_place_is_noticed(device):
     token(ht)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad([y, ht], d["x"], [torch.ones_like(y), torch.ones_like(ht)])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("every", [37, 3])
+@pytest.mark.parametrize("seg", [None, 64])
+def test_strong_decays_to_the_last_bits(device, dtype, every, seg, monkeypatch):
+    """Tokens whose step wipes the state, one in 37 or one in 3, beside steps of zero and ordinary ones, outputs and gradients. fp32
+    and the states that are handed on take no difference of long sums: the bounds of any other call. In the 16-bit outputs a pair's
+    weight is 2^(gamma_t - gamma_s) of two sums over the chunk's tokens, each rounded to fp32 once: half a step of the largest."""
+    if seg:
+        monkeypatch.setattr(ss, "_segment_tokens", lambda *a: seg)
+    T, H, P, N = 260, 2, 32, 32
+    i = _inputs((1, T), H, P, 1, N, dtype, 93, 1, rate=1.0)
+    dt = torch.full((1, T, H), 0.05)
+    dt[:, ::every] = 2000.0
+    dt[:, 5::41] = 0.0
+    i["dt"], i["dt_bias"] = dt.to(dtype), None
+    i["x"] = i["x"].clone()
+    i["x"][:, dt[0, :, 0] == 2000] = 0  # their own write is not what is looked at
+    gen = torch.Generator().manual_seed(94)
+    dy, dht = torch.randn(1, T, H, P, generator=gen).to(dtype), torch.randn(1, H, N, P, generator=gen)
+    (y, last, g), (ym, lastm, gm) = _oracle(i, [T], softplus=False, dy=dy, dht=dht)
+    g2 = np.maximum(_np(i["dt"])[0] * _np(i["A"]), -104.0) * np.log2(np.e)
+    deepest = max(abs(g2[t:t + 64].sum(0)).max() for t in range(0, T, 64))
+    weights = 0.0 if dtype == torch.float32 else 2 * np.spacing(np.float32(deepest)) / 2 * np.log(2)
+    d = _to(i, device, grad=True)
+    got, ht = _call(d, softplus=False)
+    _check("y", got, y, _bound(dtype, T, y, ym, N) + weights * ym, dtype)
+    _check("last", ht, last, _bound(dtype, T, last, lastm, 0, False))
+    names = [k for k in NAMES if k != "dt_bias"]
+    for k, a in zip(names, torch.autograd.grad([got, ht], [d[k] for k in names], [dy.to(device), dht.to(device)])):
+        wide = {"x": N, "B": P * H, "C": P * H, "h0": 0, "D": T * P}.get(k, N * P + T)
+        extra = weights * gm[k] if k in ("x", "B", "C") else 0.0
+        if k == "dt" and dtype != torch.float32:
+            # What passes a token is a prefix sum, over 16 tokens, of the pairs that begin minus those that end there. Behind a token that
+            # wipes the state nothing passes, but the sum of up to 16 terms each way is off by 32 half-steps of the pairs before it, and
+            # the terms by as many of their own; gm of the chunk's first tokens bounds all pairs that end later.
+            top = np.concatenate([np.repeat(gm[k][t:t + 64].max(0, keepdims=True), len(gm[k][t:t + 64]), 0) for t in range(0, T, 64)])
+            extra = 64 * HALF32 * top
+        bound = _bound(dtype, T, g[k], gm[k], wide, k in ("x", "B", "C")) + extra
+        # a step of 2000 leaves gradients beyond fp16's range: infinite with their sign, or the largest value, and nothing else
+        a, most = a.detach().double().cpu().numpy().reshape(g[k].shape), torch.finfo(d[k].dtype).max
+        slack = (bound + _half(d[k].dtype) * abs(g[k])) * 2
+        beyond = abs(g[k]) + slack > most
+        assert (a[beyond] * np.sign(g[k][beyond]) >= np.minimum(most, abs(g[k]) - slack)[beyond]).all(), k
+        _check(k, torch.from_numpy(np.where(beyond, g[k], a)), g[k], bound, d[k].dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_decay_gradients_of_a_training_step(device, dtype, monkeypatch):
+    """A_log and dt_bias of every layer of a block in a training step, against float64 on what the layer's scan was given: sums of both
+    signs over all tokens, within the bounds of the scan's own tests and the rounding to the parameters' type."""
+    lens = [70, 0, 1, 30]
+    torch.manual_seed(95)
+    model = block.StateSpaceBlock(64, 3, residual_scale=0.7, d_state=16, head_dim=16, expand=2, n_groups=2).to(dtype).to(device)
+    calls, upstream = [], {}
+    scan = block.state_space_scan
+
+    def recorded(x, dt, A, B, C, **k):
+        y, state = scan(x, dt, A, B, C, **k)
+        n = len(calls)
+        calls.append(dict(x=x, dt=dt, A=A, B=B, C=C, D=k["D"], dt_bias=k["dt_bias"], h0=None))
+        y.register_hook(lambda grad: upstream.update({n: grad.clone()}))
+        return y, state
+
+    monkeypatch.setattr(block, "state_space_scan", recorded)
+    x = torch.randn(1, sum(lens), 64, device=device).to(dtype)
+    out, _ = model(x, torch.tensor([0, 70, 70, 71, 101], device=device))
+    out.backward(torch.randn_like(out))
+    assert len(calls) == len(upstream) == 3
+    for n, layer in enumerate(model.layers):
+        i = {k: None if t is None else t.detach().cpu() for k, t in calls[n].items()}
+        (_, _, g), (_, _, gm) = _oracle(i, lens, dy=upstream[n].cpu())
+        N, P = i["B"].shape[-1], i["x"].shape[-1]
+        bound = lambda k: _bound(dtype, max(lens), g[k], gm[k], N * P + sum(lens), False)  # noqa: E731
+        A = _np(i["A"])
+        _check("A_log", layer.A_log.grad, g["A"] * A, (bound("A") + 4 * HALF32 * gm["A"]) * abs(A), dtype)
+        _check("dt_bias", layer.dt_bias.grad, g["dt_bias"], bound("dt_bias"), dtype)
