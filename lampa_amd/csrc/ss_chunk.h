@@ -128,6 +128,12 @@ struct ScTile {
       v[k] = x;
     }
   }
+  // Values of a 16-bit type with their sign bits changed where `bits` (two to a word) has ones.
+  __device__ __forceinline__ void flip(unsigned bits) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int k = 0; k < W / 32; ++k) v[k] = __builtin_bit_cast(sc_x8<T>, __builtin_bit_cast(u32x4, v[k]) ^ bits);
+  }
   // Stored in the column order of op_perm32: a lane's share of a 32-wide contraction step is one 16-byte piece.
   __device__ __forceinline__ void put(T* tile, int stride) const {
 #pragma unroll
@@ -157,6 +163,13 @@ struct ScTile {
     return bad;
   }
 };
+
+// The matrix instructions round an accumulator that is smaller than the products added to it towards minus infinity (measured: 1.5
+// beside an accumulator of +-0.75 last places comes out as 1.5 + 0 and 1.5 - 1). What is formed that way is too small by about 2^-25 of
+// the largest summand, whatever its sign, which sums over all tokens (dA, d dt_bias) do not average out as they do ordinary
+// rounding. So the gradients work on dy with its sign changed in every other chunk, and change the signs of what comes out back:
+// everything of theirs is linear in dy, and the errors of one chunk make up for those of the next.
+__device__ __forceinline__ unsigned sc_flip_bits(float sign) { return sign < 0.0f ? 0x80008000u : 0u; }
 
 // What a chunk's steps and decays come to, one entry a token. gamma is summed up in 64 bits: it reaches -200 and beyond where a
 // head decays fast, and the exponents of neighbouring tokens are differences of it, which have to be right to 2^-24 for dA and

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
   }
   ScTile<T, NP> pB, pC;
   ScTile<T, 64> pX, pY;
-  float pdt = 0.0f, dD = 0.0f;
+  float pdt = 0.0f, dD = 0.0f, sign = -1.0f;  // sign: of R, of dy in this chunk, and of all that is made from them
   const int64_t chunks = (seg.t1 - seg.t0 + 63) / 64;
   auto fetch = [&](int64_t c) {
     const int64_t t0 = seg.t0 + 64 * c;
@@ -104,6 +104,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
     const int64_t t0 = seg.t0 + 64 * c;
     const int n_tok = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
     if (!AHEAD) fetch(c);
+    sign = -sign;
+    pY.flip(sc_flip_bits(sign));
     pB.put(tb, KS);
     pC.put(tc, KS);
     pX.put(tx, VS);
@@ -186,7 +188,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
       for (int q = 0; q < 4; ++q) S[q] = kept[(nt0 * 4 + q) * 64 + lane];
     }
 
-    const float end = dec.end;
+    const float end = dec.end, D_sign = sign * D;
+    float dD_chunk = 0.0f;
     // dx of this wave's 16 columns: lane = token 16 st + i, registers = columns 4 g .. + 3
     {
       x8 vy[2];
@@ -227,7 +230,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           dot = __builtin_fmaf((float)xv[r], acc[st][r], dot);
-          dD = __builtin_fmaf((float)xv[r], (float)dyv[r], dD);
+          dD_chunk = __builtin_fmaf((float)xv[r], (float)dyv[r], dD_chunk);
         }
         dot += __shfl_xor(dot, 16);
         dot += __shfl_xor(dot, 32);
@@ -239,10 +242,10 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
           if (2 * kk + 1 >= st) near = mfma16(vy[kk], *reinterpret_cast<const x8*>(m1 + s * MS + 32 * kk + 8 * g), near);
         if (F16) near = near * back1[s] + acc[st];
         if (s < n_tok) {
-          const float ds = dec.delta[s];
+          const float ds = sign * dec.delta[s];
           x4 o;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[r] = (T)__builtin_fmaf(ds, near[r], D * (float)dyv[r]);
+          for (int r = 0; r < 4; ++r) o[r] = (T)__builtin_fmaf(ds, near[r], D_sign * (float)dyv[r]);
           const int c0 = 16 * wave + 4 * g;
           T* dst = reinterpret_cast<T*>(reinterpret_cast<char*>(dxb + (t0 + 16 * st) * row_p) + (unsigned)(i * (int)row_p + c0) * (unsigned)sizeof(T));
           if constexpr (VEC) {
@@ -255,6 +258,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
         }
       }
     }
+    dD = __builtin_fmaf(sign, dD_chunk, dD);
     sc_fence();
     // dB and dC of this wave's columns n: lane = token, registers = columns 4 g .. + 3 of a tile
     float dot = 0.0f;
@@ -351,6 +355,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
                 dc[st] = mfma16(vb[kk], q, dc[st]);
               }
             }
+          db[st] *= sign;
+          dc[st] *= sign;
           if (s < n_tok) {
             const int64_t row = ((t0 + 16 * st) * parts + blockIdx.y) * a.N;
             const unsigned at = (unsigned)(i * (int)(parts * a.N) + c0) * 4u;
@@ -379,19 +385,23 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
     if (lane == 0) dot_part[wave] = dot;
 
     sc_fence();
-    // R in front of the chunk, both ways round.
+    // R in front of the chunk, both ways round, with the sign of the next chunk's dy.
     {
       float wt[2][8];
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) sc_row_weights(dec.grow, kk, lane, wt[kk]);
+      for (int kk = 0; kk < 2; ++kk) {
+        sc_row_weights(dec.grow, kk, lane, wt[kk]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) wt[kk][e] = -wt[kk][e];
+      }
       auto add = [&](f32x4& acc, const x8 (&left)[2], const x8 (&right)[2][PARTS], float back) {
         if constexpr (F16) {
           f32x4 d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) d = sc_mfma_left(left[kk], right[kk], d);
-          acc = acc * end + d * back;
+          acc = d * back - acc * end;
         } else {
-          acc *= end;
+          acc *= -end;
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) acc = sc_mfma_left(left[kk], right[kk], acc);
         }
@@ -460,8 +470,8 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
       if (lane == 0) before = 0.0f;
       if (lane < n_tok) {
         const int64_t at = (t0 + lane) * parts + blockIdx.y;
-        w.dg[at] = (pairs + before) + (later + all);
-        w.reach[at] = col + diag[lane] + left;
+        w.dg[at] = sign * ((pairs + before) + (later + all));
+        w.reach[at] = sign * (col + diag[lane] + left);
       }
     }
   }
@@ -479,7 +489,7 @@ __global__ void __launch_bounds__(SC_BLOCK, 2) sc_grad_kernel(lampa_ss_args a, S
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int n = 16 * nt + 4 * g + r;
-        if (n < a.N && p < a.P) out[(int64_t)n * a.P + p] = R[nt][r];
+        if (n < a.N && p < a.P) out[(int64_t)n * a.P + p] = -sign * R[nt][r];
       }
   }
 }

@@ -43,7 +43,7 @@ __device__ __forceinline__ void sc_map(const lampa_ss_args& a, const SsGrad& w, 
   }
   ScTile<T, NP> pk;
   ScTile<T, 64> pv;
-  float pdt = 0.0f, sum = 0.0f;
+  float pdt = 0.0f, sum = 0.0f, sign = 1.0f;  // sign (REV): of S, and of dy in this chunk
   auto fetch = [&](int64_t c) {
     const int64_t t0 = seg.t0 + 64 * (REV ? chunks - 1 - c : c);
     const int n = (int)(seg.t1 - t0 < 64 ? seg.t1 - t0 : 64);
@@ -63,12 +63,16 @@ __device__ __forceinline__ void sc_map(const lampa_ss_args& a, const SsGrad& w, 
 #pragma unroll
         for (int r = 0; r < 4; ++r) keep[sc_kept_at(nt, wave, 4 * g + r, i)] = S[nt][r];
     }
+    if (REV) {
+      sign = -sign;
+      pv.flip(sc_flip_bits(sign));
+    }
     pk.put(tk, KS);
     pv.put(tv, VS);
     if (wave == 0) sc_decays(dec, nullptr, pdt, n, bias, A, a.softplus);
     lds_barrier();
     if (c + 1 < chunks) fetch(c + 1);
-    const float end = dec.end;
+    const float end = REV ? -dec.end : dec.end;
     sum += dec.sum;
     sc_x8<T> v[2];
     sc_columns<T>(tv, VS, 16 * wave, lane, v);
@@ -95,7 +99,7 @@ __device__ __forceinline__ void sc_map(const lampa_ss_args& a, const SsGrad& w, 
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int n = 16 * nt + 4 * (lane0 >> 4) + r;
-      if (n < a.N && p < a.P) local[(int64_t)n * a.P + p] = S[nt][r];
+      if (n < a.N && p < a.P) local[(int64_t)n * a.P + p] = REV ? sign * S[nt][r] : S[nt][r];
     }
   if (!REV && threadIdx.x == 0 && pb == 0) a.slot_decay[(int64_t)blockIdx.x * a.H + h] = __builtin_amdgcn_exp2f(sum);
 }

@@ -348,3 +348,35 @@ def test_decay_gradients_of_a_training_step(device, dtype, monkeypatch):
         A = _np(i["A"])
         _check("A_log", layer.A_log.grad, g["A"] * A, (bound("A") + 4 * HALF32 * gm["A"]) * abs(A), dtype)
         _check("dt_bias", layer.dt_bias.grad, g["dt_bias"], bound("dt_bias"), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_decay_gradient_has_no_bias(device, dtype):
+    """dA is a sum over all tokens of delta_t dg_t. Errors of a token's dg that are as likely above as below add up like a random walk,
+    ones that lean to one side like the number of tokens. A dg is four sums in fp32, off by two half-steps (2^-23) of dg's usual size,
+    the same for the 64 tokens of a chunk at worst and independent between chunks: 4 sigma of their sum is
+    4 * 2^-23 * sqrt(64 T) * rms(delta dg). (A lean of one half-step would come to T / (8 sqrt(64 T)) = 2.2 times that.)"""
+    T, H, P, N = 19200, 4, 32, 32
+    gen = torch.Generator(device=device).manual_seed(96)
+    r = lambda *s: torch.randn(*s, generator=gen, device=device)  # noqa: E731
+    silu = torch.nn.functional.silu
+    x, B, C, dy = silu(r(1, T, H, P)).to(dtype), silu(r(1, T, 1, N)).to(dtype), silu(r(1, T, 1, N)).to(dtype), r(1, T, H, P).to(dtype)
+    A, delta = torch.tensor([-1.0, -2.0, -4.0, -8.0], device=device), torch.nn.functional.softplus(r(1, T, H) * 0.7 - 4.3)
+    leaf = A.clone().requires_grad_(True)
+    y, _ = ss.state_space_scan(x, delta, leaf, B, C)
+    dA, = torch.autograd.grad(y, leaf, dy)
+    xs, ds, Bs, Cs, ys = (t[0].double() for t in (x, delta, B, C, dy))
+    decay = torch.exp(ds * A.double())
+    states = torch.zeros(T + 1, H, N, P, dtype=torch.float64, device=device)
+    for t in range(T):
+        states[t + 1] = decay[t, :, None, None] * states[t] + (ds[t, :, None] * Bs[t])[:, :, None] * xs[t][:, None, :]
+    R = torch.zeros(H, N, P, dtype=torch.float64, device=device)
+    dg = torch.empty(T, H, dtype=torch.float64, device=device)
+    for t in range(T - 1, -1, -1):
+        R += Cs[t, 0][None, :, None] * ys[t][:, None, :]
+        R *= decay[t, :, None, None]
+        dg[t] = (R * states[t]).sum((-1, -2))
+    terms = ds * dg
+    bound = 4 * 2.0 ** -23 * (64 * T) ** 0.5 * terms.pow(2).mean(0).sqrt()
+    off = (dA.double() - terms.sum(0)).abs()
+    assert (off <= bound + 2.0 ** -24 * dA.abs()).all(), (off / bound).tolist()
