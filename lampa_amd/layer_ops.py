@@ -287,6 +287,10 @@ def causal_conv1d(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: 
     with_state = initial_state is not None or output_final_state
     if not with_state:
         require_cuda(cu_seqlens)
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"causal_conv1d: the residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if bias is not None and bias.numel() != D:
+        raise ValueError(f"causal_conv1d: the bias must hold {D} values, got {tuple(bias.shape)}")
     if weight is None:
         weight = torch.ones(D, 1, device=x.device)
     grad = _wants_grad(x, weight, bias, residual)

@@ -380,3 +380,15 @@ def test_the_decay_gradient_has_no_bias(device, dtype):
     bound = 4 * 2.0 ** -23 * (64 * T) ** 0.5 * terms.pow(2).mean(0).sqrt()
     off = (dA.double() - terms.sum(0)).abs()
     assert (off <= bound + 2.0 ** -24 * dA.abs()).all(), (off / bound).tolist()
+
+
+def test_a_residual_or_bias_of_another_size_is_refused(device):
+    """The kernels read a row of the residual for each of x and a value of the bias for each channel: nothing is broadcast."""
+    x, w = torch.zeros(2, 5, 16, device=device), torch.zeros(16, 4, device=device)
+    for leaf in (x, x.clone().requires_grad_(True)):
+        for shape in ((1, 5, 16), (2, 1, 16), (2, 5, 8)):
+            with pytest.raises(ValueError, match="residual"):
+                lo.causal_conv1d(leaf, w, residual=torch.zeros(*shape, device=device))
+        for size in (1, 8, 32):
+            with pytest.raises(ValueError, match="bias"):
+                lo.causal_conv1d(leaf, w, torch.zeros(size, device=device))
