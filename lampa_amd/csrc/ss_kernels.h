@@ -8,8 +8,10 @@
 struct SsGrad {
   float* adjoints;           // [slots, H, N, P]: the segments' local adjoints, then the adjoint at each segment's end
   float *dB_part, *dC_part;  // [tokens, H * blocks, N]: one part for each head and block of 64 columns of x
-  float* dg;                 // [tokens, H, blocks]: the decay exponent's gradient (chunks), or dy_t . (S_t^T C_t) (token-serial)
-  float* reach;              // [tokens, H, blocks]: x_t . (R_t^T B_t)
+  float* dg;                 // [tokens, H, blocks]: the decay exponent's gradient (chunks), or dy_t . ((a_t S_{t-1})^T C_t) (token-serial)
+  float* reach;              // chunks: [tokens, H, blocks]: x_t . (R_t^T B_t)
+  float* behind;             // token-serial: [tokens, H, blocks]: x_t . ((a_{t+1} R_{t+1})^T B_t), reach without the token's own output
+  float* pair;               // token-serial: [tokens, H, 1 + blocks]: C_t . B_t, and dy_t . x_t of each block
   float* chunk_states;       // chunks: the state in front of every 64 tokens, [rows, H, blocks, N padded, 64]
                              // token-serial: the state behind every SS_DOT, [rows, H, N, P]
   float* chunk_dots;         // token-serial: <R, S> behind every SS_DOT tokens, [rows, H, blocks]

@@ -52,8 +52,11 @@ static int ss_join(const lampa_ss_args& a, float* states, const float* init, flo
 
 // From the gradient of the decays to those of dt, A and dt_bias. One workgroup takes 256 tokens of a segment and head,
 // a wave 64, a lane one. Where dg has not been summed up yet (fp32), it is here, SS_DOT tokens at a time from their end:
-// dg_t = dg_{t+1} + read_t - delta_t reach_t, behind the last of them <R, S>. Starting anew that often keeps rounding errors of
-// the sum, which pass on to every earlier token of it, from adding up (dA off by 2.5e-5 over segments of 256 tokens, 6e-6 over 64).
+// dg_t = dg_{t+1} + read_t - delta_t behind_t, behind the last of them <R, S>: what ends at t minus what begins there. What a token
+// passes to its own output is in neither. It does not cross a token; where decays are fast it is most of both, e^|g| of dg, and its
+// rounding stayed in dg (ddt off by 22 half-steps at g = -3, now 4; 48 883 tokens at g = -1.2: dA 2.5e-6, now 2.5e-7). Starting anew
+// that often keeps rounding errors of the sum, which pass on to every earlier token of it, from adding up (dA off by 2.5e-5 over
+// segments of 256 tokens, 6e-6 over 64).
 template <typename T>
 __global__ void __launch_bounds__(SS_BLOCK) ss_decay_grad_kernel(lampa_ss_args a, SsGrad w, bool summed) {
   const SsSegment seg = ss_segment(a, blockIdx.x);
@@ -71,10 +74,20 @@ __global__ void __launch_bounds__(SS_BLOCK) ss_decay_grad_kernel(lampa_ss_args a
       raw = ss_load_dt<T>(a.dt, a.dt_dtype, tok * a.dt_stride + h) + bias;
       delta = ss_delta(raw, 0.0f, a.softplus);
       for (int i = 0; i < reads; ++i) dg += w.dg[(tok * a.H + h) * reads + i];
-      for (int i = 0; i < npb; ++i) reach += w.reach[(tok * a.H + h) * npb + i];
+      if (summed) {
+        for (int i = 0; i < npb; ++i) reach += w.reach[(tok * a.H + h) * npb + i];
+      } else {
+        const float* pair = w.pair + (tok * a.H + h) * (1 + npb);
+        float behind = 0.0f, own = 0.0f;
+        for (int i = 0; i < npb; ++i) {
+          behind += w.behind[(tok * a.H + h) * npb + i];
+          own += pair[1 + i];
+        }
+        dg -= delta * behind;
+        reach = __builtin_fmaf(pair[0], own, behind);
+      }
     }
     if (!summed && !seg.outside) {
-      if (on) dg -= delta * reach;
 #pragma unroll
       for (int off = 1; off < SS_DOT; off <<= 1) {
         const float later = __shfl_down(dg, off);
@@ -205,7 +218,9 @@ static int64_t ss_grad_layout(const lampa_ss_args& a, char* base, SsGrad* w) {
   take(g.dC_part, a.n_tokens * a.H * npb * a.N);
   const bool serial = a.dtype == GDR_FP32;
   take(g.dg, a.n_tokens * a.H * npb * (serial ? nnb : 1));
-  take(g.reach, a.n_tokens * a.H * npb);
+  take(g.reach, serial ? 0 : a.n_tokens * a.H * npb);
+  take(g.behind, serial ? a.n_tokens * a.H * npb : 0);
+  take(g.pair, serial ? a.n_tokens * a.H * (1 + npb) : 0);
   take(g.chunk_states, ss_rows(&a, serial ? SS_DOT : 64) * a.H * (serial ? (int64_t)a.N * a.P : npb * ss_chunk_n(a.N) * 64));
   take(g.chunk_dots, serial ? ss_rows(&a, SS_DOT) * a.H * npb : 0);
   take(g.param_part, slots * ss_pieces(a) * a.H * 2);

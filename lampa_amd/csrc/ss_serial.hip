@@ -8,9 +8,14 @@
 // tokens at a time and read as broadcasts, so a token costs 3 vector instructions a row and no reduction across lanes.
 // One wave a workgroup; nothing is shared between waves, so no barrier waits for another wave.
 //
-// Bound by the latency of a token (about 0.5 us with one wave a SIMD: 3 instructions a row, the staged rows' reads, and the
-// stores), so segments are short. Measured, fp32: gradients of 6 007 packed tokens x 4 heads, P = N = 32, 241 us for the four
-// walks in segments of 64; 77 tokens x 2 sequences whole 50 us.
+// Bound by the latency of a token (0.4 to 0.6 us with one wave a SIMD: 3 instructions a row, the staged rows' reads, and the
+// stores), so segments are short. Measured, fp32: 6 007 packed tokens x 4 heads, P = N = 32, in segments of 64: y 26, dC 40, dx 39, dB
+// 25 us, local states and adjoints 18 each; 77 tokens x 2 sequences whole 28 us; forward of 20 000 x 8 x 64 at N = 64 / 128 in all 235 /
+// 404 us.
+//
+// Errors: a token's part of a later state is a product of as many fp32 decays as lie between them, each rounded, where exponents
+// summed up in 64 bits would be rounded once: y is off by 3e-7 at 77 tokens of slow decay against 6e-8, and by 4e-8 either way where
+// heads forget within a few tokens.
 #include "ss_kernels.h"
 
 #define SS_TILE 8  // tokens staged at once; SS_DOT is a multiple of it
@@ -25,7 +30,9 @@ template <int ROWS, int LG, int KIND, bool MAP>
 __global__ void __launch_bounds__(64, (ss_serial_waves<ROWS, KIND, MAP>())) ss_serial_kernel(lampa_ss_args a, SsGrad w) {
   constexpr bool REV = KIND == SS_DX || KIND == SS_DB;  // from the end of the segment
   constexpr bool LANE_P = KIND == SS_Y || KIND == SS_DX;
-  constexpr bool SUMS = !MAP && (KIND == SS_DC || KIND == SS_DX);  // a dot with a second lane vector, C or x, for each token
+  // Walks that also leave dots of their read-outs with a second lane vector, C or x: these read out what the state holds without the
+  // token's own part, U_t (Q_t . U_t for the rows), which goes to the output alone.
+  constexpr bool SUMS = !MAP && (KIND == SS_DC || KIND == SS_DX);
   constexpr int PIECES = ROWS * SS_TILE / 64, RL = ROWS / LG, COLS = 64 / LG;
   const SsSegment seg = ss_segment(a, blockIdx.x);
   if (!seg.live) return;
@@ -122,7 +129,9 @@ __global__ void __launch_bounds__(64, (ss_serial_waves<ROWS, KIND, MAP>())) ss_s
     }
     pdt = ((const float*)a.dt)[(t0 + (lane < last ? lane : last)) * a.dt_stride + h];
   };
-  // The states kept every SS_DOT tokens: written in front of the adjoints' walk, read by it one ahead.
+  // The states kept every SS_DOT tokens: written in front of the adjoints' walk, read by it one ahead, but for 64 whole rows, which two
+  // waves a SIMD have no room to hold twice (136 registers spilled, gradients of 60 000 x 8 x 64 2 620 us against 2 230).
+  constexpr bool AHEAD = !(ROWS == 64 && LG == 1);
   auto kept_of = [&](int64_t done) { return w.chunk_states + ((ss_row_of(seg, SS_DOT) + (done - 1) / SS_DOT) * a.H + h) * per_h; };
   float kept[KIND == SS_DX && !MAP ? RL : 1];
   auto fetch_kept = [&](int64_t done) {
@@ -139,7 +148,7 @@ __global__ void __launch_bounds__(64, (ss_serial_waves<ROWS, KIND, MAP>())) ss_s
   float dD = 0.0f;
   if (tiles) {
     fetch(0);
-    if constexpr (KIND == SS_DX && !MAP) fetch_kept(count);
+    if constexpr (KIND == SS_DX && !MAP && AHEAD) fetch_kept(count);
   }
   for (int64_t tile = 0; tile < tiles; ++tile) {
     const int64_t t0 = base_of(tile);
@@ -175,16 +184,25 @@ __global__ void __launch_bounds__(64, (ss_serial_waves<ROWS, KIND, MAP>())) ss_s
       const int64_t done = t0 + n - seg.t0;
       if (tile == 0 || done % SS_DOT == 0) {
         float dot = 0.0f;
+        if constexpr (!AHEAD) fetch_kept(done);
 #pragma unroll
         for (int r = 0; r < RL; ++r) dot = __builtin_fmaf(S[r], kept[r], dot);
         dot = ss_wave_sum(dot) * carry;
         if (lane == 0) w.chunk_dots[((ss_row_of(seg, SS_DOT) + (done - 1) / SS_DOT) * a.H + h) * npb + pb] = dot;
         const int64_t next = (done - 1) / SS_DOT * SS_DOT;
-        if (next > 0) fetch_kept(next);
+        if (AHEAD && next > 0) fetch_kept(next);
       }
+    }
+    float own = 0.0f;  // U_t . Q_t of token lane / 8
+    if constexpr (SUMS) {
+#pragma unroll
+      for (int r = 0; r < ROWS / 8; ++r) own = __builtin_fmaf(lu[lane >> 3][(lane & 7) + 8 * r], lq[lane >> 3][(lane & 7) + 8 * r], own);
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) own += __shfl_xor(own, off);
     }
     // Tokens behind the segment's last one have no step, no input and a decay of one: every tile is walked whole, without a branch,
     // so that the staged rows of the next tokens are read while one is worked on.
+    auto own_of = [&](int t) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(own), 8 * t)); };
     float outs[MAP ? 1 : SS_TILE];
 #pragma unroll
     for (int i = 0; i < SS_TILE; ++i) {
@@ -195,13 +213,18 @@ __global__ void __launch_bounds__(64, (ss_serial_waves<ROWS, KIND, MAP>())) ss_s
       float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int r = 0; r < RL; ++r) {
+        if (SUMS) o[r & 3] = __builtin_fmaf(lq[t][row0 + r], S[r], o[r & 3]);
         S[r] = __builtin_fmaf(lu[t][row0 + r], v, S[r] * s);
-        if (!MAP) o[r & 3] = __builtin_fmaf(lq[t][row0 + r], S[r], o[r & 3]);
+        // both at once: left alone, the old and the new state are kept side by side (64 rows x 64 lanes: 31 to 196 registers spilled,
+        // gradients of 60 000 x 8 x 64 2 790 us against 2 230)
+        if (SUMS) asm("" : "+v"(S[r]), "+v"(o[r & 3]));
+        if (!MAP && !SUMS) o[r & 3] = __builtin_fmaf(lq[t][row0 + r], S[r], o[r & 3]);
         if (RL > 64 && r % 32 == 31) __builtin_amdgcn_sched_barrier(0);  // no registers for the rows of more tokens
       }
       carry = decay;
       if constexpr (!MAP) {
         float out = (o[0] + o[1]) + (o[2] + o[3]);
+        if (SUMS) out *= s;
 #pragma unroll
         for (int off = COLS; off < 64; off <<= 1) out += __shfl_xor(out, off);
         // made here and now: used only under a condition, it would be formed there, from every token's state
@@ -210,11 +233,11 @@ __global__ void __launch_bounds__(64, (ss_serial_waves<ROWS, KIND, MAP>())) ss_s
           outs[t] = __builtin_fmaf(D, lv[t][lane], out);
         } else if constexpr (KIND == SS_DX) {
           const float xv = le[t][lane];
-          outs[t] = __builtin_fmaf(delta, out, D * lv[t][lane]);
+          outs[t] = __builtin_fmaf(delta, __builtin_fmaf(own_of(t), v, out), D * lv[t][lane]);
           if (lane < COLS) dD = __builtin_fmaf(xv, lv[t][lane], dD);
           le[t][lane] = lane < COLS ? xv * out : 0.0f;
         } else if constexpr (KIND == SS_DC) {
-          outs[t] = out;
+          outs[t] = __builtin_fmaf(own_of(t), v, out);
           le[t][lane] = lane < COLS ? le[t][lane] * out : 0.0f;
         } else {
           outs[t] = delta * out;
@@ -236,9 +259,15 @@ __global__ void __launch_bounds__(64, (ss_serial_waves<ROWS, KIND, MAP>())) ss_s
       for (int off = 1; off < 8; off <<= 1) sum += __shfl_xor(sum, off);
       const int t = lane >> 3;
       if ((lane & 7) == 0 && t < n) {
-        const int64_t row = ((t0 + t) * a.H + h) * npb + pb;
-        if constexpr (KIND == SS_DX) w.reach[row] = sum;
-        else w.dg[row * nnb + lane_block] = sum;
+        const int64_t row = (t0 + t) * a.H + h;
+        float* pair = w.pair + row * (1 + npb);
+        if constexpr (KIND == SS_DX) {
+          w.behind[row * npb + pb] = sum;
+          if (pb == 0) pair[0] = own;
+        } else {
+          w.dg[(row * npb + pb) * nnb + lane_block] = sum;
+          if (lane_block == 0) pair[1 + pb] = own;
+        }
       }
     }
     if constexpr (KIND == SS_DC && !MAP) {

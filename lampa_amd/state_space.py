@@ -34,10 +34,11 @@ def _segment_tokens(longest: int, total: int, heads: int, N: int, dtype, grad: b
     """Length of the segments that run in parallel, a multiple of 64: as many workgroups as the chip holds at once, in one round.
     ``heads`` counts blocks of 64 columns. The chunk kernels (16-bit types) run two workgroups a CU, three without gradients and
     N <= 64; the token-serial ones (float32) one wave a workgroup, eight a CU. 60 000 tokens x 8 heads, segments of 256 / 640 /
-    960 / 1920 tokens: forward at N = 64 126 / 97 / 106 / - us, with gradients at N = 128 1098 / - / 810 / 1039 us. Segments of
-    fewer tokens than `shortest` are not worth the two further launches of joining them: fp32 gradients of 6 007 tokens x 4
-    heads with 64 / 128 / 256 tokens 335 / 579 / 1061 us, but 77 tokens whole 48 us, in two segments 72; 16-bit forward of 15 000
-    x 6 with 64 / 256 / 512 tokens 41 / 42 / 58 us."""
+    960 / 1920 tokens: forward at N = 64 120 / 95 / 108 / 167 us, with gradients at N = 128 996 / 893 / 779 / 977 us; fp32, 20 000 x
+    8, with gradients at N = 64, 64 / 128 / 192 / 640 tokens: 1007 / 980 / 1266 / 3398 us. Segments of fewer tokens than `shortest`
+    are not worth the two further launches of joining them: fp32 gradients of 6 007 tokens x 4 heads with 64 / 128 / 256 tokens 194 /
+    305 / 549 us, but 77 tokens whole 27 us, in two segments 45; 16-bit forward of 15 000 x 6 with 64 / 256 / 512 tokens 37 / 45 / 63
+    us, where 256 leave a quarter of the states to hold."""
     serial = dtype == torch.float32
     per_cu = 8 if serial else 3 if N <= 64 and not grad else 2
     shortest = 256 if not serial else 128 if longest <= 128 else 64

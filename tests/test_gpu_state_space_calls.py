@@ -350,36 +350,70 @@ def test_decay_gradients_of_a_training_step(device, dtype, monkeypatch):
         _check("dt_bias", layer.dt_bias.grad, g["dt_bias"], bound("dt_bias"), dtype)
 
 
+def _decay_gradient(device, x, delta, A, B, C, dy):
+    """What the decay's gradient is made of, in float64, token by token: dg_t = <R_t, a_t S_{t-1}> and x_t . (R_t^T B_t), both [T, H]."""
+    xs, ds, Bs, Cs, ys = (t[0].double() for t in (x, delta, B, C, dy))
+    T, H, P = xs.shape
+    N = Bs.shape[-1]
+    decay = torch.exp(ds * A.double())
+    states = torch.zeros(T + 1, H, N, P, dtype=torch.float64, device=device)
+    for t in range(T):
+        states[t + 1] = decay[t, :, None, None] * states[t] + (ds[t, :, None] * Bs[t])[:, :, None] * xs[t][:, None, :]
+    R = torch.zeros(H, N, P, dtype=torch.float64, device=device)
+    dg, reach = (torch.empty(T, H, dtype=torch.float64, device=device) for _ in range(2))
+    for t in range(T - 1, -1, -1):
+        R += Cs[t, 0][None, :, None] * ys[t][:, None, :]
+        reach[t] = (R * Bs[t, 0][None, :, None] * xs[t][:, None, :]).sum((-1, -2))
+        R *= decay[t, :, None, None]
+        dg[t] = (R * states[t]).sum((-1, -2))
+    return dg, reach
+
+
+def _decaying(device, dtype, rates, step, T, P, N):
+    H = len(rates)
+    gen = torch.Generator(device=device).manual_seed(96)
+    r = lambda *s: torch.randn(*s, generator=gen, device=device)  # noqa: E731
+    silu = torch.nn.functional.silu
+    x, B, C, dy = silu(r(1, T, H, P)).to(dtype), silu(r(1, T, 1, N)).to(dtype), silu(r(1, T, 1, N)).to(dtype), r(1, T, H, P).to(dtype)
+    A, delta = -torch.tensor(rates, device=device), torch.nn.functional.softplus(r(1, T, H) * 0.7 + float(np.log(np.expm1(step))))
+    leaves = [A.clone().requires_grad_(True), delta.clone().requires_grad_(True)]
+    y, _ = ss.state_space_scan(x, leaves[1], leaves[0], B, C)
+    return (A, delta[0], *torch.autograd.grad(y, leaves, dy), *_decay_gradient(device, x, delta, A, B, C, dy))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_the_decay_gradient_has_no_bias(device, dtype):
     """dA is a sum over all tokens of delta_t dg_t. Errors of a token's dg that are as likely above as below add up like a random walk,
     ones that lean to one side like the number of tokens. A dg is four sums in fp32, off by two half-steps (2^-23) of dg's usual size,
     the same for the 64 tokens of a chunk at worst and independent between chunks: 4 sigma of their sum is
     4 * 2^-23 * sqrt(64 T) * rms(delta dg). (A lean of one half-step would come to T / (8 sqrt(64 T)) = 2.2 times that.)"""
-    T, H, P, N = 19200, 4, 32, 32
-    gen = torch.Generator(device=device).manual_seed(96)
-    r = lambda *s: torch.randn(*s, generator=gen, device=device)  # noqa: E731
-    silu = torch.nn.functional.silu
-    x, B, C, dy = silu(r(1, T, H, P)).to(dtype), silu(r(1, T, 1, N)).to(dtype), silu(r(1, T, 1, N)).to(dtype), r(1, T, H, P).to(dtype)
-    A, delta = torch.tensor([-1.0, -2.0, -4.0, -8.0], device=device), torch.nn.functional.softplus(r(1, T, H) * 0.7 - 4.3)
-    leaf = A.clone().requires_grad_(True)
-    y, _ = ss.state_space_scan(x, delta, leaf, B, C)
-    dA, = torch.autograd.grad(y, leaf, dy)
-    xs, ds, Bs, Cs, ys = (t[0].double() for t in (x, delta, B, C, dy))
-    decay = torch.exp(ds * A.double())
-    states = torch.zeros(T + 1, H, N, P, dtype=torch.float64, device=device)
-    for t in range(T):
-        states[t + 1] = decay[t, :, None, None] * states[t] + (ds[t, :, None] * Bs[t])[:, :, None] * xs[t][:, None, :]
-    R = torch.zeros(H, N, P, dtype=torch.float64, device=device)
-    dg = torch.empty(T, H, dtype=torch.float64, device=device)
-    for t in range(T - 1, -1, -1):
-        R += Cs[t, 0][None, :, None] * ys[t][:, None, :]
-        R *= decay[t, :, None, None]
-        dg[t] = (R * states[t]).sum((-1, -2))
-    terms = ds * dg
+    T = 19200
+    A, delta, dA, _, dg, _ = _decaying(device, dtype, (1.0, 2.0, 4.0, 8.0), 0.013, T, 32, 32)
+    terms = delta.double() * dg
     bound = 4 * 2.0 ** -23 * (64 * T) ** 0.5 * terms.pow(2).mean(0).sqrt()
     off = (dA.double() - terms.sum(0)).abs()
     assert (off <= bound + 2.0 ** -24 * dA.abs()).all(), (off / bound).tolist()
+
+
+@pytest.mark.parametrize("rates,step", [((1.0, 2.0, 4.0, 8.0), 0.013), ((6.0, 10.0, 15.0, 30.0), 0.1)])
+@pytest.mark.parametrize("P,N", [(32, 32), (8, 64), (64, 64), (80, 100)])
+def test_the_exact_decay_gradient_where_little_passes_a_token(device, rates, step, P, N):
+    """fp32: dg is summed up from the end of 16 tokens, each of which adds what ends there and takes away what begins there: two sums off
+    by two half-steps each, of dg's usual size if a token's own output, which is e^|delta A| as large, is in neither. So the k-th dg
+    from the end is off by 2 sqrt(2 k) half-steps (8.2 rms over the 16), and ddt = A dg + reach by that times A and by four half-steps
+    of reach; 1.25 times their sum in squares is allowed. In dA = sum delta_t dg_t the error of a token's sums comes with the deltas
+    of all tokens before it in the 16; 4 sigma."""
+    T, hs = 4800, 2.0 ** -24
+    A, delta, dA, ddt, dg, reach = _decaying(device, torch.float32, rates, step, T, P, N)
+    A, delta = A.double(), delta.double()
+    rms = lambda t: t.pow(2).mean(0).sqrt()  # noqa: E731
+    off = rms(ddt[0].double() - (A * dg + reach))
+    bound = 1.25 * hs * ((8.2 * A * rms(dg)) ** 2 + (4 * rms(reach)) ** 2).sqrt()
+    assert (off <= bound).all(), (off / bound).tolist()
+    carried = delta.view(T // 16, 16, -1).cumsum(1).flatten(0, 1)
+    bound = 4 * 2 * 2 ** 0.5 * hs * rms(dg) * carried.pow(2).sum(0).sqrt() + hs * dA.abs()
+    off = (dA.double() - (delta * dg).sum(0)).abs()
+    assert (off <= bound).all(), (off / bound).tolist()
 
 
 def test_a_residual_or_bias_of_another_size_is_refused(device):
