@@ -258,7 +258,7 @@ class _CausalConv(torch.autograd.Function):
                 T, _ACT[ctx.activation], _code(x.dtype), ptr(dx), ptr(dwb), ptr(ws), size, stream_of(x)),
                 "lampa_causal_conv1d_bwd")
         dw = dwb[:, :W].to(weight.dtype).reshape(weight.shape) if ctx.needs_input_grad[1] else None
-        db = dwb[:, W].to(bias.dtype) if ctx.needs_input_grad[2] else None
+        db = dwb[:, W].to(bias.dtype).reshape(bias.shape) if ctx.needs_input_grad[2] else None
         return dx, dw, db, dy.to(ctx.residual_dtype) if ctx.needs_input_grad[3] else None, None, None, None, None
 
 
@@ -297,7 +297,7 @@ def causal_conv1d(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: 
     if with_state or grad:
         what = "causal_conv1d"
         _same_device(what, x, weight, bias, residual, initial_state)
-        if weight.numel() % D or weight.shape[0] != D or (bias is not None and tuple(bias.shape) != (D,)):
+        if weight.numel() % D or (with_state and (weight.shape[0] != D or (bias is not None and tuple(bias.shape) != (D,)))):
             raise ValueError(f"{what}: expected weight [{D}, W] and bias [{D}], got {tuple(weight.shape)} and "
                              f"{None if bias is None else tuple(bias.shape)}")
         W = weight.numel() // D

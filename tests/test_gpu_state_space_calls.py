@@ -426,3 +426,21 @@ def test_a_residual_or_bias_of_another_size_is_refused(device):
         for size in (1, 8, 32):
             with pytest.raises(ValueError, match="bias"):
                 lo.causal_conv1d(leaf, w, torch.zeros(size, device=device))
+
+
+def test_taps_and_bias_of_other_shapes_train(device):
+    """Without a state the taps may come in any shape of D x W values and the bias in any of D, with gradients as without."""
+    gen = torch.Generator().manual_seed(11)
+    x, w, b = (torch.randn(*s, generator=gen).to(device) for s in ((2, 9, 16), (16, 4), (16,)))
+    with torch.no_grad():
+        want = lo.causal_conv1d(x, w, b, activation="silu")
+    flat = [t.clone().requires_grad_(True) for t in (w, b)]
+    grads = torch.autograd.grad(lo.causal_conv1d(x, *flat, activation="silu").sum(), flat)
+    for shape, bias_shape in (((16, 1, 4), (1, 16)), ((64,), (16, 1)), ((1, 16, 4), (1, 1, 16))):
+        leaves = [w.reshape(shape).clone().requires_grad_(True), b.reshape(bias_shape).clone().requires_grad_(True)]
+        with torch.no_grad():
+            assert torch.equal(lo.causal_conv1d(x, *leaves, activation="silu"), want)
+        y = lo.causal_conv1d(x, *leaves, activation="silu")
+        assert torch.equal(y, want)
+        for a, c, leaf in zip(torch.autograd.grad(y.sum(), leaves), grads, leaves):
+            assert a.shape == leaf.shape and torch.equal(a.reshape(c.shape), c)
