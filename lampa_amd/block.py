@@ -21,8 +21,8 @@ import torch.nn.functional as F
 
 from . import lsh
 from .gated_delta import chunk_gated_delta_rule
-from .layer_ops import (PROJ_CONV_HIDDEN, FusedRMSNormSwishGate, RMSNorm, ShortConvolution, causal_conv1d, causal_conv1d_split,
-                        causal_conv1d_step, gdr_gates, norm_proj, norm_proj_supported, proj_conv, residual_norm)
+from .layer_ops import (PROJ_CONV_HIDDEN, FusedRMSNormSwishGate, RMSNorm, ShortConvolution, _sequences, causal_conv1d,
+                        causal_conv1d_split, causal_conv1d_step, gdr_gates, norm_proj, norm_proj_supported, proj_conv, residual_norm)
 from .state_space import state_space_scan, state_space_step
 
 
@@ -241,7 +241,8 @@ class StateSpaceLayer(nn.Module):
     def forward(self, hidden_states: torch.Tensor, cu_seqlens=None, cache=None, output_cache: bool = False):
         """hidden_states [B, T, hidden] -> (out [B, T, hidden], cache or None). ``cache`` = (the last inputs of the convolution
         [sequences, conv_dim, conv_size], the states [sequences, heads, d_state, head_dim] float32) as a call or ``step`` left
-        them; no gradient runs through the convolution's part."""
+        them; no gradient runs through the convolution's part. ``cu_seqlens`` as ``state_space_scan`` takes it."""
+        cu_seqlens = _sequences("StateSpaceLayer", cu_seqlens, *hidden_states.shape[:2], hidden_states.device)
         z, xbc, dt = self._split(hidden_states)
         conv_cache, state = (None, None) if cache is None else cache
         conv = causal_conv1d(xbc, self.conv_weight, self.conv_bias, activation="silu", cu_seqlens=cu_seqlens,
@@ -286,6 +287,7 @@ class StateSpaceBlock(nn.Module):
 
     def forward(self, x: torch.Tensor, cu_seqlens=None, caches=None, output_caches: bool = False):
         """x [B, T, hidden] -> (normed output [B, T, hidden], the layers' caches or None)."""
+        cu_seqlens = _sequences("StateSpaceBlock", cu_seqlens, *x.shape[:2], x.device)
         h, residual = self._enter(x)
         new = []
         for i, layer in enumerate(self.layers):

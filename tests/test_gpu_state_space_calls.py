@@ -444,3 +444,23 @@ def test_taps_and_bias_of_other_shapes_train(device):
         assert torch.equal(y, want)
         for a, c, leaf in zip(torch.autograd.grad(y.sum(), leaves), grads, leaves):
             assert a.shape == leaf.shape and torch.equal(a.reshape(c.shape), c)
+
+
+@pytest.mark.parametrize("whole", [False, True])
+def test_boundaries_on_the_host_for_a_layer_and_a_block(device, whole):
+    """With and without caches, trained or not: the bits of boundaries on the GPU, and a check of what they hold."""
+    torch.manual_seed(12)
+    args = dict(d_state=16, head_dim=16, expand=2, n_groups=2)
+    model = (block.StateSpaceBlock(64, 2, **args) if whole else block.StateSpaceLayer(64, **args)).to(device)
+    x = torch.randn(1, 50, 64, device=device)
+    host = torch.tensor([0, 20, 20, 50])
+    for caches in (False, True):
+        want = model(x, host.to(device), **{"output_caches" if whole else "output_cache": caches})[0]
+        got = model(x, host, **{"output_caches" if whole else "output_cache": caches})[0]
+        assert torch.equal(got, want)
+        with torch.no_grad():
+            assert torch.equal(model(x, host)[0], model(x, host.to(device))[0])
+        for a, b in zip(torch.autograd.grad(got.sum(), list(model.parameters())), torch.autograd.grad(want.sum(), list(model.parameters()))):
+            assert torch.equal(a, b)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        model(x, torch.tensor([0, 20, 49]))
