@@ -8,9 +8,9 @@
 //
 // LPR lanes (or, at 256, a whole workgroup) share a row, each holding 8 consecutive channels in each of STEPS strides.
 //
-// Measured, 60 000 x 512 in bf16 beside an fp32 residual, post-norm, a gate for each token, a scale: forward 77 us (430 MB, 5.6
-// TB/s), gradients 147 us (676 MB, 4.6 TB/s) with the next row's operands under way (190 us without) and 8 us for the sums over
-// the workgroups' rows.
+// Measured, 60 000 x 512 in bf16 beside an fp32 residual, post-norm, a gate for each token, a scale: forward 81 us (430 MB, 5.3
+// TB/s), gradients 167 us (676 MB, 4.1 TB/s; 147 at best) with the next row's operands under way (190 us without) and 9 us for the
+// sums over the workgroups' rows.
 #include "gdr_common.h"
 #include "row_sums.h"
 

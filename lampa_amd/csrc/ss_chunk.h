@@ -12,10 +12,11 @@
 // two or three operands of the input type each, value and remainders (ScParts): the state is handed from chunk to chunk and out
 // to the caller in fp32, and its sums are what the gradient of the decays is made of.
 //
-// Measured, 60 000 tokens x 8 heads of 64 in bf16, one group of B and C. N = 64, forward: local states 32 us, join 15, outputs 64 (137
+// Measured, 60 000 tokens x 8 heads of 64 in bf16, one group of B and C. N = 64, forward: local states 29 us, join 11, outputs 62 (137
 // MB; 600 vector instructions a wave and chunk keep the vector units two thirds busy, the matrix cores a sixth). N = 128 with
-// gradients: local states 62, join 33 both ways, outputs 115, kept states and local adjoints 163 (of them 246 MB of kept
-// states written), gradients 350, sums of dB and dC over the heads 125 (490 MB, 3.9 TB/s).
+// gradients: local states 56, join 11 and 13 from the end, outputs 105, kept states and local adjoints 153 (of them 246 MB of kept
+// states written), gradients 330, sums of dB and dC over the heads 125 (490 MB, 3.9 TB/s). fp16, whose operands are scaled: 134 us
+// forward at N = 64 where bf16 takes 116 (with the host), 531 against 497 with gradients.
 #pragma once
 #include "ss_kernels.h"
 
