@@ -104,7 +104,8 @@ __device__ __forceinline__ void sc_map(const lampa_ss_args& a, const SsGrad& w, 
   if (!REV && threadIdx.x == 0 && pb == 0) a.slot_decay[(int64_t)blockIdx.x * a.H + h] = __builtin_amdgcn_exp2f(sum);
 }
 
-// Waves a SIMD that fit without spilling (element-by-element loads and fp16's scales take more registers).
+// Waves a SIMD that fit (element-by-element loads and fp16's scales take more registers; of all variants one, bf16 element by element
+// at N = 64 with three parts, spills two).
 template <typename T, int NP, bool VEC>
 constexpr int sc_map_waves() { return !VEC ? (NP <= 64 && __is_same(T, __bf16) ? 3 : 2) : NP <= 32 ? 5 : NP <= 64 ? 4 : (__is_same(T, __bf16) ? 3 : 2); }
 
