@@ -532,6 +532,57 @@ int lampa_residual_norm_bwd(const void* x, const void* residual, const float* we
                             float* dweight, float* dpost_weight, float* dscale, void* workspace, int64_t workspace_bytes,
                             void* stream);
 
+/* ------------------------------------------------------------------------------------------------ gated recurrence */
+
+/* The gated linear recurrence of one channel, and its gradients (models/baselines/full_mamba2.py:221-430 has the mixers it stands
+ * beside):  a = exp(A sigmoid(decay_gate)), u = [sqrt(1 - a^2)] sigmoid(input_gate) x, h_t = a_t h_{t-1} + u_t, y = act(gate) h.
+ * x, decay_gate, input_gate (NULL: factor 1), gate (NULL: y = h) of dtype, rows of D contiguous values `*_stride` elements
+ * apart; A fp32 [D] (at most 0); h0, ht fp32 [n_seq, D] or NULL; y, dy and the gradients dx .. dgate contiguous [n_tokens, D].
+ * Sequences: n_seq of seq_len tokens, or cu_seqlens [n_seq + 1] on the device (held inside the tokens and made monotone; rows behind
+ * the last boundary get zero). tile_states fp32 [lampa_lr_slots, D]: written by the forward where it is not NULL, read
+ * by the gradients. dA fp32 [D], dh0 fp32 [n_seq, D] (with h0). Workspace: lampa_lr_workspace_bytes for the pass in question,
+ * of a call's own while it runs. */
+typedef struct lampa_lr_args {
+  const void* x;
+  const void* decay_gate;
+  const void* input_gate;
+  const void* gate;
+  const float* A;
+  const float* h0;
+  void* y;
+  float* ht;
+  float* tile_states;
+  const int64_t* cu_seqlens;
+  const void* dy;
+  const float* dht; /* NULL: zero */
+  void* dx;
+  void* d_decay_gate;
+  void* d_input_gate;
+  void* d_gate;
+  float* dA;
+  float* dh0;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t n_tokens;
+  int64_t seq_len;
+  int64_t x_stride, decay_stride, input_stride, gate_stride;
+  int32_t n_seq, D, dtype;
+  int32_t activation; /* of the gate: 0 none, 1 SiLU, 2 sigmoid */
+  int32_t normalize;  /* the factor sqrt(1 - a^2) */
+  int32_t reserved;
+} lampa_lr_args;
+
+int64_t lampa_lr_slots(const lampa_lr_args* args);
+int64_t lampa_lr_workspace_bytes(const lampa_lr_args* args, int backward);
+int lampa_lr_scan_fwd(const lampa_lr_args* args, void* stream);
+int lampa_lr_scan_bwd(const lampa_lr_args* args, void* stream);
+
+/* One token for each of n sequences: x, gates [n, D] (row strides in elements), state fp32 [n, D] read, new_state written (may be
+ * the same pointer: in place), y [n, D]. */
+int lampa_lr_step(const void* x, int64_t x_stride, const void* decay_gate, int64_t decay_stride, const void* input_gate,
+                  int64_t input_stride, const void* gate, int64_t gate_stride, const float* A, const float* state, float* new_state,
+                  void* y, int64_t n, int D, int dtype, int activation, int normalize, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

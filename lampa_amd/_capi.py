@@ -98,6 +98,11 @@ _SIGNATURES = {
     "lampa_ss_bwd_workspace_bytes": (_i64, [_vp]),
     "lampa_ss_scan_bwd": (_i32, [_vp, _vp]),
     "lampa_ss_step": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64] + [_vp] * 6 + [_i32] * 8 + [_vp]),
+    "lampa_lr_slots": (_i64, [_vp]),
+    "lampa_lr_workspace_bytes": (_i64, [_vp, _i32]),
+    "lampa_lr_scan_fwd": (_i32, [_vp, _vp]),
+    "lampa_lr_scan_bwd": (_i32, [_vp, _vp]),
+    "lampa_lr_step": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp]),
     "lampa_causal_conv1d_state_fwd": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp,
                                              _vp]),
     "lampa_causal_conv1d_step": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _i32, _i32, _vp]),
