@@ -583,6 +583,35 @@ int lampa_lr_step(const void* x, int64_t x_stride, const void* decay_gate, int64
                   int64_t input_stride, const void* gate, int64_t gate_stride, const float* A, const float* state, float* new_state,
                   void* y, int64_t n, int D, int dtype, int activation, int normalize, void* stream);
 
+/* -------------------------------------------------------------------------------------------- gated feed-forward block */
+
+/* y = (act(x Wg^T) * (x Wu^T)) Wd^T and its gradients (GatedMLP, models/hattention/modeling_gated_deltaproduct.py:310-324).
+ * x [rows, D] of dtype with row stride x_stride; w_gate, w_up [F, D], w_down [D, F], y, dy, dx [rows, D] and the weights'
+ * gradients (the weights' shapes and type) contiguous. dx and any of the weights' gradients may be NULL: not wanted. D and F multiples of 8,
+ * everything 16-byte aligned. activation 0 none, 1 SiLU, 2 sigmoid. Workspace: lampa_ff_workspace_bytes for the pass in
+ * question (and the gradients asked for), of a call's own while it runs. */
+typedef struct lampa_ff_args {
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* w_down;
+  void* y;
+  const void* dy;
+  void* dx;
+  void* dw_gate;
+  void* dw_up;
+  void* dw_down;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t rows;
+  int64_t x_stride;
+  int32_t D, F, dtype, activation;
+} lampa_ff_args;
+
+int64_t lampa_ff_workspace_bytes(const lampa_ff_args* args, int backward);
+int lampa_ff_fwd(const lampa_ff_args* args, void* stream);
+int lampa_ff_bwd(const lampa_ff_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

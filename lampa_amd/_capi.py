@@ -103,6 +103,9 @@ _SIGNATURES = {
     "lampa_lr_scan_fwd": (_i32, [_vp, _vp]),
     "lampa_lr_scan_bwd": (_i32, [_vp, _vp]),
     "lampa_lr_step": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp]),
+    "lampa_ff_workspace_bytes": (_i64, [_vp, _i32]),
+    "lampa_ff_fwd": (_i32, [_vp, _vp]),
+    "lampa_ff_bwd": (_i32, [_vp, _vp]),
     "lampa_causal_conv1d_state_fwd": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp,
                                              _vp]),
     "lampa_causal_conv1d_step": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _i32, _i32, _vp]),

@@ -1,0 +1,53 @@
+// Shared by the kernels of the gated feed-forward block (gfx950).
+//   forward:    G = x Wg^T,  U = x Wu^T,  S = act(G) * U,  y = S Wd^T
+//   gradients:  dS = dy Wd,  dG = dS * U * act'(G),  dU = dS * act(G),
+//               dx = dG Wg + dU Wu,  dWg = dG^T x,  dWu = dU^T x,  dWd = dy^T S.
+// Products run on the matrix cores with fp32 sums (16-bit inputs on the 16-bit instructions, fp32 inputs on the fp32 ones).
+// S, dG and dU are operands of further products: for 16-bit inputs they are rounded to the input type once (half a step of each, which
+// the outputs' own rounding equals), act and act' are taken from the unrounded fp32 sums in both passes.
+#pragma once
+#include "../../include/lampa_amd.h"
+#include "gdr_ops.h"
+
+enum { FF_ACT_NONE = 0, FF_ACT_SILU = 1, FF_ACT_SIGMOID = 2 };
+#define FF_OFF 0x80000000u  // byte offset past the end of every buffer
+
+__device__ __forceinline__ float ff_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+template <int ACT>
+__device__ __forceinline__ float ff_act(float g) {
+  if constexpr (ACT == FF_ACT_NONE) return g;
+  const float s = ff_sigmoid(g);
+  return ACT == FF_ACT_SILU ? g * s : s;
+}
+// (act(g), act'(g))
+template <int ACT>
+__device__ __forceinline__ void ff_act_slope(float g, float& value, float& slope) {
+  if constexpr (ACT == FF_ACT_NONE) {
+    value = g;
+    slope = 1.0f;
+  } else {
+    const float s = ff_sigmoid(g);
+    value = ACT == FF_ACT_SILU ? g * s : s;
+    slope = ACT == FF_ACT_SILU ? __builtin_fmaf(value, 1.0f - s, s) : s * (1.0f - s);
+  }
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t ff_buffer(const void* base, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes > 0 ? (unsigned)bytes : 0u, 0x00020000);
+}
+typedef unsigned ff_u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ ff_u32x4 ff_load16(__amdgpu_buffer_rsrc_t buf, unsigned offset) {
+  return __builtin_bit_cast(ff_u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, offset, 0, 0));
+}
+
+// Four consecutive values, rounded to T.
+template <typename T>
+__device__ __forceinline__ void ff_store4(T* p, float a, float b, float c, float d) {
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<vec4*>(p) = vec4{GdrElem<T>::from_float(a), GdrElem<T>::from_float(b), GdrElem<T>::from_float(c), GdrElem<T>::from_float(d)};
+}
+
+// The general form (ff_gemm.hip): hidden values through memory.
+int64_t ff_gemm_workspace(const lampa_ff_args* a, int backward);
+int ff_gemm_fwd(const lampa_ff_args* a, hipStream_t s);
+int ff_gemm_bwd(const lampa_ff_args* a, hipStream_t s);

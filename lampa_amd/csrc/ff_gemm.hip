@@ -1,0 +1,473 @@
+// The gated feed-forward block for any width: tiled matrix products whose epilogues hold what is elementwise (ff_common.h has the
+// mathematics). Hidden values go through memory between the products.
+//   hidden:  S from x, Wg and Wu in one kernel (both products share x's tiles);
+//   grads:   G, U from x and dS from dy and Wd^T in one kernel, which leaves S, dG and dU;
+//   product: y = S Wd^T; dx = dG Wg + dU Wu as one sum over both (on transposed weights: all operands then lie along their
+//            contraction);
+//   weights: dWg, dWu, dWd over the rows, split over the rows where that fills the GPU, the parts summed in a fixed order.
+// A workgroup has 4 waves in 2 x 2 over a tile of 128 x 128 of the output (64 hidden columns of each product for `hidden` and
+// `grads`), tiles of 128 bytes of the contraction in LDS, double buffered, the next one under way in registers. Rows of 128 bytes
+// are stored with their 16-byte pieces permuted by the row (piece ^ row % 8), so that the 32 rows of an operand read do not
+// meet in the same banks.
+#include "ff_common.h"
+
+#define MM_BLOCK 256
+#define MM_ROWS 128       // rows of a tile
+#define MM_ROW_BYTES 128  // of the contraction
+#define MM_TILE (MM_ROWS * MM_ROW_BYTES)
+
+template <typename T>
+__device__ __forceinline__ f32x16 mm_mac(ff_u32x4 a, ff_u32x4 b, f32x16 c) {
+  if constexpr (sizeof(T) == 2) {
+    return mfma32(__builtin_bit_cast(typename OpVec<T>::x8, a), __builtin_bit_cast(typename OpVec<T>::x8, b), c);
+  } else {  // 8 values of the contraction: lane half hh holds 4 hh .. + 3, step j pairs j and 4 + j
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+    return c;
+  }
+}
+
+// A tile's operand: 64 rows (or 128) of a row-major matrix, `step` elements apart.
+struct MmSide {
+  __amdgpu_buffer_rsrc_t buf;  // from the tile's first row to the end of its last one
+  unsigned step;               // bytes between rows
+};
+template <typename T>
+__device__ __forceinline__ MmSide mm_side(const T* base, int64_t first, int64_t rows, int64_t stride, int K) {
+  const int64_t left = rows - first;
+  const int64_t n = left < 0 ? 0 : (left < MM_ROWS ? left : MM_ROWS);
+  return {ff_buffer(base + (n ? first * stride : 0), n ? ((n - 1) * stride + K) * (int64_t)sizeof(T) : 0), (unsigned)(stride * sizeof(T))};
+}
+
+// acc[m][b] += (B rows b) . (A rows m) over K: register r of a lane is B row 8 (r / 4) + 4 hh + r % 4 of its block, A row = lane % 32.
+// The wave's A blocks are rows 64 wm and 64 wm + 32, its B blocks rows 32 wn and 64 + 32 wn (the second from b1).
+template <typename T, int NB>
+__device__ __forceinline__ void mm_phase(const MmSide& a, const MmSide& b0, const MmSide& b1, int K, unsigned char* lds,
+                                         f32x16 (&acc)[2][NB]) {
+  constexpr int BR = 64 * NB, BCH = BR * 8 / MM_BLOCK, EPC = 16 / sizeof(T), STAGE = MM_TILE + BR * MM_ROW_BYTES;
+  const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, hh = lane >> 5, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
+  const int steps = (K * (int)sizeof(T) + MM_ROW_BYTES - 1) / MM_ROW_BYTES;
+  ff_u32x4 ra[4], rb[BCH];
+  auto fetch = [&](int step) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int id = tid + i * MM_BLOCK, row = id >> 3, at = step * MM_ROW_BYTES + (id & 7) * 16;
+      ra[i] = ff_load16(a.buf, at < K * (int)sizeof(T) ? row * a.step + at : FF_OFF);
+    }
+#pragma unroll
+    for (int i = 0; i < BCH; ++i) {
+      const int id = tid + i * MM_BLOCK, row = id >> 3, at = step * MM_ROW_BYTES + (id & 7) * 16;
+      const unsigned off = at < K * (int)sizeof(T) ? (row & 63) * b0.step + at : FF_OFF;
+      rb[i] = ff_load16(i * MM_BLOCK / 8 >= 64 ? b1.buf : b0.buf, off);  // 32 rows a step of i
+    }
+  };
+  auto stage = [&](int which) {
+    unsigned char* p = lds + which * STAGE;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int id = tid + i * MM_BLOCK, row = id >> 3;
+      *reinterpret_cast<ff_u32x4*>(p + row * MM_ROW_BYTES + (((id & 7) ^ (row & 7)) * 16)) = ra[i];
+    }
+#pragma unroll
+    for (int i = 0; i < BCH; ++i) {
+      const int id = tid + i * MM_BLOCK, row = id >> 3;
+      *reinterpret_cast<ff_u32x4*>(p + MM_TILE + row * MM_ROW_BYTES + (((id & 7) ^ (row & 7)) * 16)) = rb[i];
+    }
+  };
+  fetch(0);
+  stage(0);
+  __syncthreads();
+  for (int step = 0; step < steps; ++step) {
+    if (step + 1 < steps) fetch(step + 1);
+    const unsigned char* p = lds + (step & 1) * STAGE;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      ff_u32x4 fa[2], fb[NB];
+      const int piece = ((ks * 2 + hh) ^ (ln & 7)) * 16;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) fa[m] = *reinterpret_cast<const ff_u32x4*>(p + (64 * wm + 32 * m + ln) * MM_ROW_BYTES + piece);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        fb[b] = *reinterpret_cast<const ff_u32x4*>(p + MM_TILE + (64 * b + 32 * wn + ln) * MM_ROW_BYTES + piece);
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[m][b] = mm_mac<T>(fb[b], fa[m], acc[m][b]);
+    }
+    if (step + 1 < steps) stage((step + 1) & 1);
+    __syncthreads();
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void mm_clear(f32x16 (&acc)[2][N]) {
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[m][b][r] = 0.0f;
+}
+
+// Tiles of the output, in columns first within strips of 8 row tiles: the strip's rows of x stay in L2 while the columns pass.
+__device__ __forceinline__ void mm_place(int64_t row_tiles, int col_tiles, int64_t& rt, int& ct) {
+  const int64_t per = 8 * (int64_t)col_tiles, strip = blockIdx.x / per, in = blockIdx.x % per;
+  const int64_t high = row_tiles - strip * 8 < 8 ? row_tiles - strip * 8 : 8;
+  rt = strip * 8 + in % high;
+  ct = (int)(in / high);
+}
+
+// ------------------------------------------------------------------------------------------------ S = act(x Wg^T) (x Wu^T)
+template <typename T, int ACT>
+__global__ void __launch_bounds__(MM_BLOCK) ff_hidden_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ wg,
+                                                             const T* __restrict__ wu, int64_t rows, int D, int F,
+                                                             T* __restrict__ hidden) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * 2 * MM_TILE];
+  int64_t rt;
+  int ct;
+  mm_place((rows + MM_ROWS - 1) / MM_ROWS, (F + 63) / 64, rt, ct);
+  const int64_t r0 = rt * MM_ROWS;
+  const int f0 = ct * 64;
+  f32x16 acc[2][2];
+  mm_clear(acc);
+  mm_phase<T, 2>(mm_side(x, r0, rows, x_stride, D), mm_side(wg, f0, F, D, D), mm_side(wu, f0, F, D, D), D, lds, acc);
+  const int lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const int64_t row = r0 + 64 * wm + 32 * m + ln;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int f = f0 + 32 * wn + 8 * q + 4 * hh;
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = ff_act<ACT>(acc[m][0][4 * q + k]) * acc[m][1][4 * q + k];
+      if (row < rows && f < F) ff_store4(hidden + row * F + f, v[0], v[1], v[2], v[3]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ S, dG, dU
+template <typename T, int ACT>
+__global__ void __launch_bounds__(MM_BLOCK) ff_grads_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ dy,
+                                                            const T* __restrict__ wg, const T* __restrict__ wu,
+                                                            const T* __restrict__ wd_t, int64_t rows, int D, int F,
+                                                            T* __restrict__ hidden, T* __restrict__ dg, T* __restrict__ du) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * 2 * MM_TILE];
+  int64_t rt;
+  int ct;
+  mm_place((rows + MM_ROWS - 1) / MM_ROWS, (F + 63) / 64, rt, ct);
+  const int64_t r0 = rt * MM_ROWS;
+  const int f0 = ct * 64;
+  f32x16 acc[2][2], ds[2][1];
+  mm_clear(acc);
+  mm_clear(ds);
+  mm_phase<T, 2>(mm_side(x, r0, rows, x_stride, D), mm_side(wg, f0, F, D, D), mm_side(wu, f0, F, D, D), D, lds, acc);
+  const MmSide wd = mm_side(wd_t, f0, F, D, D);
+  mm_phase<T, 1>(mm_side(dy, r0, rows, D, D), wd, wd, D, lds, ds);
+  const int lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const int64_t row = r0 + 64 * wm + 32 * m + ln;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int f = f0 + 32 * wn + 8 * q + 4 * hh;
+      float v[4], g[4], u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float value, slope;
+        ff_act_slope<ACT>(acc[m][0][4 * q + k], value, slope);
+        const float up = acc[m][1][4 * q + k], d = ds[m][0][4 * q + k];
+        v[k] = value * up;
+        g[k] = d * up * slope;
+        u[k] = d * value;
+      }
+      if (row < rows && f < F) {
+        if (hidden) ff_store4(hidden + row * F + f, v[0], v[1], v[2], v[3]);
+        ff_store4(dg + row * F + f, g[0], g[1], g[2], g[3]);
+        ff_store4(du + row * F + f, u[0], u[1], u[2], u[3]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ out = A0 B0^T (+ A1 B1^T)
+template <typename T>
+__global__ void __launch_bounds__(MM_BLOCK) ff_product_kernel(const T* __restrict__ a0, const T* __restrict__ b0, const T* __restrict__ a1,
+                                                              const T* __restrict__ b1, int64_t rows, int N, int K,
+                                                              T* __restrict__ out) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * 2 * MM_TILE];
+  int64_t rt;
+  int ct;
+  mm_place((rows + MM_ROWS - 1) / MM_ROWS, (N + 127) / 128, rt, ct);
+  const int64_t r0 = rt * MM_ROWS;
+  const int n0 = ct * 128;
+  f32x16 acc[2][2];
+  mm_clear(acc);
+  for (int p = 0; p < (a1 ? 2 : 1); ++p) {
+    const T* b = p ? b1 : b0;
+    mm_phase<T, 2>(mm_side(p ? a1 : a0, r0, rows, K, K), mm_side(b, n0, N, K, K), mm_side(b, n0 + 64, N, K, K), K, lds, acc);
+  }
+  const int lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const int64_t row = r0 + 64 * wm + 32 * m + ln;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = n0 + 64 * b + 32 * wn + 8 * q + 4 * hh;
+        if (row < rows && n < N)
+          ff_store4(out + row * N + n, acc[m][b][4 * q], acc[m][b][4 * q + 1], acc[m][b][4 * q + 2], acc[m][b][4 * q + 3]);
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ weights' gradients
+// Up to three products C[M, N] = sum over rows t of A[t, m] B[t, n], one behind the other in the grid; part `split` of a product goes
+// over rows [split * per, ..) and leaves its sums in parts + split * part_step + at.
+struct FfWeightJob {
+  const void *A, *B;
+  int64_t a_stride, b_stride, at;
+  int M, N, tiles;  // tiles of 128 x 128
+};
+struct FfWeightJobs {
+  FfWeightJob job[3];
+  int n, splits;
+  int64_t rows, per, part_step;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(MM_BLOCK) ff_weights_kernel(const FfWeightJobs jobs, float* __restrict__ parts) {
+  constexpr int BK = 128 / sizeof(T);              // rows of a step
+  constexpr int STRIDE = sizeof(T) == 2 ? 144 : 132;  // elements between a tile's rows: four rows of 32 bytes side by side fill 128
+  constexpr int EPC = 16 / sizeof(T), CPR = 128 / EPC, CH = BK * CPR / MM_BLOCK;
+  __shared__ __attribute__((aligned(16))) T lds[2][2][BK * STRIDE];
+  int tile = blockIdx.x, j = 0;
+  while (j + 1 < jobs.n && tile >= jobs.job[j].tiles) tile -= jobs.job[j++].tiles;
+  const FfWeightJob& job = jobs.job[j];
+  const int ntiles = (job.N + 127) / 128, m0 = tile / ntiles * 128, n0 = tile % ntiles * 128;
+  const int64_t begin = (int64_t)blockIdx.y * jobs.per, end = begin + jobs.per < jobs.rows ? begin + jobs.per : jobs.rows;
+  const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, hh = lane >> 5, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
+  f32x16 acc[2][2];
+  mm_clear(acc);
+  ff_u32x4 ra[CH], rb[CH];
+  auto fetch = [&](int64_t t0) {
+    const int64_t n = end - t0 < BK ? end - t0 : BK;
+    const __amdgpu_buffer_rsrc_t ab = ff_buffer((const T*)job.A + t0 * job.a_stride + m0, ((n - 1) * job.a_stride + job.M - m0) * (int64_t)sizeof(T));
+    const __amdgpu_buffer_rsrc_t bb = ff_buffer((const T*)job.B + t0 * job.b_stride + n0, ((n - 1) * job.b_stride + job.N - n0) * (int64_t)sizeof(T));
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int id = tid + i * MM_BLOCK, row = id / CPR, c = id % CPR * EPC;
+      ra[i] = ff_load16(ab, m0 + c < job.M ? (unsigned)((row * job.a_stride + c) * sizeof(T)) : FF_OFF);
+      rb[i] = ff_load16(bb, n0 + c < job.N ? (unsigned)((row * job.b_stride + c) * sizeof(T)) : FF_OFF);
+    }
+  };
+  auto stage = [&](int which) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int id = tid + i * MM_BLOCK, row = id / CPR, c = id % CPR * EPC;
+      *reinterpret_cast<ff_u32x4*>(&lds[which][0][row * STRIDE + c]) = ra[i];
+      *reinterpret_cast<ff_u32x4*>(&lds[which][1][row * STRIDE + c]) = rb[i];
+    }
+  };
+  auto operand = [&](const T* arr, int col0, int row0) -> ff_u32x4 {
+    if constexpr (sizeof(T) == 2) {
+      return __builtin_bit_cast(ff_u32x4, op_ld_kappa_tr<T>(arr, STRIDE, col0, row0, lane));
+    } else {
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = arr[(row0 + 4 * hh + e) * STRIDE + col0 + ln];
+      return __builtin_bit_cast(ff_u32x4, v);
+    }
+  };
+  if (begin < end) {
+    fetch(begin);
+    stage(0);
+    __syncthreads();
+    int which = 0;
+    for (int64_t t0 = begin; t0 < end; t0 += BK, which ^= 1) {
+      const bool more = t0 + BK < end;
+      if (more) fetch(t0 + BK);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const int row0 = ks * BK / 4;
+        ff_u32x4 fa[2], fb[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          fa[k] = operand(lds[which][0], 64 * wm + 32 * k, row0);
+          fb[k] = operand(lds[which][1], 64 * wn + 32 * k, row0);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) acc[m][b] = mm_mac<T>(fb[b], fa[m], acc[m][b]);
+      }
+      if (more) stage(which ^ 1);
+      __syncthreads();
+    }
+  }
+  float* out = parts + blockIdx.y * jobs.part_step + job.at;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const int row = m0 + 64 * wm + 32 * m + ln;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = n0 + 64 * wn + 32 * b + 8 * q + 4 * hh;
+        if (row < job.M && n < job.N)
+          *reinterpret_cast<f32x4*>(out + (int64_t)row * job.N + n) =
+              f32x4{acc[m][b][4 * q], acc[m][b][4 * q + 1], acc[m][b][4 * q + 2], acc[m][b][4 * q + 3]};
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ small kernels
+template <typename T>
+__global__ void __launch_bounds__(256) ff_reduce_kernel(const float* __restrict__ rows, int n, int64_t cols, int64_t step, T* __restrict__ out) {
+  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (c >= cols) return;
+  f32x4 sum = *reinterpret_cast<const f32x4*>(rows + c);
+  for (int r = 1; r < n; ++r) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(rows + r * step + c);
+    sum += v;
+  }
+  ff_store4(out + c, sum[0], sum[1], sum[2], sum[3]);
+}
+
+// out [cols, rows] = in [rows, cols]^T in tiles of 32 x 32; three matrices side by side in the grid's third dimension.
+struct FfTurns {
+  const void* in[3];
+  void* out[3];
+  int rows[3], cols[3];
+};
+template <typename T>
+__global__ void __launch_bounds__(256) ff_turn_kernel(const FfTurns t) {
+  __shared__ T tile[32][33];
+  const int z = blockIdx.z, rows = t.rows[z], cols = t.cols[z], r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
+  if (r0 >= rows || c0 >= cols) return;
+  const T* in = (const T*)t.in[z];
+  T* out = (T*)t.out[z];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+#pragma unroll
+  for (int k = 0; k < 32; k += 8)
+    if (r0 + y + k < rows && c0 + x < cols) tile[y + k][x] = in[(int64_t)(r0 + y + k) * cols + c0 + x];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 32; k += 8)
+    if (c0 + y + k < cols && r0 + x < rows) out[(int64_t)(c0 + y + k) * rows + r0 + x] = tile[x][y + k];
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static int64_t ff_size(const lampa_ff_args* a) { return a->dtype == GDR_FP32 ? 4 : 2; }
+static int64_t ff_area(int64_t n, int64_t elem) { return lampa_align_up(n * elem, 256); }
+
+// Parts of the weights' gradients: as many as make about four workgroups a CU, of 256 rows or more each.
+static int ff_splits(const lampa_ff_args* a) {
+  const int64_t tiles = ((a->F + 127) / 128) * (int64_t)((a->D + 127) / 128) * ((a->dw_gate != nullptr) + (a->dw_up != nullptr) + (a->dw_down != nullptr));
+  const int64_t want = tiles ? (512 + tiles - 1) / tiles : 1, most = (a->rows + 255) / 256;
+  const int64_t n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n);
+}
+
+struct FfAreas {
+  int64_t hidden, dg, du, turned, parts, total;  // turned: Wd^T, Wg^T, Wu^T one behind the other
+};
+static FfAreas ff_areas(const lampa_ff_args* a, int backward) {
+  const int64_t e = ff_size(a), h = ff_area(a->rows * a->F, e), w = ff_area((int64_t)a->D * a->F, e);
+  FfAreas l{};
+  l.hidden = 0;
+  l.dg = h;
+  l.du = l.dg + (backward ? h : 0);
+  l.turned = l.du + (backward ? h : 0);
+  l.parts = l.turned + (backward ? 3 * w : 0);
+  l.total = l.parts + (backward ? ff_area((int64_t)ff_splits(a) * 3 * a->D * a->F, 4) : 0);
+  return l;
+}
+int64_t ff_gemm_workspace(const lampa_ff_args* a, int backward) { return ff_areas(a, backward).total; }
+
+static unsigned ff_tiles(int64_t rows, int cols, int wide) {
+  return (unsigned)((rows + MM_ROWS - 1) / MM_ROWS * ((cols + wide - 1) / wide));
+}
+
+template <typename T, int ACT>
+static int ff_fwd_go(const lampa_ff_args* a, hipStream_t s) {
+  T* hidden = (T*)a->workspace;
+  LAMPA_PROF(s, "start");
+  hipLaunchKernelGGL((ff_hidden_kernel<T, ACT>), dim3(ff_tiles(a->rows, a->F, 64)), dim3(MM_BLOCK), 0, s, (const T*)a->x, a->x_stride,
+                     (const T*)a->w_gate, (const T*)a->w_up, a->rows, a->D, a->F, hidden);
+  LAMPA_PROF(s, "ff_hidden_kernel");
+  hipLaunchKernelGGL((ff_product_kernel<T>), dim3(ff_tiles(a->rows, a->D, 128)), dim3(MM_BLOCK), 0, s, (const T*)hidden,
+                     (const T*)a->w_down, (const T*)nullptr, (const T*)nullptr, a->rows, a->D, a->F, (T*)a->y);
+  LAMPA_PROF(s, "ff_product_kernel");
+  return lampa_launch_status();
+}
+
+template <typename T, int ACT>
+static int ff_bwd_go(const lampa_ff_args* a, hipStream_t s) {
+  const FfAreas l = ff_areas(a, 1);
+  char* ws = (char*)a->workspace;
+  const int64_t w = ff_area((int64_t)a->D * a->F, sizeof(T));
+  T *hidden = (T*)(ws + l.hidden), *dg = (T*)(ws + l.dg), *du = (T*)(ws + l.du);
+  T *wd_t = (T*)(ws + l.turned), *wg_t = (T*)(ws + l.turned + w), *wu_t = (T*)(ws + l.turned + 2 * w);
+  float* parts = (float*)(ws + l.parts);
+  const bool weights = a->dw_gate || a->dw_up || a->dw_down;
+  LAMPA_PROF(s, "start");
+  const FfTurns turns{{a->w_down, a->w_gate, a->w_up}, {wd_t, wg_t, wu_t}, {a->D, a->F, a->F}, {a->F, a->D, a->D}};
+  const int most = a->D > a->F ? a->D : a->F;
+  hipLaunchKernelGGL((ff_turn_kernel<T>), dim3((most + 31) / 32, (most + 31) / 32, a->dx ? 3 : 1), dim3(256), 0, s, turns);
+  LAMPA_PROF(s, "ff_turn_kernel");
+  hipLaunchKernelGGL((ff_grads_kernel<T, ACT>), dim3(ff_tiles(a->rows, a->F, 64)), dim3(MM_BLOCK), 0, s, (const T*)a->x, a->x_stride,
+                     (const T*)a->dy, (const T*)a->w_gate, (const T*)a->w_up, (const T*)wd_t, a->rows, a->D, a->F,
+                     a->dw_down ? hidden : (T*)nullptr, dg, du);
+  LAMPA_PROF(s, "ff_grads_kernel");
+  if (a->dx) {
+    hipLaunchKernelGGL((ff_product_kernel<T>), dim3(ff_tiles(a->rows, a->D, 128)), dim3(MM_BLOCK), 0, s, (const T*)dg, (const T*)wg_t,
+                       (const T*)du, (const T*)wu_t, a->rows, a->D, a->F, (T*)a->dx);
+    LAMPA_PROF(s, "ff_product_kernel");
+  }
+  if (weights) {
+    FfWeightJobs jobs{};
+    jobs.splits = ff_splits(a);
+    jobs.rows = a->rows;
+    jobs.per = lampa_align_up((a->rows + jobs.splits - 1) / jobs.splits, 64);
+    const int64_t size = (int64_t)a->D * a->F;
+    T* outs[3];
+    int tiles = 0;
+    auto add = [&](void* out, const void* A, int64_t as, const void* B, int64_t bs, int M, int N) {
+      if (!out) return;
+      FfWeightJob& j = jobs.job[jobs.n];
+      j = FfWeightJob{A, B, as, bs, jobs.n * size, M, N, (M + 127) / 128 * ((N + 127) / 128)};
+      tiles += j.tiles;
+      outs[jobs.n++] = (T*)out;
+    };
+    add(a->dw_gate, dg, a->F, a->x, a->x_stride, a->F, a->D);
+    add(a->dw_up, du, a->F, a->x, a->x_stride, a->F, a->D);
+    add(a->dw_down, a->dy, a->D, hidden, a->F, a->D, a->F);
+    jobs.part_step = jobs.n * size;
+    hipLaunchKernelGGL((ff_weights_kernel<T>), dim3((unsigned)tiles, (unsigned)jobs.splits), dim3(MM_BLOCK), 0, s, jobs, parts);
+    LAMPA_PROF(s, "ff_weights_kernel");
+    for (int j = 0; j < jobs.n; ++j) {
+      hipLaunchKernelGGL((ff_reduce_kernel<T>), dim3((unsigned)((size / 4 + 255) / 256)), dim3(256), 0, s, parts + jobs.job[j].at,
+                         jobs.splits, size, jobs.part_step, outs[j]);
+      LAMPA_PROF(s, "ff_reduce_kernel");
+    }
+  }
+  return lampa_launch_status();
+}
+
+#define FF_TYPES(GO)                                                                                               \
+  switch (a->dtype * 3 + a->activation) {                                                                          \
+    case 0: return GO<__bf16, 0>(a, s);                                                                            \
+    case 1: return GO<__bf16, 1>(a, s);                                                                            \
+    case 2: return GO<__bf16, 2>(a, s);                                                                            \
+    case 3: return GO<_Float16, 0>(a, s);                                                                          \
+    case 4: return GO<_Float16, 1>(a, s);                                                                          \
+    case 5: return GO<_Float16, 2>(a, s);                                                                          \
+    case 6: return GO<float, 0>(a, s);                                                                             \
+    case 7: return GO<float, 1>(a, s);                                                                             \
+    default: return GO<float, 2>(a, s);                                                                            \
+  }
+int ff_gemm_fwd(const lampa_ff_args* a, hipStream_t s) { FF_TYPES(ff_fwd_go) }
+int ff_gemm_bwd(const lampa_ff_args* a, hipStream_t s) { FF_TYPES(ff_bwd_go) }
