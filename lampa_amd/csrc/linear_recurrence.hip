@@ -16,6 +16,8 @@
 #include "gdr_common.h"
 #include "row_sums.h"
 
+#pragma clang fp contract(off)  // fused only where it is written: the kernels for one and two channels a lane give the same bits
+
 #define LR_FWD_BLOCK 256
 #define LR_TOK 16    // tokens of a forward run
 #define LR_BWD_BLOCK 512
@@ -184,10 +186,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t lr_buffer(const void* base, in
 
 __device__ __forceinline__ float lr_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
-// a and, of log a = l, m = sqrt(1 - a^2): near a = 1 the difference would lose its digits, so 1 - exp(-t), t = -2 l, is summed as its
-// series there (8 terms: t^8 / 9! = 1e-8 of it at t = 1/2).
-__device__ __forceinline__ float lr_unit(float l, float a) {
-  const float t = -2.0f * l;
+// a = exp(l) and k = 1 - a, near a = 1 without loss: there k is the sum of its series in t = -l (8 terms: t^8 / 9! = 1e-8 of it at
+// t = 1/2) and a = 1 - k is off by its own rounding alone. (The exponential instruction's error, up to a step of a and not
+// the same in both directions, adds up over the thousands of tokens that such a channel remembers: 7e-6 of dA at 6 007 tokens.)
+// `small`, the same in the whole wave: |l| is below 1/2 whatever the gates hold.
+__device__ __forceinline__ void lr_decay(float l, bool small, float& a, float& k) {
+  const float t = -l;
   float p = __builtin_fmaf(t, -1.0f / 8.0f, 1.0f);
   p = __builtin_fmaf(t * (-1.0f / 7.0f), p, 1.0f);
   p = __builtin_fmaf(t * (-1.0f / 6.0f), p, 1.0f);
@@ -195,8 +199,15 @@ __device__ __forceinline__ float lr_unit(float l, float a) {
   p = __builtin_fmaf(t * (-1.0f / 4.0f), p, 1.0f);
   p = __builtin_fmaf(t * (-1.0f / 3.0f), p, 1.0f);
   p = __builtin_fmaf(t * (-1.0f / 2.0f), p, 1.0f);
-  return __builtin_amdgcn_sqrtf(t < 0.5f ? t * p : __builtin_fmaf(-a, a, 1.0f));
+  k = t * p;
+  a = 1.0f - k;
+  if (!small && !(__builtin_fabsf(t) < 0.5f)) {
+    a = __expf(l);
+    k = 1.0f - a;
+  }
 }
+// sqrt(1 - a^2) of a and 1 - a.
+__device__ __forceinline__ float lr_unit(float a, float k) { return __builtin_amdgcn_sqrtf(k * (1.0f + a)); }
 __device__ __forceinline__ float lr_act(float z, int act) {
   if (act == LR_ACT_NONE) return z;
   const float s = lr_sigmoid(z);
@@ -392,13 +403,15 @@ __global__ void __launch_bounds__(LR_FWD_BLOCK) lr_fwd_kernel(const LrArgs a) {
   }
   const int64_t left = s.t1 - s.t0 - row;
   const int n = left < 0 ? 0 : (left < LR_TOK ? (int)left : LR_TOK);  // tokens of this run
-  float A[V], P[V], H[V], av[LR_TOK][V], uv[LR_TOK][V];
+  float A[V], P[V], H[V], L[V], av[LR_TOK][V], uv[LR_TOK][V];
+  bool small = true;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     A[v] = on ? a.A[c + v] : 0.0f;
-    P[v] = 1.0f;
-    H[v] = 0.0f;
+    small = small && __builtin_fabsf(A[v]) < 0.5f;
+    H[v] = L[v] = 0.0f;
   }
+  small = __all(small);
 #pragma unroll
   for (int j = 0; j < LR_TOK; ++j) {
     float rv[V], xv[V], iv[V];
@@ -407,16 +420,22 @@ __global__ void __launch_bounds__(LR_FWD_BLOCK) lr_fwd_kernel(const LrArgs a) {
     if constexpr (HASI) lr_widen<T, V>(ri[j], iv);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float l = A[v] * lr_sigmoid(rv[v]);
-      float d = __expf(l), u = xv[v];
+      float l = A[v] * lr_sigmoid(rv[v]), d, k, u = xv[v];
+      lr_decay(l, small, d, k);
       if constexpr (HASI) u *= lr_sigmoid(iv[v]);
-      if (a.normalize) u *= lr_unit(l, d);
-      if (j >= n) { d = 1.0f; u = 0.0f; }
+      if (a.normalize) u *= lr_unit(d, k);
+      if (j >= n) { l = 0.0f; d = 1.0f; u = 0.0f; }
       av[j][v] = d;
       uv[j][v] = u;
-      P[v] *= d;
+      L[v] += l;
       H[v] = __builtin_fmaf(d, H[v], u);
     }
+  }
+  // from the sum of the exponents: a product of 16 rounded factors would be off by 16 roundings, tile after tile
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float k;
+    lr_decay(L[v], false, P[v], k);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) maps[threadIdx.x][v] = float2{P[v], H[v]};
@@ -537,15 +556,17 @@ __global__ void __launch_bounds__(LR_BWD_BLOCK) lr_bwd_kernel(const LrArgs a) {
   }
   const int64_t left = s.t1 - s.t0 - row;
   const int n = left < 0 ? 0 : (left < TOK ? (int)left : TOK);
-  float A[V], h[V], P[V], H[V], C[V], av[TOK][V], dv[TOK][V], hv[TOK + 1][V];
+  float A[V], h[V], P[V], L[V], H[V], C[V], av[TOK][V], dv[TOK][V], hv[TOK + 1][V];
+  bool small = true;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     A[v] = on ? a.A[c + v] : 0.0f;
+    small = small && __builtin_fabsf(A[v]) < 0.5f;
     h[v] = on ? a.tile_states[slot * a.D + c + v] : 0.0f;
-    P[v] = 1.0f;
-    H[v] = C[v] = 0.0f;
+    L[v] = H[v] = C[v] = 0.0f;
     hv[0][v] = 0.0f;
   }
+  small = __all(small);
 #pragma unroll
   for (int j = 0; j < TOK; ++j) {
     float rv[V], xv[V], iv[V], zv[V], dy[V];
@@ -556,18 +577,23 @@ __global__ void __launch_bounds__(LR_BWD_BLOCK) lr_bwd_kernel(const LrArgs a) {
     if constexpr (HASZ) lr_widen<T, V>(rz[j], zv);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float l = A[v] * lr_sigmoid(rv[v]);
-      float d = __expf(l), u = xv[v];
+      float l = A[v] * lr_sigmoid(rv[v]), d, k, u = xv[v];
+      lr_decay(l, small, d, k);
       if constexpr (HASI) u *= lr_sigmoid(iv[v]);
-      if (a.normalize) u *= lr_unit(l, d);
-      if (j >= n) { d = 1.0f; u = 0.0f; }
+      if (a.normalize) u *= lr_unit(d, k);
+      if (j >= n) { l = 0.0f; d = 1.0f; u = 0.0f; }
       av[j][v] = d;
       dv[j][v] = dy[v];
       if constexpr (HASZ) dv[j][v] *= lr_act(zv[v], a.act);
       H[v] = __builtin_fmaf(d, H[v], u);
       hv[j + 1][v] = H[v];  // from a state of zero
-      P[v] *= d;
+      L[v] += l;
     }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float k;
+    lr_decay(L[v], false, P[v], k);
   }
 #pragma unroll
   for (int j = TOK - 1; j >= 0; --j) {
@@ -645,7 +671,9 @@ __global__ void __launch_bounds__(LR_BWD_BLOCK) lr_bwd_kernel(const LrArgs a) {
       const float G = dv[j][v] + g[v];
       float into = si, dl = d * hv[j][v];  // d h / d x, d h / d log a
       if (a.normalize) {
-        const float m = lr_unit(l, d);
+        float same, k;
+        lr_decay(l, small, same, k);
+        const float m = lr_unit(d, k);
         into *= m;
         // a token that keeps all (m = 0) has no slope through m
         dl = __builtin_fmaf(-si * xv[v], m == 0.0f ? 0.0f : d * d * __builtin_amdgcn_rcpf(m), dl);
@@ -700,10 +728,10 @@ __global__ void __launch_bounds__(256) lr_step_kernel(const T* __restrict__ x, i
   const int c = (int)(at % D);
   const float xv = GdrElem<T>::to_float(x[b * xs + c]), rv = GdrElem<T>::to_float(r[b * rs + c]);
   const float iv = gi ? GdrElem<T>::to_float(gi[b * is + c]) : 0.0f, zv = z ? GdrElem<T>::to_float(z[b * zs + c]) : 0.0f;
-  const float l = A[c] * lr_sigmoid(rv), d = __expf(l);
-  float u = xv;
+  float d, k, u = xv;
+  lr_decay(A[c] * lr_sigmoid(rv), false, d, k);
   if (gi) u *= lr_sigmoid(iv);
-  if (normalize) u *= lr_unit(l, d);
+  if (normalize) u *= lr_unit(d, k);
   const float h = __builtin_fmaf(d, state[at], u);
   new_state[at] = h;
   y[at] = GdrElem<T>::from_float(z ? h * lr_act(zv, act) : h);
