@@ -7,8 +7,10 @@
 // Bound by bytes: every input is read once and every output written once, in one pass. A workgroup takes a tile of tokens of
 // one sequence x 2 LR channels: LR lanes side by side over channels, 256 / LR runs of LR_TOK tokens one after the other. A run's
 // effect on the state is the map h -> P h + H with P = prod a; the runs' maps are joined in LDS, and the tile's map is left for the
-// tiles behind it. Tiles of LR_GROUP form a group: a tile composes the maps of its group before it and starts from the state
-// that the group before left, always in this order, so repeated calls give the same bits. Maps and states are words that
+// tiles behind it. LR_GROUP tiles form a group, whose last tile leaves the group's map as soon as it has the others'; LR_GROUP
+// groups form a block, whose last tile leaves the state. A tile starts from the state before its block under the maps of the
+// block's groups before its own and of its group's tiles before it: two steps behind the slowest of them, where a chain of
+// states would cost a step a tile. The order is always this one, so repeated calls give the same bits. Maps and states are words that
 // are written whole and hold a pattern no result has until then, so the value is its own flag and no fence is needed.
 // Tiles are handed out by a counter, in the order in which they wait for each other: a tile waits only for tiles that were
 // handed out before it, so every wait ends.
@@ -16,13 +18,15 @@
 #include "gdr_common.h"
 #include "row_sums.h"
 
+#include <type_traits>
+
 #pragma clang fp contract(off)  // fused only where it is written: the kernels for one and two channels a lane give the same bits
 
 #define LR_FWD_BLOCK 256
 #define LR_TOK 16    // tokens of a forward run
 #define LR_BWD_BLOCK 512
 #define LR_BWD_TOK 8  // tokens of a run of the gradients: tiles of the same length
-#define LR_GROUP 32  // tiles of a group
+#define LR_GROUP 16  // tiles of a group, groups of a block
 #define LR_POLLS (1 << 22)  // polls a wait may take (seconds); it then ends with NaN
 #define LR_EMPTY64 0xffffffffffffffffull
 #define LR_EMPTY32 0xffffffffu
@@ -88,11 +92,14 @@ __device__ __forceinline__ LrTile lr_tile(const LrSeqs& q, int64_t slot) {
   return s;
 }
 
-// Words of a call: a counter, the tiles' maps [slots, D] (P low, H high), the groups' states [slots / LR_GROUP + 1, D], the
+#define LR_BLOCK_TILES (LR_GROUP * LR_GROUP)
+
+// Words of a call: a counter, the tiles' maps [slots, D] (P low, H high), the groups' [slots / LR_GROUP + 1, D], the blocks' states
+// [slots / LR_BLOCK_TILES + 1, D] (a slot's group and block: tiles that leave theirs are that many slots or more apart), the
 // boundaries in order.
 struct LrWords {
   unsigned* ticket;
-  unsigned long long* maps;
+  unsigned long long *maps, *group_maps;
   unsigned* states;
   int64_t* cu;
 };
@@ -189,21 +196,24 @@ __device__ __forceinline__ float lr_sigmoid(float x) { return __builtin_amdgcn_r
 // a = exp(l) and k = 1 - a, near a = 1 without loss: there k is the sum of its series in t = -l (8 terms: t^8 / 9! = 1e-8 of it at
 // t = 1/2) and a = 1 - k is off by its own rounding alone. (The exponential instruction's error, up to a step of a and not
 // the same in both directions, adds up over the thousands of tokens that such a channel remembers: 7e-6 of dA at 6 007 tokens.)
-// `small`, the same in the whole wave: |l| is below 1/2 whatever the gates hold.
-__device__ __forceinline__ void lr_decay(float l, bool small, float& a, float& k) {
+// SMALL: |l| is below 1/2 whatever the gates hold.
+template <bool SMALL>
+__device__ __forceinline__ void lr_decay(float l, float& a, float& k) {
   const float t = -l;
-  float p = __builtin_fmaf(t, -1.0f / 8.0f, 1.0f);
-  p = __builtin_fmaf(t * (-1.0f / 7.0f), p, 1.0f);
-  p = __builtin_fmaf(t * (-1.0f / 6.0f), p, 1.0f);
-  p = __builtin_fmaf(t * (-1.0f / 5.0f), p, 1.0f);
-  p = __builtin_fmaf(t * (-1.0f / 4.0f), p, 1.0f);
-  p = __builtin_fmaf(t * (-1.0f / 3.0f), p, 1.0f);
-  p = __builtin_fmaf(t * (-1.0f / 2.0f), p, 1.0f);
+  float p = __builtin_fmaf(t, -1.0f / 40320.0f, 1.0f / 5040.0f);
+  p = __builtin_fmaf(t, p, -1.0f / 720.0f);
+  p = __builtin_fmaf(t, p, 1.0f / 120.0f);
+  p = __builtin_fmaf(t, p, -1.0f / 24.0f);
+  p = __builtin_fmaf(t, p, 1.0f / 6.0f);
+  p = __builtin_fmaf(t, p, -0.5f);
+  p = __builtin_fmaf(t, p, 1.0f);
   k = t * p;
   a = 1.0f - k;
-  if (!small && !(__builtin_fabsf(t) < 0.5f)) {
-    a = __expf(l);
-    k = 1.0f - a;
+  if constexpr (!SMALL) {
+    const float e = __expf(l);
+    const bool far = !(__builtin_fabsf(t) < 0.5f);
+    a = far ? e : a;
+    k = far ? 1.0f - e : k;
   }
 }
 // sqrt(1 - a^2) of a and 1 - a.
@@ -222,41 +232,25 @@ __device__ __forceinline__ void lr_put_map(unsigned long long* p, float P, float
 __device__ __forceinline__ void lr_put_state(unsigned* p, float h) {
   __hip_atomic_store(p, lr_bits(h), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-template <int V>
-__device__ __forceinline__ void lr_get_states(const unsigned* p, float (&h)[V]) {
-  unsigned w[V];
-  bool ok;
-  int polls = 0;
-  do {
-    ok = true;
+// N words of a lane's V channels, the first n of them wanted, `step` words apart; `ok`: none of them is empty. AGAIN: only those that
+// were are asked for.
+template <int V, int N, bool AGAIN>
+__device__ __forceinline__ void lr_look(const unsigned long long* at, int64_t step, int n, unsigned long long (&w)[N][V], bool& ok) {
+  ok = true;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      w[v] = __hip_atomic_load(p + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      ok = ok && w[v] != LR_EMPTY32;
-    }
-    if (!ok) __builtin_amdgcn_s_sleep(1);
-  } while (!ok && ++polls < LR_POLLS);
+  for (int k = 0; k < N; ++k)
 #pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = __uint_as_float(w[v]);  // the empty pattern is a NaN
+    for (int v = 0; v < V; ++v)
+      if (k < n && (!AGAIN || w[k][v] == LR_EMPTY64))
+        w[k][v] = __hip_atomic_load(at + k * step + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int v = 0; v < V; ++v) ok = ok && (k >= n || w[k][v] != LR_EMPTY64);
 }
-// (P, H) <- the maps of tiles p0 .. p0 + n - 1 (n <= N), one behind the other, `step` words apart.
+// (P, H) <- the maps of the first n words, one behind the other.
 template <int V, int N>
-__device__ __forceinline__ void lr_get_maps(const unsigned long long* at, int64_t step, int n, float (&P)[V], float (&H)[V]) {
-  unsigned long long w[N][V];
-  bool ok;
-  int polls = 0;
-  do {
-    ok = true;
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (k < n) {
-          w[k][v] = __hip_atomic_load(at + k * step + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          ok = ok && w[k][v] != LR_EMPTY64;
-        }
-    if (!ok) __builtin_amdgcn_s_sleep(1);
-  } while (!ok && ++polls < LR_POLLS);
+__device__ __forceinline__ void lr_compose(const unsigned long long (&w)[N][V], int n, float (&P)[V], float (&H)[V]) {
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     P[v] = 1.0f;
@@ -307,48 +301,94 @@ __device__ __forceinline__ void lr_job(const LrArgs& a, int64_t& slot, int& cb) 
   if (BACK) slot = a.slots - 1 - slot;
 }
 
-// What a tile of the forward starts from (or, BACK, what reaches a tile from behind): the state of the group before it under the
-// maps of its group before it. `place` counts tiles in the order of the walk, `dir` is its direction; `sm` holds one map
-// per thread. Every thread gets the value of its channels.
+// What a tile of the forward starts from (or, BACK, what reaches a tile from behind), in every thread for its channels; leaves the
+// group's map and the block's state where the tile is the last of one. `place` counts the sequence's tiles in the order of the walk,
+// Pt and Ht are the tile's own map (in the threads of run `writer`), `more`: tiles follow.
 template <int V, int BLOCK, bool BACK>
 __device__ __forceinline__ void lr_enter(const LrArgs& a, const LrTile& s, int64_t slot, int place, int c, bool on, int lane, int run,
-                                         const float* first, float2 (*sm)[V], float (*base)[V], float (&h)[V]) {
-  const int runs = BLOCK / a.lanes, pos = place % LR_GROUP;
+                                         int writer, bool more, const float (&Pt)[V], const float (&Ht)[V], const float* first,
+                                         float2 (*sm)[V], float (*base)[V], float (&h)[V]) {
+  const int runs = BLOCK / a.lanes, pos = place % LR_GROUP, grp = place / LR_GROUP % LR_GROUP;
   const int64_t dir = BACK ? 1 : -1;  // towards the tiles that were walked before
-  float P[V], H[V];
+  // each run takes `per` places of the group, and of the block's groups, oldest first
+  constexpr int MOST = LR_GROUP * 64 / BLOCK, PER = MOST < 1 ? 1 : MOST;  // 64 lanes side by side; fewer lanes, more runs
+  const int per = runs >= LR_GROUP ? 1 : LR_GROUP / runs, p0 = run * per;
+  const int nt = on ? (pos - p0 < per ? pos - p0 : per) : 0, ng = on ? (grp - p0 < per ? grp - p0 : per) : 0;
+  const unsigned long long* tiles = a.w.maps + (slot + dir * (pos - p0)) * a.D + c;
+  // group g of the block before this one's: its last tile lies pos + 1 + LR_GROUP (grp - 1 - g) tiles away
+  const int64_t last0 = slot + dir * (pos + 1 + (int64_t)LR_GROUP * (grp - 1 - p0));
+  const unsigned long long* groups = a.w.group_maps + last0 / LR_GROUP * a.D + c;
+  const bool from_block = run == 0 && on && place >= LR_BLOCK_TILES;
+  const unsigned* state = a.w.states + (slot + dir * (place % LR_BLOCK_TILES + 1)) / LR_BLOCK_TILES * a.D + c;
+  unsigned long long wt[PER][V], wg[PER][V];
+  unsigned ws[V];
+  bool have_tiles, have_groups;
+  lr_look<V, PER, false>(tiles, -dir * a.D, nt, wt, have_tiles);
+  lr_look<V, PER, false>(groups, -dir * a.D, ng, wg, have_groups);
+  bool have_state = true;
+  auto look_state = [&]() {
+    if (!from_block) return;
+    have_state = true;
 #pragma unroll
-  for (int v = 0; v < V; ++v) { P[v] = 1.0f; H[v] = 0.0f; }
-  // the run's share of the group's maps, oldest first: places [run * per, run * per + per) of the group
-  constexpr int PER = LR_GROUP * 64 / BLOCK;  // with 64 lanes side by side; fewer lanes, more runs, fewer maps for each
-  const int per = runs >= LR_GROUP ? 1 : LR_GROUP / runs;
-  const int p0 = run * per, n = pos - p0 < per ? pos - p0 : per;
-  if (n > 0 && on) lr_get_maps<V, PER>(a.w.maps + (slot + dir * (pos - p0)) * a.D + c, -dir * a.D, n, P, H);
+    for (int v = 0; v < V; ++v) {
+      ws[v] = __hip_atomic_load(state + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      have_state = have_state && ws[v] != LR_EMPTY32;
+    }
+  };
+  look_state();
+  // a wait that runs out leaves empty words, which are NaN
+  for (int polls = 0; !have_tiles && polls < LR_POLLS; ++polls) {
+    __builtin_amdgcn_s_sleep(2);
+    lr_look<V, PER, true>(tiles, -dir * a.D, nt, wt, have_tiles);
+  }
+  float P[V], H[V];
+  lr_compose<V, PER>(wt, nt, P, H);
 #pragma unroll
   for (int v = 0; v < V; ++v) sm[threadIdx.x][v] = float2{P[v], H[v]};
-  if (run == 0) {
-    float b[V];
+  __syncthreads();
+  float Pg[V], Hg[V];  // the tiles of the group before this one
 #pragma unroll
-    for (int v = 0; v < V; ++v) b[v] = 0.0f;
-    if (on) {
-      if (place >= LR_GROUP) {
-        lr_get_states<V>(a.w.states + ((slot + dir * (pos + 1)) / LR_GROUP) * a.D + c, b);
-      } else if (first) {
+  for (int v = 0; v < V; ++v) { Pg[v] = 1.0f; Hg[v] = 0.0f; }
+  for (int k = 0; k < runs && k * per < pos; ++k) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) b[v] = first[(int64_t)s.seq * a.D + c + v];
-      }
+    for (int v = 0; v < V; ++v) {
+      const float2 m = sm[k * a.lanes + lane][v];
+      Hg[v] = __builtin_fmaf(m.x, Hg[v], m.y);
+      Pg[v] *= m.x;
     }
+  }
+  if (run == writer && on && more && pos == LR_GROUP - 1) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) base[lane][v] = b[v];
+    for (int v = 0; v < V; ++v)
+      lr_put_map(a.w.group_maps + slot / LR_GROUP * a.D + c + v, Pt[v] * Pg[v], __builtin_fmaf(Pt[v], Hg[v], Ht[v]));
+  }
+  for (int polls = 0; !(have_groups && have_state) && polls < LR_POLLS; ++polls) {
+    __builtin_amdgcn_s_sleep(2);
+    lr_look<V, PER, true>(groups, -dir * a.D, ng, wg, have_groups);
+    look_state();
+  }
+  lr_compose<V, PER>(wg, ng, P, H);
+  __syncthreads();  // the tiles' maps have been read
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    sm[threadIdx.x][v] = float2{P[v], H[v]};
+    if (run == 0) base[lane][v] = from_block ? __uint_as_float(ws[v]) : (on && first ? first[(int64_t)s.seq * a.D + c + v] : 0.0f);
   }
   __syncthreads();
 #pragma unroll
   for (int v = 0; v < V; ++v) h[v] = base[lane][v];
-  for (int k = 0; k < runs && k * per < pos; ++k) {
+  for (int k = 0; k < runs && k * per < grp; ++k) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float2 m = sm[k * a.lanes + lane][v];
       h[v] = __builtin_fmaf(m.x, h[v], m.y);
     }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    h[v] = __builtin_fmaf(Pg[v], h[v], Hg[v]);
+    if (run == writer && on && more && place % LR_BLOCK_TILES == LR_BLOCK_TILES - 1)
+      lr_put_state(a.w.states + slot / LR_BLOCK_TILES * a.D + c + v, __builtin_fmaf(Pt[v], h[v], Ht[v]));
   }
 }
 
@@ -411,31 +451,35 @@ __global__ void __launch_bounds__(LR_FWD_BLOCK) lr_fwd_kernel(const LrArgs a) {
     small = small && __builtin_fabsf(A[v]) < 0.5f;
     H[v] = L[v] = 0.0f;
   }
-  small = __all(small);
+  // plain: every token is there and |A| < 1/2 throughout the wave, as in most of a call
+  auto gates = [&](auto plain) {
+    constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
-  for (int j = 0; j < LR_TOK; ++j) {
-    float rv[V], xv[V], iv[V];
-    lr_widen<T, V>(rr[j], rv);
-    lr_widen<T, V>(rx[j], xv);
-    if constexpr (HASI) lr_widen<T, V>(ri[j], iv);
+    for (int j = 0; j < LR_TOK; ++j) {
+      float rv[V], xv[V], iv[V];
+      lr_widen<T, V>(rr[j], rv);
+      lr_widen<T, V>(rx[j], xv);
+      if constexpr (HASI) lr_widen<T, V>(ri[j], iv);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float l = A[v] * lr_sigmoid(rv[v]), d, k, u = xv[v];
-      lr_decay(l, small, d, k);
-      if constexpr (HASI) u *= lr_sigmoid(iv[v]);
-      if (a.normalize) u *= lr_unit(d, k);
-      if (j >= n) { l = 0.0f; d = 1.0f; u = 0.0f; }
-      av[j][v] = d;
-      uv[j][v] = u;
-      L[v] += l;
-      H[v] = __builtin_fmaf(d, H[v], u);
+      for (int v = 0; v < V; ++v) {
+        float l = A[v] * lr_sigmoid(rv[v]), d, k, u = xv[v];
+        lr_decay<PLAIN>(l, d, k);
+        if constexpr (HASI) u *= lr_sigmoid(iv[v]);
+        if (a.normalize) u *= lr_unit(d, k);
+        if (!PLAIN && j >= n) { l = 0.0f; d = 1.0f; u = 0.0f; }
+        av[j][v] = d;
+        uv[j][v] = u;
+        L[v] += l;
+        H[v] = __builtin_fmaf(d, H[v], u);
+      }
     }
-  }
+  };
+  if (__all(small && n == LR_TOK)) gates(std::true_type()); else gates(std::false_type());
   // from the sum of the exponents: a product of 16 rounded factors would be off by 16 roundings, tile after tile
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     float k;
-    lr_decay(L[v], false, P[v], k);
+    lr_decay<false>(L[v], P[v], k);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) maps[threadIdx.x][v] = float2{P[v], H[v]};
@@ -460,12 +504,10 @@ __global__ void __launch_bounds__(LR_FWD_BLOCK) lr_fwd_kernel(const LrArgs a) {
     if (last_run && on && !last_tile) lr_put_map(a.w.maps + slot * a.D + c + v, Pt[v], Ht[v]);
   }
   float h[V];
-  lr_enter<V, LR_FWD_BLOCK, false>(a, s, slot, s.index, c, on, lane, run, a.h0, before, base, h);
+  lr_enter<V, LR_FWD_BLOCK, false>(a, s, slot, s.index, c, on, lane, run, runs - 1, !last_tile, Pt, Ht, a.h0, before, base, h);
   if (on) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if (last_run && !last_tile && s.index % LR_GROUP == LR_GROUP - 1)
-        lr_put_state(a.w.states + (slot / LR_GROUP) * a.D + c + v, __builtin_fmaf(Pt[v], h[v], Ht[v]));
       if (run == 0 && a.tile_states) a.tile_states[slot * a.D + c + v] = h[v];
     }
   }
@@ -492,7 +534,7 @@ __global__ void __launch_bounds__(LR_FWD_BLOCK) lr_fwd_kernel(const LrArgs a) {
 
 // ------------------------------------------------------------------------------------------------ gradients
 template <typename T, int V, bool HASI, bool HASZ>
-__global__ void __launch_bounds__(LR_BWD_BLOCK) lr_bwd_kernel(const LrArgs a) {
+__global__ void __launch_bounds__(LR_BWD_BLOCK, sizeof(T) == 2 ? 4 : 2) lr_bwd_kernel(const LrArgs a) {
   typedef typename LrRaw<T, V>::type raw;
   constexpr int E = sizeof(T), TOK = LR_BWD_TOK;
   __shared__ float2 maps[LR_BWD_BLOCK][V], before[LR_BWD_BLOCK][V];
@@ -556,7 +598,7 @@ __global__ void __launch_bounds__(LR_BWD_BLOCK) lr_bwd_kernel(const LrArgs a) {
   }
   const int64_t left = s.t1 - s.t0 - row;
   const int n = left < 0 ? 0 : (left < TOK ? (int)left : TOK);
-  float A[V], h[V], P[V], L[V], H[V], C[V], av[TOK][V], dv[TOK][V], hv[TOK + 1][V];
+  float A[V], h[V], P[V], L[V], H[V], C[V], av[TOK][V], hv[TOK + 1][V];
   bool small = true;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -566,34 +608,39 @@ __global__ void __launch_bounds__(LR_BWD_BLOCK) lr_bwd_kernel(const LrArgs a) {
     L[v] = H[v] = C[v] = 0.0f;
     hv[0][v] = 0.0f;
   }
-  small = __all(small);
+  const bool plain = __all(small && n == TOK);
+  float dv[TOK][V];  // what reaches h from y; not kept over the wait, formed again behind it
+  auto gates = [&](auto simple) {
+    constexpr bool PLAIN = decltype(simple)::value;
 #pragma unroll
-  for (int j = 0; j < TOK; ++j) {
-    float rv[V], xv[V], iv[V], zv[V], dy[V];
-    lr_widen<T, V>(rr[j], rv);
-    lr_widen<T, V>(rx[j], xv);
-    lr_widen<T, V>(rdy[j], dy);
-    if constexpr (HASI) lr_widen<T, V>(ri[j], iv);
-    if constexpr (HASZ) lr_widen<T, V>(rz[j], zv);
+    for (int j = 0; j < TOK; ++j) {
+      float rv[V], xv[V], iv[V], zv[V], dy[V];
+      lr_widen<T, V>(rr[j], rv);
+      lr_widen<T, V>(rx[j], xv);
+      lr_widen<T, V>(rdy[j], dy);
+      if constexpr (HASI) lr_widen<T, V>(ri[j], iv);
+      if constexpr (HASZ) lr_widen<T, V>(rz[j], zv);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float l = A[v] * lr_sigmoid(rv[v]), d, k, u = xv[v];
-      lr_decay(l, small, d, k);
-      if constexpr (HASI) u *= lr_sigmoid(iv[v]);
-      if (a.normalize) u *= lr_unit(d, k);
-      if (j >= n) { l = 0.0f; d = 1.0f; u = 0.0f; }
-      av[j][v] = d;
-      dv[j][v] = dy[v];
-      if constexpr (HASZ) dv[j][v] *= lr_act(zv[v], a.act);
-      H[v] = __builtin_fmaf(d, H[v], u);
-      hv[j + 1][v] = H[v];  // from a state of zero
-      L[v] += l;
+      for (int v = 0; v < V; ++v) {
+        float l = A[v] * lr_sigmoid(rv[v]), d, k, u = xv[v];
+        lr_decay<PLAIN>(l, d, k);
+        if constexpr (HASI) u *= lr_sigmoid(iv[v]);
+        if (a.normalize) u *= lr_unit(d, k);
+        if (!PLAIN && j >= n) { l = 0.0f; d = 1.0f; u = 0.0f; }
+        av[j][v] = d;
+        dv[j][v] = dy[v];
+        if constexpr (HASZ) dv[j][v] *= lr_act(zv[v], a.act);
+        H[v] = __builtin_fmaf(d, H[v], u);
+        hv[j + 1][v] = H[v];  // from a state of zero
+        L[v] += l;
+      }
     }
-  }
+  };
+  if (plain) gates(std::true_type()); else gates(std::false_type());
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     float k;
-    lr_decay(L[v], false, P[v], k);
+    lr_decay<false>(L[v], P[v], k);
   }
 #pragma unroll
   for (int j = TOK - 1; j >= 0; --j) {
@@ -633,11 +680,7 @@ __global__ void __launch_bounds__(LR_BWD_BLOCK) lr_bwd_kernel(const LrArgs a) {
     Pt[v] = Pa[v] * P[v];
     if (run == 0 && on && !first_tile) lr_put_map(a.w.maps + slot * a.D + c + v, Pt[v], Ct[v]);
   }
-  lr_enter<V, LR_BWD_BLOCK, true>(a, s, slot, place, c, on, lane, run, a.dht, before, base, g);
-  if (run == 0 && on && !first_tile && place % LR_GROUP == LR_GROUP - 1) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) lr_put_state(a.w.states + (slot / LR_GROUP) * a.D + c + v, __builtin_fmaf(Pt[v], g[v], Ct[v]));
-  }
+  lr_enter<V, LR_BWD_BLOCK, true>(a, s, slot, place, c, on, lane, run, 0, !first_tile, Pt, Ct, a.dht, before, base, g);
 #pragma unroll
   for (int v = 0; v < V; ++v) g[v] = __builtin_fmaf(Pa[v], g[v], Ca[v]);
   // hv[j] <- the state before token j: h under the decays so far, and what has come in since
@@ -656,48 +699,53 @@ __global__ void __launch_bounds__(LR_BWD_BLOCK) lr_bwd_kernel(const LrArgs a) {
   float dA[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) dA[v] = 0.0f;
+  auto grads = [&](auto simple) {
+    constexpr bool PLAIN = decltype(simple)::value;
 #pragma unroll
-  for (int j = TOK - 1; j >= 0; --j) {
-    float rv[V], xv[V], iv[V], zv[V], dy[V], dx[V], dr[V], di[V], dz[V];
-    lr_widen<T, V>(rr[j], rv);
-    lr_widen<T, V>(rx[j], xv);
-    lr_widen<T, V>(rdy[j], dy);
-    if constexpr (HASI) lr_widen<T, V>(ri[j], iv);
-    if constexpr (HASZ) lr_widen<T, V>(rz[j], zv);
+    for (int j = TOK - 1; j >= 0; --j) {
+      float rv[V], xv[V], iv[V], zv[V], dy[V], dx[V], dr[V], di[V], dz[V];
+      lr_widen<T, V>(rr[j], rv);
+      lr_widen<T, V>(rx[j], xv);
+      lr_widen<T, V>(rdy[j], dy);
+      if constexpr (HASI) lr_widen<T, V>(ri[j], iv);
+      if constexpr (HASZ) lr_widen<T, V>(rz[j], zv);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float sr = lr_sigmoid(rv[v]), l = A[v] * sr, d = av[j][v];
-      const float si = HASI ? lr_sigmoid(iv[v]) : 1.0f;
-      const float G = dv[j][v] + g[v];
-      float into = si, dl = d * hv[j][v];  // d h / d x, d h / d log a
-      if (a.normalize) {
-        float same, k;
-        lr_decay(l, small, same, k);
-        const float m = lr_unit(d, k);
-        into *= m;
-        // a token that keeps all (m = 0) has no slope through m
-        dl = __builtin_fmaf(-si * xv[v], m == 0.0f ? 0.0f : d * d * __builtin_amdgcn_rcpf(m), dl);
-      }
-      dl *= G;
-      dx[v] = G * into;
-      if constexpr (HASI) di[v] = dx[v] * xv[v] * (1.0f - si);
-      dr[v] = dl * l * (1.0f - sr);
-      if (j < n) dA[v] = __builtin_fmaf(dl, sr, dA[v]);
-      if constexpr (HASZ) {
-        float slope = 1.0f;
-        if (a.act != LR_ACT_NONE) {
-          const float sz = lr_sigmoid(zv[v]);
-          slope = a.act == LR_ACT_SILU ? sz * __builtin_fmaf(zv[v], 1.0f - sz, 1.0f) : sz * (1.0f - sz);
+      for (int v = 0; v < V; ++v) {
+        const float sr = lr_sigmoid(rv[v]), l = A[v] * sr;
+        const float si = HASI ? lr_sigmoid(iv[v]) : 1.0f;
+        float d, k, dh = dy[v], slope = 1.0f;
+        lr_decay<PLAIN>(l, d, k);
+        if constexpr (HASZ) {
+          dh *= lr_act(zv[v], a.act);
+          if (a.act != LR_ACT_NONE) {
+            const float sz = lr_sigmoid(zv[v]);
+            slope = a.act == LR_ACT_SILU ? sz * __builtin_fmaf(zv[v], 1.0f - sz, 1.0f) : sz * (1.0f - sz);
+          }
         }
-        dz[v] = dy[v] * hv[j + 1][v] * slope;
+        const float G = dh + g[v];
+        float into = si, dl = d * hv[j][v];  // d h / d x, d h / d log a
+        if (a.normalize) {
+          const float m = lr_unit(d, k);
+          into *= m;
+          // a token that keeps all (m = 0) has no slope through m
+          dl = __builtin_fmaf(-si * xv[v], m == 0.0f ? 0.0f : d * d * __builtin_amdgcn_rcpf(m), dl);
+        }
+        dl *= G;
+        dx[v] = G * into;
+        if constexpr (HASI) di[v] = dx[v] * xv[v] * (1.0f - si);
+        dr[v] = dl * l * (1.0f - sr);
+        if (PLAIN || j < n) dA[v] = __builtin_fmaf(dl, sr, dA[v]);
+        if constexpr (HASZ) dz[v] = dy[v] * hv[j + 1][v] * slope;
+        if (!PLAIN && j >= n) d = 1.0f;
+        g[v] = d * G;
       }
-      g[v] = d * G;
+      lr_store<raw>(dxb, yo + j * ystep, lr_narrow<T, V>(dx));
+      lr_store<raw>(drb, yo + j * ystep, lr_narrow<T, V>(dr));
+      if constexpr (HASI) lr_store<raw>(dib, yo + j * ystep, lr_narrow<T, V>(di));
+      if constexpr (HASZ) lr_store<raw>(dzb, yo + j * ystep, lr_narrow<T, V>(dz));
     }
-    lr_store<raw>(dxb, yo + j * ystep, lr_narrow<T, V>(dx));
-    lr_store<raw>(drb, yo + j * ystep, lr_narrow<T, V>(dr));
-    if constexpr (HASI) lr_store<raw>(dib, yo + j * ystep, lr_narrow<T, V>(di));
-    if constexpr (HASZ) lr_store<raw>(dzb, yo + j * ystep, lr_narrow<T, V>(dz));
-  }
+  };
+  if (plain) grads(std::true_type()); else grads(std::false_type());
   if (a.dh0 && first_tile && run == 0 && on) {
 #pragma unroll
     for (int v = 0; v < V; ++v) a.dh0[(int64_t)s.seq * a.D + c + v] = g[v];
@@ -729,7 +777,7 @@ __global__ void __launch_bounds__(256) lr_step_kernel(const T* __restrict__ x, i
   const float xv = GdrElem<T>::to_float(x[b * xs + c]), rv = GdrElem<T>::to_float(r[b * rs + c]);
   const float iv = gi ? GdrElem<T>::to_float(gi[b * is + c]) : 0.0f, zv = z ? GdrElem<T>::to_float(z[b * zs + c]) : 0.0f;
   float d, k, u = xv;
-  lr_decay(A[c] * lr_sigmoid(rv), false, d, k);
+  lr_decay<false>(A[c] * lr_sigmoid(rv), d, k);
   if (gi) u *= lr_sigmoid(iv);
   if (normalize) u *= lr_unit(d, k);
   const float h = __builtin_fmaf(d, state[at], u);
@@ -782,8 +830,8 @@ static LrLayout lr_layout(const lampa_lr_args* a, int backward) {
   const int64_t slots = lr_slots(a);
   LrLayout l;
   l.maps = 256;
-  l.states = l.maps + (lr_handed_out(a) ? lampa_align_up(slots * a->D * 8, 256) : 0);
-  l.cu = l.states + (lr_handed_out(a) ? lampa_align_up((slots / LR_GROUP + 1) * a->D * 4, 256) : 0);
+  l.states = l.maps + (lr_handed_out(a) ? lampa_align_up((slots + slots / LR_GROUP + 1) * a->D * 8, 256) : 0);
+  l.cu = l.states + (lr_handed_out(a) ? lampa_align_up((slots / LR_BLOCK_TILES + 1) * a->D * 4, 256) : 0);
   l.parts = l.cu + (lr_handed_out(a) && a->cu_seqlens ? lampa_align_up(((int64_t)a->n_seq + 1) * 8, 256) : 0);
   l.total = l.parts + (backward ? slots * a->D * 4 : 0);
   return l;
@@ -818,10 +866,11 @@ static int lr_setup(const lampa_lr_args* a, int backward, LrArgs& k, int V, hipS
   k.dy = a->dy; k.dht = a->dht; k.dx = a->dx; k.dr = a->d_decay_gate; k.di = a->d_input_gate; k.dz = a->d_gate;
   k.dh0 = a->dh0; k.dA_parts = (float*)(ws + l.parts);
   k.xs = a->x_stride; k.rs = a->decay_stride; k.is = a->input_stride; k.zs = a->gate_stride;
-  k.w = LrWords{(unsigned*)ws, (unsigned long long*)(ws + l.maps), (unsigned*)(ws + l.states), (int64_t*)(ws + l.cu)};
+  k.slots = lr_slots(a);
+  k.w = LrWords{(unsigned*)ws, (unsigned long long*)(ws + l.maps), (unsigned long long*)(ws + l.maps) + k.slots * a->D,
+                 (unsigned*)(ws + l.states), (int64_t*)(ws + l.cu)};
   k.handed_out = lr_handed_out(a);
   k.q = LrSeqs{a->cu_seqlens ? (k.handed_out ? (const int64_t*)(ws + l.cu) : a->cu_seqlens) : nullptr, a->seq_len, a->n_tokens, a->n_seq, tile};
-  k.slots = lr_slots(a);
   k.D = a->D;
   k.lanes = lanes_of_tile;
   k.cblocks = (a->D + k.lanes * V - 1) / (k.lanes * V);
@@ -830,7 +879,7 @@ static int lr_setup(const lampa_lr_args* a, int backward, LrArgs& k, int V, hipS
   if (k.slots * k.cblocks > 0x7fffffff) return LAMPA_ERR_UNSUPPORTED;
   LAMPA_PROF(s, "start");
   if (k.handed_out) {
-    const int64_t n_maps = k.slots * a->D, n_states = (k.slots / LR_GROUP + 1) * a->D;
+    const int64_t n_maps = (k.slots + k.slots / LR_GROUP + 1) * a->D, n_states = (k.slots / LR_BLOCK_TILES + 1) * a->D;
     const int64_t blocks = (n_maps + 1023) / 1024;
     hipLaunchKernelGGL(lr_init_kernel, dim3((unsigned)(blocks < 1 ? 1 : (blocks < 1024 ? blocks : 1024))), dim3(256), 0, s, k.w, n_maps,
                        n_states, a->cu_seqlens, a->n_seq, a->n_tokens);
