@@ -23,7 +23,7 @@ static int ff_check_operands(const lampa_ff_args* a, int64_t size) {
 
 extern "C" int64_t lampa_ff_workspace_bytes(const lampa_ff_args* a, int backward) {
   const int rc = ff_check(a);
-  return rc != LAMPA_OK ? rc : ff_gemm_workspace(a, backward);
+  return rc != LAMPA_OK ? rc : ff_fused_takes(a) ? ff_fused_workspace(a, backward) : ff_gemm_workspace(a, backward);
 }
 
 extern "C" int lampa_ff_fwd(const lampa_ff_args* a, void* stream) {
@@ -33,7 +33,7 @@ extern "C" int lampa_ff_fwd(const lampa_ff_args* a, void* stream) {
   if (rc != LAMPA_OK) return rc;
   if (a->rows && !a->y) return LAMPA_ERR_INVALID;
   if (!a->rows) return LAMPA_OK;
-  return ff_gemm_fwd(a, (hipStream_t)stream);
+  return ff_fused_takes(a) ? ff_fused_fwd(a, (hipStream_t)stream) : ff_gemm_fwd(a, (hipStream_t)stream);
 }
 
 // Without rows nothing is launched: the caller clears the weights' gradients itself.
@@ -44,5 +44,5 @@ extern "C" int lampa_ff_bwd(const lampa_ff_args* a, void* stream) {
   if (rc != LAMPA_OK) return rc;
   if (a->rows && !a->dy) return LAMPA_ERR_INVALID;
   if (!a->rows || (!a->dx && !a->dw_gate && !a->dw_up && !a->dw_down)) return LAMPA_OK;
-  return ff_gemm_bwd(a, (hipStream_t)stream);
+  return ff_fused_takes(a) ? ff_fused_bwd(a, (hipStream_t)stream) : ff_gemm_bwd(a, (hipStream_t)stream);
 }

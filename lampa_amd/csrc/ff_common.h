@@ -47,7 +47,28 @@ __device__ __forceinline__ void ff_store4(T* p, float a, float b, float c, float
   *reinterpret_cast<vec4*>(p) = vec4{GdrElem<T>::from_float(a), GdrElem<T>::from_float(b), GdrElem<T>::from_float(c), GdrElem<T>::from_float(d)};
 }
 
+// out[c] = sum over n rows, `step` values apart, of rows[c], in order; cols a multiple of 4.
+template <typename T>
+static __global__ void __launch_bounds__(256) ff_reduce_kernel(const float* __restrict__ rows, int n, int64_t cols, int64_t step, T* __restrict__ out) {
+  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (c >= cols) return;
+  f32x4 sum = *reinterpret_cast<const f32x4*>(rows + c);
+  for (int r = 1; r < n; ++r) sum += *reinterpret_cast<const f32x4*>(rows + r * step + c);
+  ff_store4(out + c, sum[0], sum[1], sum[2], sum[3]);
+}
+template <typename T>
+static int ff_reduce(const float* rows, int n, int64_t cols, int64_t step, T* out, hipStream_t s) {
+  hipLaunchKernelGGL((ff_reduce_kernel<T>), dim3((unsigned)((cols / 4 + 255) / 256)), dim3(256), 0, s, rows, n, cols, step, out);
+  LAMPA_PROF(s, "ff_reduce_kernel");
+  return lampa_launch_status();
+}
+
 // The general form (ff_gemm.hip): hidden values through memory.
 int64_t ff_gemm_workspace(const lampa_ff_args* a, int backward);
 int ff_gemm_fwd(const lampa_ff_args* a, hipStream_t s);
 int ff_gemm_bwd(const lampa_ff_args* a, hipStream_t s);
+// 16-bit types and D <= 128 (ff_fused.hip): hidden values in registers.
+bool ff_fused_takes(const lampa_ff_args* a);
+int64_t ff_fused_workspace(const lampa_ff_args* a, int backward);
+int ff_fused_fwd(const lampa_ff_args* a, hipStream_t s);
+int ff_fused_bwd(const lampa_ff_args* a, hipStream_t s);

@@ -324,18 +324,6 @@ __global__ void __launch_bounds__(MM_BLOCK) ff_weights_kernel(const FfWeightJobs
 }
 
 // ------------------------------------------------------------------------------------------------ small kernels
-template <typename T>
-__global__ void __launch_bounds__(256) ff_reduce_kernel(const float* __restrict__ rows, int n, int64_t cols, int64_t step, T* __restrict__ out) {
-  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (c >= cols) return;
-  f32x4 sum = *reinterpret_cast<const f32x4*>(rows + c);
-  for (int r = 1; r < n; ++r) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(rows + r * step + c);
-    sum += v;
-  }
-  ff_store4(out + c, sum[0], sum[1], sum[2], sum[3]);
-}
-
 // out [cols, rows] = in [rows, cols]^T in tiles of 32 x 32; three matrices side by side in the grid's third dimension.
 struct FfTurns {
   const void* in[3];
@@ -449,9 +437,8 @@ static int ff_bwd_go(const lampa_ff_args* a, hipStream_t s) {
     hipLaunchKernelGGL((ff_weights_kernel<T>), dim3((unsigned)tiles, (unsigned)jobs.splits), dim3(MM_BLOCK), 0, s, jobs, parts);
     LAMPA_PROF(s, "ff_weights_kernel");
     for (int j = 0; j < jobs.n; ++j) {
-      hipLaunchKernelGGL((ff_reduce_kernel<T>), dim3((unsigned)((size / 4 + 255) / 256)), dim3(256), 0, s, parts + jobs.job[j].at,
-                         jobs.splits, size, jobs.part_step, outs[j]);
-      LAMPA_PROF(s, "ff_reduce_kernel");
+      const int rc = ff_reduce<T>(parts + jobs.job[j].at, jobs.splits, size, jobs.part_step, outs[j], s);
+      if (rc != LAMPA_OK) return rc;
     }
   }
   return lampa_launch_status();
