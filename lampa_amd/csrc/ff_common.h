@@ -40,6 +40,10 @@ __device__ __forceinline__ ff_u32x4 ff_load16(__amdgpu_buffer_rsrc_t buf, unsign
   return __builtin_bit_cast(ff_u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, offset, 0, 0));
 }
 
+// Everything that this wave has asked memory for has come. Before a loop with loads of its own: a register loaded in front of the loop
+// would otherwise be waited for inside it, and the loop's own loads, which are counted in order, with it.
+__device__ __forceinline__ void ff_loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // Four consecutive values, rounded to T.
 template <typename T>
 __device__ __forceinline__ void ff_store4(T* p, float a, float b, float c, float d) {

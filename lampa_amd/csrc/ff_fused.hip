@@ -1,8 +1,7 @@
 // The gated feed-forward block for 16-bit types and narrow blocks (D <= 128): hidden values never leave the registers
 // (ff_common.h has the mathematics).
 //   out:      y (or, BACK, dx): a wave keeps 32 rows of x (and dy) as operands and their outputs as sums; the hidden columns pass in
-//             chunks of 32, whose weights the workgroup's 4 waves share in LDS (double buffered, the next chunk under way in
-//             registers). Products are formed transposed, hidden columns x rows: the sums of the first products, rounded, are
+//             chunks of 32, whose weights the workgroup's waves share in LDS (the next chunk under way in registers). Products are formed transposed, hidden columns x rows: the sums of the first products, rounded, are
 //             then the operands of the next as they lie in the registers.
 //   weights:  a wave keeps 32 hidden columns (their weights as operands, the sums of the three gradients: 16 DB values a lane each)
 //             and the rows pass in tiles of 32 in LDS; workgroups share the rows out and leave their sums in fp32.
@@ -11,7 +10,8 @@
 #include "ff_common.h"
 
 #define FU_BLOCK 256
-#define FU_ROWS 128  // rows of a workgroup of `out`
+#define FU_WIDE 8   // waves of a workgroup of `out` where the rows fill the GPU
+#define FU_AHEAD 2  // steps that operands are read ahead of their products
 #define FU_CHUNK 32  // hidden columns of a chunk
 
 template <typename T>
@@ -30,28 +30,63 @@ struct FuOut {
   int D, F, chunks;  // chunks of a workgroup
 };
 
-// A 16-wide step's operand whose rows are the 32 columns col0 .. of a tile and whose contraction runs over the tile's rows.
+// Row-major tiles of up to 128 columns that are read both along their rows (16 bytes a lane, 32 rows side by side) and turned (four rows
+// of 16 columns for each 16 lanes): the 16-byte pieces of a row are permuted by three bits of the row, piece ^ fu_twist(row), so
+// that neither kind of read meets itself in a bank. Rows are a multiple of 128 bytes.
+__device__ __forceinline__ int fu_twist(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+template <typename T, int STRIDE>
+__device__ __forceinline__ void fu_put(T* tile, int row, int c, ff_u32x4 v) {
+  *reinterpret_cast<ff_u32x4*>(tile + row * STRIDE + ((c >> 3) ^ fu_twist(row)) * 8) = v;
+}
+// Row `row`, columns c .. c + 7.
+template <typename T, int STRIDE>
+__device__ __forceinline__ typename OpVec<T>::x8 fu_along(const T* tile, int row, int c) {
+  return *reinterpret_cast<const typename OpVec<T>::x8*>(tile + row * STRIDE + ((c >> 3) ^ fu_twist(row)) * 8);
+}
+// A 16-wide step's operand whose rows are the 32 columns col0 .. of a tile and whose contraction runs over the tile's rows row0 .., in
+// slot order (op_ld_kappa_tr of gdr_ops.h on a permuted tile).
 template <typename T, int STRIDE>
 __device__ __forceinline__ typename OpVec<T>::x8 fu_turned(const T* tile, int col0, int row0, int lane) {
-  return op_ld_kappa_tr<T>(tile, STRIDE, col0, row0, lane);
+  const int L = lane & 15, blk = (lane >> 4) & 1, hh = lane >> 5, row = row0 + 4 * hh + (L >> 2);
+  const int piece = (col0 >> 3) + 2 * blk + ((L & 3) >> 1);
+  const T* p = tile + row * STRIDE + (piece ^ fu_twist(row)) * 8 + (L & 1) * 4;
+  const typename OpVec<T>::x4 lo = op_lds_read_tr4<T>(p), hi = op_lds_read_tr4<T>(p + 8 * STRIDE);  // 8 rows on: the same twist
+  typename OpVec<T>::x8 out;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) { out[s] = lo[s]; out[4 + s] = hi[s]; }
+  return out;
 }
 
-template <typename T, int ACT, int DB, bool BACK>
-__global__ void __launch_bounds__(FU_BLOCK, 2) ff_out_kernel(const FuOut a) {
+// WAVES waves of 32 rows each.
+template <typename T, int ACT, int DB, int WAVES, bool BACK>
+__global__ void __launch_bounds__(64 * WAVES, 2) ff_out_kernel(const FuOut a) {
   typedef typename OpVec<T>::x8 x8;
   typedef typename OpVec<T>::x4 x4;
-  constexpr int KS = 2 * DB, WIDE = DB * 32, GS = WIDE + 8, DS = 40;       // elements between the rows of the tiles
-  constexpr int PIECES = 128 * DB, LOADS = (PIECES + FU_BLOCK - 1) / FU_BLOCK;  // 16-byte pieces of each matrix's chunk
-  constexpr int STAGE = 2 * FU_CHUNK * GS + WIDE * DS;
-  __shared__ __attribute__((aligned(16))) T lds[2 * STAGE];
+  constexpr int KS = 2 * DB, WIDE = DB * 32, GS = (DB + 1) / 2 * 64, DS = BACK ? 32 : 40;  // elements between the rows of the tiles
+  constexpr int BLOCK = 64 * WAVES, PIECES = 128 * DB, LOADS = (PIECES + BLOCK - 1) / BLOCK;  // 16-byte pieces of each matrix's chunk
+  constexpr int STAGE = 2 * FU_CHUNK * GS + WIDE * DS, ROWS = 32 * WAVES;
+  // BACK: two chunks; forward: three. At the end 32 rows of outputs for each wave.
+  constexpr int LOOP = (BACK ? 2 : 3) * STAGE, OUTS = WAVES * 32 * (WIDE + 8), LDS = LOOP > OUTS ? LOOP : OUTS;
+  __shared__ __attribute__((aligned(16))) T lds[LDS];
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, hh = lane >> 5, wave = tid >> 6;
   const int D = a.D, F = a.F;
-  const int64_t r0 = (int64_t)blockIdx.x * FU_ROWS;
+  const int64_t r0 = (int64_t)blockIdx.x * ROWS;
   const int64_t left = a.rows - r0;
-  const int here = left < FU_ROWS ? (int)left : FU_ROWS;
+  const int here = left < ROWS ? (int)left : ROWS;
   const int c0 = blockIdx.y * a.chunks, all = (F + FU_CHUNK - 1) / FU_CHUNK, c1 = c0 + a.chunks < all ? c0 + a.chunks : all;
 
   ff_u32x4 rg[LOADS], ru[LOADS], rd[LOADS];
+  // where this thread's pieces lie in a chunk, and in its tiles
+  unsigned from[LOADS], from_down[LOADS];
+  int at[LOADS], at_down[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int id = tid + i * BLOCK, row = id / (DB * 4), c = id % (DB * 4) * 8, d = id / 4, f = id % 4 * 8;
+    from[i] = c < D ? (unsigned)(row * D + c) * 2 : FF_OFF;
+    from_down[i] = d < D ? (unsigned)(d * F + f) * 2 : FF_OFF;
+    at[i] = row * GS + ((c >> 3) ^ fu_twist(row)) * 8;
+    at_down[i] = 2 * FU_CHUNK * GS + d * DS + (BACK ? f ^ (d & 2 ? 16 : 0) : f);  // BACK: read turned, rows 2, 3 of four the other way round
+  }
   auto fetch = [&](int chunk) {
     const int f0 = chunk * FU_CHUNK, n = F - f0 < FU_CHUNK ? F - f0 : FU_CHUNK;
     const __amdgpu_buffer_rsrc_t gb = ff_buffer((const T*)a.wg + (int64_t)f0 * D, (int64_t)n * D * 2);
@@ -59,38 +94,41 @@ __global__ void __launch_bounds__(FU_BLOCK, 2) ff_out_kernel(const FuOut a) {
     const __amdgpu_buffer_rsrc_t db = ff_buffer((const T*)a.wd + f0, ((int64_t)(D - 1) * F + n) * 2);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int id = tid + i * FU_BLOCK;
-      if (PIECES % FU_BLOCK && id >= PIECES) break;
-      const int row = id / (DB * 4), c = id % (DB * 4) * 8;
-      rg[i] = fu_load(gb, (unsigned)(row * D) * 2, c, D);
-      ru[i] = fu_load(ub, (unsigned)(row * D) * 2, c, D);
-      const int d = id / 4, f = id % 4 * 8;
-      rd[i] = ff_load16(db, f < n && d < D ? (unsigned)(d * F + f) * 2 : FF_OFF);
+      if (PIECES % BLOCK && tid + i * BLOCK >= PIECES) break;
+      rg[i] = ff_load16(gb, from[i]);
+      ru[i] = ff_load16(ub, from[i]);
+    }
+    if (n == FU_CHUNK) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) rd[i] = ff_load16(db, from_down[i]);
+    } else {  // the columns behind the last are the next row's
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) rd[i] = ff_load16(db, tid % 4 * 8 < n ? from_down[i] : FF_OFF);
     }
   };
   auto stage = [&](int which) {
-    T *g = lds + which * STAGE, *u = g + FU_CHUNK * GS, *w = u + FU_CHUNK * GS;
+    T* p = lds + which * STAGE;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int id = tid + i * FU_BLOCK;
-      if (PIECES % FU_BLOCK && id >= PIECES) break;
-      const int row = id / (DB * 4), c = id % (DB * 4) * 8;
-      *reinterpret_cast<ff_u32x4*>(g + row * GS + c) = rg[i];
-      *reinterpret_cast<ff_u32x4*>(u + row * GS + c) = ru[i];
-      const int d = id / 4, f = id % 4 * 8;
-      if constexpr (BACK) {
-        *reinterpret_cast<ff_u32x4*>(w + d * DS + f) = rd[i];
-      } else {  // groups of four in slot order within each 16 columns: the share of a step is then one 16-byte piece
-        const x8 v = fu_op<T>(rd[i]);
-        T* p = w + d * DS + (f & 16) + (f & 8 ? 4 : 0);
-        *reinterpret_cast<x4*>(p) = x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<x4*>(p + 8) = x4{v[4], v[5], v[6], v[7]};
-      }
+      if (PIECES % BLOCK && tid + i * BLOCK >= PIECES) break;
+      *reinterpret_cast<ff_u32x4*>(p + at[i]) = rg[i];
+      *reinterpret_cast<ff_u32x4*>(p + FU_CHUNK * GS + at[i]) = ru[i];
+      *reinterpret_cast<ff_u32x4*>(p + at_down[i]) = rd[i];
     }
   };
+  // Wd as the operand whose rows are the chunk's hidden columns, contraction over its rows d0 .. in slot order
+  auto down_turned = [&](const T* w, int d0) {
+    const int L = lane & 15, blk = (lane >> 4) & 1, row = d0 + 4 * hh + (L >> 2);
+    const T* p = w + row * DS + ((16 * blk + 4 * (L & 3)) ^ (row & 2 ? 16 : 0));
+    const x4 lo = op_lds_read_tr4<T>(p), hi = op_lds_read_tr4<T>(p + 8 * DS);
+    return x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
 
+  // Row of a chunk's Wg and Wu that is row ln of the first products: chosen so that the 8 sums a lane holds for a step of the last
+  // product are 8 hidden columns in line, as Wd has them (BACK reads Wd and both turned, in the order the sums lie in anyway).
+  const int gl = BACK ? ln : (ln & 16) | ((ln & 4) << 1) | ((ln & 8) >> 1) | (ln & 3);
   fetch(c0);
-  // this wave's 32 rows
+  // this wave's rows
   x8 xo[KS], dyo[BACK ? KS : 1];
   {
     const int row = 32 * wave + ln;
@@ -113,69 +151,178 @@ __global__ void __launch_bounds__(FU_BLOCK, 2) ff_out_kernel(const FuOut a) {
   }
   f32x16 out[DB];
 #pragma unroll
-  for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) out[d][r] = 0.0f;
+      for (int r = 0; r < 16; ++r) out[d][r] = 0.0f;
   stage(0);
-  __syncthreads();
-  for (int chunk = c0; chunk < c1; ++chunk) {
-    if (chunk + 1 < c1) fetch(chunk + 1);
-    const int which = (chunk - c0) & 1;
-    const T *g = lds + which * STAGE, *u = g + FU_CHUNK * GS, *w = u + FU_CHUNK * GS;
-    f32x16 G, U, S;
+  ff_loads_done();
+  if (c0 + 1 < c1) fetch(c0 + 1);
+  lds_barrier();
+  if constexpr (!BACK) {
+    // Chunk c + 1's first products run while chunk c's elementwise part does, pinned side by side in steps: the matrix cores work
+    // through a product while the wave issues what does not depend on it.
+    f32x16 Ga, Ua, Gb, Ub;
+    auto first = [&](const T* g, f32x16& G, f32x16& U, auto between) {
+      const T* u = g + FU_CHUNK * GS;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) G[r] = U[r] = S[r] = 0.0f;
+      for (int r = 0; r < 16; ++r) G[r] = U[r] = 0.0f;
+      x8 ga[KS], ua[KS];
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      G = mfma32(*reinterpret_cast<const x8*>(g + ln * GS + 16 * k + 8 * hh), xo[k], G);
-      U = mfma32(*reinterpret_cast<const x8*>(u + ln * GS + 16 * k + 8 * hh), xo[k], U);
-      if constexpr (BACK) S = mfma32(fu_turned<T, DS>(w, 0, 16 * k, lane), dyo[k], S);
+      for (int k = 0; k < KS + FU_AHEAD; ++k) {
+        if (k < KS) {
+          ga[k] = fu_along<T, GS>(g, gl, 16 * k + 8 * hh);
+          ua[k] = fu_along<T, GS>(u, gl, 16 * k + 8 * hh);
+        }
+        if (k >= FU_AHEAD) {
+          const int m = k - FU_AHEAD;
+          G = mfma32(ga[m], xo[m], G);
+          U = mfma32(ua[m], xo[m], U);
+          between(m);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    int slot = 0;  // of the chunk being finished
+    auto next_slot = [](int s) { return s == 2 ? 0 : s + 1; };
+    auto one = [&](int chunk, f32x16& G, f32x16& U, f32x16& G1, f32x16& U1) {
+      const int s1 = next_slot(slot), s2 = next_slot(s1);
+      if (chunk + 2 < c1) stage(s2);  // requested a whole chunk ago
+      if (chunk + 3 < c1) fetch(chunk + 3);
+      const T* w = lds + slot * STAGE + 2 * FU_CHUNK * GS;
+      x8 h[2];
+      auto act = [&](int k) {
+#pragma unroll
+        for (int r = 16 * k / KS; r < 16 * (k + 1) / KS; ++r) h[r / 8][r % 8] = (T)(ff_act<ACT>(G[r]) * U[r]);
+      };
+      if (chunk + 1 < c1) {
+        first(lds + s1 * STAGE, G1, U1, act);
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) act(k);
+      }
+      x8 da[2 * DB];
+#pragma unroll
+      for (int m = 0; m < 2 * DB + FU_AHEAD; ++m) {
+        if (m < 2 * DB) da[m] = *reinterpret_cast<const x8*>(w + (32 * (m % DB) + ln) * DS + 16 * (m / DB) + 8 * hh);
+        if (m >= FU_AHEAD) out[(m - FU_AHEAD) % DB] = mfma32(da[m - FU_AHEAD], h[(m - FU_AHEAD) / DB], out[(m - FU_AHEAD) % DB]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      lds_barrier();
+      slot = s1;
+    };
+    first(lds, Ga, Ua, [](int) {});
+    if (c0 + 1 < c1) stage(1);
+    if (c0 + 2 < c1) fetch(c0 + 2);
+    lds_barrier();
+    for (int chunk = c0; chunk < c1; chunk += 2) {
+      one(chunk, Ga, Ua, Gb, Ub);
+      if (chunk + 1 < c1) one(chunk + 1, Gb, Ub, Ga, Ua);
     }
-    if constexpr (!BACK) {
+  } else {
+    for (int chunk = c0; chunk < c1; ++chunk) {
+      const int which = (chunk - c0) & 1;
+      if (chunk + 1 < c1) stage(which ^ 1);  // requested a whole chunk ago
+      if (chunk + 2 < c1) fetch(chunk + 2);
+      const T *g = lds + which * STAGE, *u = g + FU_CHUNK * GS, *w = u + FU_CHUNK * GS;
+      f32x16 G, U, S;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) G[r] = ff_act<ACT>(G[r]) * U[r];
+        for (int r = 0; r < 16; ++r) G[r] = U[r] = S[r] = 0.0f;
+      // operands are read FU_AHEAD steps ahead of their products, held there by the barriers (left to itself the compiler reads each just
+      // before its product and waits)
+      {
+        x8 ga[KS], ua[KS], wa[BACK ? KS : 1];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const x8 h = acc_to_op<T>(G, 8 * s);
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-          out[d] = mfma32(*reinterpret_cast<const x8*>(w + (32 * d + ln) * DS + 16 * s + 8 * hh), h, out[d]);
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float value, slope;
-        ff_act_slope<ACT>(G[r], value, slope);
-        G[r] = S[r] * U[r] * slope;
-        U[r] = S[r] * value;
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const x8 dg = acc_to_op<T>(G, 8 * s), du = acc_to_op<T>(U, 8 * s);
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          out[d] = mfma32(fu_turned<T, GS>(g, 32 * d, 16 * s, lane), dg, out[d]);
-          out[d] = mfma32(fu_turned<T, GS>(u, 32 * d, 16 * s, lane), du, out[d]);
+        for (int k = 0; k < KS + FU_AHEAD; ++k) {
+          if (k < KS) {
+            ga[k] = fu_along<T, GS>(g, gl, 16 * k + 8 * hh);
+            ua[k] = fu_along<T, GS>(u, gl, 16 * k + 8 * hh);
+            if constexpr (BACK) wa[k] = down_turned(w, 16 * k);
+          }
+          if (k >= FU_AHEAD) {
+            const int m = k - FU_AHEAD;
+            {
+              G = mfma32(ga[m], xo[m], G);
+              U = mfma32(ua[m], xo[m], U);
+              if constexpr (BACK) S = mfma32(wa[m], dyo[m], S);
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
+      x8 da[2 * DB], db[BACK ? 2 * DB : 1];
+      auto last_operands = [&](int m) {
+        const int s = m / DB, d = m % DB;
+        if constexpr (BACK) {
+          da[m] = fu_turned<T, GS>(g, 32 * d, 16 * s, lane);
+          db[m] = fu_turned<T, GS>(u, 32 * d, 16 * s, lane);
+        } else {
+          da[m] = *reinterpret_cast<const x8*>(w + (32 * d + ln) * DS + 16 * s + 8 * hh);
+        }
+      };
+#pragma unroll
+      for (int m = 0; m < FU_AHEAD && m < 2 * DB; ++m) last_operands(m);
+      __builtin_amdgcn_sched_barrier(0);
+      x8 h0[2], h1[2];
+      {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if constexpr (BACK) {
+            float value, slope;
+            ff_act_slope<ACT>(G[r], value, slope);
+            h0[r / 8][r % 8] = (T)(S[r] * U[r] * slope);
+            h1[r / 8][r % 8] = (T)(S[r] * value);
+          } else {
+            h0[r / 8][r % 8] = (T)(ff_act<ACT>(G[r]) * U[r]);
+          }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 2 * DB; ++m) {
+        const int s = m / DB, d = m % DB;
+        if (m + FU_AHEAD < 2 * DB) last_operands(m + FU_AHEAD);
+        {
+          out[d] = mfma32(da[m], h0[s], out[d]);
+          if constexpr (BACK) out[d] = mfma32(db[m], h1[s], out[d]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      lds_barrier();
     }
-    if (chunk + 1 < c1) stage(which ^ 1);
-    __syncthreads();
   }
-  const int row = 32 * wave + ln;
-  if (row >= here) return;
+  if (a.parts) {
+    {
+      const int row = 32 * wave + ln;
+      if (row >= here) return;
 #pragma unroll
-  for (int d = 0; d < DB; ++d)
+      for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int c = 32 * d + 8 * q + 4 * hh;
-      if (c >= D) continue;
-      if (a.parts)
-        *reinterpret_cast<f32x4*>(a.parts + ((int64_t)blockIdx.y * a.rows + r0 + row) * D + c) =
-            f32x4{out[d][4 * q], out[d][4 * q + 1], out[d][4 * q + 2], out[d][4 * q + 3]};
-      else
-        ff_store4((T*)a.out + (r0 + row) * D + c, out[d][4 * q], out[d][4 * q + 1], out[d][4 * q + 2], out[d][4 * q + 3]);
+        for (int q = 0; q < 4; ++q) {
+          const int c = 32 * d + 8 * q + 4 * hh;
+          if (c < D)
+            *reinterpret_cast<f32x4*>(a.parts + ((int64_t)blockIdx.y * a.rows + r0 + row) * D + c) =
+                f32x4{out[d][4 * q], out[d][4 * q + 1], out[d][4 * q + 2], out[d][4 * q + 3]};
+        }
     }
+    return;
+  }
+  // through LDS (the tiles have been read), so that a row is written in pieces of 16 bytes side by side
+  constexpr int OS = WIDE + 8;
+  T* o = lds + wave * 32 * OS;
+  const __amdgpu_buffer_rsrc_t ob = ff_buffer((T*)a.out + r0 * D, (int64_t)here * D * 2);
+  {
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        ff_store4(o + ln * OS + 32 * d + 8 * q + 4 * hh, out[d][4 * q], out[d][4 * q + 1], out[d][4 * q + 2], out[d][4 * q + 3]);
+    lds_fence();
+#pragma unroll
+    for (int i = 0; i < 2 * DB; ++i) {
+      const int id = lane + 64 * i, row = id / (DB * 4), c = id % (DB * 4) * 8;
+      const ff_u32x4 v = *reinterpret_cast<const ff_u32x4*>(o + row * OS + c);
+      __builtin_amdgcn_raw_buffer_store_b128(v, ob, c < D ? (unsigned)((32 * wave + row) * D + c) * 2 : FF_OFF, 0, 0);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ weights' gradients
@@ -189,15 +336,17 @@ struct FuWeights {
 template <typename T, int ACT, int DB>
 __global__ void __launch_bounds__(FU_BLOCK, 1) ff_fused_weights_kernel(const FuWeights a) {
   typedef typename OpVec<T>::x8 x8;
-  constexpr int KS = 2 * DB, WIDE = DB * 32, XS = WIDE + 8, TILE = 32 * XS;
+  constexpr int KS = 2 * DB, XS = (DB + 1) / 2 * 64, TILE = 32 * XS;
   constexpr int PIECES = 128 * DB, LOADS = (PIECES + FU_BLOCK - 1) / FU_BLOCK;
   __shared__ __attribute__((aligned(16))) T lds[2][2 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, hh = lane >> 5, wave = tid >> 6;
   const int D = a.D, F = a.F, f0 = blockIdx.x * 128 + 32 * wave, f = f0 + ln;
   const int64_t begin = (int64_t)blockIdx.y * a.per, end = begin + a.per < a.rows ? begin + a.per : a.rows;
+  const int tiles = end > begin ? (int)((end - begin + 31) / 32) : 0;
 
   ff_u32x4 rx[LOADS], ry[LOADS];
-  auto fetch = [&](int64_t t0) {
+  auto fetch = [&](int tile) {
+    const int64_t t0 = begin + 32 * (int64_t)tile;
     const int n = end - t0 < 32 ? (int)(end - t0) : 32;
     const __amdgpu_buffer_rsrc_t xb = ff_buffer((const T*)a.x + t0 * a.x_stride, ((n - 1) * a.x_stride + D) * 2);
     const __amdgpu_buffer_rsrc_t yb = ff_buffer((const T*)a.dy + t0 * D, (int64_t)n * D * 2);
@@ -216,11 +365,11 @@ __global__ void __launch_bounds__(FU_BLOCK, 1) ff_fused_weights_kernel(const FuW
       const int id = tid + i * FU_BLOCK;
       if (PIECES % FU_BLOCK && id >= PIECES) break;
       const int row = id / (DB * 4), c = id % (DB * 4) * 8;
-      *reinterpret_cast<ff_u32x4*>(&lds[which][row * XS + c]) = rx[i];
-      *reinterpret_cast<ff_u32x4*>(&lds[which][TILE + row * XS + c]) = ry[i];
+      fu_put<T, XS>(lds[which], row, c, rx[i]);
+      fu_put<T, XS>(lds[which] + TILE, row, c, ry[i]);
     }
   };
-  if (begin < end) fetch(begin);
+  if (tiles) fetch(0);
   x8 wg[KS], wu[KS], wd[KS];
   {
     const __amdgpu_buffer_rsrc_t gb = ff_buffer(a.wg, (int64_t)F * D * 2), ub = ff_buffer(a.wu, (int64_t)F * D * 2);
@@ -241,46 +390,65 @@ __global__ void __launch_bounds__(FU_BLOCK, 1) ff_fused_weights_kernel(const FuW
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dwg[d][r] = dwu[d][r] = dwd[d][r] = 0.0f;
-  if (begin < end) {
+  if (tiles) {
     stage(0);
-    __syncthreads();
-    int which = 0;
-    for (int64_t t0 = begin; t0 < end; t0 += 32, which ^= 1) {
-      const bool more = t0 + 32 < end;
-      if (more) fetch(t0 + 32);
+    ff_loads_done();
+    if (tiles > 1) fetch(1);
+    lds_barrier();
+    for (int tile = 0; tile < tiles; ++tile) {
+      const int which = tile & 1;
+      if (tile + 1 < tiles) stage(which ^ 1);  // requested a whole tile ago
+      if (tile + 2 < tiles) fetch(tile + 2);
       const T *x = lds[which], *y = x + TILE;
       f32x16 G, U, S;
 #pragma unroll
       for (int r = 0; r < 16; ++r) G[r] = U[r] = S[r] = 0.0f;
+      // operands are read FU_AHEAD steps ahead of their products, held there by the barriers (left to itself the compiler reads each
+      // just before its product and waits)
+      x8 xa[KS], ya[KS];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const x8 xa = *reinterpret_cast<const x8*>(x + ln * XS + 16 * k + 8 * hh), ya = *reinterpret_cast<const x8*>(y + ln * XS + 16 * k + 8 * hh);
-        G = mfma32(xa, wg[k], G);
-        U = mfma32(xa, wu[k], U);
-        S = mfma32(ya, wd[k], S);
+      for (int k = 0; k < KS + FU_AHEAD; ++k) {
+        if (k < KS) {
+          xa[k] = fu_along<T, XS>(x, ln, 16 * k + 8 * hh);
+          ya[k] = fu_along<T, XS>(y, ln, 16 * k + 8 * hh);
+        }
+        if (k >= FU_AHEAD) {
+          const int m = k - FU_AHEAD;
+          G = mfma32(xa[m], wg[m], G);
+          U = mfma32(xa[m], wu[m], U);
+          S = mfma32(ya[m], wd[m], S);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
+      x8 xt[2 * DB], yt[2 * DB];
+#pragma unroll
+      for (int m = 0; m < FU_AHEAD && m < 2 * DB; ++m) {
+        xt[m] = fu_turned<T, XS>(x, 32 * (m % DB), 16 * (m / DB), lane);
+        yt[m] = fu_turned<T, XS>(y, 32 * (m % DB), 16 * (m / DB), lane);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      x8 dg[2], du[2], h[2];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float value, slope;
         ff_act_slope<ACT>(G[r], value, slope);
-        const float s = S[r], up = U[r];
-        S[r] = value * up;
-        U[r] = s * value;
-        G[r] = s * up * slope;
+        h[r / 8][r % 8] = (T)(value * U[r]);
+        du[r / 8][r % 8] = (T)(S[r] * value);
+        dg[r / 8][r % 8] = (T)(S[r] * U[r] * slope);
       }
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const x8 dg = acc_to_op<T>(G, 8 * s), du = acc_to_op<T>(U, 8 * s), h = acc_to_op<T>(S, 8 * s);
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          const x8 xt = fu_turned<T, XS>(x, 32 * d, 16 * s, lane), yt = fu_turned<T, XS>(y, 32 * d, 16 * s, lane);
-          dwg[d] = mfma32(xt, dg, dwg[d]);
-          dwu[d] = mfma32(xt, du, dwu[d]);
-          dwd[d] = mfma32(yt, h, dwd[d]);
+      for (int m = 0; m < 2 * DB; ++m) {
+        const int s = m / DB, d = m % DB, n = m + FU_AHEAD;
+        if (n < 2 * DB) {
+          xt[n] = fu_turned<T, XS>(x, 32 * (n % DB), 16 * (n / DB), lane);
+          yt[n] = fu_turned<T, XS>(y, 32 * (n % DB), 16 * (n / DB), lane);
         }
+        dwg[d] = mfma32(xt[m], dg[s], dwg[d]);
+        dwu[d] = mfma32(xt[m], du[s], dwu[d]);
+        dwd[d] = mfma32(yt[m], h[s], dwd[d]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (more) stage(which ^ 1);
-      __syncthreads();
+      lds_barrier();
     }
   }
   if (f >= F) return;
@@ -336,15 +504,16 @@ bool ff_fused_takes(const lampa_ff_args* a) { return a->dtype != GDR_FP32 && a->
 // How the chunks of hidden columns are shared out: over one workgroup where the rows alone fill half the GPU (every further share
 // writes and reads the outputs' fp32 parts), else over as many as make one workgroup a CU.
 struct FuShare {
-  int splits, chunks;
+  int splits, chunks, waves;
 };
 static FuShare fu_share(const lampa_ff_args* a) {
-  const int64_t tiles = (a->rows + FU_ROWS - 1) / FU_ROWS;
+  const int waves = a->rows > 128 * 256 ? FU_WIDE : 4;
+  const int64_t tiles = (a->rows + 32 * waves - 1) / (32 * waves);
   const int all = (a->F + FU_CHUNK - 1) / FU_CHUNK;
   const int64_t want = tiles < 1 ? 1 : 256 / tiles;
-  const int n = want < 1 ? 1 : (want < all ? (int)want : all);
+  const int n = want < 1 || waves > 4 ? 1 : (want < all ? (int)want : all);
   const int chunks = (all + n - 1) / n;
-  return {(all + chunks - 1) / chunks, chunks};
+  return {(all + chunks - 1) / chunks, chunks, waves};
 }
 // The rows of the weights' gradients: one workgroup of 128 hidden columns a CU.
 static int fu_weight_splits(const lampa_ff_args* a) {
@@ -363,13 +532,19 @@ static int fu_out(const lampa_ff_args* a, hipStream_t s) {
   const FuShare sh = fu_share(a);
   T* out = (T*)(BACK ? a->dx : a->y);
   FuOut k{a->x, a->dy, a->w_gate, a->w_up, a->w_down, out, sh.splits > 1 ? (float*)a->workspace : nullptr, a->rows, a->x_stride, a->D, a->F, sh.chunks};
-  const dim3 grid((unsigned)((a->rows + FU_ROWS - 1) / FU_ROWS), (unsigned)sh.splits), block(FU_BLOCK);
+  const int rows = 32 * sh.waves;
+  const dim3 grid((unsigned)((a->rows + rows - 1) / rows), (unsigned)sh.splits), block(64 * sh.waves);
+#define FU_GO(DB)                                                                                       \
+  if (sh.waves == 4) hipLaunchKernelGGL((ff_out_kernel<T, ACT, DB, 4, BACK>), grid, block, 0, s, k);          \
+  else hipLaunchKernelGGL((ff_out_kernel<T, ACT, DB, FU_WIDE, BACK>), grid, block, 0, s, k);                  \
+  break;
   switch ((a->D + 31) / 32) {
-    case 1: hipLaunchKernelGGL((ff_out_kernel<T, ACT, 1, BACK>), grid, block, 0, s, k); break;
-    case 2: hipLaunchKernelGGL((ff_out_kernel<T, ACT, 2, BACK>), grid, block, 0, s, k); break;
-    case 3: hipLaunchKernelGGL((ff_out_kernel<T, ACT, 3, BACK>), grid, block, 0, s, k); break;
-    default: hipLaunchKernelGGL((ff_out_kernel<T, ACT, 4, BACK>), grid, block, 0, s, k); break;
+    case 1: FU_GO(1)
+    case 2: FU_GO(2)
+    case 3: FU_GO(3)
+    default: FU_GO(4)
   }
+#undef FU_GO
   LAMPA_PROF(s, BACK ? "ff_out_kernel_back" : "ff_out_kernel");
   const int rc = lampa_launch_status();
   if (rc != LAMPA_OK || sh.splits == 1) return rc;

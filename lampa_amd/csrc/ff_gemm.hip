@@ -77,9 +77,11 @@ __device__ __forceinline__ void mm_phase(const MmSide& a, const MmSide& b0, cons
   };
   fetch(0);
   stage(0);
-  __syncthreads();
+  if (steps > 1) fetch(1);
+  lds_barrier();
   for (int step = 0; step < steps; ++step) {
-    if (step + 1 < steps) fetch(step + 1);
+    if (step + 1 < steps) stage((step + 1) & 1);  // requested a whole step ago
+    if (step + 2 < steps) fetch(step + 2);
     const unsigned char* p = lds + (step & 1) * STAGE;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
@@ -95,8 +97,7 @@ __device__ __forceinline__ void mm_phase(const MmSide& a, const MmSide& b0, cons
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[m][b] = mm_mac<T>(fb[b], fa[m], acc[m][b]);
     }
-    if (step + 1 < steps) stage((step + 1) & 1);
-    __syncthreads();
+    lds_barrier();
   }
 }
 
@@ -284,11 +285,12 @@ __global__ void __launch_bounds__(MM_BLOCK) ff_weights_kernel(const FfWeightJobs
   if (begin < end) {
     fetch(begin);
     stage(0);
-    __syncthreads();
+    if (begin + BK < end) fetch(begin + BK);
+    lds_barrier();
     int which = 0;
     for (int64_t t0 = begin; t0 < end; t0 += BK, which ^= 1) {
-      const bool more = t0 + BK < end;
-      if (more) fetch(t0 + BK);
+      if (t0 + BK < end) stage(which ^ 1);  // requested a whole step ago
+      if (t0 + 2 * BK < end) fetch(t0 + 2 * BK);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         const int row0 = ks * BK / 4;
@@ -303,8 +305,7 @@ __global__ void __launch_bounds__(MM_BLOCK) ff_weights_kernel(const FfWeightJobs
 #pragma unroll
           for (int b = 0; b < 2; ++b) acc[m][b] = mm_mac<T>(fb[b], fa[m], acc[m][b]);
       }
-      if (more) stage(which ^ 1);
-      __syncthreads();
+      lds_barrier();
     }
   }
   float* out = parts + blockIdx.y * jobs.part_step + job.at;
