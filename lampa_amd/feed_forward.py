@@ -5,6 +5,7 @@
 ``gated_feed_forward`` is the operator of the reference's ``GatedMLP`` (``models/hattention/modeling_gated_deltaproduct.py:310-324``)
 with its gradients; the layer is ``lampa_amd.block.GatedFeedForward``. GPU tensors only; there is no CPU path.
 """
+import functools
 import struct
 from typing import Optional
 
@@ -24,30 +25,43 @@ _ARGS = struct.Struct("=11Q3q4i")
 
 def _matrix(x):
     """x [..., D] as (rows, elements between them): itself where its rows lie evenly, 16-byte aligned and not too far apart, else a copy."""
-    x2 = x.detach().reshape(-1, x.shape[-1])
-    step = x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
-    if (x2.shape[1] > 1 and x2.stride(1) != 1) or step < x2.shape[1] or step % 8 or step > MAX_STRIDE or x2.data_ptr() % 16:
-        x2, step = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device).copy_(x2), x2.shape[1]
+    D = x.shape[-1]
+    if x.dim() == 2 and x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, D
+    x2 = x.detach().reshape(-1, D)
+    step = x2.stride(0) if x2.shape[0] > 1 else D
+    if x2.stride(1) != 1 or step < D or step % 8 or step > MAX_STRIDE or x2.data_ptr() % 16:
+        x2, step = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device).copy_(x2), D
     return x2, step
 
 
-def _launch(name, backward, x, weights, act, y=None, dy=None, grads=(None,) * 4):
+@functools.lru_cache(maxsize=4096)
+def _workspace(rows, D, F, dtype, backward, wanted):
+    """Bytes of a pass's workspace; ``wanted``: the gradients of x, w_gate, w_up and w_down that are asked for."""
+    args = _ARGS.pack(0, 0, 0, 0, 0, 0, *wanted, 0, 0, rows, D, D, F, dtype, 0)
+    return check(_capi.lib().lampa_ff_workspace_bytes(args, backward), "lampa_ff_workspace_bytes")
+
+
+def _launch(call, name, x, w_gate, w_up, w_down, act, y, dy, grads):
     x2, step = _matrix(x)
     rows, D = x2.shape
-    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    w = [_packed(t.detach()) for t in weights]
-    pack = lambda ws, size: _ARGS.pack(p(x2), *(p(t) for t in w), p(y), p(dy), *(p(t) for t in grads), p(ws), size, rows, step, D,  # noqa: E731
-                                       w[0].shape[0], _DTYPES[x.dtype], act)
-    lib = _capi.lib()
-    with _on_device(x.get_device()):
-        size = check(lib.lampa_ff_workspace_bytes(pack(None, 0), backward), "lampa_ff_workspace_bytes")
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        check(getattr(lib, name)(pack(ws, size), stream_of(x)), name)
+    F, code, dev = w_gate.shape[0], _DTYPES[x.dtype], x.device
+    w_gate, w_up, w_down = _packed(w_gate), _packed(w_up), _packed(w_down)
+    grads = tuple([0 if g is None else g.data_ptr() for g in grads])
+    size = _workspace(rows, D, F, code, int(dy is not None), tuple([int(g != 0) for g in grads]))
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    args = _ARGS.pack(x2.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), 0 if y is None else y.data_ptr(),
+                      0 if dy is None else dy.data_ptr(), *grads, ws.data_ptr() if size else 0, size, rows, step, D, F, code, act)
+    with _on_device(dev.index):
+        check(call(args, stream_of(x)), name)
+
+
+_NO_GRADS = (None,) * 4
 
 
 def _forward(x, w_gate, w_up, w_down, act):
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _launch("lampa_ff_fwd", 0, x, (w_gate, w_up, w_down), act, y=y)
+    _launch(_capi.lib().lampa_ff_fwd, "lampa_ff_fwd", x, w_gate, w_up, w_down, act, y, None, _NO_GRADS)
     return y
 
 
@@ -66,7 +80,7 @@ class _GatedFeedForward(torch.autograd.Function):
         make = torch.empty if x.numel() else torch.zeros  # without rows nothing is launched
         grads = tuple(make(t.shape, dtype=t.dtype, device=t.device) if need else None
                       for t, need in zip(tensors, ctx.needs_input_grad))
-        _launch("lampa_ff_bwd", 1, x, tensors[1:], ctx.act, dy=_packed(dy.to(x.dtype)), grads=grads)
+        _launch(_capi.lib().lampa_ff_bwd, "lampa_ff_bwd", *tensors, ctx.act, None, _packed(dy.to(x.dtype)), grads)
         return (*grads, None)
 
 

@@ -10,6 +10,7 @@ token for each sequence on a kept state. It is the per-channel counterpart of ``
 ``models/baselines/full_mamba2.py:221-430``) and follows its names, state handling and return tuples. GPU tensors only; there is
 no CPU path.
 """
+import functools
 import struct
 import weakref
 from typing import Optional
@@ -34,26 +35,28 @@ def _rows(t, D):
     apart (a token of each of several long sequences)."""
     if t is None:
         return None, D
-    t, step = _tokens(t.detach(), D)
+    t, step = _tokens(t, D)
     if step > MAX_STRIDE:
-        return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t), D
+        return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t.detach()), D
     return t, step
 
 
-def _pack(call, A, h0, y, ht, tiles, cu, grads, ws, size):
-    (x, xs), (r, rs), (i, is_), (z, zs), act, normalize, n_seq = call
-    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+@functools.lru_cache(maxsize=4096)
+def _sizes(B, T, D, n_seq, packed, dtype, backward):
+    """(tiles, bytes of a pass's workspace) of a call."""
+    args = _ARGS.pack(*(0,) * 9, int(packed), *(0,) * 9, 0, B * T, T, D, D, D, D, n_seq, D, dtype, 0, 0, 0)
+    lib = _capi.lib()
+    return check(lib.lampa_lr_slots(args), "lampa_lr_slots"), check(lib.lampa_lr_workspace_bytes(args, backward), "lampa_lr_workspace_bytes")
+
+
+def _pack(x, r, i, z, A, h0, y, ht, tiles, cu, grads, ws, size, act, normalize, n_seq):
+    (x, xs), (r, rs), (i, is_), (z, zs) = x, r, i, z
     B, T, D = x.shape
-    return _ARGS.pack(p(x), p(r), p(i), p(z), p(A), p(h0), p(y), p(ht), p(tiles), p(cu), *(p(t) for t in grads), p(ws), size, B * T, T,
-                      xs, rs, is_, zs, n_seq, D, _DTYPES[x.dtype], act, int(normalize), 0)
+    pointers = [0 if t is None else t.data_ptr() for t in (x, r, i, z, A, h0, y, ht, tiles, cu, *grads, ws)]
+    return _ARGS.pack(*pointers, size, B * T, T, xs, rs, is_, zs, n_seq, D, _DTYPES[x.dtype], act, int(normalize), 0)
 
 
 _NO_GRADS = (None,) * 8
-
-
-def _call(x, r, i, z, act, normalize, n_seq):
-    D = x.shape[-1]
-    return _rows(x, D), _rows(r, D), _rows(i, D), _rows(z, D), act, normalize, n_seq
 
 
 def _scan_launch(x, r, A, i, z, act, normalize, h0, want_final, cu, keep=False):
@@ -61,17 +64,15 @@ def _scan_launch(x, r, A, i, z, act, normalize, h0, want_final, cu, keep=False):
     B, T, D = x.shape
     n_seq = B if cu is None else cu.numel() - 1
     dev = x.device
-    call = _call(x, r, i, z, act, normalize, n_seq)
-    A, h0 = _plain_f32(A), _plain_f32(h0)
+    slots, size = _sizes(B, T, D, n_seq, cu is not None, _DTYPES[x.dtype], 0)
     y = torch.empty((B, T, D), dtype=x.dtype, device=dev)
     ht = torch.empty((n_seq, D), dtype=torch.float32, device=dev) if want_final else None
-    lib = _capi.lib()
+    tiles = torch.empty((slots, D), dtype=torch.float32, device=dev) if keep else None
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    args = _pack(_rows(x, D), _rows(r, D), _rows(i, D), _rows(z, D), _plain_f32(A), _plain_f32(h0), y, ht, tiles, cu, _NO_GRADS, ws, size, act,
+                 normalize, n_seq)
     with _on_device(dev.index):
-        probe = _pack(call, A, h0, y, ht, None, cu, _NO_GRADS, None, 0)
-        tiles = torch.empty((check(lib.lampa_lr_slots(probe), "lampa_lr_slots"), D), dtype=torch.float32, device=dev) if keep else None
-        size = check(lib.lampa_lr_workspace_bytes(probe, 0), "lampa_lr_workspace_bytes")
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        check(lib.lampa_lr_scan_fwd(_pack(call, A, h0, y, ht, tiles, cu, _NO_GRADS, ws, size), stream_of(y)), "lampa_lr_scan_fwd")
+        check(_capi.lib().lampa_lr_scan_fwd(args, stream_of(y)), "lampa_lr_scan_fwd")
     return y, ht, tiles
 
 
@@ -79,19 +80,18 @@ def _scan_backward(x, r, A, i, z, act, normalize, h0, cu, tiles, dy, dht):
     B, T, D = x.shape
     n_seq = B if cu is None else cu.numel() - 1
     dev = x.device
-    call = _call(x, r, i, z, act, normalize, n_seq)
-    A, h0, dht = _plain_f32(A), _plain_f32(h0), _plain_f32(dht)
+    _, size = _sizes(B, T, D, n_seq, cu is not None, _DTYPES[x.dtype], 1)
+    h0 = _plain_f32(h0)
     dy = torch.zeros((B, T, D), dtype=x.dtype, device=dev) if dy is None else dy.to(x.dtype).contiguous()
     new = lambda t: None if t is None else torch.empty((B, T, D), dtype=x.dtype, device=dev)  # noqa: E731
     dx, dr, di, dz = new(x), new(r), new(i), new(z)
     dA = torch.empty(D, dtype=torch.float32, device=dev)
     dh0 = None if h0 is None else torch.empty((n_seq, D), dtype=torch.float32, device=dev)
-    grads = (dy, dht, dx, dr, di, dz, dA, dh0)
-    lib = _capi.lib()
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    args = _pack(_rows(x, D), _rows(r, D), _rows(i, D), _rows(z, D), _plain_f32(A), h0, None, None, tiles, cu,
+                 (dy, _plain_f32(dht), dx, dr, di, dz, dA, dh0), ws, size, act, normalize, n_seq)
     with _on_device(dev.index):
-        size = check(lib.lampa_lr_workspace_bytes(_pack(call, A, h0, None, None, tiles, cu, grads, None, 0), 1), "lampa_lr_workspace_bytes")
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        check(lib.lampa_lr_scan_bwd(_pack(call, A, h0, None, None, tiles, cu, grads, ws, size), stream_of(dx)), "lampa_lr_scan_bwd")
+        check(_capi.lib().lampa_lr_scan_bwd(args, stream_of(dx)), "lampa_lr_scan_bwd")
     return dx, dr, dA, di, dz, dh0
 
 
