@@ -5,16 +5,16 @@
 //   product: y = S Wd^T; dx = dG Wg + dU Wu as one sum over both (on transposed weights: all operands then lie along their
 //            contraction);
 //   weights: dWg, dWu, dWd over the rows, split over the rows where that fills the GPU, the parts summed in a fixed order.
-// A workgroup has 4 waves in 2 x 2 over a tile of 128 x 128 of the output (64 hidden columns of each product for `hidden` and
-// `grads`), tiles of 128 bytes of the contraction in LDS, double buffered, the next one under way in registers. Rows of 128 bytes
+// A workgroup has 4 waves in 2 x 2 over a tile of 128 (or 64) x 128 of the output (64 hidden columns of each product for `hidden` and
+// `grads`), tiles of 128 bytes of the contraction in LDS, double buffered, the next one under way in registers. A product with few
+// tiles has its contraction shared out and the parts summed in order. Rows of 128 bytes
 // are stored with their 16-byte pieces permuted by the row (piece ^ row % 8), so that the 32 rows of an operand read do not
 // meet in the same banks.
 #include "ff_common.h"
 
 #define MM_BLOCK 256
-#define MM_ROWS 128       // rows of a tile
 #define MM_ROW_BYTES 128  // of the contraction
-#define MM_TILE (MM_ROWS * MM_ROW_BYTES)
+#define MM_STAGE(MB) ((64 * (MB) + 128) * MM_ROW_BYTES)  // one step's tiles: 64 MB rows of x against 128 of the weights
 
 template <typename T>
 __device__ __forceinline__ f32x16 mm_mac(ff_u32x4 a, ff_u32x4 b, f32x16 c) {
@@ -36,22 +36,23 @@ struct MmSide {
 template <typename T>
 __device__ __forceinline__ MmSide mm_side(const T* base, int64_t first, int64_t rows, int64_t stride, int K) {
   const int64_t left = rows - first;
-  const int64_t n = left < 0 ? 0 : (left < MM_ROWS ? left : MM_ROWS);
+  const int64_t n = left < 0 ? 0 : (left < 128 ? left : 128);
   return {ff_buffer(base + (n ? first * stride : 0), n ? ((n - 1) * stride + K) * (int64_t)sizeof(T) : 0), (unsigned)(stride * sizeof(T))};
 }
 
 // acc[m][b] += (B rows b) . (A rows m) over K: register r of a lane is B row 8 (r / 4) + 4 hh + r % 4 of its block, A row = lane % 32.
-// The wave's A blocks are rows 64 wm and 64 wm + 32, its B blocks rows 32 wn and 64 + 32 wn (the second from b1).
-template <typename T, int NB>
+// The wave's MB A blocks are rows 32 (MB wm + m), its B blocks rows 32 wn and 64 + 32 wn (the second from b1).
+template <typename T, int MB, int NB>
 __device__ __forceinline__ void mm_phase(const MmSide& a, const MmSide& b0, const MmSide& b1, int K, unsigned char* lds,
-                                         f32x16 (&acc)[2][NB]) {
-  constexpr int BR = 64 * NB, BCH = BR * 8 / MM_BLOCK, EPC = 16 / sizeof(T), STAGE = MM_TILE + BR * MM_ROW_BYTES;
+                                         f32x16 (&acc)[MB][NB]) {
+  constexpr int BR = 64 * NB, BCH = BR * 8 / MM_BLOCK, AR = 64 * MB, ACH = AR * 8 / MM_BLOCK, ATILE = AR * MM_ROW_BYTES;
+  constexpr int STAGE = MM_STAGE(MB);
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, hh = lane >> 5, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   const int steps = (K * (int)sizeof(T) + MM_ROW_BYTES - 1) / MM_ROW_BYTES;
-  ff_u32x4 ra[4], rb[BCH];
+  ff_u32x4 ra[ACH], rb[BCH];
   auto fetch = [&](int step) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < ACH; ++i) {
       const int id = tid + i * MM_BLOCK, row = id >> 3, at = step * MM_ROW_BYTES + (id & 7) * 16;
       ra[i] = ff_load16(a.buf, at < K * (int)sizeof(T) ? row * a.step + at : FF_OFF);
     }
@@ -65,14 +66,14 @@ __device__ __forceinline__ void mm_phase(const MmSide& a, const MmSide& b0, cons
   auto stage = [&](int which) {
     unsigned char* p = lds + which * STAGE;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < ACH; ++i) {
       const int id = tid + i * MM_BLOCK, row = id >> 3;
       *reinterpret_cast<ff_u32x4*>(p + row * MM_ROW_BYTES + (((id & 7) ^ (row & 7)) * 16)) = ra[i];
     }
 #pragma unroll
     for (int i = 0; i < BCH; ++i) {
       const int id = tid + i * MM_BLOCK, row = id >> 3;
-      *reinterpret_cast<ff_u32x4*>(p + MM_TILE + row * MM_ROW_BYTES + (((id & 7) ^ (row & 7)) * 16)) = rb[i];
+      *reinterpret_cast<ff_u32x4*>(p + ATILE + row * MM_ROW_BYTES + (((id & 7) ^ (row & 7)) * 16)) = rb[i];
     }
   };
   fetch(0);
@@ -83,60 +84,80 @@ __device__ __forceinline__ void mm_phase(const MmSide& a, const MmSide& b0, cons
     if (step + 1 < steps) stage((step + 1) & 1);  // requested a whole step ago
     if (step + 2 < steps) fetch(step + 2);
     const unsigned char* p = lds + (step & 1) * STAGE;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      ff_u32x4 fa[2], fb[NB];
+    // operands are read a step ahead of their products, held there by the barriers
+    ff_u32x4 fa[2][MB], fb[2][NB];
+    auto read = [&](int ks) {
       const int piece = ((ks * 2 + hh) ^ (ln & 7)) * 16;
 #pragma unroll
-      for (int m = 0; m < 2; ++m) fa[m] = *reinterpret_cast<const ff_u32x4*>(p + (64 * wm + 32 * m + ln) * MM_ROW_BYTES + piece);
+      for (int m = 0; m < MB; ++m) fa[ks & 1][m] = *reinterpret_cast<const ff_u32x4*>(p + (32 * (MB * wm + m) + ln) * MM_ROW_BYTES + piece);
 #pragma unroll
       for (int b = 0; b < NB; ++b)
-        fb[b] = *reinterpret_cast<const ff_u32x4*>(p + MM_TILE + (64 * b + 32 * wn + ln) * MM_ROW_BYTES + piece);
+        fb[ks & 1][b] = *reinterpret_cast<const ff_u32x4*>(p + ATILE + (64 * b + 32 * wn + ln) * MM_ROW_BYTES + piece);
+    };
+    read(0);
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+    for (int ks = 0; ks < 4; ++ks) {
+      if (ks + 1 < 4) read(ks + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) acc[m][b] = mm_mac<T>(fb[b], fa[m], acc[m][b]);
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[m][b] = mm_mac<T>(fb[ks & 1][b], fa[ks & 1][m], acc[m][b]);
+      __builtin_amdgcn_sched_barrier(0);
     }
     lds_barrier();
   }
 }
 
-template <int N>
-__device__ __forceinline__ void mm_clear(f32x16 (&acc)[2][N]) {
+template <int M, int N>
+__device__ __forceinline__ void mm_clear(f32x16 (&acc)[M][N]) {
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < M; ++m)
 #pragma unroll
     for (int b = 0; b < N; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[m][b][r] = 0.0f;
 }
 
-// Tiles of the output, in columns first within strips of 8 row tiles: the strip's rows of x stay in L2 while the columns pass.
+// Workgroup -> tile of the output. Workgroups go round robin over the 8 XCDs, each with an L2 of its own.
+// mm_place: an XCD takes every 8th row tile and all columns, a strip of 8 row tiles at a time: its rows stay in L2 while the columns pass.
 __device__ __forceinline__ void mm_place(int64_t row_tiles, int col_tiles, int64_t& rt, int& ct) {
   const int64_t per = 8 * (int64_t)col_tiles, strip = blockIdx.x / per, in = blockIdx.x % per;
   const int64_t high = row_tiles - strip * 8 < 8 ? row_tiles - strip * 8 : 8;
   rt = strip * 8 + in % high;
   ct = (int)(in / high);
 }
+// mm_place_columns: an XCD takes every 8th column tile and all rows, row tile by row tile: its part of the weights stays in L2 while the rows
+// pass. For weights that L2 does not hold as a whole. The grid is 8 x column tiles of an XCD x row tiles; false: no tile.
+__device__ __forceinline__ bool mm_place_columns(int col_tiles, int64_t& rt, int& ct) {
+  const int each = (col_tiles + 7) / 8, in = blockIdx.x / 8;
+  ct = (int)(blockIdx.x % 8) + 8 * (in % each);
+  rt = in / each;
+  return ct < col_tiles;
+}
 
 // ------------------------------------------------------------------------------------------------ S = act(x Wg^T) (x Wu^T)
-template <typename T, int ACT>
-__global__ void __launch_bounds__(MM_BLOCK) ff_hidden_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ wg,
+template <typename T, int ACT, int MB>
+__global__ void __launch_bounds__(MM_BLOCK, 2) ff_hidden_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ wg,
                                                              const T* __restrict__ wu, int64_t rows, int D, int F,
-                                                             T* __restrict__ hidden) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * 2 * MM_TILE];
+                                                             T* __restrict__ hidden, bool columns) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * MM_STAGE(MB)];
   int64_t rt;
   int ct;
-  mm_place((rows + MM_ROWS - 1) / MM_ROWS, (F + 63) / 64, rt, ct);
-  const int64_t r0 = rt * MM_ROWS;
+  if (columns) {
+    if (!mm_place_columns((F + 63) / 64, rt, ct)) return;
+  } else {
+    mm_place((rows + 64 * MB - 1) / (64 * MB), (F + 63) / 64, rt, ct);
+  }
+  const int64_t r0 = rt * (64 * MB);
   const int f0 = ct * 64;
-  f32x16 acc[2][2];
+  f32x16 acc[MB][2];
   mm_clear(acc);
-  mm_phase<T, 2>(mm_side(x, r0, rows, x_stride, D), mm_side(wg, f0, F, D, D), mm_side(wu, f0, F, D, D), D, lds, acc);
+  mm_phase<T, MB, 2>(mm_side(x, r0, rows, x_stride, D), mm_side(wg, f0, F, D, D), mm_side(wu, f0, F, D, D), D, lds, acc);
   const int lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const int64_t row = r0 + 64 * wm + 32 * m + ln;
+  for (int m = 0; m < MB; ++m) {
+    const int64_t row = r0 + 32 * (MB * wm + m) + ln;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int f = f0 + 32 * wn + 8 * q + 4 * hh;
@@ -149,27 +170,32 @@ __global__ void __launch_bounds__(MM_BLOCK) ff_hidden_kernel(const T* __restrict
 }
 
 // ------------------------------------------------------------------------------------------------ S, dG, dU
-template <typename T, int ACT>
-__global__ void __launch_bounds__(MM_BLOCK) ff_grads_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ dy,
+template <typename T, int ACT, int MB>
+__global__ void __launch_bounds__(MM_BLOCK, 2) ff_grads_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ dy,
                                                             const T* __restrict__ wg, const T* __restrict__ wu,
                                                             const T* __restrict__ wd_t, int64_t rows, int D, int F,
-                                                            T* __restrict__ hidden, T* __restrict__ dg, T* __restrict__ du) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * 2 * MM_TILE];
+                                                            T* __restrict__ hidden, T* __restrict__ dg, T* __restrict__ du,
+                                                            bool columns) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * MM_STAGE(MB)];
   int64_t rt;
   int ct;
-  mm_place((rows + MM_ROWS - 1) / MM_ROWS, (F + 63) / 64, rt, ct);
-  const int64_t r0 = rt * MM_ROWS;
+  if (columns) {
+    if (!mm_place_columns((F + 63) / 64, rt, ct)) return;
+  } else {
+    mm_place((rows + 64 * MB - 1) / (64 * MB), (F + 63) / 64, rt, ct);
+  }
+  const int64_t r0 = rt * (64 * MB);
   const int f0 = ct * 64;
-  f32x16 acc[2][2], ds[2][1];
+  f32x16 acc[MB][2], ds[MB][1];
   mm_clear(acc);
   mm_clear(ds);
-  mm_phase<T, 2>(mm_side(x, r0, rows, x_stride, D), mm_side(wg, f0, F, D, D), mm_side(wu, f0, F, D, D), D, lds, acc);
+  mm_phase<T, MB, 2>(mm_side(x, r0, rows, x_stride, D), mm_side(wg, f0, F, D, D), mm_side(wu, f0, F, D, D), D, lds, acc);
   const MmSide wd = mm_side(wd_t, f0, F, D, D);
-  mm_phase<T, 1>(mm_side(dy, r0, rows, D, D), wd, wd, D, lds, ds);
+  mm_phase<T, MB, 1>(mm_side(dy, r0, rows, D, D), wd, wd, D, lds, ds);
   const int lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const int64_t row = r0 + 64 * wm + 32 * m + ln;
+  for (int m = 0; m < MB; ++m) {
+    const int64_t row = r0 + 32 * (MB * wm + m) + ln;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int f = f0 + 32 * wn + 8 * q + 4 * hh;
@@ -193,33 +219,38 @@ __global__ void __launch_bounds__(MM_BLOCK) ff_grads_kernel(const T* __restrict_
 }
 
 // ------------------------------------------------------------------------------------------------ out = A0 B0^T (+ A1 B1^T)
-template <typename T>
-__global__ void __launch_bounds__(MM_BLOCK) ff_product_kernel(const T* __restrict__ a0, const T* __restrict__ b0, const T* __restrict__ a1,
-                                                              const T* __restrict__ b1, int64_t rows, int N, int K,
-                                                              T* __restrict__ out) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * 2 * MM_TILE];
+// Part blockIdx.y takes `span` of the contraction's columns (of both products); with more than one part the sums go to parts
+// [splits, rows, N] in fp32.
+template <typename T, int MB>
+__global__ void __launch_bounds__(MM_BLOCK, 2) ff_product_kernel(const T* __restrict__ a0, const T* __restrict__ b0,
+                                                                              const T* __restrict__ a1, const T* __restrict__ b1,
+                                                                              int64_t rows, int N, int K, int span, T* __restrict__ out,
+                                                                              float* __restrict__ parts) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * MM_STAGE(MB)];
   int64_t rt;
   int ct;
-  mm_place((rows + MM_ROWS - 1) / MM_ROWS, (N + 127) / 128, rt, ct);
-  const int64_t r0 = rt * MM_ROWS;
-  const int n0 = ct * 128;
-  f32x16 acc[2][2];
+  mm_place((rows + 64 * MB - 1) / (64 * MB), (N + 127) / 128, rt, ct);
+  const int64_t r0 = rt * (64 * MB);
+  const int n0 = ct * 128, k0 = blockIdx.y * span, width = K - k0 < span ? K - k0 : span;
+  f32x16 acc[MB][2];
   mm_clear(acc);
   for (int p = 0; p < (a1 ? 2 : 1); ++p) {
-    const T* b = p ? b1 : b0;
-    mm_phase<T, 2>(mm_side(p ? a1 : a0, r0, rows, K, K), mm_side(b, n0, N, K, K), mm_side(b, n0 + 64, N, K, K), K, lds, acc);
+    const T *a = (p ? a1 : a0) + k0, *b = (p ? b1 : b0) + k0;
+    mm_phase<T, MB, 2>(mm_side(a, r0, rows, K, width), mm_side(b, n0, N, K, width), mm_side(b, n0 + 64, N, K, width), width, lds, acc);
   }
   const int lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const int64_t row = r0 + 64 * wm + 32 * m + ln;
+  for (int m = 0; m < MB; ++m) {
+    const int64_t row = r0 + 32 * (MB * wm + m) + ln;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int n = n0 + 64 * b + 32 * wn + 8 * q + 4 * hh;
-        if (row < rows && n < N)
-          ff_store4(out + row * N + n, acc[m][b][4 * q], acc[m][b][4 * q + 1], acc[m][b][4 * q + 2], acc[m][b][4 * q + 3]);
+        if (row >= rows || n >= N) continue;
+        const f32x4 v = {acc[m][b][4 * q], acc[m][b][4 * q + 1], acc[m][b][4 * q + 2], acc[m][b][4 * q + 3]};
+        if (parts) *reinterpret_cast<f32x4*>(parts + ((int64_t)blockIdx.y * rows + row) * N + n) = v;
+        else ff_store4(out + row * N + n, v[0], v[1], v[2], v[3]);
       }
   }
 }
@@ -325,6 +356,21 @@ __global__ void __launch_bounds__(MM_BLOCK) ff_weights_kernel(const FfWeightJobs
 }
 
 // ------------------------------------------------------------------------------------------------ small kernels
+// The parts of up to three gradients (one behind the other in a part) in order, in one launch.
+template <typename T>
+struct FfSums {
+  T* out[3];
+};
+template <typename T>
+__global__ void __launch_bounds__(256) ff_sums_kernel(const float* __restrict__ parts, int n, int64_t cols, int64_t step, FfSums<T> to) {
+  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (c >= cols) return;
+  const float* p = parts + blockIdx.y * cols + c;
+  f32x4 sum = *reinterpret_cast<const f32x4*>(p);
+  for (int r = 1; r < n; ++r) sum += *reinterpret_cast<const f32x4*>(p + r * step);
+  ff_store4(to.out[blockIdx.y] + c, sum[0], sum[1], sum[2], sum[3]);
+}
+
 // out [cols, rows] = in [rows, cols]^T in tiles of 32 x 32; three matrices side by side in the grid's third dimension.
 struct FfTurns {
   const void* in[3];
@@ -360,37 +406,89 @@ static int ff_splits(const lampa_ff_args* a) {
   return (int)(n < 1 ? 1 : n);
 }
 
+// Rows of a tile (64 times this): 128 where that leaves two workgroups a CU, as many as it holds, else 64, so that few rows, and fp32
+// products, which take 16 times as long, spread over the GPU (fp32 gradients of 2 000 rows, D = 512, F = 1024: 67 us with tiles of
+// 128 from one workgroup a CU on, 63 so). 256 rows, one workgroup a CU, take longer at 8 192 x 768, F = 2048: 92 us against 75.
+static int ff_row_blocks(int64_t rows, int cols, int wide) { return (rows + 127) / 128 * ((cols + wide - 1) / wide) >= 512 ? 2 : 1; }
+// How a product's contraction is shared out: where its tiles leave CUs idle, over as many workgroups as fill them, of 4 steps or more.
+struct FfSplit {
+  int mb, n, span;
+};
+static FfSplit ff_split(const lampa_ff_args* a) {
+  FfSplit s;
+  s.mb = ff_row_blocks(a->rows, a->D, 128);
+  const int64_t tiles = (a->rows + 64 * s.mb - 1) / (64 * s.mb) * ((a->D + 127) / 128);
+  const int step = MM_ROW_BYTES / (int)ff_size(a), steps = (a->F + step - 1) / step;
+  const int64_t want = tiles ? 256 / tiles : 1;
+  int n = (int)(want < steps / 4 ? want : steps / 4);
+  if (n < 1) n = 1;
+  const int per = (steps + n - 1) / n;
+  s.n = (steps + per - 1) / per;
+  s.span = per * step;
+  return s;
+}
+
 struct FfAreas {
-  int64_t hidden, dg, du, turned, parts, total;  // turned: Wd^T, Wg^T, Wu^T one behind the other
+  int64_t hidden, dg, du, turned, sums, parts, total;  // turned: Wd^T, Wg^T, Wu^T one behind the other
 };
 static FfAreas ff_areas(const lampa_ff_args* a, int backward) {
   const int64_t e = ff_size(a), h = ff_area(a->rows * a->F, e), w = ff_area((int64_t)a->D * a->F, e);
+  const FfSplit sp = ff_split(a);
   FfAreas l{};
   l.hidden = 0;
   l.dg = h;
   l.du = l.dg + (backward ? h : 0);
   l.turned = l.du + (backward ? h : 0);
-  l.parts = l.turned + (backward ? 3 * w : 0);
+  l.sums = l.turned + (backward ? 3 * w : 0);
+  l.parts = l.sums + (sp.n > 1 ? ff_area((int64_t)sp.n * a->rows * a->D, 4) : 0);
   l.total = l.parts + (backward ? ff_area((int64_t)ff_splits(a) * 3 * a->D * a->F, 4) : 0);
   return l;
 }
 int64_t ff_gemm_workspace(const lampa_ff_args* a, int backward) { return ff_areas(a, backward).total; }
 
-static unsigned ff_tiles(int64_t rows, int cols, int wide) {
-  return (unsigned)((rows + MM_ROWS - 1) / MM_ROWS * ((cols + wide - 1) / wide));
+static unsigned ff_tiles(int64_t rows, int mb, int cols, int wide) {
+  return (unsigned)((rows + 64 * mb - 1) / (64 * mb) * ((cols + wide - 1) / wide));
+}
+
+// Tiles shared out by columns: where Wg and Wu together are more than half an XCD's L2 of 4 MB and there are two tiles or more for
+// each (8 192 x 768, F = 2048: hidden 72 us against 76, grads 134 against 141).
+static bool ff_by_columns(const lampa_ff_args* a) { return 2 * (int64_t)a->D * a->F * ff_size(a) > 1 << 21 && a->F >= 1024; }
+static unsigned ff_column_tiles(int64_t rows, int mb, int F) {
+  return (unsigned)(8 * (((F + 63) / 64 + 7) / 8) * ((rows + 64 * mb - 1) / (64 * mb)));
+}
+
+#define FF_ROWS(MB, GO) \
+  if ((MB) == 1) GO(1); else GO(2);
+
+template <typename T>
+static int ff_product_go(const lampa_ff_args* a, const T* a0, const T* b0, const T* a1, const T* b1, T* out, float* sums, hipStream_t s) {
+  const FfSplit sp = ff_split(a);
+#define FF_GO(MB)                                                                                                                   \
+  hipLaunchKernelGGL((ff_product_kernel<T, MB>), dim3(ff_tiles(a->rows, MB, a->D, 128), (unsigned)sp.n), dim3(MM_BLOCK), 0, s, a0, b0, a1, \
+                     b1, a->rows, a->D, a->F, sp.span, out, sp.n > 1 ? sums : (float*)nullptr)
+  FF_ROWS(sp.mb, FF_GO)
+#undef FF_GO
+  LAMPA_PROF(s, "ff_product_kernel");
+  const int rc = lampa_launch_status();
+  if (rc != LAMPA_OK || sp.n == 1) return rc;
+  return ff_reduce<T>(sums, sp.n, a->rows * a->D, a->rows * a->D, out, s);
 }
 
 template <typename T, int ACT>
 static int ff_fwd_go(const lampa_ff_args* a, hipStream_t s) {
+  const FfAreas l = ff_areas(a, 0);
   T* hidden = (T*)a->workspace;
+  const bool columns = ff_by_columns(a);
   LAMPA_PROF(s, "start");
-  hipLaunchKernelGGL((ff_hidden_kernel<T, ACT>), dim3(ff_tiles(a->rows, a->F, 64)), dim3(MM_BLOCK), 0, s, (const T*)a->x, a->x_stride,
-                     (const T*)a->w_gate, (const T*)a->w_up, a->rows, a->D, a->F, hidden);
+#define FF_GO(MB)                                                                                                                    \
+  hipLaunchKernelGGL((ff_hidden_kernel<T, ACT, MB>), dim3(columns ? ff_column_tiles(a->rows, MB, a->F) : ff_tiles(a->rows, MB, a->F, 64)), dim3(MM_BLOCK), 0, s, (const T*)a->x, a->x_stride, \
+                     (const T*)a->w_gate, (const T*)a->w_up, a->rows, a->D, a->F, hidden, columns)
+  FF_ROWS(ff_row_blocks(a->rows, a->F, 64), FF_GO)
+#undef FF_GO
   LAMPA_PROF(s, "ff_hidden_kernel");
-  hipLaunchKernelGGL((ff_product_kernel<T>), dim3(ff_tiles(a->rows, a->D, 128)), dim3(MM_BLOCK), 0, s, (const T*)hidden,
-                     (const T*)a->w_down, (const T*)nullptr, (const T*)nullptr, a->rows, a->D, a->F, (T*)a->y);
-  LAMPA_PROF(s, "ff_product_kernel");
-  return lampa_launch_status();
+  const int rc = lampa_launch_status();
+  if (rc != LAMPA_OK) return rc;
+  return ff_product_go<T>(a, hidden, (const T*)a->w_down, nullptr, nullptr, (T*)a->y, (float*)((char*)a->workspace + l.sums), s);
 }
 
 template <typename T, int ACT>
@@ -401,47 +499,49 @@ static int ff_bwd_go(const lampa_ff_args* a, hipStream_t s) {
   T *hidden = (T*)(ws + l.hidden), *dg = (T*)(ws + l.dg), *du = (T*)(ws + l.du);
   T *wd_t = (T*)(ws + l.turned), *wg_t = (T*)(ws + l.turned + w), *wu_t = (T*)(ws + l.turned + 2 * w);
   float* parts = (float*)(ws + l.parts);
-  const bool weights = a->dw_gate || a->dw_up || a->dw_down;
+  const bool weights = a->dw_gate || a->dw_up || a->dw_down, columns = ff_by_columns(a);
   LAMPA_PROF(s, "start");
   const FfTurns turns{{a->w_down, a->w_gate, a->w_up}, {wd_t, wg_t, wu_t}, {a->D, a->F, a->F}, {a->F, a->D, a->D}};
   const int most = a->D > a->F ? a->D : a->F;
   hipLaunchKernelGGL((ff_turn_kernel<T>), dim3((most + 31) / 32, (most + 31) / 32, a->dx ? 3 : 1), dim3(256), 0, s, turns);
   LAMPA_PROF(s, "ff_turn_kernel");
-  hipLaunchKernelGGL((ff_grads_kernel<T, ACT>), dim3(ff_tiles(a->rows, a->F, 64)), dim3(MM_BLOCK), 0, s, (const T*)a->x, a->x_stride,
-                     (const T*)a->dy, (const T*)a->w_gate, (const T*)a->w_up, (const T*)wd_t, a->rows, a->D, a->F,
-                     a->dw_down ? hidden : (T*)nullptr, dg, du);
+#define FF_GO(MB)                                                                                                                     \
+  hipLaunchKernelGGL((ff_grads_kernel<T, ACT, MB>), dim3(columns ? ff_column_tiles(a->rows, MB, a->F) : ff_tiles(a->rows, MB, a->F, 64)), dim3(MM_BLOCK), 0, s, (const T*)a->x, a->x_stride, \
+                     (const T*)a->dy, (const T*)a->w_gate, (const T*)a->w_up, (const T*)wd_t, a->rows, a->D, a->F,                          \
+                     a->dw_down ? hidden : (T*)nullptr, dg, du, columns)
+  FF_ROWS(ff_row_blocks(a->rows, a->F, 64), FF_GO)
+#undef FF_GO
   LAMPA_PROF(s, "ff_grads_kernel");
+  int rc = lampa_launch_status();
+  if (rc != LAMPA_OK) return rc;
   if (a->dx) {
-    hipLaunchKernelGGL((ff_product_kernel<T>), dim3(ff_tiles(a->rows, a->D, 128)), dim3(MM_BLOCK), 0, s, (const T*)dg, (const T*)wg_t,
-                       (const T*)du, (const T*)wu_t, a->rows, a->D, a->F, (T*)a->dx);
-    LAMPA_PROF(s, "ff_product_kernel");
+    rc = ff_product_go<T>(a, dg, wg_t, du, wu_t, (T*)a->dx, (float*)(ws + l.sums), s);
+    if (rc != LAMPA_OK) return rc;
   }
-  if (weights) {
-    FfWeightJobs jobs{};
-    jobs.splits = ff_splits(a);
-    jobs.rows = a->rows;
-    jobs.per = lampa_align_up((a->rows + jobs.splits - 1) / jobs.splits, 64);
-    const int64_t size = (int64_t)a->D * a->F;
-    T* outs[3];
-    int tiles = 0;
-    auto add = [&](void* out, const void* A, int64_t as, const void* B, int64_t bs, int M, int N) {
-      if (!out) return;
-      FfWeightJob& j = jobs.job[jobs.n];
-      j = FfWeightJob{A, B, as, bs, jobs.n * size, M, N, (M + 127) / 128 * ((N + 127) / 128)};
-      tiles += j.tiles;
-      outs[jobs.n++] = (T*)out;
-    };
-    add(a->dw_gate, dg, a->F, a->x, a->x_stride, a->F, a->D);
-    add(a->dw_up, du, a->F, a->x, a->x_stride, a->F, a->D);
-    add(a->dw_down, a->dy, a->D, hidden, a->F, a->D, a->F);
-    jobs.part_step = jobs.n * size;
-    hipLaunchKernelGGL((ff_weights_kernel<T>), dim3((unsigned)tiles, (unsigned)jobs.splits), dim3(MM_BLOCK), 0, s, jobs, parts);
-    LAMPA_PROF(s, "ff_weights_kernel");
-    for (int j = 0; j < jobs.n; ++j) {
-      const int rc = ff_reduce<T>(parts + jobs.job[j].at, jobs.splits, size, jobs.part_step, outs[j], s);
-      if (rc != LAMPA_OK) return rc;
-    }
-  }
+  if (!weights) return LAMPA_OK;
+  FfWeightJobs jobs{};
+  jobs.splits = ff_splits(a);
+  jobs.rows = a->rows;
+  jobs.per = lampa_align_up((a->rows + jobs.splits - 1) / jobs.splits, 64);
+  const int64_t size = (int64_t)a->D * a->F;
+  FfSums<T> outs{};
+  int tiles = 0;
+  auto add = [&](void* out, const void* A, int64_t as, const void* B, int64_t bs, int M, int N) {
+    if (!out) return;
+    FfWeightJob& j = jobs.job[jobs.n];
+    j = FfWeightJob{A, B, as, bs, jobs.n * size, M, N, (M + 127) / 128 * ((N + 127) / 128)};
+    tiles += j.tiles;
+    outs.out[jobs.n++] = (T*)out;
+  };
+  add(a->dw_gate, dg, a->F, a->x, a->x_stride, a->F, a->D);
+  add(a->dw_up, du, a->F, a->x, a->x_stride, a->F, a->D);
+  add(a->dw_down, a->dy, a->D, hidden, a->F, a->D, a->F);
+  jobs.part_step = jobs.n * size;
+  hipLaunchKernelGGL((ff_weights_kernel<T>), dim3((unsigned)tiles, (unsigned)jobs.splits), dim3(MM_BLOCK), 0, s, jobs, parts);
+  LAMPA_PROF(s, "ff_weights_kernel");
+  hipLaunchKernelGGL((ff_sums_kernel<T>), dim3((unsigned)((size / 4 + 255) / 256), (unsigned)jobs.n), dim3(256), 0, s, parts, jobs.splits,
+                     size, jobs.part_step, outs);
+  LAMPA_PROF(s, "ff_sums_kernel");
   return lampa_launch_status();
 }
 
