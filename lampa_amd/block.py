@@ -12,6 +12,10 @@ else runs in this package's HIP kernels. Forward only.
 ``models/baselines/full_mamba2.py:221-430``): projection -> short convolution + SiLU -> selective scan -> gated norm -> output
 projection, with the norms at the borders fused with the residual add. They train (every operator has its gradients), take
 packed sequences, and continue from caches with whole prompts or one token at a time.
+
+``GatedRecurrentLayer``, ``GatedFeedForward`` and ``GatedRecurrentBlock`` are a block of a mixer with a per-channel recurrence and a
+gated feed-forward block behind each mixer (the wiring of ``GatedDeltaProductBlock``, ``modeling_gated_deltaproduct.py:995-1056``,
+whose second half is the reference's ``GatedMLP``, ``:310-324``), trained, prefilled and stepped in the same way.
 """
 import math
 
@@ -20,9 +24,11 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import lsh
+from .feed_forward import gated_feed_forward
 from .gated_delta import chunk_gated_delta_rule
 from .layer_ops import (PROJ_CONV_HIDDEN, FusedRMSNormSwishGate, RMSNorm, ShortConvolution, _sequences, causal_conv1d,
                         causal_conv1d_split, causal_conv1d_step, gdr_gates, norm_proj, norm_proj_supported, proj_conv, residual_norm)
+from .linear_recurrence import gated_recurrence, gated_recurrence_step
 from .state_space import state_space_scan, state_space_step
 
 
@@ -303,3 +309,104 @@ class StateSpaceBlock(nn.Module):
         for i, layer in enumerate(self.layers):
             h, residual = self._border(i, layer.step(h, caches[i]), residual)
         return h
+
+
+class GatedFeedForward(nn.Module):
+    """``GatedMLP`` (``modeling_gated_deltaproduct.py:310-324``): down_proj(act(gate_proj(x)) * up_proj(x)). Without
+    ``intermediate_size`` it is two thirds of ``hidden_ratio * hidden_size``, rounded up to a multiple of 256."""
+
+    def __init__(self, hidden_size: int = 128, hidden_ratio: float = 4, intermediate_size: int = None, activation: str = "silu"):
+        super().__init__()
+        if intermediate_size is None:
+            intermediate_size = 256 * -(-int(hidden_size * hidden_ratio * 2 / 3) // 256)
+        self.hidden_size, self.intermediate_size, self.activation = hidden_size, intermediate_size, activation
+        self.gate_proj = nn.Linear(hidden_size, intermediate_size, bias=False)
+        self.up_proj = nn.Linear(hidden_size, intermediate_size, bias=False)
+        self.down_proj = nn.Linear(intermediate_size, hidden_size, bias=False)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """x [..., hidden] -> [..., hidden]."""
+        return gated_feed_forward(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, self.activation)
+
+
+class GatedRecurrentLayer(nn.Module):
+    """in_proj -> x | z; causal convolution + SiLU over x; decay and input gates from it; gated linear recurrence with
+    A = -exp(A_log), its output gated by silu(z); out_proj. ``expand * hidden_size`` channels."""
+
+    def __init__(self, hidden_size: int = 128, expand: int = 2, conv_size: int = 4):
+        super().__init__()
+        inner = expand * hidden_size
+        self.hidden_size, self.inner, self.conv_size = hidden_size, inner, conv_size
+        self.in_proj = nn.Linear(hidden_size, 2 * inner, bias=False)
+        bound = conv_size ** -0.5
+        self.conv_weight = nn.Parameter(torch.empty(inner, conv_size).uniform_(-bound, bound))
+        self.conv_bias = nn.Parameter(torch.empty(inner).uniform_(-bound, bound))
+        self.gate_proj = nn.Linear(inner, 2 * inner)
+        # a token with an open decay gate keeps 0.9 .. 0.999 of the state
+        self.A_log = nn.Parameter(torch.log(-torch.log(torch.empty(inner).uniform_(0.9, 0.999))))
+        self.out_proj = nn.Linear(inner, hidden_size, bias=False)
+
+    def _gates(self, x):
+        return self.gate_proj(x).split([self.inner, self.inner], dim=-1)
+
+    def forward(self, hidden_states: torch.Tensor, cu_seqlens=None, cache=None, output_cache: bool = False):
+        """hidden_states [B, T, hidden] -> (out [B, T, hidden], cache or None). ``cache`` = (the last inputs of the convolution
+        [sequences, inner, conv_size], the states [sequences, inner] float32) as a call or ``step`` left them; no gradient runs
+        through the convolution's part. ``cu_seqlens`` as ``gated_recurrence`` takes it."""
+        cu_seqlens = _sequences("GatedRecurrentLayer", cu_seqlens, *hidden_states.shape[:2], hidden_states.device)
+        x, z = self.in_proj(hidden_states).split([self.inner, self.inner], dim=-1)
+        conv_cache, state = (None, None) if cache is None else cache
+        conv = causal_conv1d(x, self.conv_weight, self.conv_bias, activation="silu", cu_seqlens=cu_seqlens,
+                             initial_state=conv_cache, output_final_state=output_cache)
+        x, conv_cache = conv if output_cache else (conv, None)
+        r, i = self._gates(x)
+        y, state = gated_recurrence(x, r, -torch.exp(self.A_log.float()), input_gate=i, gate=z, gate_activation="silu",
+                                    initial_state=state, output_final_state=output_cache, cu_seqlens=cu_seqlens)
+        return self.out_proj(y), (conv_cache, state) if output_cache else None
+
+    @torch.no_grad()
+    def step(self, hidden_states: torch.Tensor, cache):
+        """One token for each sequence: hidden_states [sequences, hidden] -> [sequences, hidden]; the cache is moved on in place."""
+        x, z = self.in_proj(hidden_states).split([self.inner, self.inner], dim=-1)
+        x = causal_conv1d_step(x, cache[0], self.conv_weight, self.conv_bias, "silu")
+        r, i = self._gates(x)
+        y = gated_recurrence_step(x, r, -torch.exp(self.A_log.float()), cache[1], input_gate=i, gate=z, gate_activation="silu")
+        return self.out_proj(y)
+
+
+class GatedRecurrentBlock(nn.Module):
+    """``n_layers`` pre-norm residual pairs of a ``GatedRecurrentLayer`` and a ``GatedFeedForward``, and a final norm. The residual
+    add and the next norm are one operator; ``residual_in_fp32`` keeps the stream in float32 beside 16-bit layers."""
+
+    def __init__(self, hidden_size: int = 128, n_layers: int = 4, hidden_ratio: float = 4, intermediate_size: int = None,
+                 residual_in_fp32: bool = True, norm_eps: float = 1e-5, **layer_args):
+        super().__init__()
+        self.layers = nn.ModuleList([GatedRecurrentLayer(hidden_size, **layer_args) for _ in range(n_layers)])
+        self.feed_forward = nn.ModuleList([GatedFeedForward(hidden_size, hidden_ratio, intermediate_size) for _ in range(n_layers)])
+        self.norm_weights = nn.ParameterList([nn.Parameter(torch.ones(hidden_size)) for _ in range(2 * n_layers + 1)])
+        self.residual_in_fp32, self.norm_eps = residual_in_fp32, norm_eps
+
+    def _run(self, x, mix):
+        """x through all pairs; ``mix(i, h)`` is layer i's mixer."""
+        h = residual_norm(x, None, self.norm_weights[0], eps=self.norm_eps)
+        residual = x.float() if self.residual_in_fp32 else x
+        for i, feed_forward in enumerate(self.feed_forward):
+            h, residual = residual_norm(mix(i, h), residual, self.norm_weights[2 * i + 1], eps=self.norm_eps)
+            h, residual = residual_norm(feed_forward(h), residual, self.norm_weights[2 * i + 2], eps=self.norm_eps)
+        return h
+
+    def forward(self, x: torch.Tensor, cu_seqlens=None, caches=None, output_caches: bool = False):
+        """x [B, T, hidden] -> (normed output [B, T, hidden], the layers' caches or None)."""
+        cu_seqlens = _sequences("GatedRecurrentBlock", cu_seqlens, *x.shape[:2], x.device)
+        new = [None] * len(self.layers)
+
+        def mix(i, h):
+            out, new[i] = self.layers[i](h, cu_seqlens, None if caches is None else caches[i], output_caches)
+            return out
+
+        return self._run(x, mix), new if output_caches else None
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, caches):
+        """One token for each sequence: x [sequences, hidden]; the caches are moved on in place."""
+        return self._run(x, lambda i, h: self.layers[i].step(h, caches[i]))
