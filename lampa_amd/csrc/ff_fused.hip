@@ -22,6 +22,17 @@ __device__ __forceinline__ ff_u32x4 fu_load(__amdgpu_buffer_rsrc_t buf, unsigned
   return ff_load16(buf, c < D ? row_bytes + (unsigned)c * 2 : FF_OFF);
 }
 
+// v as element i of an operand, and, TWO, what its rounding left as that of another (none where there is no finite rest).
+template <bool TWO, typename T>
+__device__ __forceinline__ void fu_parts(float v, T& high, T& low, int i) {
+  const auto h = (__typeof__(high[0]))v;
+  high[i] = h;
+  if constexpr (TWO) {
+    const float rest = v - (float)h;
+    low[i] = (__typeof__(high[0]))(__builtin_fabsf(rest) < __builtin_inff() ? rest : 0.0f);
+  }
+}
+
 struct FuOut {
   const void *x, *dy, *wg, *wu, *wd;
   void* out;     // [rows, D] of the type, or
@@ -57,11 +68,14 @@ __device__ __forceinline__ typename OpVec<T>::x8 fu_turned(const T* tile, int co
   return out;
 }
 
-// WAVES waves of 32 rows each.
+// WAVES waves of 32 rows each. With 4, where the GPU has room (fu_share), hidden values enter the last products as two parts, their
+// rounding and what it left: what a few outputs are off by would else hang on a handful of roundings (one token of 128 columns: up to
+// 1.6 times the output's own rounding). With FU_WIDE, as one: their roundings, as large as the output's own, cost a third of the time.
 template <typename T, int ACT, int DB, int WAVES, bool BACK>
-__global__ void __launch_bounds__(64 * WAVES, 2) ff_out_kernel(const FuOut a) {
+__global__ void __launch_bounds__(64 * WAVES, WAVES == 4 ? 1 : 2) ff_out_kernel(const FuOut a) {
   typedef typename OpVec<T>::x8 x8;
   typedef typename OpVec<T>::x4 x4;
+  constexpr bool TWO = WAVES == 4;
   constexpr int KS = 2 * DB, WIDE = DB * 32, GS = (DB + 1) / 2 * 64, DS = BACK ? 32 : 40;  // elements between the rows of the tiles
   constexpr int BLOCK = 64 * WAVES, PIECES = 128 * DB, LOADS = (PIECES + BLOCK - 1) / BLOCK;  // 16-byte pieces of each matrix's chunk
   constexpr int STAGE = 2 * FU_CHUNK * GS + WIDE * DS, ROWS = 32 * WAVES;
@@ -151,9 +165,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ff_out_kernel(const FuOut a) {
   }
   f32x16 out[DB];
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+  for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) out[d][r] = 0.0f;
+    for (int r = 0; r < 16; ++r) out[d][r] = 0.0f;
   stage(0);
   ff_loads_done();
   if (c0 + 1 < c1) fetch(c0 + 1);
@@ -189,10 +203,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ff_out_kernel(const FuOut a) {
       if (chunk + 2 < c1) stage(s2);  // requested a whole chunk ago
       if (chunk + 3 < c1) fetch(chunk + 3);
       const T* w = lds + slot * STAGE + 2 * FU_CHUNK * GS;
-      x8 h[2];
+      x8 h[2], low[2];
       auto act = [&](int k) {
 #pragma unroll
-        for (int r = 16 * k / KS; r < 16 * (k + 1) / KS; ++r) h[r / 8][r % 8] = (T)(ff_act<ACT>(G[r]) * U[r]);
+        for (int r = 16 * k / KS; r < 16 * (k + 1) / KS; ++r) fu_parts<TWO>(ff_act<ACT>(G[r]) * U[r], h[r / 8], low[r / 8], r % 8);
       };
       if (chunk + 1 < c1) {
         first(lds + s1 * STAGE, G1, U1, act);
@@ -204,7 +218,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ff_out_kernel(const FuOut a) {
 #pragma unroll
       for (int m = 0; m < 2 * DB + FU_AHEAD; ++m) {
         if (m < 2 * DB) da[m] = *reinterpret_cast<const x8*>(w + (32 * (m % DB) + ln) * DS + 16 * (m / DB) + 8 * hh);
-        if (m >= FU_AHEAD) out[(m - FU_AHEAD) % DB] = mfma32(da[m - FU_AHEAD], h[(m - FU_AHEAD) / DB], out[(m - FU_AHEAD) % DB]);
+        if (m >= FU_AHEAD) {
+          const int n = m - FU_AHEAD;
+          out[n % DB] = mfma32(da[n], h[n / DB], out[n % DB]);
+          if constexpr (TWO) out[n % DB] = mfma32(da[n], low[n / DB], out[n % DB]);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
       lds_barrier();
@@ -226,63 +244,50 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ff_out_kernel(const FuOut a) {
       const T *g = lds + which * STAGE, *u = g + FU_CHUNK * GS, *w = u + FU_CHUNK * GS;
       f32x16 G, U, S;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) G[r] = U[r] = S[r] = 0.0f;
+      for (int r = 0; r < 16; ++r) G[r] = U[r] = S[r] = 0.0f;
       // operands are read FU_AHEAD steps ahead of their products, held there by the barriers (left to itself the compiler reads each just
       // before its product and waits)
-      {
-        x8 ga[KS], ua[KS], wa[BACK ? KS : 1];
+      x8 ga[KS], ua[KS], wa[KS];
 #pragma unroll
-        for (int k = 0; k < KS + FU_AHEAD; ++k) {
-          if (k < KS) {
-            ga[k] = fu_along<T, GS>(g, gl, 16 * k + 8 * hh);
-            ua[k] = fu_along<T, GS>(u, gl, 16 * k + 8 * hh);
-            if constexpr (BACK) wa[k] = down_turned(w, 16 * k);
-          }
-          if (k >= FU_AHEAD) {
-            const int m = k - FU_AHEAD;
-            {
-              G = mfma32(ga[m], xo[m], G);
-              U = mfma32(ua[m], xo[m], U);
-              if constexpr (BACK) S = mfma32(wa[m], dyo[m], S);
-            }
-          }
-          __builtin_amdgcn_sched_barrier(0);
+      for (int k = 0; k < KS + FU_AHEAD; ++k) {
+        if (k < KS) {
+          ga[k] = fu_along<T, GS>(g, gl, 16 * k + 8 * hh);
+          ua[k] = fu_along<T, GS>(u, gl, 16 * k + 8 * hh);
+          wa[k] = down_turned(w, 16 * k);
         }
+        if (k >= FU_AHEAD) {
+          const int m = k - FU_AHEAD;
+          G = mfma32(ga[m], xo[m], G);
+          U = mfma32(ua[m], xo[m], U);
+          S = mfma32(wa[m], dyo[m], S);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      x8 da[2 * DB], db[BACK ? 2 * DB : 1];
+      x8 da[2 * DB], db[2 * DB];
       auto last_operands = [&](int m) {
-        const int s = m / DB, d = m % DB;
-        if constexpr (BACK) {
-          da[m] = fu_turned<T, GS>(g, 32 * d, 16 * s, lane);
-          db[m] = fu_turned<T, GS>(u, 32 * d, 16 * s, lane);
-        } else {
-          da[m] = *reinterpret_cast<const x8*>(w + (32 * d + ln) * DS + 16 * s + 8 * hh);
-        }
+        da[m] = fu_turned<T, GS>(g, 32 * (m % DB), 16 * (m / DB), lane);
+        db[m] = fu_turned<T, GS>(u, 32 * (m % DB), 16 * (m / DB), lane);
       };
 #pragma unroll
       for (int m = 0; m < FU_AHEAD && m < 2 * DB; ++m) last_operands(m);
       __builtin_amdgcn_sched_barrier(0);
-      x8 h0[2], h1[2];
-      {
+      x8 dg[2], du[2], dg_low[2], du_low[2];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          if constexpr (BACK) {
-            float value, slope;
-            ff_act_slope<ACT>(G[r], value, slope);
-            h0[r / 8][r % 8] = (T)(S[r] * U[r] * slope);
-            h1[r / 8][r % 8] = (T)(S[r] * value);
-          } else {
-            h0[r / 8][r % 8] = (T)(ff_act<ACT>(G[r]) * U[r]);
-          }
-        }
+      for (int r = 0; r < 16; ++r) {
+        float value, slope;
+        ff_act_slope<ACT>(G[r], value, slope);
+        fu_parts<TWO>(S[r] * U[r] * slope, dg[r / 8], dg_low[r / 8], r % 8);
+        fu_parts<TWO>(S[r] * value, du[r / 8], du_low[r / 8], r % 8);
       }
 #pragma unroll
       for (int m = 0; m < 2 * DB; ++m) {
         const int s = m / DB, d = m % DB;
         if (m + FU_AHEAD < 2 * DB) last_operands(m + FU_AHEAD);
-        {
-          out[d] = mfma32(da[m], h0[s], out[d]);
-          if constexpr (BACK) out[d] = mfma32(db[m], h1[s], out[d]);
+        out[d] = mfma32(da[m], dg[s], out[d]);
+        out[d] = mfma32(db[m], du[s], out[d]);
+        if constexpr (TWO) {
+          out[d] = mfma32(da[m], dg_low[s], out[d]);
+          out[d] = mfma32(db[m], du_low[s], out[d]);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -290,38 +295,33 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ff_out_kernel(const FuOut a) {
     }
   }
   if (a.parts) {
-    {
-      const int row = 32 * wave + ln;
-      if (row >= here) return;
+    const int row = 32 * wave + ln;
+    if (row >= here) return;
+    float* p = a.parts + ((int64_t)blockIdx.y * a.rows + r0 + row) * D;
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int c = 32 * d + 8 * q + 4 * hh;
-          if (c < D)
-            *reinterpret_cast<f32x4*>(a.parts + ((int64_t)blockIdx.y * a.rows + r0 + row) * D + c) =
-                f32x4{out[d][4 * q], out[d][4 * q + 1], out[d][4 * q + 2], out[d][4 * q + 3]};
-        }
-    }
+      for (int q = 0; q < 4; ++q) {
+        const int c = 32 * d + 8 * q + 4 * hh;
+        if (c < D) *reinterpret_cast<f32x4*>(p + c) = f32x4{out[d][4 * q], out[d][4 * q + 1], out[d][4 * q + 2], out[d][4 * q + 3]};
+      }
     return;
   }
   // through LDS (the tiles have been read), so that a row is written in pieces of 16 bytes side by side
   constexpr int OS = WIDE + 8;
   T* o = lds + wave * 32 * OS;
   const __amdgpu_buffer_rsrc_t ob = ff_buffer((T*)a.out + r0 * D, (int64_t)here * D * 2);
-  {
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+  for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        ff_store4(o + ln * OS + 32 * d + 8 * q + 4 * hh, out[d][4 * q], out[d][4 * q + 1], out[d][4 * q + 2], out[d][4 * q + 3]);
-    lds_fence();
+    for (int q = 0; q < 4; ++q)
+      ff_store4(o + ln * OS + 32 * d + 8 * q + 4 * hh, out[d][4 * q], out[d][4 * q + 1], out[d][4 * q + 2], out[d][4 * q + 3]);
+  lds_fence();
 #pragma unroll
-    for (int i = 0; i < 2 * DB; ++i) {
-      const int id = lane + 64 * i, row = id / (DB * 4), c = id % (DB * 4) * 8;
-      const ff_u32x4 v = *reinterpret_cast<const ff_u32x4*>(o + row * OS + c);
-      __builtin_amdgcn_raw_buffer_store_b128(v, ob, c < D ? (unsigned)((32 * wave + row) * D + c) * 2 : FF_OFF, 0, 0);
-    }
+  for (int i = 0; i < 2 * DB; ++i) {
+    const int id = lane + 64 * i, row = id / (DB * 4), c = id % (DB * 4) * 8;
+    const ff_u32x4 v = *reinterpret_cast<const ff_u32x4*>(o + row * OS + c);
+    __builtin_amdgcn_raw_buffer_store_b128(v, ob, c < D ? (unsigned)((32 * wave + row) * D + c) * 2 : FF_OFF, 0, 0);
   }
 }
 
