@@ -78,9 +78,10 @@ class _GatedFeedForward(torch.autograd.Function):
         tensors = ctx.saved_tensors
         x = tensors[0]
         make = torch.empty if x.numel() else torch.zeros  # without rows nothing is launched
-        grads = tuple(make(t.shape, dtype=t.dtype, device=t.device) if need else None
-                      for t, need in zip(tensors, ctx.needs_input_grad))
-        _launch(_capi.lib().lampa_ff_bwd, "lampa_ff_bwd", *tensors, ctx.act, None, _packed(dy.to(x.dtype)), grads)
+        grads = [make(t.shape, dtype=t.dtype, device=t.device) if need else None for t, need in zip(tensors, ctx.needs_input_grad)]
+        if dy.dtype != x.dtype:
+            dy = dy.to(x.dtype)
+        _launch(_capi.lib().lampa_ff_bwd, "lampa_ff_bwd", *tensors, ctx.act, None, _packed(dy), grads)
         return (*grads, None)
 
 

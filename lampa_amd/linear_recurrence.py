@@ -35,10 +35,13 @@ def _rows(t, D):
     apart (a token of each of several long sequences)."""
     if t is None:
         return None, D
-    t, step = _tokens(t, D)
-    if step > MAX_STRIDE:
-        return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t.detach()), D
-    return t, step
+    B, T, _ = t.shape
+    sb, step, inner = t.stride()
+    if T == 1:
+        step = sb if B > 1 else D
+    if (inner == 1 or D == 1) and D <= step <= MAX_STRIDE and (B == 1 or T == 1 or sb == T * step):
+        return t, step
+    return torch.empty((B, T, D), dtype=t.dtype, device=t.device).copy_(t.detach()), D
 
 
 @functools.lru_cache(maxsize=4096)
@@ -82,9 +85,13 @@ def _scan_backward(x, r, A, i, z, act, normalize, h0, cu, tiles, dy, dht):
     dev = x.device
     _, size = _sizes(B, T, D, n_seq, cu is not None, _DTYPES[x.dtype], 1)
     h0 = _plain_f32(h0)
-    dy = torch.zeros((B, T, D), dtype=x.dtype, device=dev) if dy is None else dy.to(x.dtype).contiguous()
-    new = lambda t: None if t is None else torch.empty((B, T, D), dtype=x.dtype, device=dev)  # noqa: E731
-    dx, dr, di, dz = new(x), new(r), new(i), new(z)
+    if dy is None:
+        dy = torch.zeros((B, T, D), dtype=x.dtype, device=dev)
+    elif dy.dtype != x.dtype or not dy.is_contiguous():
+        dy = dy.to(x.dtype).contiguous()
+    dx, dr = torch.empty_like(dy), torch.empty_like(dy)
+    di = None if i is None else torch.empty_like(dy)
+    dz = None if z is None else torch.empty_like(dy)
     dA = torch.empty(D, dtype=torch.float32, device=dev)
     dh0 = None if h0 is None else torch.empty((n_seq, D), dtype=torch.float32, device=dev)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
@@ -117,7 +124,11 @@ class _GatedRecurrence(torch.autograd.Function):
             raise RuntimeError("gated_recurrence: the final state has been modified by an inplace operation (a step that moved it "
                                "on) before the gradients of the call that returned it; give gated_recurrence_step a new_state")
         dx, dr, dA, di, dz, dh0 = _scan_backward(x, r, A, i, z, ctx.act, ctx.normalize, h0, cu, tiles, dy, dht)
-        return (dx, dr, dA.to(A.dtype), di, dz, None if h0 is None else dh0.to(h0.dtype), None, None, None, None, None)
+        if A.dtype != torch.float32:
+            dA = dA.to(A.dtype)
+        if h0 is not None and h0.dtype != torch.float32:
+            dh0 = dh0.to(h0.dtype)
+        return dx, dr, dA, di, dz, dh0, None, None, None, None, None
 
 
 def _check_operands(what, x, decay_gate, A, input_gate, gate, gate_activation, dims):
