@@ -303,11 +303,12 @@ __device__ __forceinline__ void lr_job(const LrArgs& a, int64_t& slot, int& cb) 
 
 // What a tile of the forward starts from (or, BACK, what reaches a tile from behind), in every thread for its channels; leaves the
 // group's map and the block's state where the tile is the last of one. `place` counts the sequence's tiles in the order of the walk,
-// Pt and Ht are the tile's own map (in the threads of run `writer`), `more`: tiles follow.
-template <int V, int BLOCK, bool BACK>
+// Pt and Ht are the tile's own map (in the threads of run `writer`), `more`: tiles follow; `meanwhile` is called once the first look is
+// under way, for loads that nobody waits for.
+template <int V, int BLOCK, bool BACK, typename F>
 __device__ __forceinline__ void lr_enter(const LrArgs& a, const LrTile& s, int64_t slot, int place, int c, bool on, int lane, int run,
                                          int writer, bool more, const float (&Pt)[V], const float (&Ht)[V], const float* first,
-                                         float2 (*sm)[V], float (*base)[V], float (&h)[V]) {
+                                         float2 (*sm)[V], float (*base)[V], float (&h)[V], F meanwhile) {
   const int runs = BLOCK / a.lanes, pos = place % LR_GROUP, grp = place / LR_GROUP % LR_GROUP;
   const int64_t dir = BACK ? 1 : -1;  // towards the tiles that were walked before
   // each run takes `per` places of the group, and of the block's groups, oldest first
@@ -336,6 +337,7 @@ __device__ __forceinline__ void lr_enter(const LrArgs& a, const LrTile& s, int64
     }
   };
   look_state();
+  meanwhile();
   // a wait that runs out leaves empty words, which are NaN
   for (int polls = 0; !have_tiles && polls < LR_POLLS; ++polls) {
     __builtin_amdgcn_s_sleep(2);
@@ -418,7 +420,7 @@ __global__ void __launch_bounds__(LR_FWD_BLOCK) lr_fwd_kernel(const LrArgs a) {
     for (int j = 0; j < LR_TOK; ++j) lr_store<raw>(yb, yo + j * a.D * E, lr_narrow<T, V>(zero));
     return;
   }
-  raw rr[LR_TOK], rx[LR_TOK], ri[HASI ? LR_TOK : 1], rz[HASZ ? LR_TOK : 1];
+  raw rr[LR_TOK], rx[LR_TOK], ri[HASI ? LR_TOK : 1];
   {
     const __amdgpu_buffer_rsrc_t rb = lr_buffer(a.r, a.rs, E, s, a.D), xb = lr_buffer(a.x, a.xs, E, s, a.D);
     const unsigned ro = on ? (unsigned)(row * a.rs + c) * E : LR_OFF, xo = on ? (unsigned)(row * a.xs + c) * E : LR_OFF;
@@ -433,12 +435,6 @@ __global__ void __launch_bounds__(LR_FWD_BLOCK) lr_fwd_kernel(const LrArgs a) {
       const unsigned io = on ? (unsigned)(row * a.is + c) * E : LR_OFF, istep = (unsigned)a.is * E;
 #pragma unroll
       for (int j = 0; j < LR_TOK; ++j) ri[j] = lr_load<raw>(ib, io + j * istep);
-    }
-    if constexpr (HASZ) {
-      const __amdgpu_buffer_rsrc_t zb = lr_buffer(a.z, a.zs, E, s, a.D);
-      const unsigned zo = on ? (unsigned)(row * a.zs + c) * E : LR_OFF, zstep = (unsigned)a.zs * E;
-#pragma unroll
-      for (int j = 0; j < LR_TOK; ++j) rz[j] = lr_load<raw>(zb, zo + j * zstep);
     }
   }
   const int64_t left = s.t1 - s.t0 - row;
@@ -504,7 +500,15 @@ __global__ void __launch_bounds__(LR_FWD_BLOCK) lr_fwd_kernel(const LrArgs a) {
     if (last_run && on && !last_tile) lr_put_map(a.w.maps + slot * a.D + c + v, Pt[v], Ht[v]);
   }
   float h[V];
-  lr_enter<V, LR_FWD_BLOCK, false>(a, s, slot, s.index, c, on, lane, run, runs - 1, !last_tile, Pt, Ht, a.h0, before, base, h);
+  raw rz[HASZ ? LR_TOK : 1];
+  lr_enter<V, LR_FWD_BLOCK, false>(a, s, slot, s.index, c, on, lane, run, runs - 1, !last_tile, Pt, Ht, a.h0, before, base, h, [&]() {
+    if constexpr (HASZ) {  // the output's gate: not needed for the map that others wait for
+      const __amdgpu_buffer_rsrc_t zb = lr_buffer(a.z, a.zs, E, s, a.D);
+      const unsigned zo = on ? (unsigned)(row * a.zs + c) * E : LR_OFF, zstep = (unsigned)a.zs * E;
+#pragma unroll
+      for (int j = 0; j < LR_TOK; ++j) rz[j] = lr_load<raw>(zb, zo + j * zstep);
+    }
+  });
   if (on) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -680,7 +684,7 @@ __global__ void __launch_bounds__(LR_BWD_BLOCK, sizeof(T) == 2 ? 4 : 2) lr_bwd_k
     Pt[v] = Pa[v] * P[v];
     if (run == 0 && on && !first_tile) lr_put_map(a.w.maps + slot * a.D + c + v, Pt[v], Ct[v]);
   }
-  lr_enter<V, LR_BWD_BLOCK, true>(a, s, slot, place, c, on, lane, run, 0, !first_tile, Pt, Ct, a.dht, before, base, g);
+  lr_enter<V, LR_BWD_BLOCK, true>(a, s, slot, place, c, on, lane, run, 0, !first_tile, Pt, Ct, a.dht, before, base, g, []() {});
 #pragma unroll
   for (int v = 0; v < V; ++v) g[v] = __builtin_fmaf(Pa[v], g[v], Ca[v]);
   // hv[j] <- the state before token j: h under the decays so far, and what has come in since
