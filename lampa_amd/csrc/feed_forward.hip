@@ -33,7 +33,8 @@ extern "C" int lampa_ff_fwd(const lampa_ff_args* a, void* stream) {
   if (rc != LAMPA_OK) return rc;
   if (a->rows && !a->y) return LAMPA_ERR_INVALID;
   if (!a->rows) return LAMPA_OK;
-  return ff_fused_takes(a) ? ff_fused_fwd(a, (hipStream_t)stream) : ff_gemm_fwd(a, (hipStream_t)stream);
+  hipStream_t s = (hipStream_t)stream;
+  return !ff_fused_takes(a) ? ff_gemm_fwd(a, s) : a->dtype == GDR_BF16 ? ff_fused_fwd_bf16(a, s) : ff_fused_fwd_fp16(a, s);
 }
 
 // Without rows nothing is launched: the caller clears the weights' gradients itself.
@@ -44,5 +45,6 @@ extern "C" int lampa_ff_bwd(const lampa_ff_args* a, void* stream) {
   if (rc != LAMPA_OK) return rc;
   if (a->rows && !a->dy) return LAMPA_ERR_INVALID;
   if (!a->rows || (!a->dx && !a->dw_gate && !a->dw_up && !a->dw_down)) return LAMPA_OK;
-  return ff_fused_takes(a) ? ff_fused_bwd(a, (hipStream_t)stream) : ff_gemm_bwd(a, (hipStream_t)stream);
+  hipStream_t s = (hipStream_t)stream;
+  return !ff_fused_takes(a) ? ff_gemm_bwd(a, s) : a->dtype == GDR_BF16 ? ff_fused_bwd_bf16(a, s) : ff_fused_bwd_fp16(a, s);
 }

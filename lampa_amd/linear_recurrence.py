@@ -21,7 +21,7 @@ from torch.autograd.graph import increment_version
 from . import _capi
 from ._capi import check, ptr, stream_of
 from .gated_delta import _direct
-from .layer_ops import _ACT, _DTYPES, _ForwardOnly, _on_device, _plain_f32, _same_device, _sequences, _tokens, _wants_grad
+from .layer_ops import _ACT, _DTYPES, _ForwardOnly, _on_device, _plain_f32, _same_device, _sequences, _wants_grad
 
 MAX_CHANNELS = 1 << 20
 MAX_STRIDE = 1 << 20  # elements between tokens: the kernels form offsets inside a tile in 32 bits
@@ -193,9 +193,13 @@ def gated_recurrence(x: torch.Tensor, decay_gate: torch.Tensor, A: torch.Tensor,
 
 
 def _step_rows(t, D):
+    """(t, elements between rows) of t [n, D] whose rows are contiguous."""
     if t is None:
         return None, D
-    return (t, D) if t.is_contiguous() else _tokens(t.unsqueeze(0), D)
+    step, inner = t.stride()
+    if t.shape[0] == 1:
+        step = D
+    return (t, step) if (inner == 1 or D == 1) and step >= D else (t.contiguous(), D)
 
 
 def _step_launch(x, r, A, i, z, act, normalize, state, target):
