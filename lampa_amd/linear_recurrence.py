@@ -156,7 +156,8 @@ def gated_recurrence(x: torch.Tensor, decay_gate: torch.Tensor, A: torch.Tensor,
                      initial_state: Optional[torch.Tensor] = None, output_final_state: bool = False,
                      cu_seqlens: Optional[torch.Tensor] = None):
     """x, decay_gate, input_gate, gate [B, T, D] of one type (they may be column slices of wider tensors); A [D], the log of what a
-    token with an open decay gate keeps: at most 0 (above 0 the normalised recurrence is NaN; without ``normalize`` it grows).
+    token with an open decay gate keeps: at most 0 (above 0 the normalised recurrence is NaN; without ``normalize`` it grows, and past
+    float32's range within a sequence it may be NaN where the recurrence, on zeros, is not).
     ``input_gate`` None: a factor of 1; ``gate`` None: y = h; ``gate_activation`` ``None`` / ``'sigmoid'`` / ``'silu'`` /
     ``'swish'``; ``normalize=False`` leaves the factor sqrt(1 - a^2) out. Any D up to 2^20. Returns (y [B, T, D] in x's type,
     final state [sequences, D] float32 or None).
