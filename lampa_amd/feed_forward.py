@@ -92,8 +92,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     2^17. Returns [..., D] in x's type.
 
     Products have fp32 sums; for 16-bit types the hidden values act(.) * (.) (and, in the gradients, theirs) are rounded to the type
-    as the next product's operands (in float16 a hidden value past its range is infinite). Differentiable in every tensor (first order; the gradients compute the hidden values again, so
-    nothing but the inputs is kept; repeated calls give the same bits)."""
+    as the next product's operands (in float16 a hidden value past its range is infinite). Differentiable in every tensor (first
+    order; the gradients compute the hidden values again, so nothing but the inputs is kept; repeated calls give the same bits)."""
     what = "gated_feed_forward"
     _same_device(what, x, w_gate, w_up, w_down)
     if activation not in _ACT:

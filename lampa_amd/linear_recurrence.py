@@ -72,8 +72,8 @@ def _scan_launch(x, r, A, i, z, act, normalize, h0, want_final, cu, keep=False):
     ht = torch.empty((n_seq, D), dtype=torch.float32, device=dev) if want_final else None
     tiles = torch.empty((slots, D), dtype=torch.float32, device=dev) if keep else None
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    args = _pack(_rows(x, D), _rows(r, D), _rows(i, D), _rows(z, D), _plain_f32(A), _plain_f32(h0), y, ht, tiles, cu, _NO_GRADS, ws, size, act,
-                 normalize, n_seq)
+    held = _rows(x, D), _rows(r, D), _rows(i, D), _rows(z, D), _plain_f32(A), _plain_f32(h0)  # copies among them live until the launch
+    args = _pack(*held, y, ht, tiles, cu, _NO_GRADS, ws, size, act, normalize, n_seq)
     with _on_device(dev.index):
         check(_capi.lib().lampa_lr_scan_fwd(args, stream_of(y)), "lampa_lr_scan_fwd")
     return y, ht, tiles
@@ -95,8 +95,9 @@ def _scan_backward(x, r, A, i, z, act, normalize, h0, cu, tiles, dy, dht):
     dA = torch.empty(D, dtype=torch.float32, device=dev)
     dh0 = None if h0 is None else torch.empty((n_seq, D), dtype=torch.float32, device=dev)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    args = _pack(_rows(x, D), _rows(r, D), _rows(i, D), _rows(z, D), _plain_f32(A), h0, None, None, tiles, cu,
-                 (dy, _plain_f32(dht), dx, dr, di, dz, dA, dh0), ws, size, act, normalize, n_seq)
+    dht = _plain_f32(dht)
+    held = _rows(x, D), _rows(r, D), _rows(i, D), _rows(z, D), _plain_f32(A), h0  # copies among them live until the launch
+    args = _pack(*held, None, None, tiles, cu, (dy, dht, dx, dr, di, dz, dA, dh0), ws, size, act, normalize, n_seq)
     with _on_device(dev.index):
         check(_capi.lib().lampa_lr_scan_bwd(args, stream_of(dx)), "lampa_lr_scan_bwd")
     return dx, dr, dA, di, dz, dh0
