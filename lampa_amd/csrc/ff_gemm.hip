@@ -45,6 +45,11 @@ __device__ __forceinline__ MmSide mm_side(const T* base, int64_t first, int64_t 
   return {ff_buffer(base + (n ? first * stride : 0), n ? ((n - 1) * stride + K) * (int64_t)sizeof(T) : 0), (unsigned)(stride * sizeof(T))};
 }
 
+// 16 bytes of each lane from memory to LDS: lane l's go to p + 16 l, zeros where its offset is out of range.
+__device__ __forceinline__ void mm_load_lds(__amdgpu_buffer_rsrc_t buf, unsigned char* p, unsigned offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (__attribute__((address_space(3))) void*)p, 16, offset, 0, 0, 0);
+}
+
 // acc[m][b] += (B rows b) . (A rows m) over K: register r of a lane is B row 8 (r / 4) + 4 hh + r % 4 of its block, A row = lane % 32.
 // The wave's MB A blocks are rows 32 (MB wm + m), its B blocks rows 32 wn and 64 + 32 wn (the second from b1).
 template <typename T, int MB, int NB>
@@ -54,40 +59,24 @@ __device__ __forceinline__ void mm_phase(const MmSide& a, const MmSide& b0, cons
   constexpr int STAGE = MM_STAGE(MB);
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, hh = lane >> 5, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   const int steps = (K * (int)sizeof(T) + MM_ROW_BYTES - 1) / MM_ROW_BYTES;
-  ff_u32x4 ra[ACH], rb[BCH];
-  auto fetch = [&](int step) {
+  // A wave's load of 64 pieces of 16 bytes fills 8 rows of 128 bytes in LDS, lane by lane; which piece of the row a lane asks for makes
+  // the permutation. Loads come in the order they were asked for, so the wait for a step leaves the later steps' loads under way.
+  auto fetch = [&](int step, int which) {
+    unsigned char* p = lds + which * STAGE + __builtin_amdgcn_readfirstlane(wave) * 1024;
+    const int row = tid >> 3, at = step * MM_ROW_BYTES + ((tid & 7) ^ (row & 7)) * 16;
+    const bool in = at < K * (int)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < ACH; ++i) {
-      const int id = tid + i * MM_BLOCK, row = id >> 3, at = step * MM_ROW_BYTES + (id & 7) * 16;
-      ra[i] = ff_load16(a.buf, at < K * (int)sizeof(T) ? row * a.step + at : FF_OFF);
-    }
+    for (int i = 0; i < ACH; ++i) mm_load_lds(a.buf, p + i * 4096, in ? (row + 32 * i) * a.step + at : FF_OFF);
 #pragma unroll
-    for (int i = 0; i < BCH; ++i) {
-      const int id = tid + i * MM_BLOCK, row = id >> 3, at = step * MM_ROW_BYTES + (id & 7) * 16;
-      const unsigned off = at < K * (int)sizeof(T) ? (row & 63) * b0.step + at : FF_OFF;
-      rb[i] = ff_load16(i * MM_BLOCK / 8 >= 64 ? b1.buf : b0.buf, off);  // 32 rows a step of i
-    }
+    for (int i = 0; i < BCH; ++i)
+      mm_load_lds(i >= 2 ? b1.buf : b0.buf, p + ATILE + i * 4096, in ? (row + 32 * (i & 1)) * b0.step + at : FF_OFF);
   };
-  auto stage = [&](int which) {
-    unsigned char* p = lds + which * STAGE;
-#pragma unroll
-    for (int i = 0; i < ACH; ++i) {
-      const int id = tid + i * MM_BLOCK, row = id >> 3;
-      *reinterpret_cast<ff_u32x4*>(p + row * MM_ROW_BYTES + (((id & 7) ^ (row & 7)) * 16)) = ra[i];
-    }
-#pragma unroll
-    for (int i = 0; i < BCH; ++i) {
-      const int id = tid + i * MM_BLOCK, row = id >> 3;
-      *reinterpret_cast<ff_u32x4*>(p + ATILE + row * MM_ROW_BYTES + (((id & 7) ^ (row & 7)) * 16)) = rb[i];
-    }
-  };
-  fetch(0);
-  stage(0);
-  if (steps > 1) fetch(1);
-  lds_barrier();
+  fetch(0, 0);
   for (int step = 0; step < steps; ++step) {
-    if (step + 1 < steps) stage((step + 1) & 1);  // requested a whole step ago
-    if (step + 2 < steps) fetch(step + 2);
+    // this step's tiles are there for all waves, and the last step's are free
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    if (step + 1 < steps) fetch(step + 1, (step + 1) & 1);
     const unsigned char* p = lds + (step & 1) * STAGE;
     // operands are read a step ahead of their products, held there by the barriers
     ff_u32x4 fa[2][MB], fb[2][NB];
@@ -110,8 +99,8 @@ __device__ __forceinline__ void mm_phase(const MmSide& a, const MmSide& b0, cons
         for (int b = 0; b < NB; ++b) acc[m][b] = mm_mac<T>(fb[ks & 1][b], fa[ks & 1][m], acc[m][b]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    lds_barrier();
   }
+  lds_barrier();  // the tiles are free
 }
 
 template <int M, int N>
