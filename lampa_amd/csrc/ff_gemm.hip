@@ -6,15 +6,16 @@
 //            contraction);
 //   weights: dWg, dWu, dWd over the rows, split over the rows where that fills the GPU, the parts summed in a fixed order.
 // A workgroup has 4 waves in 2 x 2 over a tile of 128 (or 64) x 128 of the output (64 hidden columns of each product for `hidden` and
-// `grads`), tiles of 128 bytes of the contraction in LDS, double buffered, the next one under way in registers. A product with few
-// tiles has its contraction shared out and the parts summed in order. Rows of 128 bytes
-// are stored with their 16-byte pieces permuted by the row (piece ^ row % 8), so that the 32 rows of an operand read do not
-// meet in the same banks.
+// `grads`), tiles of 128 bytes of the contraction in LDS, double buffered, the next one on its way from memory to LDS past the registers
+// (through them: hidden 72 us, grads 134, weights 138). A product with few tiles has its contraction shared out and the parts summed
+// in order. Rows of 128 bytes are stored with their 16-byte pieces permuted by the row (piece ^ row / 2 % 8): 16 rows of an operand
+// read, 8 even and 8 odd ones, fill the 256 bytes of the banks once.
 //
-// Measured, 8 192 x 768, 2 048 hidden columns, bf16 (the library's 8 192 x 4 096 x 768 product alone 0.88 PFLOP/s): hidden 72 us (51.5 GFLOP,
-// 0.72 PFLOP/s), grads 134 us (77 GFLOP), y and dx about 45 and 76 us (25.8 and 51.5 GFLOP), weights 133 us (77 GFLOP). LDS
-// bounds them: a wave's 64 x 64 read and write 1.5 times what the matrix cores' time holds (without staging hidden takes 48 us, grads
-// 82). fp32, 1 501 x 96, 256 hidden columns: 8, 13, 13 and 24 us.
+// Measured, 8 192 x 768, 2 048 hidden columns, bf16 (the library's 8 192 x 4 096 x 768 product alone 0.88 PFLOP/s): hidden 66 us (51.5 GFLOP,
+// 0.78 PFLOP/s), grads 115 us (77 GFLOP), y and dx together 123 us (77 GFLOP), weights 118 us (77 GFLOP). The matrix cores are
+// busy for half of the time. It is neither LDS alone (without the conflicts of piece ^ row % 8, half of its cycles, hidden and grads
+// take 1% less), nor the loads: steps of 64 bytes, three ahead, take 72 and 136 us against 69 and 122, tiles of 256 rows by 8 waves, two
+// steps ahead, 72 and 125. fp32, 1 501 x 96, 256 hidden columns: 8, 13, 13 and 24 us.
 #include "ff_common.h"
 
 #define MM_BLOCK 256
@@ -60,10 +61,10 @@ __device__ __forceinline__ void mm_phase(const MmSide& a, const MmSide& b0, cons
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, hh = lane >> 5, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   const int steps = (K * (int)sizeof(T) + MM_ROW_BYTES - 1) / MM_ROW_BYTES;
   // A wave's load of 64 pieces of 16 bytes fills 8 rows of 128 bytes in LDS, lane by lane; which piece of the row a lane asks for makes
-  // the permutation. Loads come in the order they were asked for, so the wait for a step leaves the later steps' loads under way.
+  // the permutation.
   auto fetch = [&](int step, int which) {
     unsigned char* p = lds + which * STAGE + __builtin_amdgcn_readfirstlane(wave) * 1024;
-    const int row = tid >> 3, at = step * MM_ROW_BYTES + ((tid & 7) ^ (row & 7)) * 16;
+    const int row = tid >> 3, at = step * MM_ROW_BYTES + ((tid & 7) ^ (row >> 1 & 7)) * 16;
     const bool in = at < K * (int)sizeof(T);
 #pragma unroll
     for (int i = 0; i < ACH; ++i) mm_load_lds(a.buf, p + i * 4096, in ? (row + 32 * i) * a.step + at : FF_OFF);
@@ -81,7 +82,7 @@ __device__ __forceinline__ void mm_phase(const MmSide& a, const MmSide& b0, cons
     // operands are read a step ahead of their products, held there by the barriers
     ff_u32x4 fa[2][MB], fb[2][NB];
     auto read = [&](int ks) {
-      const int piece = ((ks * 2 + hh) ^ (ln & 7)) * 16;
+      const int piece = ((ks * 2 + hh) ^ (ln >> 1 & 7)) * 16;
 #pragma unroll
       for (int m = 0; m < MB; ++m) fa[ks & 1][m] = *reinterpret_cast<const ff_u32x4*>(p + (32 * (MB * wm + m) + ln) * MM_ROW_BYTES + piece);
 #pragma unroll
@@ -264,11 +265,10 @@ struct FfWeightJobs {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(MM_BLOCK) ff_weights_kernel(const FfWeightJobs jobs, float* __restrict__ parts) {
-  constexpr int BK = 128 / sizeof(T);              // rows of a step
-  constexpr int STRIDE = sizeof(T) == 2 ? 144 : 132;  // elements between a tile's rows: four rows of 32 bytes side by side fill 128
+__global__ void __launch_bounds__(MM_BLOCK, 2) ff_weights_kernel(const FfWeightJobs jobs, float* __restrict__ parts) {
+  constexpr int BK = 128 / sizeof(T);  // rows of a step
   constexpr int EPC = 16 / sizeof(T), CPR = 128 / EPC, CH = BK * CPR / MM_BLOCK;
-  __shared__ __attribute__((aligned(16))) T lds[2][2][BK * STRIDE];
+  __shared__ __attribute__((aligned(16))) T lds[2][2][BK * 128];
   int tile = blockIdx.x, j = 0;
   while (j + 1 < jobs.n && tile >= jobs.job[j].tiles) tile -= jobs.job[j++].tiles;
   const FfWeightJob& job = jobs.job[j];
@@ -277,60 +277,70 @@ __global__ void __launch_bounds__(MM_BLOCK) ff_weights_kernel(const FfWeightJobs
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, hh = lane >> 5, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   f32x16 acc[2][2];
   mm_clear(acc);
-  ff_u32x4 ra[CH], rb[CH];
-  auto fetch = [&](int64_t t0) {
+  // Rows of 128 columns in LDS, their pieces permuted so that the rows of an operand read meet in no bank. 16 bits: a read takes 64
+  // bytes of each of 8 rows, 16 lanes 32 bytes of 4 rows; 32 bytes of row r go to place ^ twist(r % 4) of 8, different in
+  // any 128 bytes for the 4 rows and in 256 for both halves. fp32: the lane halves read 128 bytes of rows 4 apart.
+  auto twist = [](int r) { return (r << 1) ^ (r & 1) ^ (r >> 1); };
+  auto fetch = [&](int64_t t0, T* to) {
     const int64_t n = end - t0 < BK ? end - t0 : BK;
     const __amdgpu_buffer_rsrc_t ab = ff_buffer((const T*)job.A + t0 * job.a_stride + m0, ((n - 1) * job.a_stride + job.M - m0) * (int64_t)sizeof(T));
     const __amdgpu_buffer_rsrc_t bb = ff_buffer((const T*)job.B + t0 * job.b_stride + n0, ((n - 1) * job.b_stride + job.N - n0) * (int64_t)sizeof(T));
+    const int row = tid / CPR, piece = tid % CPR, c = (sizeof(T) == 2 ? piece ^ (twist(row & 3) << 1) : piece ^ ((row & 4) << 1)) * EPC;
+    unsigned char* p = reinterpret_cast<unsigned char*>(to) + __builtin_amdgcn_readfirstlane(wave) * 1024;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int id = tid + i * MM_BLOCK, row = id / CPR, c = id % CPR * EPC;
-      ra[i] = ff_load16(ab, m0 + c < job.M ? (unsigned)((row * job.a_stride + c) * sizeof(T)) : FF_OFF);
-      rb[i] = ff_load16(bb, n0 + c < job.N ? (unsigned)((row * job.b_stride + c) * sizeof(T)) : FF_OFF);
-    }
-  };
-  auto stage = [&](int which) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int id = tid + i * MM_BLOCK, row = id / CPR, c = id % CPR * EPC;
-      *reinterpret_cast<ff_u32x4*>(&lds[which][0][row * STRIDE + c]) = ra[i];
-      *reinterpret_cast<ff_u32x4*>(&lds[which][1][row * STRIDE + c]) = rb[i];
+      const int r = row + i * (MM_BLOCK / CPR);
+      mm_load_lds(ab, p + i * 4096, m0 + c < job.M ? (unsigned)((r * job.a_stride + c) * sizeof(T)) : FF_OFF);
+      mm_load_lds(bb, p + BK * 128 * sizeof(T) + i * 4096, n0 + c < job.N ? (unsigned)((r * job.b_stride + c) * sizeof(T)) : FF_OFF);
     }
   };
   auto operand = [&](const T* arr, int col0, int row0) -> ff_u32x4 {
-    if constexpr (sizeof(T) == 2) {
-      return __builtin_bit_cast(ff_u32x4, op_ld_kappa_tr<T>(arr, STRIDE, col0, row0, lane));
+    if constexpr (sizeof(T) == 2) {  // as op_ld_kappa_tr takes it
+      const int L = lane & 15;
+      const T* q = arr + (row0 + 4 * hh + (L >> 2)) * 128 + ((col0 / 16 + ((lane >> 4) & 1)) ^ twist(L >> 2)) * 16 + 4 * (L & 3);
+      const typename OpVec<T>::x4 lo = op_lds_read_tr4<T>(q), hi = op_lds_read_tr4<T>(q + 8 * 128);
+      typename OpVec<T>::x8 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v[e] = lo[e]; v[4 + e] = hi[e]; }
+      return __builtin_bit_cast(ff_u32x4, v);
     } else {
       f32x4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = arr[(row0 + 4 * hh + e) * STRIDE + col0 + ln];
+      for (int e = 0; e < 4; ++e) v[e] = arr[(row0 + 4 * hh + e) * 128 + (col0 ^ (32 * hh)) + ln];
       return __builtin_bit_cast(ff_u32x4, v);
     }
   };
   if (begin < end) {
-    fetch(begin);
-    stage(0);
-    if (begin + BK < end) fetch(begin + BK);
-    lds_barrier();
+    fetch(begin, lds[0][0]);
     int which = 0;
     for (int64_t t0 = begin; t0 < end; t0 += BK, which ^= 1) {
-      if (t0 + BK < end) stage(which ^ 1);  // requested a whole step ago
-      if (t0 + 2 * BK < end) fetch(t0 + 2 * BK);
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const int row0 = ks * BK / 4;
-        ff_u32x4 fa[2], fb[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          fa[k] = operand(lds[which][0], 64 * wm + 32 * k, row0);
-          fb[k] = operand(lds[which][1], 64 * wn + 32 * k, row0);
-        }
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int b = 0; b < 2; ++b) acc[m][b] = mm_mac<T>(fb[b], fa[m], acc[m][b]);
-      }
+      // this step's rows are there for all waves, and the last step's are free
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       lds_barrier();
+      // the next step's rows go to `there`, this step's are at `here`: told apart, so that reads do not wait for the loads
+      auto step = [&](T* __restrict__ there, const T* __restrict__ here) {
+        if (t0 + BK < end) fetch(t0 + BK, there);
+        ff_u32x4 fa[2][2], fb[2][2];
+        auto read = [&](int ks) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            fa[ks & 1][k] = operand(here, 64 * wm + 32 * k, ks * BK / 4);
+            fb[ks & 1][k] = operand(here + BK * 128, 64 * wn + 32 * k, ks * BK / 4);
+          }
+        };
+        read(0);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          if (ks + 1 < 4) read(ks + 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) acc[m][b] = mm_mac<T>(fb[ks & 1][b], fa[ks & 1][m], acc[m][b]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      step(lds[which ^ 1][0], lds[which][0]);
     }
   }
   float* out = parts + blockIdx.y * jobs.part_step + job.at;
@@ -400,17 +410,20 @@ static int ff_splits(const lampa_ff_args* a) {
   return (int)(n < 1 ? 1 : n);
 }
 
-// Rows of a tile (64 times this): 128 where that leaves two workgroups a CU, as many as it holds, else 64, so that few rows, and fp32
-// products, which take 16 times as long, spread over the GPU (fp32 gradients of 2 000 rows, D = 512, F = 1024: 67 us with tiles of
-// 128 from one workgroup a CU on, 63 so). 256 rows, one workgroup a CU, take longer at 8 192 x 768, F = 2048: 92 us against 75.
-static int ff_row_blocks(int64_t rows, int cols, int wide) { return (rows + 127) / 128 * ((cols + wide - 1) / wide) >= 512 ? 2 : 1; }
+// Rows of a tile (64 times this). 128 where that leaves a workgroup a CU (16 bits: y and dx of 8 192 x 768, 384 tiles, 62 us on average
+// against 69; of 4 100 x 1 024, 264 tiles, 53 against 59; hidden of 1 280 rows, 320 tiles, 16 against 17), in fp32, whose products
+// take 16 times as long, where it leaves two (gradients of 2 000 rows, D = 512, F = 1024: 67 us with tiles of 128 from one on,
+// 63 so); else 64, so that few rows spread over the GPU.
+static int ff_row_blocks(const lampa_ff_args* a, int cols, int wide) {
+  return (a->rows + 127) / 128 * ((cols + wide - 1) / wide) >= (a->dtype == GDR_FP32 ? 512 : 256) ? 2 : 1;
+}
 // How a product's contraction is shared out: where its tiles leave CUs idle, over as many workgroups as fill them, of 4 steps or more.
 struct FfSplit {
   int mb, n, span;
 };
 static FfSplit ff_split(const lampa_ff_args* a) {
   FfSplit s;
-  s.mb = ff_row_blocks(a->rows, a->D, 128);
+  s.mb = ff_row_blocks(a, a->D, 128);
   const int64_t tiles = (a->rows + 64 * s.mb - 1) / (64 * s.mb) * ((a->D + 127) / 128);
   const int step = MM_ROW_BYTES / (int)ff_size(a), steps = (a->F + step - 1) / step;
   const int64_t want = tiles ? 256 / tiles : 1;
@@ -445,7 +458,7 @@ static unsigned ff_tiles(int64_t rows, int mb, int cols, int wide) {
 }
 
 // Tiles shared out by columns: where Wg and Wu together are more than half an XCD's L2 of 4 MB and there are two tiles or more for
-// each (8 192 x 768, F = 2048: hidden 72 us against 76, grads 134 against 141).
+// each (8 192 x 768, F = 2048: hidden 69 us against 72, grads 121 against 130).
 static bool ff_by_columns(const lampa_ff_args* a) { return 2 * (int64_t)a->D * a->F * ff_size(a) > 1 << 21 && a->F >= 1024; }
 static unsigned ff_column_tiles(int64_t rows, int mb, int F) {
   return (unsigned)(8 * (((F + 63) / 64 + 7) / 8) * ((rows + 64 * mb - 1) / (64 * mb)));
@@ -477,7 +490,7 @@ static int ff_fwd_go(const lampa_ff_args* a, hipStream_t s) {
 #define FF_GO(MB)                                                                                                                    \
   hipLaunchKernelGGL((ff_hidden_kernel<T, ACT, MB>), dim3(columns ? ff_column_tiles(a->rows, MB, a->F) : ff_tiles(a->rows, MB, a->F, 64)), dim3(MM_BLOCK), 0, s, (const T*)a->x, a->x_stride, \
                      (const T*)a->w_gate, (const T*)a->w_up, a->rows, a->D, a->F, hidden, columns)
-  FF_ROWS(ff_row_blocks(a->rows, a->F, 64), FF_GO)
+  FF_ROWS(ff_row_blocks(a, a->F, 64), FF_GO)
 #undef FF_GO
   LAMPA_PROF(s, "ff_hidden_kernel");
   const int rc = lampa_launch_status();
@@ -503,7 +516,7 @@ static int ff_bwd_go(const lampa_ff_args* a, hipStream_t s) {
   hipLaunchKernelGGL((ff_grads_kernel<T, ACT, MB>), dim3(columns ? ff_column_tiles(a->rows, MB, a->F) : ff_tiles(a->rows, MB, a->F, 64)), dim3(MM_BLOCK), 0, s, (const T*)a->x, a->x_stride, \
                      (const T*)a->dy, (const T*)a->w_gate, (const T*)a->w_up, (const T*)wd_t, a->rows, a->D, a->F,                          \
                      a->dw_down ? hidden : (T*)nullptr, dg, du, columns)
-  FF_ROWS(ff_row_blocks(a->rows, a->F, 64), FF_GO)
+  FF_ROWS(ff_row_blocks(a, a->F, 64), FF_GO)
 #undef FF_GO
   LAMPA_PROF(s, "ff_grads_kernel");
   int rc = lampa_launch_status();
