@@ -48,6 +48,7 @@ struct LrSeqs {
   const int64_t* cu;  // device [n_seq + 1] or null: dense sequences of len tokens
   int64_t len, n_tokens;
   int n_seq, tile;    // tokens of a tile
+  bool one_tile;      // no more tokens than a tile: cu are the caller's boundaries, which nobody has put in order
 };
 struct LrTile {
   int64_t t0, t1;  // its tokens
@@ -60,11 +61,27 @@ __device__ __forceinline__ int64_t lr_bound(const LrSeqs& q, int i) {
   if (!q.cu) return (int64_t)i * q.len;
   if (i == 0) return 0;
   if (i > q.n_seq) return q.n_tokens;
-  const int64_t c = q.cu[i];
-  return c < 0 ? 0 : (c > q.n_tokens ? q.n_tokens : c);
+  return q.cu[i];
+}
+// Boundary i of a call of one tile: the largest of the first i as the caller gave them, held inside the tokens; by the whole wave.
+__device__ __forceinline__ int lr_bound_of_one_tile(const LrSeqs& q, int i) {
+  const int n = (int)q.n_tokens;
+  if (i > q.n_seq) return n;
+  int most = 0;
+  for (int64_t k = 1 + (threadIdx.x & 63); k <= i; k += 64) {
+    const int64_t c = q.cu[k];
+    const int in = c < 0 ? 0 : (c > n ? n : (int)c);
+    most = in > most ? in : most;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const int other = __shfl_xor(most, d);
+    most = other > most ? other : most;
+  }
+  return __builtin_amdgcn_readfirstlane(most);
 }
 // Sequence i takes its slots from floor(begin / tile) + i on: room for its ceil(length / tile) tiles (one where it is empty)
-// without knowing the lengths on the host.
+// without knowing the lengths on the host. In a call of one tile slot i is sequence i's.
 __device__ __forceinline__ LrTile lr_tile(const LrSeqs& q, int64_t slot) {
   LrTile s;
   int64_t b, e;
@@ -77,6 +94,14 @@ __device__ __forceinline__ LrTile lr_tile(const LrSeqs& q, int64_t slot) {
     s.first = s.seq * per;
     b = (int64_t)s.seq * q.len;
     e = b + q.len;
+  } else if (q.one_tile) {
+    s.live = slot <= q.n_seq;
+    s.seq = s.live ? (int)slot : q.n_seq;  // the rows behind the last sequence count as sequence n_seq
+    s.index = 0;
+    s.first = slot;
+    s.outside = s.seq == q.n_seq;
+    b = lr_bound_of_one_tile(q, s.seq);
+    e = lr_bound_of_one_tile(q, s.seq + 1);
   } else {
     int lo = 0, hi = q.n_seq;  // the rows behind the last sequence count as sequence n_seq
     while (lo < hi) {
@@ -881,7 +906,8 @@ static int lr_setup(const lampa_lr_args* a, int backward, LrArgs& k, int V, hipS
   k.w = LrWords{(unsigned*)ws, (unsigned long long*)(ws + l.maps), (unsigned long long*)(ws + l.maps) + k.slots * a->D,
                  (unsigned*)(ws + l.states), (int64_t*)(ws + l.cu)};
   k.handed_out = lr_handed_out(a);
-  k.q = LrSeqs{a->cu_seqlens ? (k.handed_out ? (const int64_t*)(ws + l.cu) : a->cu_seqlens) : nullptr, a->seq_len, a->n_tokens, a->n_seq, tile};
+  k.q = LrSeqs{a->cu_seqlens ? (k.handed_out ? (const int64_t*)(ws + l.cu) : a->cu_seqlens) : nullptr, a->seq_len, a->n_tokens, a->n_seq, tile,
+               !k.handed_out};
   k.D = a->D;
   k.lanes = lanes_of_tile;
   k.cblocks = (a->D + k.lanes * V - 1) / (k.lanes * V);
