@@ -241,6 +241,7 @@ def gated_recurrence_step(x: torch.Tensor, decay_gate: torch.Tensor, A: torch.Te
     target, act = state if new_state is None else new_state, _ACT[gate_activation]
     increment_version(target)  # written through its pointer: a backward that saved it must notice
     launch = lambda: _step_launch(x, decay_gate, A, input_gate, gate, act, bool(normalize), state, target)  # noqa: E731
-    if _wants_grad(x, decay_gate, A, input_gate, gate, state):
+    # a traced call has to be in the graph as a function; asking `_direct` takes a microsecond of a step's 13
+    if _wants_grad(x, decay_gate, A, input_gate, gate, state) or torch._C._get_tracing_state() is not None:
         return _ForwardOnly.apply(launch, x, decay_gate, A, input_gate, gate, state)
     return launch()

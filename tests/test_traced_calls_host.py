@@ -1,0 +1,55 @@
+"""A traced call is in the graph as the operator, not as the empty tensor that its kernel would have filled. The library is replaced here;
+nothing is launched."""
+import contextlib
+
+import pytest
+import torch
+
+from lampa_amd import feed_forward as ff
+from lampa_amd import linear_recurrence as lr
+from lampa_amd.gated_delta import _direct
+
+
+class Library:
+    def __getattr__(self, name):
+        return lambda *args: 0
+
+
+@pytest.fixture(autouse=True)
+def replaced(monkeypatch):
+    for module in (ff, lr):
+        monkeypatch.setattr(module, "_same_device", lambda *args: 0)
+        monkeypatch.setattr(module, "_on_device", lambda index: contextlib.nullcontext())
+        monkeypatch.setattr(module, "stream_of", lambda t: 0)
+        monkeypatch.setattr(module._capi, "lib", Library)
+    monkeypatch.setattr(lr, "_sizes", lambda *args: (2, 256))
+
+
+W = [torch.randn(8, 16), torch.randn(8, 16), torch.randn(16, 8)]
+A = -torch.rand(16)
+CALLS = {
+    "_GatedFeedForward": lambda x: ff.gated_feed_forward(x, *W),
+    "_GatedRecurrence": lambda x: lr.gated_recurrence(x[None], x[None], A)[0],
+    "_ForwardOnly": lambda x: lr.gated_recurrence_step(x, x, A, torch.zeros(4, 16)),
+}
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("grad", [False, True])
+def test_the_operator_is_in_the_graph(name, grad):
+    with torch.set_grad_enabled(grad):
+        graph = torch.jit.trace(CALLS[name], (torch.randn(4, 16),), check_trace=False).graph
+    (out,) = graph.outputs()
+    assert f"^{name}" in str(graph) and "aten::empty" not in str(out.node())
+
+
+def test_parameters_without_gradients_go_to_the_launcher():
+    """A module's weights under no_grad are plain tensors; where a gradient can be asked for, or in a subclass, they are not."""
+    class Other(torch.Tensor):
+        pass
+
+    weight = torch.nn.Parameter(torch.zeros(2))
+    assert not _direct(weight) and not _direct(torch.zeros(2).as_subclass(Other))
+    with torch.no_grad():
+        assert _direct(weight) and not _direct(torch.zeros(2).as_subclass(Other))
