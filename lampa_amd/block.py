@@ -325,8 +325,12 @@ class GatedFeedForward(nn.Module):
         self.down_proj = nn.Linear(intermediate_size, hidden_size, bias=False)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        """x [..., hidden] -> [..., hidden]."""
-        return gated_feed_forward(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, self.activation)
+        """x [..., hidden] -> [..., hidden]. Under autocast in its type, as the linear layers it stands for."""
+        tensors = x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight
+        if torch.is_autocast_enabled("cuda"):
+            dtype = torch.get_autocast_dtype("cuda")
+            tensors = [t if t.dtype == torch.float64 else t.to(dtype) for t in tensors]
+        return gated_feed_forward(*tensors, self.activation)
 
 
 class GatedRecurrentLayer(nn.Module):
