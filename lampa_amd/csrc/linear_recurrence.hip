@@ -311,26 +311,29 @@ struct LrArgs {
   int64_t xs, rs, is, zs;
   LrSeqs q;
   LrWords w;
-  int64_t slots;
+  int64_t slots, jobs;    // tiles, and their workgroups
   int D, lanes, cblocks;  // lanes side by side, workgroups over the channels
   int act, normalize;
   int handed_out;  // tiles wait for each other and are handed out by the counter
 };
 
-// The workgroup's tile and block of channels. BACK: in the order of the gradients, last tiles first.
+// The workgroup's tile and block of channels; false: none (the grid's last row is not full). BACK: in the order of the gradients, last
+// tiles first.
 template <bool BACK>
-__device__ __forceinline__ void lr_job(const LrArgs& a, int64_t& slot, int& cb) {
+__device__ __forceinline__ bool lr_job(const LrArgs& a, int64_t& slot, int& cb) {
   __shared__ unsigned ticket;
-  unsigned job = blockIdx.x;
+  unsigned job = blockIdx.y * gridDim.x + blockIdx.x;
   if (a.handed_out) {
     if (threadIdx.x == 0) ticket = atomicAdd(a.w.ticket, 1u);
     __syncthreads();
     job = ticket;
   }
   job = __builtin_amdgcn_readfirstlane(job);  // the same for all: tiles' places and buffers stay in scalar registers
+  if (job >= a.jobs) return false;
   slot = job / (unsigned)a.cblocks;
   cb = (int)(job % (unsigned)a.cblocks);
   if (BACK) slot = a.slots - 1 - slot;
+  return true;
 }
 
 // What a tile of the forward starts from (or, BACK, what reaches a tile from behind), in every thread for its channels; leaves the
@@ -435,7 +438,7 @@ __global__ void __launch_bounds__(LR_FWD_BLOCK) lr_fwd_kernel(const LrArgs a) {
   __shared__ float base[64][V];
   int64_t slot;
   int cb;
-  lr_job<false>(a, slot, cb);
+  if (!lr_job<false>(a, slot, cb)) return;
   const LrTile s = lr_tile(a.q, slot);
   if (!s.live) return;
   const int lane = threadIdx.x % a.lanes, run = threadIdx.x / a.lanes, runs = LR_FWD_BLOCK / a.lanes;
@@ -577,7 +580,7 @@ __global__ void __launch_bounds__(LR_BWD_BLOCK, sizeof(T) == 2 ? 4 : 2) lr_bwd_k
   __shared__ float base[64][V], carry[LR_BWD_BLOCK][V];
   int64_t slot;
   int cb;
-  lr_job<true>(a, slot, cb);
+  if (!lr_job<true>(a, slot, cb)) return;
   const LrTile s = lr_tile(a.q, slot);
   const int lane = threadIdx.x % a.lanes, run = threadIdx.x / a.lanes, runs = LR_BWD_BLOCK / a.lanes;
   const int c = (cb * a.lanes + lane) * V;
@@ -806,7 +809,7 @@ __global__ void __launch_bounds__(256) lr_step_kernel(const T* __restrict__ x, i
                                                       const T* __restrict__ gi, int64_t is, const T* __restrict__ z, int64_t zs,
                                                       const float* __restrict__ A, const float* state, float* new_state,
                                                       T* __restrict__ y, int64_t total, int D, int act, int normalize) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t at = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
   if (at >= total) return;
   const int64_t b = at / D;
   const int c = (int)(at % D);
@@ -913,7 +916,8 @@ static int lr_setup(const lampa_lr_args* a, int backward, LrArgs& k, int V, hipS
   k.cblocks = (a->D + k.lanes * V - 1) / (k.lanes * V);
   k.act = a->activation;
   k.normalize = a->normalize;
-  if (k.slots * k.cblocks > 0x7fffffff) return LAMPA_ERR_UNSUPPORTED;
+  k.jobs = k.slots * k.cblocks;
+  if (k.jobs > 0x7fffffff) return LAMPA_ERR_UNSUPPORTED;
   LAMPA_PROF(s, "start");
   if (k.handed_out) {
     const int64_t n_maps = (k.slots + k.slots / LR_GROUP + 1) * a->D, n_states = (k.slots / LR_BLOCK_TILES + 1) * a->D;
@@ -926,9 +930,15 @@ static int lr_setup(const lampa_lr_args* a, int backward, LrArgs& k, int V, hipS
   return LAMPA_OK;
 }
 
+// Workgroups in rows of LR_GRID_ROW: a launch takes fewer than 2^32 threads along one dimension.
+#define LR_GRID_ROW (1 << 22)
+static dim3 lr_grid(int64_t n) {
+  return dim3((unsigned)(n < LR_GRID_ROW ? n : LR_GRID_ROW), (unsigned)((n + LR_GRID_ROW - 1) / LR_GRID_ROW));
+}
+
 template <typename T, int V>
 static void lr_fwd_go(const LrArgs& k, hipStream_t s) {
-  const dim3 grid((unsigned)(k.slots * k.cblocks)), block(LR_FWD_BLOCK);
+  const dim3 grid = lr_grid(k.jobs), block(LR_FWD_BLOCK);
 #define LR_GO(I, Z) hipLaunchKernelGGL((lr_fwd_kernel<T, V, I, Z>), grid, block, 0, s, k)
   if (k.i) { if (k.z) LR_GO(true, true); else LR_GO(true, false); }
   else { if (k.z) LR_GO(false, true); else LR_GO(false, false); }
@@ -936,7 +946,7 @@ static void lr_fwd_go(const LrArgs& k, hipStream_t s) {
 }
 template <typename T, int V>
 static void lr_bwd_go(const LrArgs& k, hipStream_t s) {
-  const dim3 grid((unsigned)(k.slots * k.cblocks)), block(LR_BWD_BLOCK);
+  const dim3 grid = lr_grid(k.jobs), block(LR_BWD_BLOCK);
 #define LR_GO(I, Z) hipLaunchKernelGGL((lr_bwd_kernel<T, V, I, Z>), grid, block, 0, s, k)
   if (k.i) { if (k.z) LR_GO(true, true); else LR_GO(true, false); }
   else { if (k.z) LR_GO(false, true); else LR_GO(false, false); }
@@ -995,7 +1005,7 @@ static int lr_step_go(const void* x, int64_t xs, const void* r, int64_t rs, cons
                       const float* A, const float* state, float* new_state, void* y, int64_t total, int D, int act, int normalize,
                       hipStream_t s) {
   LAMPA_PROF(s, "start");
-  hipLaunchKernelGGL((lr_step_kernel<T>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, (const T*)x, xs, (const T*)r, rs,
+  hipLaunchKernelGGL((lr_step_kernel<T>), lr_grid((total + 255) / 256), dim3(256), 0, s, (const T*)x, xs, (const T*)r, rs,
                      (const T*)i, is, (const T*)z, zs, A, state, new_state, (T*)y, total, D, act, normalize);
   LAMPA_PROF(s, "lr_step_kernel");
   return lampa_launch_status();
