@@ -5,8 +5,8 @@ static int ff_check(const lampa_ff_args* a) {
   if (!a || a->rows < 0 || a->D < 1 || a->F < 1 || a->dtype < 0 || a->dtype > 2 || a->activation < 0 || a->activation > 2)
     return LAMPA_ERR_INVALID;
   if (a->D % 8 || a->F % 8 || a->D > (1 << 17) || a->F > (1 << 17)) return LAMPA_ERR_UNSUPPORTED;
-  // output tiles are numbered, and offsets inside a tile formed, in 32 bits
-  if (a->rows > (int64_t)1 << 31 || (a->rows + 127) / 128 * ((a->F + 63) / 64) > 0x7fffffff) return LAMPA_ERR_UNSUPPORTED;
+  // a launch takes fewer than 2^32 threads along one dimension: 512 for 256 rows, 256 for a tile of 128 rows x 64 hidden columns
+  if (a->rows > ((int64_t)1 << 31) - 256 || (a->rows + 127) / 128 * ((a->F + 63) / 64) >= 1 << 24) return LAMPA_ERR_UNSUPPORTED;
   return LAMPA_OK;
 }
 static int ff_check_operands(const lampa_ff_args* a, int64_t size) {
