@@ -1,7 +1,9 @@
-"""The gated recurrence at its edges: results that are zero by definition, boundaries out of order in short calls."""
+"""The gated recurrence at its edges: results that are zero by definition, boundaries out of order in short calls, steps in every
+type."""
 import pytest
 import torch
 
+from lampa_amd.linear_recurrence import gated_recurrence_step
 from test_gpu_linear_recurrence import _bounds, _call, _close, _expected, _gpu, _inputs
 
 pytestmark = pytest.mark.gpu
@@ -59,3 +61,21 @@ def test_boundaries_out_of_order_in_calls_of_one_tile(case):
         _close("last", last, *want["last"])
         for k in names:
             _close(k, grads[k][:, :end] if k in "xriz" else grads[k], *want[k])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
+@pytest.mark.parametrize("D,act,normalize", [(33, "silu", True), (512, "sigmoid", False), (130, None, True)])
+def test_steps_in_the_other_types(D, act, normalize, dtype):
+    """The token step against the definition where the other tests run it in bf16: sliced rows, with and without gates."""
+    n, T = 3, 5
+    t = _inputs((n, T), D, dtype, 43, n, i=act is not None, z=act is not None, sliced=True)
+    want = _expected(t, [T] * n, act, normalize)
+    g = _gpu(t)
+    state = g["h0"].clone()
+    for k in range(T):
+        at = {m: None if g[m] is None else g[m][:, k] for m in "xriz"}
+        y = gated_recurrence_step(at["x"], at["r"], g["A"], state, input_gate=at["i"], gate=at["z"], gate_activation=act,
+                                  normalize=normalize)
+        assert y.dtype == dtype
+        _close("y", y, want["y"][0].reshape(n, T, D)[:, k], want["y"][1].reshape(n, T, D)[:, k], dtype)
+    _close("last", state, *want["last"])
