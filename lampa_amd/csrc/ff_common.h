@@ -3,8 +3,9 @@
 //   gradients:  dS = dy Wd,  dG = dS * U * act'(G),  dU = dS * act(G),
 //               dx = dG Wg + dU Wu,  dWg = dG^T x,  dWu = dU^T x,  dWd = dy^T S.
 // Products run on the matrix cores with fp32 sums (16-bit inputs on the 16-bit instructions, fp32 inputs on the fp32 ones).
-// S, dG and dU are operands of further products: for 16-bit inputs they are rounded to the input type once (half a step of each, which
-// the outputs' own rounding equals), act and act' are taken from the unrounded fp32 sums in both passes.
+// S, dG and dU are operands of further products. For 16-bit inputs they are rounded to the input type, half a step of each, which comes to as
+// much as the outputs' own rounding; where the rows are few they enter as two parts, the rounding and what it left, so that outputs do not
+// hang on a handful of roundings (each form states its rule). act and act' are taken from the unrounded fp32 sums in both passes.
 #pragma once
 #include "../../include/lampa_amd.h"
 #include "gdr_ops.h"
@@ -49,6 +50,13 @@ template <typename T>
 __device__ __forceinline__ void ff_store4(T* p, float a, float b, float c, float d) {
   typedef T vec4 __attribute__((ext_vector_type(4)));
   *reinterpret_cast<vec4*>(p) = vec4{GdrElem<T>::from_float(a), GdrElem<T>::from_float(b), GdrElem<T>::from_float(c), GdrElem<T>::from_float(d)};
+}
+
+// What v's rounding to T leaves (none where there is no finite rest): v as two parts of T is off by half a step of half a step.
+template <typename T>
+__device__ __forceinline__ float ff_rest(float v) {
+  const float rest = v - GdrElem<T>::to_float(GdrElem<T>::from_float(v));
+  return __builtin_fabsf(rest) < __builtin_inff() ? rest : 0.0f;
 }
 
 // out[c] = sum over n rows, `step` values apart, of rows[c], in order; cols a multiple of 4.

@@ -131,11 +131,18 @@ __device__ __forceinline__ bool mm_place_columns(int col_tiles, int64_t& rt, int
   return ct < col_tiles;
 }
 
+// Four hidden values (or their gradients), and, where `low` is not 0, what their rounding leaves as many elements on.
+template <typename T>
+__device__ __forceinline__ void mm_store_parts(T* p, int64_t low, const float (&v)[4]) {
+  ff_store4(p, v[0], v[1], v[2], v[3]);
+  if (low) ff_store4(p + low, ff_rest<T>(v[0]), ff_rest<T>(v[1]), ff_rest<T>(v[2]), ff_rest<T>(v[3]));
+}
+
 // ------------------------------------------------------------------------------------------------ S = act(x Wg^T) (x Wu^T)
 template <typename T, int ACT, int MB>
 __global__ void __launch_bounds__(MM_BLOCK, 2) ff_hidden_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ wg,
                                                              const T* __restrict__ wu, int64_t rows, int D, int F,
-                                                             T* __restrict__ hidden, bool columns) {
+                                                             T* __restrict__ hidden, int64_t low, bool columns) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[2 * MM_STAGE(MB)];
   int64_t rt;
   int ct;
@@ -159,7 +166,7 @@ __global__ void __launch_bounds__(MM_BLOCK, 2) ff_hidden_kernel(const T* __restr
       float v[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] = ff_act<ACT>(acc[m][0][4 * q + k]) * acc[m][1][4 * q + k];
-      if (row < rows && f < F) ff_store4(hidden + row * F + f, v[0], v[1], v[2], v[3]);
+      if (row < rows && f < F) mm_store_parts(hidden + row * F + f, low, v);
     }
   }
 }
@@ -170,7 +177,7 @@ __global__ void __launch_bounds__(MM_BLOCK, 2) ff_grads_kernel(const T* __restri
                                                             const T* __restrict__ wg, const T* __restrict__ wu,
                                                             const T* __restrict__ wd_t, int64_t rows, int D, int F,
                                                             T* __restrict__ hidden, T* __restrict__ dg, T* __restrict__ du,
-                                                            bool columns) {
+                                                            int64_t low, bool columns) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[2 * MM_STAGE(MB)];
   int64_t rt;
   int ct;
@@ -205,9 +212,9 @@ __global__ void __launch_bounds__(MM_BLOCK, 2) ff_grads_kernel(const T* __restri
         u[k] = d * value;
       }
       if (row < rows && f < F) {
-        if (hidden) ff_store4(hidden + row * F + f, v[0], v[1], v[2], v[3]);
-        ff_store4(dg + row * F + f, g[0], g[1], g[2], g[3]);
-        ff_store4(du + row * F + f, u[0], u[1], u[2], u[3]);
+        if (hidden) mm_store_parts(hidden + row * F + f, low, v);
+        mm_store_parts(dg + row * F + f, low, g);
+        mm_store_parts(du + row * F + f, low, u);
       }
     }
   }
@@ -215,11 +222,11 @@ __global__ void __launch_bounds__(MM_BLOCK, 2) ff_grads_kernel(const T* __restri
 
 // ------------------------------------------------------------------------------------------------ out = A0 B0^T (+ A1 B1^T)
 // Part blockIdx.y takes `span` of the contraction's columns (of both products); with more than one part the sums go to parts
-// [splits, rows, N] in fp32.
+// [splits, rows, N] in fp32. `low` not 0: A0 and A1 have a second part as many elements on.
 template <typename T, int MB>
 __global__ void __launch_bounds__(MM_BLOCK, 2) ff_product_kernel(const T* __restrict__ a0, const T* __restrict__ b0,
                                                                               const T* __restrict__ a1, const T* __restrict__ b1,
-                                                                              int64_t rows, int N, int K, int span, T* __restrict__ out,
+                                                                              int64_t low, int64_t rows, int N, int K, int span, T* __restrict__ out,
                                                                               float* __restrict__ parts) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[2 * MM_STAGE(MB)];
   int64_t rt;
@@ -229,8 +236,10 @@ __global__ void __launch_bounds__(MM_BLOCK, 2) ff_product_kernel(const T* __rest
   const int n0 = ct * 128, k0 = blockIdx.y * span, width = K - k0 < span ? K - k0 : span;
   f32x16 acc[MB][2];
   mm_clear(acc);
-  for (int p = 0; p < (a1 ? 2 : 1); ++p) {
-    const T *a = (p ? a1 : a0) + k0, *b = (p ? b1 : b0) + k0;
+  const int products = a1 ? 2 : 1;
+  for (int i = 0; i < (low ? 2 * products : products); ++i) {
+    const int p = low ? i >> 1 : i;
+    const T *a = (p ? a1 : a0) + (low && i & 1 ? low : 0) + k0, *b = (p ? b1 : b0) + k0;
     mm_phase<T, MB, 2>(mm_side(a, r0, rows, K, width), mm_side(b, n0, N, K, width), mm_side(b, n0 + 64, N, K, width), width, lds, acc);
   }
   const int lane = threadIdx.x & 63, ln = lane & 31, hh = lane >> 5, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
@@ -252,15 +261,17 @@ __global__ void __launch_bounds__(MM_BLOCK, 2) ff_product_kernel(const T* __rest
 
 // ------------------------------------------------------------------------------------------------ weights' gradients
 // Up to three products C[M, N] = sum over rows t of A[t, m] B[t, n], one behind the other in the grid; part `split` of a product goes
-// over rows [split * per, ..) and leaves its sums in parts + split * part_step + at.
+// over rows [split * per, ..) and leaves its sums in parts + split * part_step + at. `twice`: A or B has a second part, a_low or b_low
+// elements on.
 struct FfWeightJob {
   const void *A, *B;
-  int64_t a_stride, b_stride, at;
+  int64_t a_stride, b_stride, a_low, b_low, at;
   int M, N, tiles;  // tiles of 128 x 128
 };
 struct FfWeightJobs {
   FfWeightJob job[3];
   int n, splits;
+  bool twice;
   int64_t rows, per, part_step;
 };
 
@@ -281,10 +292,11 @@ __global__ void __launch_bounds__(MM_BLOCK, 2) ff_weights_kernel(const FfWeightJ
   // bytes of each of 8 rows, 16 lanes 32 bytes of 4 rows; 32 bytes of row r go to place ^ twist(r % 4) of 8, different in
   // any 128 bytes for the 4 rows and in 256 for both halves. fp32: the lane halves read 128 bytes of rows 4 apart.
   auto twist = [](int r) { return (r << 1) ^ (r & 1) ^ (r >> 1); };
+  const T *A = (const T*)job.A, *B = (const T*)job.B;
   auto fetch = [&](int64_t t0, T* to) {
     const int64_t n = end - t0 < BK ? end - t0 : BK;
-    const __amdgpu_buffer_rsrc_t ab = ff_buffer((const T*)job.A + t0 * job.a_stride + m0, ((n - 1) * job.a_stride + job.M - m0) * (int64_t)sizeof(T));
-    const __amdgpu_buffer_rsrc_t bb = ff_buffer((const T*)job.B + t0 * job.b_stride + n0, ((n - 1) * job.b_stride + job.N - n0) * (int64_t)sizeof(T));
+    const __amdgpu_buffer_rsrc_t ab = ff_buffer(A + t0 * job.a_stride + m0, ((n - 1) * job.a_stride + job.M - m0) * (int64_t)sizeof(T));
+    const __amdgpu_buffer_rsrc_t bb = ff_buffer(B + t0 * job.b_stride + n0, ((n - 1) * job.b_stride + job.N - n0) * (int64_t)sizeof(T));
     const int row = tid / CPR, piece = tid % CPR, c = (sizeof(T) == 2 ? piece ^ (twist(row & 3) << 1) : piece ^ ((row & 4) << 1)) * EPC;
     unsigned char* p = reinterpret_cast<unsigned char*>(to) + __builtin_amdgcn_readfirstlane(wave) * 1024;
 #pragma unroll
@@ -310,7 +322,12 @@ __global__ void __launch_bounds__(MM_BLOCK, 2) ff_weights_kernel(const FfWeightJ
       return __builtin_bit_cast(ff_u32x4, v);
     }
   };
-  if (begin < end) {
+  for (int part = 0; part < (jobs.twice ? 2 : 1) && begin < end; ++part) {
+    if (part) {
+      A += job.a_low;
+      B += job.b_low;
+      lds_barrier();  // the first part's last rows have been read
+    }
     fetch(begin, lds[0][0]);
     int which = 0;
     for (int64_t t0 = begin; t0 < end; t0 += BK, which ^= 1) {
@@ -435,13 +452,22 @@ static FfSplit ff_split(const lampa_ff_args* a) {
   return s;
 }
 
+// 16-bit hidden values and their gradients as two parts, their rounding and what it left, where the rows are no more than a tile's: what
+// outputs are off by would else hang on a handful of roundings (by the norm, over the output's own rounding: one row of 136, 32 hidden
+// columns, up to 2.2, 21 rows up to 1.7, 128 rows up to 1.5; 1.41 on average at any number). The last products take twice the operations: at 64 rows x
+// 768, 2 048 hidden columns, bf16, 11 us against 9 and the call 22 against 20, at 32 rows 20.6 against 20.1; at 512 27 against 23, not done.
+#define FF_TWO_ROWS 64
+static bool ff_two(const lampa_ff_args* a) { return a->dtype != GDR_FP32 && a->rows <= FF_TWO_ROWS; }
+
 struct FfAreas {
+  int64_t low;  // elements from a hidden value to its second part, 0: none
   int64_t hidden, dg, du, turned, sums, parts, total;  // turned: Wd^T, Wg^T, Wu^T one behind the other
 };
 static FfAreas ff_areas(const lampa_ff_args* a, int backward) {
-  const int64_t e = ff_size(a), h = ff_area(a->rows * a->F, e), w = ff_area((int64_t)a->D * a->F, e);
+  const int64_t e = ff_size(a), one = ff_area(a->rows * a->F, e), h = ff_two(a) ? 2 * one : one, w = ff_area((int64_t)a->D * a->F, e);
   const FfSplit sp = ff_split(a);
   FfAreas l{};
+  l.low = ff_two(a) ? one / e : 0;
   l.hidden = 0;
   l.dg = h;
   l.du = l.dg + (backward ? h : 0);
@@ -468,11 +494,12 @@ static unsigned ff_column_tiles(int64_t rows, int mb, int F) {
   if ((MB) == 1) GO(1); else GO(2);
 
 template <typename T>
-static int ff_product_go(const lampa_ff_args* a, const T* a0, const T* b0, const T* a1, const T* b1, T* out, float* sums, hipStream_t s) {
+static int ff_product_go(const lampa_ff_args* a, const T* a0, const T* b0, const T* a1, const T* b1, int64_t low, T* out, float* sums,
+                         hipStream_t s) {
   const FfSplit sp = ff_split(a);
 #define FF_GO(MB)                                                                                                                   \
   hipLaunchKernelGGL((ff_product_kernel<T, MB>), dim3(ff_tiles(a->rows, MB, a->D, 128), (unsigned)sp.n), dim3(MM_BLOCK), 0, s, a0, b0, a1, \
-                     b1, a->rows, a->D, a->F, sp.span, out, sp.n > 1 ? sums : (float*)nullptr)
+                     b1, low, a->rows, a->D, a->F, sp.span, out, sp.n > 1 ? sums : (float*)nullptr)
   FF_ROWS(sp.mb, FF_GO)
 #undef FF_GO
   LAMPA_PROF(s, "ff_product_kernel");
@@ -489,13 +516,13 @@ static int ff_fwd_go(const lampa_ff_args* a, hipStream_t s) {
   LAMPA_PROF(s, "start");
 #define FF_GO(MB)                                                                                                                    \
   hipLaunchKernelGGL((ff_hidden_kernel<T, ACT, MB>), dim3(columns ? ff_column_tiles(a->rows, MB, a->F) : ff_tiles(a->rows, MB, a->F, 64)), dim3(MM_BLOCK), 0, s, (const T*)a->x, a->x_stride, \
-                     (const T*)a->w_gate, (const T*)a->w_up, a->rows, a->D, a->F, hidden, columns)
+                     (const T*)a->w_gate, (const T*)a->w_up, a->rows, a->D, a->F, hidden, l.low, columns)
   FF_ROWS(ff_row_blocks(a, a->F, 64), FF_GO)
 #undef FF_GO
   LAMPA_PROF(s, "ff_hidden_kernel");
   const int rc = lampa_launch_status();
   if (rc != LAMPA_OK) return rc;
-  return ff_product_go<T>(a, hidden, (const T*)a->w_down, nullptr, nullptr, (T*)a->y, (float*)((char*)a->workspace + l.sums), s);
+  return ff_product_go<T>(a, hidden, (const T*)a->w_down, nullptr, nullptr, l.low, (T*)a->y, (float*)((char*)a->workspace + l.sums), s);
 }
 
 template <typename T, int ACT>
@@ -515,34 +542,35 @@ static int ff_bwd_go(const lampa_ff_args* a, hipStream_t s) {
 #define FF_GO(MB)                                                                                                                     \
   hipLaunchKernelGGL((ff_grads_kernel<T, ACT, MB>), dim3(columns ? ff_column_tiles(a->rows, MB, a->F) : ff_tiles(a->rows, MB, a->F, 64)), dim3(MM_BLOCK), 0, s, (const T*)a->x, a->x_stride, \
                      (const T*)a->dy, (const T*)a->w_gate, (const T*)a->w_up, (const T*)wd_t, a->rows, a->D, a->F,                          \
-                     a->dw_down ? hidden : (T*)nullptr, dg, du, columns)
+                     a->dw_down ? hidden : (T*)nullptr, dg, du, l.low, columns)
   FF_ROWS(ff_row_blocks(a, a->F, 64), FF_GO)
 #undef FF_GO
   LAMPA_PROF(s, "ff_grads_kernel");
   int rc = lampa_launch_status();
   if (rc != LAMPA_OK) return rc;
   if (a->dx) {
-    rc = ff_product_go<T>(a, dg, wg_t, du, wu_t, (T*)a->dx, (float*)(ws + l.sums), s);
+    rc = ff_product_go<T>(a, dg, wg_t, du, wu_t, l.low, (T*)a->dx, (float*)(ws + l.sums), s);
     if (rc != LAMPA_OK) return rc;
   }
   if (!weights) return LAMPA_OK;
   FfWeightJobs jobs{};
   jobs.splits = ff_splits(a);
   jobs.rows = a->rows;
+  jobs.twice = l.low != 0;
   jobs.per = lampa_align_up((a->rows + jobs.splits - 1) / jobs.splits, 64);
   const int64_t size = (int64_t)a->D * a->F;
   FfSums<T> outs{};
   int tiles = 0;
-  auto add = [&](void* out, const void* A, int64_t as, const void* B, int64_t bs, int M, int N) {
+  auto add = [&](void* out, const void* A, int64_t as, int64_t a_low, const void* B, int64_t bs, int64_t b_low, int M, int N) {
     if (!out) return;
     FfWeightJob& j = jobs.job[jobs.n];
-    j = FfWeightJob{A, B, as, bs, jobs.n * size, M, N, (M + 127) / 128 * ((N + 127) / 128)};
+    j = FfWeightJob{A, B, as, bs, a_low, b_low, jobs.n * size, M, N, (M + 127) / 128 * ((N + 127) / 128)};
     tiles += j.tiles;
     outs.out[jobs.n++] = (T*)out;
   };
-  add(a->dw_gate, dg, a->F, a->x, a->x_stride, a->F, a->D);
-  add(a->dw_up, du, a->F, a->x, a->x_stride, a->F, a->D);
-  add(a->dw_down, a->dy, a->D, hidden, a->F, a->D, a->F);
+  add(a->dw_gate, dg, a->F, l.low, a->x, a->x_stride, 0, a->F, a->D);
+  add(a->dw_up, du, a->F, l.low, a->x, a->x_stride, 0, a->F, a->D);
+  add(a->dw_down, a->dy, a->D, 0, hidden, a->F, l.low, a->D, a->F);
   jobs.part_step = jobs.n * size;
   hipLaunchKernelGGL((ff_weights_kernel<T>), dim3((unsigned)tiles, (unsigned)jobs.splits), dim3(MM_BLOCK), 0, s, jobs, parts);
   LAMPA_PROF(s, "ff_weights_kernel");
