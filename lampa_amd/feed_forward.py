@@ -14,7 +14,7 @@ import torch
 from . import _capi
 from ._capi import check, stream_of
 from .gated_delta import _direct
-from .layer_ops import _ACT, _DTYPES, _on_device, _packed, _same_device
+from .layer_ops import _ACT, _DTYPES, _on_device, _packed, _same_device, _wants_grad
 
 MAX_WIDTH = 1 << 17   # of D and F
 MAX_STRIDE = 1 << 20  # elements between rows of x: offsets inside a tile are formed in 32 bits
@@ -112,6 +112,6 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
         raise TypeError(f"{what}: x and the weights must have one type (bfloat16, float16 or float32), got {x.dtype}, {w_gate.dtype}, "
                         f"{w_up.dtype} and {w_down.dtype}")
     act = _ACT[activation]
-    if _direct(x, w_gate, w_up, w_down):
+    if _direct(x) and not _wants_grad(w_gate, w_up, w_down):  # a module's weights without gradients too
         return _forward(x, w_gate, w_up, w_down, act)
     return _GatedFeedForward.apply(x, w_gate, w_up, w_down, act)

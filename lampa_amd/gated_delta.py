@@ -598,7 +598,6 @@ class _GatedDelta(torch.autograd.Function):
 
 
 _functorch_wrapped = torch._C._functorch.is_functorch_wrapped_tensor
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def _direct(*tensors) -> bool:
@@ -607,7 +606,7 @@ def _direct(*tensors) -> bool:
     vmap and the other functorch transforms, forward-mode gradients, tensor subclasses)."""
     grad = torch.is_grad_enabled()
     for t in tensors:
-        if t is not None and (type(t) not in _PLAIN or (grad and t.requires_grad) or _functorch_wrapped(t)):
+        if t is not None and (type(t) is not torch.Tensor or (grad and t.requires_grad) or _functorch_wrapped(t)):
             return False
     return not (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None
                 or torch._C._are_functorch_transforms_active() or _forward_ad._current_level >= 0)

@@ -7,7 +7,6 @@ import torch
 
 from lampa_amd import feed_forward as ff
 from lampa_amd import linear_recurrence as lr
-from lampa_amd.gated_delta import _direct
 
 
 class Library:
@@ -44,12 +43,13 @@ def test_the_operator_is_in_the_graph(name, grad):
     assert f"^{name}" in str(graph) and "aten::empty" not in str(out.node())
 
 
-def test_parameters_without_gradients_go_to_the_launcher():
-    """A module's weights under no_grad are plain tensors; where a gradient can be asked for, or in a subclass, they are not."""
-    class Other(torch.Tensor):
-        pass
-
-    weight = torch.nn.Parameter(torch.zeros(2))
-    assert not _direct(weight) and not _direct(torch.zeros(2).as_subclass(Other))
+def test_a_modules_weights_without_gradients_go_to_the_launcher(monkeypatch):
+    applied = []
+    monkeypatch.setattr(ff._GatedFeedForward, "apply", lambda *args: applied.append(args))
+    x, weights = torch.randn(4, 16), [torch.nn.Parameter(w) for w in W]
+    ff.gated_feed_forward(x, *weights)
+    assert len(applied) == 1
     with torch.no_grad():
-        assert _direct(weight) and not _direct(torch.zeros(2).as_subclass(Other))
+        assert ff.gated_feed_forward(x, *weights).shape == x.shape and len(applied) == 1
+        torch.func.vmap(lambda t: (ff.gated_feed_forward(x, *weights), t)[1])(x)
+    assert len(applied) == 2
