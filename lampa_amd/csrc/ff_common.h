@@ -79,8 +79,8 @@ static int ff_reduce(const float* rows, int n, int64_t cols, int64_t step, T* ou
 int64_t ff_gemm_workspace(const lampa_ff_args* a, int backward);
 int ff_gemm_fwd(const lampa_ff_args* a, hipStream_t s);
 int ff_gemm_bwd(const lampa_ff_args* a, hipStream_t s);
-// 16-bit types and D <= 128 (ff_fused.h): hidden values in registers (60 000 x 128, 512 hidden columns, bf16: forward 29 us, training
-// step 148; the general form 58 and 290). Wider blocks' sums and operands do not fit a wave's registers.
+// 16-bit types and D <= 128 (ff_fused.h): hidden values in registers (60 000 x 128, 512 hidden columns, bf16: forward 28 us, training
+// step 146; the general form 55 and 263). Wider blocks' sums and operands do not fit a wave's registers.
 static inline bool ff_fused_takes(const lampa_ff_args* a) { return a->dtype != GDR_FP32 && a->D <= 128; }
 int64_t ff_fused_workspace(const lampa_ff_args* a, int backward);
 int ff_fused_fwd_bf16(const lampa_ff_args* a, hipStream_t s);

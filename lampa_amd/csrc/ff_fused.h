@@ -10,12 +10,13 @@
 // Few rows: the chunks of hidden columns are shared out as well, and the outputs' parts summed in order.
 //
 // Measured, 60 000 rows x 128, 512 hidden columns, bf16 (a large product of the library reaches 1.3 .. 1.6 PFLOP/s on this card):
-// y 29 us (23.6 GFLOP, 0.82 PFLOP/s; its products alone, without operand reads, loads or elementwise part, 17 and reading x and writing y
-// 8), dx 48 us (39 GFLOP with the first products again), gradients of the weights 70 us (47 GFLOP) and 8 for their parts' sums (50 MB).
+// y 31 us (23.6 GFLOP, 0.76 PFLOP/s; its products alone, without operand reads, loads or elementwise part, 17 and reading x and writing y
+// 8), dx 49 us (39 GFLOP with the first products again), gradients of the weights 77 us (47 GFLOP) and 9 for their parts' sums (50 MB;
+// medians of a kernel trace, calls back to back take 28 us forward).
 // With 4 waves a workgroup y takes 34 us, with two blocks of 32 rows a wave and one wave a SIMD 42. The weights' kernel holds 192 sums
 // and 96 operands a lane, one wave a SIMD, so its products, its elementwise part and its LDS reads come one after the other; keeping
 // another tile's operands to overlap them spills (125 .. 280 us).
-// One token: 3 us for the two launches beside 17 on the host.
+// One token: two kernels of 5.4 and 5.1 us behind 16 on the host.
 // Built once for each type (ff_fused_bf16.hip, ff_fused_fp16.hip), side by side.
 #pragma once
 #include "ff_common.h"
@@ -345,8 +346,9 @@ struct FuWeights {
 };
 
 // Up to FU_TWO_ROWS rows the hidden values and their gradients enter as two parts, as in `out`: sums of few rows hang on a handful of
-// roundings (with one part, bf16, 1 row of 80 columns: 1.56 times the output's own rounding; 1.4 over many). 4 096 rows x 128, 512
-// hidden columns: 24 us against 21.
+// roundings (with one part, bf16, 1 row of 80 columns: 1.56 times the output's own rounding; 1.4 over many). The more rows
+// a sum runs over, the nearer it keeps to their average, and the more the second part costs: x 128, 512 hidden columns, 4 096 rows 24 us
+// against 21, 8 192 29 against 26, 60 000 91 against 70.
 #define FU_TWO_ROWS 4096
 template <typename T, int ACT, int DB, bool TWO>
 __global__ void __launch_bounds__(FU_BLOCK, 1) ff_fused_weights_kernel(const FuWeights a) {

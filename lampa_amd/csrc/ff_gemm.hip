@@ -11,11 +11,11 @@
 // in order. Rows of 128 bytes are stored with their 16-byte pieces permuted by the row (piece ^ row / 2 % 8): 16 rows of an operand
 // read, 8 even and 8 odd ones, fill the 256 bytes of the banks once.
 //
-// Measured, 8 192 x 768, 2 048 hidden columns, bf16 (the library's 8 192 x 4 096 x 768 product alone 0.88 PFLOP/s): hidden 66 us (51.5 GFLOP,
-// 0.78 PFLOP/s), grads 115 us (77 GFLOP), y and dx together 123 us (77 GFLOP), weights 118 us (77 GFLOP). The matrix cores are
+// Measured, 8 192 x 768, 2 048 hidden columns, bf16 (the library's 8 192 x 4 096 x 768 product alone 0.88 PFLOP/s): hidden 61 us (51.5 GFLOP,
+// 0.84 PFLOP/s), grads 116 us (77 GFLOP), y 35 and dx 62 us (77 GFLOP together), weights 125 us (77 GFLOP; medians of a kernel trace). The matrix cores are
 // busy for half of the time. It is neither LDS alone (without the conflicts of piece ^ row % 8, half of its cycles, hidden and grads
 // take 1% less), nor the loads: steps of 64 bytes, three ahead, take 72 and 136 us against 69 and 122, tiles of 256 rows by 8 waves, two
-// steps ahead, 72 and 125. fp32, 1 501 x 96, 256 hidden columns: 8, 13, 13 and 24 us.
+// steps ahead, 72 and 125. fp32, 1 501 x 96, 256 hidden columns: hidden 7, grads 12, y 9, dx 13, weights 22 us.
 #include "ff_common.h"
 
 #define MM_BLOCK 256
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(256) ff_turn_kernel(const FfTurns t) {
 static int64_t ff_size(const lampa_ff_args* a) { return a->dtype == GDR_FP32 ? 4 : 2; }
 static int64_t ff_area(int64_t n, int64_t elem) { return lampa_align_up(n * elem, 256); }
 
-// Parts of the weights' gradients: as many as make about four workgroups a CU, of 256 rows or more each.
+// Parts of the weights' gradients: as many as make about two workgroups a CU, of 256 rows or more each.
 static int ff_splits(const lampa_ff_args* a) {
   const int64_t tiles = ((a->F + 127) / 128) * (int64_t)((a->D + 127) / 128) * ((a->dw_gate != nullptr) + (a->dw_up != nullptr) + (a->dw_down != nullptr));
   const int64_t want = tiles ? (512 + tiles - 1) / tiles : 1, most = (a->rows + 255) / 256;

@@ -15,9 +15,9 @@
 // Tiles are handed out by a counter, in the order in which they wait for each other: a tile waits only for tiles that were
 // handed out before it, so every wait ends.
 //
-// Measured (a copy of 1 GiB runs at 5.1 TB/s): 60 000 x 512 in bf16, both gates: forward 99 us (307 MB, 3.1 TB/s), gradients 178 us
-// (553 MB, 3.1 TB/s); 24 packed sequences of 15 000 x 192 in fp16 19 us; fp32, 5 packed sequences of 6 007 x 128: 13 and 18 us;
-// one token of 250 x 1024 in bf16 3.3 us. What is left is that tiles under way together finish together, whose loads and whose
+// Measured (medians of a kernel trace; a copy of 1 GiB runs at 5.1 TB/s): 60 000 x 512 in bf16, both gates: forward 101 us (307 MB,
+// 3.0 TB/s), gradients 182 us (553 MB, 3.0 TB/s) and 10 for the sums of dA; 24 packed sequences of 15 000 x 192 in fp16 19 us; fp32, 5
+// packed sequences of 6 007 x 128: 13 and 18 us; one token of 250 x 1024 in bf16 3.5 us. What is left is that tiles under way together finish together, whose loads and whose
 // arithmetic (35 us of the forward) so come one after the other: the forward without any wait, on states of zero, takes 68 us. More
 // or fewer workgroups a CU, tiles of 128 or 256 tokens, fewer polls and a chain of states in place of the groups' maps change it by
 // less than 5 us; tiles of 32 take 128.
