@@ -21,7 +21,7 @@ from torch.autograd.graph import increment_version
 from . import _capi
 from ._capi import check, ptr, stream_of
 from .gated_delta import _direct
-from .layer_ops import _ACT, _DTYPES, _ForwardOnly, _on_device, _plain_f32, _same_device, _sequences, _wants_grad
+from .layer_ops import _ACT, _DTYPES, _on_device, _plain_f32, _same_device, _sequences, _wants_grad
 
 MAX_CHANNELS = 1 << 20
 MAX_STRIDE = 1 << 20  # elements between tokens: the kernels form offsets inside a tile in 32 bits
@@ -204,7 +204,9 @@ def _step_rows(t, D):
     return (t, step) if (inner == 1 or D == 1) and step >= D else (t.contiguous(), D)
 
 
-def _step_launch(x, r, A, i, z, act, normalize, state, target):
+def _step_launch(x, r, A, state, i, z, new_state, act, normalize):
+    target = state if new_state is None else new_state
+    increment_version(target)  # written through its pointer: a backward that saved it must notice
     n, D = x.shape
     (x, xs), (r, rs), (i, is_), (z, zs) = _step_rows(x, D), _step_rows(r, D), _step_rows(i, D), _step_rows(z, D)
     A = _plain_f32(A)
@@ -213,6 +215,18 @@ def _step_launch(x, r, A, i, z, act, normalize, state, target):
         check(_capi.lib().lampa_lr_step(ptr(x), xs, ptr(r), rs, ptr(i), is_, ptr(z), zs, ptr(A), ptr(state), ptr(target), ptr(y), n, D,
                                         _DTYPES[x.dtype], act, int(normalize), stream_of(y)), "lampa_lr_step")
     return y
+
+
+class _Step(torch.autograd.Function):
+    """A step in a graph: traced, or never differentiated (the backward raises)."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _step_launch(*args)
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise NotImplementedError("lampa_amd implements the forward pass of this operator only")
 
 
 def gated_recurrence_step(x: torch.Tensor, decay_gate: torch.Tensor, A: torch.Tensor, state: torch.Tensor,
@@ -238,10 +252,8 @@ def gated_recurrence_step(x: torch.Tensor, decay_gate: torch.Tensor, A: torch.Te
             raise ValueError(f"{what}: new_state overlaps state")
     if x.shape[0] == 0:
         return torch.empty_like(x)
-    target, act = state if new_state is None else new_state, _ACT[gate_activation]
-    increment_version(target)  # written through its pointer: a backward that saved it must notice
-    launch = lambda: _step_launch(x, decay_gate, A, input_gate, gate, act, bool(normalize), state, target)  # noqa: E731
+    args = x, decay_gate, A, state, input_gate, gate, new_state, _ACT[gate_activation], bool(normalize)
     # a traced call has to be in the graph as a function; asking `_direct` takes a microsecond of a step's 13
     if _wants_grad(x, decay_gate, A, input_gate, gate, state) or torch._C._get_tracing_state() is not None:
-        return _ForwardOnly.apply(launch, x, decay_gate, A, input_gate, gate, state)
-    return launch()
+        return _Step.apply(*args)
+    return _step_launch(*args)

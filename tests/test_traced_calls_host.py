@@ -1,6 +1,7 @@
 """A traced call is in the graph as the operator, not as the empty tensor that its kernel would have filled. The library is replaced here;
 nothing is launched."""
 import contextlib
+import struct
 
 import pytest
 import torch
@@ -9,9 +10,15 @@ from lampa_amd import feed_forward as ff
 from lampa_amd import linear_recurrence as lr
 
 
+read = []  # where the operators were told to read x
+
+
 class Library:
     def __getattr__(self, name):
-        return lambda *args: 0
+        def call(first, *rest):
+            read.append(struct.unpack_from("=Q", first)[0] if isinstance(first, bytes) else first)
+            return 0
+        return call
 
 
 @pytest.fixture(autouse=True)
@@ -29,7 +36,7 @@ A = -torch.rand(16)
 CALLS = {
     "_GatedFeedForward": lambda x: ff.gated_feed_forward(x, *W),
     "_GatedRecurrence": lambda x: lr.gated_recurrence(x[None], x[None], A)[0],
-    "_ForwardOnly": lambda x: lr.gated_recurrence_step(x, x, A, torch.zeros(4, 16)),
+    "_Step": lambda x: lr.gated_recurrence_step(x, x, A, torch.zeros(4, 16)),
 }
 
 
@@ -38,9 +45,13 @@ CALLS = {
 @pytest.mark.parametrize("grad", [False, True])
 def test_the_operator_is_in_the_graph(name, grad):
     with torch.set_grad_enabled(grad):
-        graph = torch.jit.trace(CALLS[name], (torch.randn(4, 16),), check_trace=False).graph
-    (out,) = graph.outputs()
-    assert f"^{name}" in str(graph) and "aten::empty" not in str(out.node())
+        graph = torch.jit.trace(CALLS[name], (torch.randn(4, 16),), check_trace=False)
+    (out,) = graph.graph.outputs()
+    assert f"^{name}" in str(graph.graph) and "aten::empty" not in str(out.node())
+    for other in (torch.randn(4, 16), torch.randn(4, 16)):  # run on other tensors, it reads those
+        read.clear()
+        graph(other)
+        assert other.data_ptr() in read
 
 
 def test_a_modules_weights_without_gradients_go_to_the_launcher(monkeypatch):
